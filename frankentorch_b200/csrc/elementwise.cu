@@ -24,9 +24,14 @@ extern "C" int* ftk_status_word(void) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (!g_status[dev]) {
     int* p = nullptr;
-    if (cudaMalloc(&p, 256) != cudaSuccess) return nullptr;
-    cudaMemset(p, 0, 256);
-    g_status[dev] = p;
+    // a first call may come while a stream is being captured, which forbids allocations in the default mode
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (cudaMalloc(&p, 256) == cudaSuccess) {
+      cudaMemset(p, 0, 256);
+      g_status[dev] = p;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
   }
   return g_status[dev];
 }

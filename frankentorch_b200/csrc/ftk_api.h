@@ -340,6 +340,89 @@ int ftk_dp_wait_params(const FtkDpComm* c, int b0, void* stream);
 }
 #endif
 
+// ---- a trained decoder and its next token (rotary_append.cu, paged_attention.cu, logits.cu) -----
+#ifdef __cplusplus
+extern "C" {
+#endif
+// Element types of the operands below
+enum { FTK_T_BF16 = 0, FTK_T_FP16 = 1, FTK_T_FP32 = 2 };
+// Tokens are [B, S, heads, hd] views (strides in elements, unit inner stride, 16-byte rows).  Pages of a cache are
+// [n_pages, heads, page, hd] views, page = 1 << page_shift; position p of sequence b is row p % page of page
+// table[b * table_stride + p / page].
+//
+// Without k_pages: queries and keys (either may be NULL) turned by position into q_out / k_out; with k_pages: keys, turned where
+// inv_freq is given, and values go to their places in the cache, queries (may be NULL) to q_out.  Token s of sequence b is at
+// position start[b] + s (start NULL: s); with counts, tokens from counts[b] on stay out of the cache and their queries as they are.
+// Angle of pair i: position * inv_freq[i]; pairs (i, i + turn / 2), or (2 i, 2 i + 1) when interleaved.
+typedef struct FtkRotaryDesc {
+  long long type, B, S, Hq, Hkv, hd, turn, interleaved, inverse;
+  const void* q;
+  long long q_bs, q_ss, q_hs;
+  const void* k;
+  long long k_bs, k_ss, k_hs;
+  const void* v;
+  long long v_bs, v_ss, v_hs;
+  void* q_out;
+  long long qo_bs, qo_ss, qo_hs;
+  void* k_out;
+  long long ko_bs, ko_ss, ko_hs;
+  const double* inv_freq;   // [turn / 2]
+  const int* start;         // [B] or NULL
+  const int* counts;        // [B] or NULL
+  void* k_pages;
+  long long kp_ps, kp_hs, kp_rs;
+  void* v_pages;
+  long long vp_ps, vp_hs, vp_rs;
+  const int* table;
+  long long table_stride, table_cols, n_pages, page_shift;
+} FtkRotaryDesc;
+int ftk_rotary(const FtkRotaryDesc* d, void* stream);
+
+// One new token per sequence: o[b, h] = sum over t < lengths[b] of softmax_t(scale q[b, h] . k[t]) v[t], keys and values of head
+// h / (Hq / Hkv); lse[b, h] the natural log of the softmax's sum.  A sequence of no tokens: o = 0, lse = -inf.
+typedef struct FtkPagedAttnDesc {
+  long long type, B, Hq, Hkv, hd;
+  double scale;
+  const void* q;
+  long long q_bs, q_hs;
+  void* o;
+  long long o_bs, o_hs;
+  float* lse;               // [B, Hq]
+  const void* k_pages;
+  long long kp_ps, kp_hs, kp_rs;
+  const void* v_pages;
+  long long vp_ps, vp_hs, vp_rs;
+  const int* table;
+  long long table_stride, table_cols, n_pages, page_shift;
+  const int* lengths;       // [B]
+} FtkPagedAttnDesc;
+int ftk_paged_attn(const FtkPagedAttnDesc* d, void* stream);
+
+// Per row r and column c < V: x = logits; x = x > 0 ? x / rep : x * rep where c is among tokens[r, 0:lengths[r]];
+// x -= freq * n + pres * (n > 0) with n the count of c among tokens[r, prompts[r]:lengths[r]]; x += bias; -inf where bit c % 32
+// of word c / 32 of `allowed` is clear.  rep / freq / pres: per row where the pointer is given, else the value.
+typedef struct FtkLogitsDesc {
+  long long type, out_type, R, V;
+  const void* logits;
+  long long ld;
+  void* out;
+  long long ldo;
+  const long long* tokens;  // or NULL
+  long long ldt, L;
+  const int* lengths;       // [R] or NULL (L)
+  const int* prompts;       // [R] or NULL (0)
+  const float *rep_rows, *freq_rows, *pres_rows;
+  double rep, freq, pres;
+  const float* bias;        // or NULL
+  long long bias_rs;        // 0: one for all rows
+  const int* allowed;       // or NULL
+  long long allowed_rs;
+} FtkLogitsDesc;
+int ftk_logits(const FtkLogitsDesc* d, void* stream);
+#ifdef __cplusplus
+}
+#endif
+
 // ---- collectives through the NVSwitch multicast object (nvls.cu) -----------------------------
 #ifdef __cplusplus
 extern "C" {

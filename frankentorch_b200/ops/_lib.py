@@ -58,6 +58,10 @@ class FtkAttnDesc(C.Structure):
 GEMM_DESC = struct.Struct("@7iP3qP3qP3qPP3qPf5iPqiPPi0q")
 ATTN_DESC = struct.Struct("@5if3P9qP3q3P3P")
 assert GEMM_DESC.size == C.sizeof(FtkGemmDesc) and ATTN_DESC.size == C.sizeof(FtkAttnDesc)
+# FtkRotaryDesc, FtkPagedAttnDesc and FtkLogitsDesc have fields of eight bytes only (flags as whole numbers, scalars as doubles)
+ROTARY_DESC = struct.Struct("@9q20q3q8q5q")
+PAGED_ATTN_DESC = struct.Struct("@5qd3q3qq8q5qq")
+LOGITS_DESC = struct.Struct("@4q4q3q2q3q3d4q")
 
 FTK_MAX_RANKS = 8
 COMM_GATHER_A, COMM_GATHER_B, COMM_SCATTER_D = 1, 2, 3
@@ -164,9 +168,10 @@ def load(build_if_missing: bool = True):
         "ftk_wait_probe": [vp, i, ll, vp, vp],
         "ftk_stream_order": [vp, vp],
     }
-    # descriptors packed by GEMM_DESC / ATTN_DESC (a second function object per entry: argument types are per object)
+    # descriptors packed by GEMM_DESC / ATTN_DESC and the like (a second function object per entry: argument types are per object)
     for name, sym in (("gemm_packed", "ftk_gemm_bf16"), ("attn_fwd_packed", "ftk_attn_fwd"),
-                      ("attn_bwd_packed", "ftk_attn_bwd")):
+                      ("attn_bwd_packed", "ftk_attn_bwd"), ("rotary_packed", "ftk_rotary"),
+                      ("paged_attn_packed", "ftk_paged_attn"), ("logits_packed", "ftk_logits")):
         fn = lib[sym]
         fn.argtypes, fn.restype = [C.c_char_p, C.c_void_p], C.c_int
         setattr(lib, name, fn)

@@ -1,0 +1,192 @@
+"""Arguments that the operators between a decoder and its next token refuse, and the page arithmetic that their kernels use,
+without a GPU: every refusal comes before anything is launched."""
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from frankentorch_b200.ops import decode as D
+from frankentorch_b200.ops.kernels import KernelError
+
+CSRC = Path(__file__).resolve().parent.parent / "frankentorch_b200" / "csrc"
+BF = torch.bfloat16
+
+
+def _z(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def _i(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _refused(match, fn, *a, **kw):
+    with pytest.raises(KernelError, match=match):
+        fn(*a, **kw)
+
+
+ROTARY = dict(q=lambda: _z(2, 3, 4, 64), k=lambda: _z(2, 3, 2, 64), inv_freq=lambda: D.rotary_frequencies(64, device="cpu"))
+
+
+@pytest.mark.parametrize("match,change", [
+    ("CUDA tensors", {}),
+    ("bf16 or fp16", {"q": lambda: _z(2, 3, 4, 64, dtype=torch.float32)}),
+    ("4 dimensions", {"q": lambda: _z(2, 12, 64)}),
+    ("k is torch.float16", {"k": lambda: _z(2, 3, 2, 64, dtype=torch.float16)}),
+    (r"k must be \[2, 3", {"k": lambda: _z(2, 4, 2, 64)}),
+    ("multiple of 16", {"q": lambda: _z(2, 3, 4, 72), "k": lambda: None}),
+    ("16 bytes", {"q": lambda: _z(2, 3, 4, 68)[..., 4:]}),
+    ("16 bytes", {"q": lambda: _z(2, 3, 64, 4).transpose(2, 3)}),
+    ("16 bytes", {"k": lambda: _z(2, 3, 2, 65)[..., :64]}),
+    ("float64", {"inv_freq": lambda: torch.zeros(32)}),
+    ("multiple of 8", {"inv_freq": lambda: torch.zeros(12, dtype=torch.float64)}),
+    ("half of the head", {"inv_freq": lambda: torch.zeros(40, dtype=torch.float64)}),
+    ("needs inv_freq", {"inv_freq": lambda: None}),
+    ("start must be", {"start": lambda: torch.zeros(2, dtype=torch.int64)}),
+    ("start must be", {"start": lambda: _i(0, 0, 0)}),
+    ("q_out must be", {"q_out": lambda: _z(2, 3, 5, 64)}),
+    ("must not share memory", {"q_out": lambda: _z(2, 3, 1, 64).expand(2, 3, 4, 64)}),
+    ("k_out is torch.float32", {"k_out": lambda: _z(2, 3, 2, 64, dtype=torch.float32)}),
+])
+def test_rotary(match, change):
+    kw = {n: f() for n, f in {**ROTARY, **change}.items()}
+    _refused(match, D.rotary, kw.pop("q"), kw.pop("k"), kw.pop("inv_freq"), **kw)
+
+
+def test_frequencies():
+    w = D.rotary_frequencies(64, base=500.0, device="cpu")
+    assert w.dtype == torch.float64 and w.shape == (32,)
+    assert [float(w[i]) for i in (0, 1, 31)] == pytest.approx([1.0, 500.0 ** (-1 / 32), 500.0 ** (-31 / 32)], rel=1e-15)
+    _refused("multiple of 16", D.rotary_frequencies, 24, device="cpu")
+
+
+APPEND = dict(k_pages=lambda: _z(5, 2, 16, 64), v_pages=lambda: _z(5, 2, 16, 64), table=lambda: torch.zeros(3, 4, dtype=torch.int32),
+              k=lambda: _z(3, 7, 2, 64), v=lambda: _z(3, 7, 2, 64), start=lambda: _i(0, 0, 0), counts=lambda: None)
+
+
+@pytest.mark.parametrize("match,change", [
+    ("CUDA tensors", {}),
+    ("bf16 or fp16", {"k": lambda: _z(3, 7, 2, 64, dtype=torch.float32)}),
+    ("differ", {"v": lambda: _z(3, 7, 1, 64)}),
+    ("v is", {"v": lambda: _z(3, 7, 2, 64, dtype=torch.float16)}),
+    ("k_pages is", {"k_pages": lambda: _z(5, 2, 16, 64, dtype=torch.float16)}),
+    ("differ", {"v_pages": lambda: _z(6, 2, 16, 64)}),
+    ("power of two", {"k_pages": lambda: _z(5, 2, 12, 64), "v_pages": lambda: _z(5, 2, 12, 64)}),
+    ("pages must be", {"k_pages": lambda: _z(5, 3, 16, 64), "v_pages": lambda: _z(5, 3, 16, 64)}),
+    ("pages must be", {"k_pages": lambda: _z(5, 2, 16, 128), "v_pages": lambda: _z(5, 2, 16, 128)}),
+    ("must not share memory", {"k_pages": lambda: _z(1, 2, 16, 64).expand(5, 2, 16, 64)}),
+    ("16 bytes", {"v_pages": lambda: _z(5, 2, 16, 68)[..., :64]}),
+    ("no pages", {"k_pages": lambda: _z(0, 2, 16, 64), "v_pages": lambda: _z(0, 2, 16, 64), "gpu": lambda: True}),
+    ("page table", {"table": lambda: torch.zeros(3, 4, dtype=torch.int64)}),
+    ("page table", {"table": lambda: torch.zeros(2, 4, dtype=torch.int32)}),
+    ("page table", {"table": lambda: torch.zeros(3, 0, dtype=torch.int32)}),
+    ("page table", {"table": lambda: torch.zeros(4, 3, dtype=torch.int32).t()}),
+    ("start must be", {"start": lambda: _i(0, 0)}),
+    ("counts must be", {"counts": lambda: torch.zeros(3)}),
+    ("inv_freq is missing", {"q": lambda: _z(3, 7, 4, 64)}),
+    ("q must be", {"q": lambda: _z(3, 6, 4, 64), "inv_freq": lambda: D.rotary_frequencies(32, device="cpu")}),
+    ("q_out without q", {"q_out": lambda: _z(3, 7, 4, 64)}),
+])
+def test_append(match, change, monkeypatch):
+    if change.get("gpu"):        # a refusal behind the check of devices
+        monkeypatch.setattr(D, "_on_device", lambda *a, **k: None)
+    kw = {n: f() for n, f in {**APPEND, **change}.items() if n != "gpu"}
+    _refused(match, D.paged_append, **kw)
+
+
+ATTEND = dict(q=lambda: _z(3, 4, 64), k_pages=lambda: _z(5, 2, 16, 64), v_pages=lambda: _z(5, 2, 16, 64),
+              table=lambda: torch.zeros(3, 4, dtype=torch.int32), lengths=lambda: _i(1, 2, 3))
+
+
+@pytest.mark.parametrize("match,change", [
+    ("CUDA tensors", {}),
+    ("bf16 or fp16", {"q": lambda: _z(3, 4, 64, dtype=torch.float32)}),
+    ("3 dimensions", {"q": lambda: _z(3, 1, 4, 64)}),
+    ("head size", {"q": lambda: _z(3, 4, 32), "k_pages": lambda: _z(5, 2, 16, 32), "v_pages": lambda: _z(5, 2, 16, 32)}),
+    ("groups", {"q": lambda: _z(3, 5, 64)}),
+    ("groups", {"k_pages": lambda: _z(5, 0, 16, 64), "v_pages": lambda: _z(5, 0, 16, 64)}),
+    ("4 dimensions", {"k_pages": lambda: _z(2, 16, 64)}),
+    ("k_pages is", {"k_pages": lambda: _z(5, 2, 16, 64, dtype=torch.float16)}),
+    ("differ", {"k_pages": lambda: _z(5, 2, 8, 64)}),
+    ("power of two", {"k_pages": lambda: _z(5, 2, 24, 64), "v_pages": lambda: _z(5, 2, 24, 64)}),
+    ("16 bytes", {"q": lambda: _z(3, 4, 65)[..., :64]}),
+    ("lengths must be", {"lengths": lambda: torch.ones(3, dtype=torch.int64)}),
+    ("lengths must be", {"lengths": lambda: _i(1, 1, 1, 1, 1, 1)[::2]}),
+    ("page table", {"table": lambda: torch.zeros(12, dtype=torch.int32)}),
+    ("out must be", {"out": lambda: _z(3, 4, 128)}),
+    ("must not share memory", {"out": lambda: _z(3, 1, 64).expand(3, 4, 64)}),
+    ("out is", {"out": lambda: _z(3, 4, 64, dtype=torch.float32)}),
+])
+def test_attention(match, change):
+    _refused(match, D.paged_attention, **{n: f() for n, f in {**ATTEND, **change}.items()})
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("CUDA tensors", {}),
+    ("bf16, fp16 or fp32", {"logits": lambda: _z(2, 40, dtype=torch.float64)}),
+    ("rows, columns", {"logits": lambda: _z(2, 2, 40)}),
+    ("rows, columns", {"logits": lambda: _z(40, 2).t()}),
+    ("does not fit", {"vocab": lambda: 41}),
+    ("does not fit", {"vocab": lambda: 0}),
+    ("leave as", {"out_dtype": lambda: torch.float16}),
+    ("leave as", {"out": lambda: _z(2, 40, dtype=torch.float16)}),
+    ("out must be", {"out": lambda: _z(2, 39)}),
+    ("out must be", {"out": lambda: _z(1, 40).expand(2, 40)}),
+    ("tokens must be", {"tokens": lambda: torch.zeros(2, 3, dtype=torch.int32)}),
+    ("tokens must be", {"tokens": lambda: torch.zeros(3, 3, dtype=torch.int64)}),
+    ("lengths without", {"lengths": lambda: _i(1, 1)}),
+    ("penalties without", {"repetition": lambda: 1.2}),
+    ("lengths must be", {"tokens": lambda: torch.zeros(2, 3, dtype=torch.int64), "lengths": lambda: _i(1)}),
+    ("must be positive", {"tokens": lambda: torch.zeros(2, 3, dtype=torch.int64), "repetition": lambda: 0.0}),
+    ("must be finite", {"tokens": lambda: torch.zeros(2, 3, dtype=torch.int64), "presence": lambda: float("nan")}),
+    ("frequency must be", {"tokens": lambda: torch.zeros(2, 3, dtype=torch.int64), "frequency": lambda: torch.zeros(3)}),
+    ("bias must be", {"bias": lambda: torch.zeros(39)}),
+    ("bias must be", {"bias": lambda: torch.zeros(3, 40)}),
+    ("bias must be", {"bias": lambda: _z(40)}),
+    ("allowed must be", {"allowed": lambda: torch.zeros(1, dtype=torch.int32)}),
+    ("allowed must be", {"allowed": lambda: torch.zeros(2, 40, dtype=torch.bool)}),
+])
+def test_logits(match, kw):
+    kw = {n: f() for n, f in kw.items()}
+    _refused(match, D.logits_process, kw.pop("logits", _z(2, 40)), **kw)
+
+
+PROBE = r"""
+#include <cassert>
+#include <cstdio>
+#include "ftk_api.h"
+#include "paged_cache.h"
+int main() {
+  const int table[] = {3, 0, 7, -1, 2, 1, 6, 2147483647};          // two sequences of four pages
+  const ftk::PagedTable t = {table, 4, 4, 7, 5};                   // seven pages of 32 rows
+  assert(ftk::paged_page(t, 0, 0) == 3 && ftk::paged_page(t, 0, 31) == 3 && ftk::paged_page(t, 0, 32) == 0);
+  assert(ftk::paged_page(t, 0, 64) == -1);                         // 7 is no page of the cache
+  assert(ftk::paged_page(t, 0, 96) == -1 && ftk::paged_page(t, 0, 127) == -1);
+  assert(ftk::paged_page(t, 0, 128) == -1);                        // behind the table: not the next sequence's page
+  assert(ftk::paged_page(t, 0, -1) == -1 && ftk::paged_page(t, 1, -128) == -1);
+  assert(ftk::paged_page(t, 1, 0) == 2 && ftk::paged_page(t, 1, 95) == 6 && ftk::paged_page(t, 1, 96) == -1);
+  assert(ftk::paged_page(t, 0, 1ll << 40) == -1);
+  assert(ftk::paged_row(t, 0) == 0 && ftk::paged_row(t, 31) == 31 && ftk::paged_row(t, 33) == 1);
+  bool bad;
+  assert(ftk::paged_length(t, 0, bad) == 0 && !bad);
+  assert(ftk::paged_length(t, 128, bad) == 128 && !bad);
+  assert(ftk::paged_length(t, 129, bad) == 128 && bad);
+  assert(ftk::paged_length(t, -1, bad) == 0 && bad);
+  const ftk::PagedTable wide = {table, 4, 1 << 20, 7, 16};         // more rows than 32 bits count
+  assert(ftk::paged_length(wide, 2147483647, bad) == 2147483647 && !bad);
+  const ftk::PagedTable one = {table, 4, 4, 7, 0};                 // pages of one row
+  assert(ftk::paged_page(one, 1, 2) == 6 && ftk::paged_row(one, 2) == 0);
+  std::printf("%zu %zu %zu\n", sizeof(FtkRotaryDesc), sizeof(FtkPagedAttnDesc), sizeof(FtkLogitsDesc));
+}
+"""
+
+
+def test_page_arithmetic_and_descriptors(tmp_path):
+    from frankentorch_b200.ops import _lib
+    src = tmp_path / "probe.cpp"
+    src.write_text(PROBE)
+    exe = tmp_path / "probe"
+    subprocess.run(["g++", "-std=c++17", "-I", str(CSRC), str(src), "-o", str(exe)], check=True, timeout=120)
+    sizes = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.split()
+    assert [int(x) for x in sizes] == [_lib.ROTARY_DESC.size, _lib.PAGED_ATTN_DESC.size, _lib.LOGITS_DESC.size]
