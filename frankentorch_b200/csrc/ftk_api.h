@@ -396,7 +396,9 @@ typedef struct FtkPagedAttnDesc {
   long long table_stride, table_cols, n_pages, page_shift;
   const int* lengths;       // [B]
 } FtkPagedAttnDesc;
-int ftk_paged_attn(const FtkPagedAttnDesc* d, void* stream);
+// Scratch of one call in bytes (0: none), or a negative value for rejected arguments.  Its contents do not outlive the call.
+long long ftk_paged_attn_scratch(const FtkPagedAttnDesc* d);
+int ftk_paged_attn(const FtkPagedAttnDesc* d, void* scratch, void* stream);
 
 // Per row r and column c < V: x = logits; x = x > 0 ? x / rep : x * rep where c is among tokens[r, 0:lengths[r]];
 // x -= freq * n + pres * (n > 0) with n the count of c among tokens[r, prompts[r]:lengths[r]]; x += bias; -inf where bit c % 32

@@ -3,6 +3,23 @@
 // Mathematics.  With scores x_t = scale q . k_t the running maximum m, the sum l = sum_t exp(x_t - m) and the accumulator
 // a = sum_t exp(x_t - m) v_t are carried over the tokens; a larger maximum rescales l and a by exp(m_old - m_new).  Two parts join
 // the same way.  o = a / l, lse = m + log(l); a part of no tokens has m = -inf, l = 0.
+//
+// What bounds it: every key and value is read once, 1 to 16 flops a byte, so it is the copy bandwidth.
+//
+// Work.  A unit is a tile of 64 tokens of one head of the cache with the (up to 16) query heads that share it, so keys and values
+// are read once for the group.  The units of all sequences and heads are one list, of which each of the (two per SM) CTAs takes an
+// equal piece: ragged batches, few long sequences and many short ones all keep every SM busy to the end.  The list is made from
+// the lengths on the device, so a captured launch follows them.  A CTA that has a whole head writes the output; pieces of one are
+// left as (m, l, a) in the call's scratch and joined by a second kernel, always in the order of the tokens.  Where the table is so
+// short that nothing is worth splitting a CTA takes one head and there is no second kernel.
+//
+// Inside a CTA each of four warps takes 16 tokens of the tile on its own, through a ring of stages in shared memory that it fills
+// with 16-byte asynchronous copies several tiles (and heads, and sequences) ahead: no barrier but the warp's own until the end of a
+// head.  Scores and the product with V are 16 x 8 x 16 matrix instructions of the warp (mma.sync): rows of a tile are the query
+// heads of the group, of which there are too few for a tile of the tensor memory's 128 rows, and a quarter of the warp
+// instructions' rate is enough to keep up with the memory.  Probabilities are needed in 16 bits there; rounding them once would
+// cost as much accuracy as the rounding of the output, so each is split into two 16-bit halves, p = hi + lo with an error of
+// 2^-17: for groups of up to 8 heads the lo halves are the rows 8 to 15 of the same instruction, which are idle otherwise.
 #include <math.h>
 
 #include "ft_sm100.cuh"
@@ -16,78 +33,445 @@ extern "C" int* ftk_status_word(void);
 namespace ftk {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;
+constexpr int PA_RING = 24 * 1024;           // bytes of a warp's ring: six stages of 16 tokens of 64 elements, three of 128
+constexpr int PA_WHOLE = 8;                  // tiles per head up to which a head is left whole
+constexpr int PA_HEADER = 8;                 // ints per CTA in front of the parts
 
-// One CTA per sequence and query head; each of its four warps takes every fourth token.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const FtkPagedAttnDesc d, int* status) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// fp16 has five bits of exponent: probabilities are carried times 2^15, so that what underflows is 2^-39 of the largest.
+template <typename T> struct PaShift { static constexpr float value = 0.f; };
+template <> struct PaShift<__half> { static constexpr float value = 15.f; };
+
+struct PagedAttn {
+  FtkPagedAttnDesc d;
+  int group, subs, sub_heads;      // query heads per head of the cache, parts of a group, heads of a part
+  int* header;                     // [CTAs][PA_HEADER]
+  float* parts;                    // [CTAs][2][rows][hd + 2]: accumulators, then maxima and sums
+};
+
+// A place in the list of tiles: tile `t` of `tiles` of unit head `h` (head of the cache times part of the group) of sequence `b`.
+struct Place {
+  int b, h, t, tiles, n;
+};
+
+template <int ROWS, int HD> struct PaSmem {
+  static constexpr int STAGE = 16 * HD * 4, STAGES = PA_RING / STAGE;
+  static constexpr int MERGE = PA_WARPS * ROWS * 64 * 4;      // accumulators of 64 columns of all warps
+  static constexpr int BYTES = PA_WARPS * PA_RING + MERGE + 2 * PA_WARPS * ROWS * 4 + PA_WARPS * STAGES * 4;
+};
+
+template <typename T, int HD, int ROWS, bool SPLIT>
+__global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
+  typedef PaSmem<ROWS, HD> SM;
+  constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 8, NT = HD / 8, KS = HD / 16;
+  constexpr float SHIFT = PaShift<T>::value;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const FtkPagedAttnDesc& d = a.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = (int)d.Hkv * a.subs;
+  unsigned char* ring = smem + warp * PA_RING;
+  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * PA_RING);
+  float* stat = merge + SM::MERGE / 4;                                     // [2][warps][ROWS]
+  unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * PA_WARPS * ROWS) + warp * STAGES;
+  const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
+  const auto length = [&](int b) {
+    bool bad;
+    const long long n = paged_length(table, d.lengths[b], bad);
+    if (bad) ft_index_ok(-1, 1, status);
+    return (int)n;
+  };
+  const auto row0 = [&](int h) { return (h / a.subs) * a.group + (h % a.subs) * a.sub_heads; };      // first query head
+  const auto rows_of = [&](int h) { return min(a.sub_heads, a.group - (h % a.subs) * a.sub_heads); };
   pdl_wait();
   pdl_trigger();
-  constexpr int V = HD / 32;       // elements of a row per lane
-  const int b = blockIdx.y, h = blockIdx.x, g = h / (int)(d.Hq / d.Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const PagedTable t = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
-  bool bad;
-  const long long n = paged_length(t, d.lengths[b], bad);
-  if (bad) ft_index_ok(-1, 1, status);
-  const T* q = (const T*)d.q + b * d.q_bs + h * d.q_hs;
-  float qv[V], acc[V], m = -INFINITY, l = 0.f;
-  const float sc = (float)d.scale * LOG2E;
+
+  // ---- this CTA's piece of the list
+  Place p;
+  long long left;                       // tiles of the piece
+  long long first_unit = 0, total = 0, per = 0;
+  if (!SPLIT) {
+    p.b = blockIdx.x / heads, p.h = blockIdx.x % heads, p.t = 0;
+    p.n = length(p.b), p.tiles = (p.n + PA_TILE - 1) / PA_TILE;
+    left = p.tiles;
+  } else {
+    // tiles in front of each thread's share of the sequences, then the sequence in which the piece begins
+    long long* sums = reinterpret_cast<long long*>(smem);
+    int* found = reinterpret_cast<int*>(sums + PA_WARPS + 1);
+    const int each = ((int)d.B + PA_WARPS * 32 - 1) / (PA_WARPS * 32);
+    const int b0 = min((int)d.B, (int)threadIdx.x * each), b1 = min((int)d.B, b0 + each);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (length(b) + PA_TILE - 1) / PA_TILE;
+    long long upto = mine;
 #pragma unroll
-  for (int i = 0; i < V; ++i) qv[i] = Half16<T>::one(q[lane * V + i]) * sc, acc[i] = 0.f;
-  for (long long p = warp; p < n; p += 4) {
-    const long long page = paged_page(t, b, p);
-    if (page < 0) {
-      ft_index_ok(-1, 1, status);
-      continue;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
     }
-    const T* k = (const T*)d.k_pages + page * d.kp_ps + g * d.kp_hs + paged_row(t, p) * d.kp_rs + lane * V;
-    const T* v = (const T*)d.v_pages + page * d.vp_ps + g * d.vp_hs + paged_row(t, p) * d.vp_rs + lane * V;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) x += qv[i] * Half16<T>::one(k[i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top;
-    const float f = exp2f(m - base), e = exp2f(x - base);
-    m = top;
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = acc[i] * f + e * Half16<T>::one(v[i]);
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    long long front = upto - mine;
+    for (int w = 0; w < PA_WARPS; ++w) {
+      if (w < warp) front += sums[w];
+      total += sums[w];
+    }
+    total *= heads;
+    per = max((total + gridDim.x - 1) / gridDim.x, 2ll);      // a part of less than two tiles costs more to join than it saves
+    first_unit = per * blockIdx.x;
+    left = min(per, total - first_unit);
+    front *= heads;
+    if (left > 0 && front <= first_unit && first_unit < front + mine * heads) {
+      for (int b = b0; b < b1; ++b) {
+        const int n = length(b), tiles = (n + PA_TILE - 1) / PA_TILE;
+        if (first_unit < front + (long long)tiles * heads) {
+          found[0] = b, found[1] = (int)((first_unit - front) / tiles), found[2] = (int)((first_unit - front) % tiles);
+          found[3] = tiles, found[4] = n;
+          break;
+        }
+        front += (long long)tiles * heads;
+      }
+    }
+    __syncthreads();
+    p = {found[0], found[1], found[2], found[3], found[4]};
+    __syncthreads();                    // the ring begins where this was
+    if (threadIdx.x == 0) a.header[(long long)blockIdx.x * PA_HEADER] = -1;
+    // sequences of no tokens are in nobody's piece
+    for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
+      if (length(b) != 0) continue;
+      for (int i = threadIdx.x; i < (int)d.Hq * HD; i += PA_WARPS * 32) ((T*)d.o)[b * d.o_bs + (i / HD) * d.o_hs + i % HD] = Half16<T>::round(0.f);
+      for (int i = threadIdx.x; i < (int)d.Hq; i += PA_WARPS * 32) d.lse[(long long)b * d.Hq + i] = -INFINITY;
+    }
+    if (left <= 0) return;
   }
-  __shared__ float sa[4][HD], sm[4], sl[4];
+
+  // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences
+  Place f = p;
+  long long to_load = left;
+  int next_page = -1;                   // lane j < 16: page of token j of the warp's part of the tile at `f`
+  const auto fetch_page = [&]() {
+    const long long tok = (long long)f.t * PA_TILE + warp * 16 + (lane & 15);
+    next_page = -1;
+    if (to_load > 0 && tok < f.n) {
+      next_page = (int)paged_page(table, f.b, tok);
+      if (next_page < 0) ft_index_ok(-1, 1, status);
+    }
+  };
+  const uint32_t ring_s = smem_u32(ring);
+  const int lrow = lane / CH, lchunk = lane % CH;
+  const auto load = [&](int stage) {
+    if (to_load > 0) {
+      const unsigned ok = __ballot_sync(0xffffffffu, next_page >= 0) & 0xffffu;
+      if (lane == 0) there[stage] = ok;
+      const int g = f.h / a.subs, tok0 = f.t * PA_TILE + warp * 16;
+      const T* kb = (const T*)d.k_pages + g * d.kp_hs + lchunk * 8;
+      const T* vb = (const T*)d.v_pages + g * d.vp_hs + lchunk * 8;
+      const uint32_t dst = ring_s + stage * STAGE;
 #pragma unroll
-  for (int i = 0; i < V; ++i) sa[warp][lane * V + i] = acc[i];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = top == -INFINITY ? 0.f : top;
-  float f[4], sum = 0.f;
+      for (int r = 0; r < 16; r += 32 / CH) {
+        const int row = r + lrow;
+        const long long page = __shfl_sync(0xffffffffu, next_page, row);
+        const long long in = paged_row(table, tok0 + row);
+        const bool t = page >= 0;
+        const uint32_t at = dst + row * (HD * 2) + ((lchunk ^ (row & 7)) << 4);
+        copy16(at, t ? kb + page * d.kp_ps + in * d.kp_rs : kb, t);
+        copy16(at + 16 * HD * 2, t ? vb + page * d.vp_ps + in * d.vp_rs : vb, t);
+      }
+      --to_load;
+      if (++f.t == f.tiles) {
+        f.t = 0;
+        if (++f.h == heads) {
+          f.h = 0;
+          f.tiles = 0;
+          while (to_load > 0 && f.tiles == 0 && f.b + 1 < (int)d.B) f.n = length(++f.b), f.tiles = (f.n + PA_TILE - 1) / PA_TILE;
+        }
+      }
+      fetch_page();
+    }
+    copy_commit();
+  };
+  fetch_page();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) f[w] = exp2f(sm[w] - base), sum += f[w] * sl[w];
-  for (int i = threadIdx.x; i < HD; i += 128) {
-    float a = 0.f;
+  for (int s = 0; s < STAGES - 1; ++s) load(s);
+
+  // ---- tiles
+  const float sc = (float)d.scale * LOG2E;
+  uint32_t q[KS][ROWS == 16 ? 4 : 2];
+  float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+  const auto begin = [&]() {            // queries of the head at `p`; rows beyond the group are zero
+    const int first = row0(p.h), rows = rows_of(p.h);
+    const T* base = (const T*)d.q + p.b * d.q_bs;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) a += f[w] * sa[w][i];
-    ((T*)d.o)[b * d.o_bs + h * d.o_hs + i] = Half16<T>::round(sum == 0.f ? 0.f : a / sum);
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < (ROWS == 16 ? 4 : 2); ++i) {
+        const int row = r0 + (ROWS == 16 && (i & 1) ? 8 : 0), col = k * 16 + c0 + ((ROWS == 16 ? i >> 1 : i) ? 8 : 0);
+        q[k][i] = row < rows ? *reinterpret_cast<const uint32_t*>(base + (first + row) * d.q_hs + col) : 0u;
+      }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  };
+  bool begun = p.t == 0;                // the piece has the beginning of the head at `p`
+  int parts = 0;
+  begin();
+  int stage = 0;
+  for (;;) {
+    if (left > 0) {
+      copy_wait<STAGES - 2>();
+      __syncwarp();
+      const uint32_t ks = ring_s + stage * STAGE, vs = ks + 16 * HD * 2;
+      const unsigned ok = there[stage];
+      const int refill = stage == 0 ? STAGES - 1 : stage - 1;
+      float s[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t b[4];
+        const int row = ((lane >> 4) << 3) + (lane & 7), ch = 2 * k + ((lane >> 3) & 1);
+        ldm4(ks + row * (HD * 2) + ((ch ^ (row & 7)) << 4), b);
+        const uint32_t qa[4] = {q[k][0], ROWS == 16 ? q[k][1] : 0u, ROWS == 16 ? q[k][ROWS == 16 ? 2 : 0] : q[k][1],
+                                ROWS == 16 ? q[k][ROWS == 16 ? 3 : 0] : 0u};
+        mma16<T>(s[0], qa, b[0], b[1]);
+        mma16<T>(s[1], qa, b[2], b[3]);
+      }
+      load(refill);                     // the stage that the tile before left: its reads are behind the warp's barrier
+      // masked scores, and the larger maximum of the row's sixteen tokens and what was there
+      uint32_t hi[4] = {}, lo[4] = {};
+      float grow[2];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < (ROWS == 16 ? 2 : 1); ++r) {
+        float x[4], top = m[r];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = (i >> 1) * 8 + c0 + (i & 1);
+          x[i] = (ok >> tok) & 1u ? s[i >> 1][2 * r + (i & 1)] * sc : -INFINITY;
+          top = fmaxf(top, x[i]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float base = top == -INFINITY ? 0.f : top;
+        moved |= top != m[r];
+        grow[r] = exp2f(m[r] - base);
+        m[r] = top;
+        float e[4], h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = exp2f(x[i] - base + SHIFT);
+        l[r] = l[r] * grow[r] + ((e[0] + e[1]) + (e[2] + e[3]));
+        hi[r] = Half16<T>::down(e[0], e[1]), hi[2 + r] = Half16<T>::down(e[2], e[3]);
+        const float2 u = Half16<T>::up(hi[r]), w = Half16<T>::up(hi[2 + r]);
+        h[0] = u.x, h[1] = u.y, h[2] = w.x, h[3] = w.y;
+        lo[r] = Half16<T>::down(e[0] - h[0], e[1] - h[1]), lo[2 + r] = Half16<T>::down(e[2] - h[2], e[3] - h[3]);
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+        const float g0 = grow[0], g1 = ROWS == 16 ? grow[ROWS == 16 ? 1 : 0] : grow[0];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i][0] *= g0, acc[i][1] *= g0, acc[i][2] *= g1, acc[i][3] *= g1;
+      }
+      if (ROWS != 16) hi[1] = lo[0], hi[3] = lo[2];
+#pragma unroll
+      for (int i = 0; i < NT; i += 2) {
+        uint32_t b[4];
+        const int row = (((lane >> 3) & 1) << 3) + (lane & 7), ch = i + (lane >> 4);
+        ldm4t(vs + row * (HD * 2) + ((ch ^ (row & 7)) << 4), b);
+        mma16<T>(acc[i], hi, b[0], b[1]);
+        mma16<T>(acc[i + 1], hi, b[2], b[3]);
+        if (ROWS == 16) {
+          mma16<T>(acc[i], lo, b[0], b[1]);
+          mma16<T>(acc[i + 1], lo, b[2], b[3]);
+        }
+      }
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      --left;
+      ++p.t;
+    }
+    if (left > 0 && p.t < p.tiles) continue;
+
+    // ---- the end of a head, or of the piece: the warps' parts become one, over 64 columns at a time
+#pragma unroll
+    for (int r = 0; r < (ROWS == 16 ? 2 : 1); ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if ((lane & 3) == 0) {
+        stat[warp * ROWS + r * 8 + r0] = m[r];
+        stat[(PA_WARPS + warp) * ROWS + r * 8 + r0] = l[r];
+      }
+    }
+    const bool whole = begun && p.t == p.tiles;
+    const int first = row0(p.h), rows = rows_of(p.h);
+    float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * ROWS * (HD + 2) : nullptr;
+#pragma unroll
+    for (int half = 0; half < HD / 64; ++half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float* to = merge + (warp * ROWS + r0) * 64 + i * 8 + c0;
+        const float* c = acc[half * 8 + i];
+        if (ROWS == 16) {
+          *reinterpret_cast<float2*>(to) = make_float2(c[0], c[1]);
+          *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(c[2], c[3]);
+        } else {
+          *reinterpret_cast<float2*>(to) = make_float2(c[0] + c[2], c[1] + c[3]);
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * 64; i += PA_WARPS * 32) {
+        const int row = i >> 6, col = half * 64 + (i & 63);
+        float top = stat[row], v = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < PA_WARPS; ++w) top = fmaxf(top, stat[w * ROWS + row]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+          const float e = exp2f(stat[w * ROWS + row] - base);
+          v += e * merge[(w * ROWS + row) * 64 + (i & 63)];
+          sum += e * stat[(PA_WARPS + w) * ROWS + row];
+        }
+        if (!SPLIT || whole) {
+          ((T*)d.o)[p.b * d.o_bs + (first + row) * d.o_hs + col] = Half16<T>::round(sum == 0.f ? 0.f : v / sum);
+          if (col == 0) d.lse[(long long)p.b * d.Hq + first + row] = sum == 0.f ? -INFINITY : (top + log2f(sum) - SHIFT) * LN2;
+        } else {
+          part[row * HD + col] = v;
+          if (col == 0) part[ROWS * HD + row] = top, part[ROWS * (HD + 1) + row] = sum;
+        }
+      }
+      __syncthreads();
+    }
+    if (!SPLIT) return;
+    if (begun && p.t < p.tiles && threadIdx.x == 0) {
+      // the part that has the beginning of its head says who has the rest, up to the CTA of the head's last tile
+      const long long behind = first_unit + min(per, total - first_unit);
+      int* h = a.header + (long long)blockIdx.x * PA_HEADER;
+      h[0] = 0, h[1] = p.b, h[2] = p.h, h[3] = parts, h[4] = (int)((behind + (p.tiles - p.t) - 1) / per);
+    }
+    parts = 1;
+    if (left <= 0) return;
+    // the next head
+    begun = true;
+    p.t = 0;
+    if (++p.h == heads) {
+      p.h = 0;
+      p.tiles = 0;
+      while (p.tiles == 0 && p.b + 1 < (int)d.B) p.n = length(++p.b), p.tiles = (p.n + PA_TILE - 1) / PA_TILE;
+    }
+    begin();
   }
-  if (threadIdx.x == 0) d.lse[(long long)b * d.Hq + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-template <typename T, int HD>
-static int launch(const FtkPagedAttnDesc& d, cudaStream_t s) {
-  return launch_pdl(paged_attn_kernel<T, HD>, dim3((unsigned)d.Hq, (unsigned)d.B), dim3(128), 0, s, d, ftk_status_word());
+// Joins the parts of a head that several CTAs had: block (c, row) that whose first part CTA c has.
+template <typename T, int HD, int ROWS>
+__global__ void __launch_bounds__(HD) paged_attn_join_kernel(const __grid_constant__ PagedAttn a) {
+  constexpr float SHIFT = PaShift<T>::value;
+  pdl_wait();
+  pdl_trigger();
+  const FtkPagedAttnDesc& d = a.d;
+  const int c = blockIdx.x, row = blockIdx.y;
+  const int* h = a.header + (long long)c * PA_HEADER;
+  if (h[0] < 0) return;
+  const int b = h[1], hd = h[2], slot = h[3], last = h[4];
+  const int rows = min(a.sub_heads, a.group - (hd % a.subs) * a.sub_heads);
+  if (row >= rows) return;
+  const auto part = [&](int i) { return a.parts + ((long long)i * 2 + (i == c ? slot : 0)) * ROWS * (HD + 2); };
+  float top = -INFINITY;
+  for (int i = c; i <= last; ++i) top = fmaxf(top, part(i)[ROWS * HD + row]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float v = 0.f, sum = 0.f;
+#pragma unroll 4
+  for (int i = c; i <= last; ++i) {
+    const float* f = part(i);
+    const float e = exp2f(f[ROWS * HD + row] - base);
+    v += e * f[row * HD + threadIdx.x];
+    sum += e * f[ROWS * (HD + 1) + row];
+  }
+  const int q = (hd / a.subs) * a.group + (hd % a.subs) * a.sub_heads + row;
+  ((T*)d.o)[b * d.o_bs + q * d.o_hs + threadIdx.x] = Half16<T>::round(sum == 0.f ? 0.f : v / sum);
+  if (threadIdx.x == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (top + log2f(sum) - SHIFT) * LN2;
+}
+
+struct Plan {
+  int subs, sub_heads, rows;
+  bool split;
+  long long ctas, bytes;
+};
+static Plan plan_of(const FtkPagedAttnDesc& d) {
+  Plan p;
+  const long long group = d.Hq / d.Hkv;
+  p.subs = (int)((group + 15) / 16);
+  p.sub_heads = (int)((group + p.subs - 1) / p.subs);
+  p.rows = p.sub_heads <= 8 ? 8 : 16;
+  const long long tiles = ((d.table_cols << d.page_shift) + PA_TILE - 1) / PA_TILE;
+  p.split = tiles > PA_WHOLE;
+  p.ctas = d.B * d.Hkv * p.subs;
+  p.bytes = 0;
+  if (p.split) {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    p.ctas = 2ll * sms;
+    p.bytes = p.ctas * (PA_HEADER * 4 + 2 * p.rows * (d.hd + 2) * 4);
+  }
+  return p;
+}
+
+template <typename T, int HD, int ROWS>
+static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaStream_t s) {
+  PagedAttn a = {d, (int)(d.Hq / d.Hkv), p.subs, p.sub_heads, (int*)scratch, nullptr};
+  a.parts = (float*)((char*)scratch + p.ctas * PA_HEADER * 4);
+  int* status = ftk_status_word();
+  const int bytes = PaSmem<ROWS, HD>::BYTES;
+  static_assert(2 * (PaSmem<ROWS, HD>::BYTES + 1024) <= 228 * 1024, "two CTAs share an SM");
+  const auto whole = paged_attn_kernel<T, HD, ROWS, false>, split = paged_attn_kernel<T, HD, ROWS, true>;
+  const auto kernel = p.split ? split : whole;
+  int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc) return rc;
+  rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(PA_WARPS * 32), bytes, s, a, status);
+  if (rc || !p.split) return rc;
+  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.ctas, (unsigned)p.sub_heads), dim3(HD), 0, s, a);
+}
+
+static bool refused(const FtkPagedAttnDesc* d) {
+  return !d || d->B <= 0 || d->B > (1 << 30) || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > (1 << 20) || (d->hd != 64 && d->hd != 128) ||
+         (d->type != FTK_T_BF16 && d->type != FTK_T_FP16) || d->page_shift < 0 || d->page_shift > 30 || d->table_cols <= 0 || d->n_pages < 0 ||
+         d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff;
 }
 
 }  // namespace ftk
 using namespace ftk;
 
-extern "C" int ftk_paged_attn(const FtkPagedAttnDesc* d, void* stream) {
-  if (!d || d->B <= 0 || d->B > 65535 || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > 65535) return -2;
-  if (!d->q || !d->o || !d->lse || !d->k_pages || !d->v_pages || !d->table || !d->lengths || d->page_shift < 0 || d->page_shift > 30)
-    return -2;
+extern "C" long long ftk_paged_attn_scratch(const FtkPagedAttnDesc* d) { return refused(d) ? -2 : plan_of(*d).bytes; }
+
+extern "C" int ftk_paged_attn(const FtkPagedAttnDesc* d, void* scratch, void* stream) {
+  if (refused(d) || !d->q || !d->o || !d->lse || !d->k_pages || !d->v_pages || !d->table || !d->lengths) return -2;
+  const Plan p = plan_of(*d);
+  if (p.split && !scratch) return -2;
   cudaStream_t s = (cudaStream_t)stream;
-  if (d->type == FTK_T_BF16 && d->hd == 64) return launch<__nv_bfloat16, 64>(*d, s);
-  if (d->type == FTK_T_BF16 && d->hd == 128) return launch<__nv_bfloat16, 128>(*d, s);
-  if (d->type == FTK_T_FP16 && d->hd == 64) return launch<__half, 64>(*d, s);
-  if (d->type == FTK_T_FP16 && d->hd == 128) return launch<__half, 128>(*d, s);
-  return -2;
+  const bool bf = d->type == FTK_T_BF16;
+  if (p.rows == 8) {
+    if (d->hd == 64) return bf ? launch<__nv_bfloat16, 64, 8>(*d, p, scratch, s) : launch<__half, 64, 8>(*d, p, scratch, s);
+    return bf ? launch<__nv_bfloat16, 128, 8>(*d, p, scratch, s) : launch<__half, 128, 8>(*d, p, scratch, s);
+  }
+  if (d->hd == 64) return bf ? launch<__nv_bfloat16, 64, 16>(*d, p, scratch, s) : launch<__half, 64, 16>(*d, p, scratch, s);
+  return bf ? launch<__nv_bfloat16, 128, 16>(*d, p, scratch, s) : launch<__half, 128, 16>(*d, p, scratch, s);
 }

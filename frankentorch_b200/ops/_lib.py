@@ -171,10 +171,16 @@ def load(build_if_missing: bool = True):
     # descriptors packed by GEMM_DESC / ATTN_DESC and the like (a second function object per entry: argument types are per object)
     for name, sym in (("gemm_packed", "ftk_gemm_bf16"), ("attn_fwd_packed", "ftk_attn_fwd"),
                       ("attn_bwd_packed", "ftk_attn_bwd"), ("rotary_packed", "ftk_rotary"),
-                      ("paged_attn_packed", "ftk_paged_attn"), ("logits_packed", "ftk_logits")):
+                      ("logits_packed", "ftk_logits")):
         fn = lib[sym]
         fn.argtypes, fn.restype = [C.c_char_p, C.c_void_p], C.c_int
         setattr(lib, name, fn)
+    fn = lib["ftk_paged_attn"]
+    fn.argtypes, fn.restype = [C.c_char_p, C.c_void_p, C.c_void_p], C.c_int
+    lib.paged_attn_packed = fn
+    fn = lib["ftk_paged_attn_scratch"]
+    fn.argtypes, fn.restype = [C.c_char_p], C.c_longlong
+    lib.paged_attn_scratch = fn
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -36,12 +36,12 @@ HEAD_SIZES = (64, 128)          # of paged_attention, as of attention_fwd
 MAX_HEAD = 1024                 # of rotary and paged_append
 
 
-def _launch(name: str, fn, desc: bytes, dev: torch.device) -> None:
+def _launch(name: str, fn, dev: torch.device, *args) -> None:
     if dev.index == K._get_device():
-        K._chk(fn(desc, K._stream()), name)
+        K._chk(fn(*args, K._stream()), name)
     else:
         with torch.cuda.device(dev):
-            K._chk(fn(desc, K._stream()), name)
+            K._chk(fn(*args, K._stream()), name)
 
 
 def _on_device(ref: torch.Tensor, **others) -> None:
@@ -167,7 +167,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
         _T16[dtype], B, S, H, Hk, hd, turned, interleaved, inverse, q.data_ptr(), *qs,
         0 if k is None else k.data_ptr(), *ks, 0, 0, 0, 0, q_out.data_ptr(), *qo, 0 if k is None else k_out.data_ptr(), *ko,
         freq, st, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    _launch("ftk_rotary", _lib.load().rotary_packed, desc, q.device)
+    _launch("ftk_rotary", _lib.load().rotary_packed, q.device, desc)
     return q_out, k_out
 
 
@@ -216,7 +216,7 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
         _T16[dtype], B, S, H, Hk, hd, turned, interleaved, 0, 0 if q is None else q.data_ptr(), *qs, k.data_ptr(), *ks,
         v.data_ptr(), *vs, 0 if q is None else q_out.data_ptr(), *qo, 0, 0, 0, 0, freq, st, ct, k_pages.data_ptr(), *kp,
         v_pages.data_ptr(), *vp, table.data_ptr(), table.stride(0), table.shape[1], k_pages.shape[0], shift)
-    _launch("ftk_rotary", _lib.load().rotary_packed, desc, k.device)
+    _launch("ftk_rotary", _lib.load().rotary_packed, k.device, desc)
     return q_out
 
 
@@ -255,7 +255,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _T16[dtype], B, H, Hk, hd, 1.0 / math.sqrt(hd) if scale is None else float(scale), q.data_ptr(), *qs[:2],
         out.data_ptr(), *os_[:2], lse.data_ptr(), k_pages.data_ptr(), *kp, v_pages.data_ptr(), *vp, table.data_ptr(),
         table.stride(0), table.shape[1], k_pages.shape[0], shift, ln)
-    _launch("ftk_paged_attn", _lib.load().paged_attn_packed, desc, q.device)
+    lib = _lib.load()
+    need = lib.paged_attn_scratch(desc)
+    scratch = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    _launch("ftk_paged_attn", lib.paged_attn_packed, q.device, desc, 0 if scratch is None else scratch.data_ptr())
     return out, lse
 
 
@@ -348,5 +351,5 @@ def logits_process(logits: torch.Tensor, *, vocab: Optional[int] = None, tokens:
     desc = _lib.LOGITS_DESC.pack(_TYPES[dtype], _TYPES[out.dtype], R, V, logits.data_ptr(), logits.stride(0), out.data_ptr(),
                                  out.stride(0), tk, ldt, L, ln, pl, rep_p, freq_p, pres_p, rep, freq, pres, bias_p, bias_rs,
                                  mask_p, mask_rs)
-    _launch("ftk_logits", _lib.load().logits_packed, desc, logits.device)
+    _launch("ftk_logits", _lib.load().logits_packed, logits.device, desc)
     return out
