@@ -20,6 +20,7 @@ import torch
 
 from ..autograd.tape import TensorTape
 from ..ops import fused as F
+from ..ops.decode import rotary_frequencies
 
 
 @dataclass
@@ -34,6 +35,12 @@ class GPTConfig:
     ln_eps: float = 1e-5
     tie_lm_head: bool = True
     name: str = "gpt2-small"
+    pos: str = "learned"            # "learned": a table of max_seq rows; "rotary": queries and keys are turned by position
+    rope_base: float = 10000.0
+
+    def require_learned_positions(self, model: str) -> None:
+        if self.pos != "learned":
+            raise ValueError(f"{model} has learned positions only, not {self.pos!r}")
 
     @property
     def padded_vocab(self) -> int:
@@ -54,7 +61,8 @@ class GPTConfig:
     def param_count(self) -> int:
         d, L = self.d_model, self.n_layer
         per_layer = 4 * d + 3 * d * d + 3 * d + d * d + d + d * self.d_ff + self.d_ff + self.d_ff * d + d
-        return self.vocab_size * d + self.max_seq * d + L * per_layer + 2 * d
+        table = self.max_seq * d if self.pos == "learned" else 0
+        return self.vocab_size * d + table + L * per_layer + 2 * d
 
 
 class ParamArena:
@@ -147,7 +155,12 @@ class GPT:
         self.tape = tape
         self.device = torch.device(device)
         d, ff, Vp = cfg.d_model, cfg.d_ff, cfg.padded_vocab
-        specs: List[Tuple[str, Tuple[int, ...]]] = [("wte.weight", (Vp, d)), ("wpe.weight", (cfg.max_seq, d))]
+        if cfg.pos not in ("learned", "rotary"):
+            raise ValueError(f"positions are 'learned' or 'rotary', not {cfg.pos!r}")
+        specs: List[Tuple[str, Tuple[int, ...]]] = [("wte.weight", (Vp, d))]
+        if cfg.pos == "learned":
+            specs.append(("wpe.weight", (cfg.max_seq, d)))
+        self.inv_freq = None if cfg.pos == "learned" else rotary_frequencies(d // cfg.n_head, cfg.rope_base, self.device)
         for l in range(cfg.n_layer):
             p = f"blocks.{l}."
             specs += [
@@ -169,7 +182,8 @@ class GPT:
                                 peer_visible=peer_visible, multicast_params=True)
         # the embeddings' gradients are complete only when the backward pass ends (the token table is
         # also the LM head): they form one bucket of their own
-        self.arena.bucket_cuts.append(self.arena.slot_end("wpe.weight"))
+        self.last_embedding = "wpe.weight" if cfg.pos == "learned" else "wte.weight"
+        self.arena.bucket_cuts.append(self.arena.slot_end(self.last_embedding))
         # the weight gradients of a block are launched together (two full waves, no split-K)
         from ..ops.fused import enable_grouped_wgrad
         enable_grouped_wgrad(tape)
@@ -252,15 +266,15 @@ class GPT:
         B, S = ids.shape
         gate = self.param_gate
         if gate is not None:
-            gate("wpe.weight")
-        x = F.embedding(tape, ids, P["wte.weight"], P["wpe.weight"], S)
+            gate(self.last_embedding)
+        x = F.embedding(tape, ids, P["wte.weight"], P.get("wpe.weight"), S)
         for l in range(cfg.n_layer):
             p = f"blocks.{l}."
             if gate is not None:
                 gate(p + "mlp.fc2.bias")
             h = F.layernorm(tape, x, P[p + "ln1.weight"], P[p + "ln1.bias"], cfg.ln_eps)
             qkv = F.linear(tape, h, P[p + "attn.qkv_proj.weight"], P[p + "attn.qkv_proj.bias"])
-            a = F.attention_packed(tape, qkv, cfg.n_head, causal=True)
+            a = F.attention_packed(tape, qkv, cfg.n_head, causal=True, inv_freq=self.inv_freq)
             x = F.linear(tape, a, P[p + "attn.out_proj.weight"], P[p + "attn.out_proj.bias"], resid=x)
             h = F.layernorm(tape, x, P[p + "ln2.weight"], P[p + "ln2.bias"], cfg.ln_eps)
             x = F.mlp_up_down(tape, h, P[p + "mlp.fc1.weight"], P[p + "mlp.fc1.bias"],

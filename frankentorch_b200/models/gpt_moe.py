@@ -47,6 +47,7 @@ class MoEConfig:
 class MoEGPT:
     def __init__(self, cfg: GPTConfig, moe: MoEConfig, tape: TensorTape, device, *,
                  group: Optional[dist.ProcessGroup], micro_batch: int, seq_len: int, seed: int = 1234):
+        cfg.require_learned_positions("MoEGPT")
         self.cfg, self.moe, self.tape, self.device = cfg, moe, tape, torch.device(device)
         self.group = group
         self.rank = dist.get_rank(group) if group is not None else 0

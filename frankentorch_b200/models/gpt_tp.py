@@ -34,6 +34,7 @@ from .gpt import GPTConfig, ParamArena
 class TensorParallelGPT:
     def __init__(self, cfg: GPTConfig, tape: TensorTape, device, *, group: Optional[dist.ProcessGroup],
                  micro_batch: int, seq_len: int, seed: int = 1234, comm_ctas: int = 0):
+        cfg.require_learned_positions("TensorParallelGPT")
         self.cfg, self.tape, self.device = cfg, tape, torch.device(device)
         self.group = group
         self.rank = dist.get_rank(group) if group is not None else 0

@@ -29,6 +29,7 @@ from .gpt import GPTConfig, ParamArena
 class Zero3GPT:
     def __init__(self, cfg: GPTConfig, tape: TensorTape, device, *, group: Optional[dist.ProcessGroup],
                  seed: int = 1234, comm_ctas: int = 0):
+        cfg.require_learned_positions("Zero3GPT")
         self.cfg, self.tape, self.device = cfg, tape, torch.device(device)
         self.group = group
         self.rank = dist.get_rank(group) if group is not None else 0

@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from ..autograd.tape import ACCUMULATED, TensorTape
+from . import decode as D
 from . import kernels as K
 
 RULE_LINEAR = "d(A@B)/dA=dOut@B^T; d(A@B)/dB=A^T@dOut"
@@ -311,12 +312,14 @@ def rmsnorm(tape: TensorTape, x: int, gamma: int, eps: float = 1e-6) -> int:
     return tape.record("rms_norm", [x, gamma], _as(y, xv), vjp, "d(rms_norm(x))/dx,dgamma")
 
 
-def attention_packed(tape: TensorTape, qkv: int, n_heads: int, *, causal: bool = True,
-                     scale: Optional[float] = None) -> int:
+def attention_packed(tape: TensorTape, qkv: int, n_heads: int, *, causal: bool = True, scale: Optional[float] = None,
+                     inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False) -> int:
     """Multi-head attention over packed ``[B, S, 3*d]`` projections -> ``[B, S, d]``.
 
     Heads are addressed in place through strided TMA maps: no split/permute copies
-    (the reference reshapes to [N*H, S, hd], ft-nn/src/lib.rs:5145-5167).
+    (the reference reshapes to [N*H, S, hd], ft-nn/src/lib.rs:5145-5167).  With ``inv_freq`` the queries and keys
+    are turned by their positions 0 .. S-1 first (:func:`.decode.rotary`); the projections keep their value, the
+    turned copies are what the backward pass keeps, and their gradients are turned back on the way into ``dqkv``.
     """
     qv = tape.value(qkv)
     B, S, d3 = qv.shape
@@ -324,16 +327,24 @@ def attention_packed(tape: TensorTape, qkv: int, n_heads: int, *, causal: bool =
     hd = d // n_heads
     split = lambda t: (t if d3 == 3 * d else t[:, :, :3 * d]).view(B, S, 3, n_heads, hd).unbind(2)      # noqa: E731
     q, k, v = split(qv)
+    if inv_freq is not None:
+        turned = qv.new_empty((2, B, S, n_heads, hd)).unbind(0)
+        q, k = D.rotary(q, k, inv_freq, interleaved=interleaved, q_out=turned[0], k_out=turned[1])
     o, lse = K.attention_fwd(q, k, v, causal=causal, scale=scale)
 
     def vjp(go, targets):
         dqkv = torch.empty_like(qv)
         dq, dk, dv = split(dqkv)
-        K.attention_bwd(q, k, v, o, lse, go.reshape(B, S, n_heads, hd), causal=causal, scale=scale,
-                        dq=dq, dk=dk, dv=dv)
+        go = go.reshape(B, S, n_heads, hd)
+        if inv_freq is None:
+            K.attention_bwd(q, k, v, o, lse, go, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)
+        else:
+            tq, tk, _ = K.attention_bwd(q, k, v, o, lse, go, causal=causal, scale=scale, dv=dv)
+            D.rotary(tq, tk, inv_freq, interleaved=interleaved, inverse=True, q_out=dq, k_out=dk)
         return [dqkv]
 
-    return tape.record("sdpa", [qkv], o.view(B, S, d), vjp, "d(sdpa(q,k,v))/dq,dk,dv [flash, recompute P]")
+    return tape.record("sdpa", [qkv], o.view(B, S, d), vjp, "d(sdpa(q,k,v))/dq,dk,dv [flash, recompute P%s]"
+                       % ("" if inv_freq is None else ", rotary"))
 
 
 def embedding(tape: TensorTape, ids: torch.Tensor, wte: int, wpe: Optional[int], S: int) -> int:

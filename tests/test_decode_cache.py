@@ -1,0 +1,79 @@
+"""Page bookkeeping of the decoder's cache and what the decoder refuses, without a GPU."""
+import pytest
+import torch
+
+from frankentorch_b200.autograd.tape import TensorTape
+from frankentorch_b200.models.gpt import GPT, GPTConfig
+from frankentorch_b200.models.gpt_decode import CacheFull, GPTDecoder, PagedKVCache
+
+
+def _cache(**kw):
+    return PagedKVCache(2, 3, 64, **{**dict(pages=6, batch=3, max_tokens=40, page=8, device="cpu"), **kw})
+
+
+def test_pages_are_given_and_taken_back():
+    c = _cache()
+    assert c.k.shape == (2, 6, 3, 8, 64) and c.v.shape == c.k.shape and c.table.shape == (3, 5)
+    c.reserve(0, 1)
+    c.reserve(1, 17)
+    first = c.table.clone()
+    c.reserve(0, 8)                                   # still one page
+    assert torch.equal(c.table, first) and c.free_pages == 2
+    c.reserve(0, 9)
+    held = c.table[0, :2].tolist() + c.table[1, :3].tolist()
+    assert len(set(held)) == 5 and all(0 <= p < 6 for p in held)
+    assert c.table[0, 0] == first[0, 0]               # what a sequence has stays where it is
+    with pytest.raises(CacheFull, match="2 pages, 1 are free"):
+        c.reserve(2, 16)
+    assert c.free_pages == 1
+    c.release(1)
+    assert c.free_pages == 4
+    c.reserve(2, 32)
+    now = c.table[0, :2].tolist() + c.table[2, :4].tolist()
+    assert len(set(now)) == 6 and c.free_pages == 0
+    c.release(1)                                      # nothing held: nothing given back twice
+    assert c.free_pages == 0
+
+
+@pytest.mark.parametrize("kw", [dict(page=12), dict(page=0), dict(pages=0), dict(batch=0), dict(max_tokens=0)])
+def test_cache_refuses(kw):
+    with pytest.raises(ValueError):
+        _cache(**kw)
+    with pytest.raises(ValueError, match="41 tokens"):
+        _cache().reserve(0, 41)
+
+
+def _model(**kw):
+    cfg = GPTConfig(**{**dict(n_layer=1, d_model=128, n_head=2, d_ff=256, vocab_size=100, max_seq=32, name="t"), **kw})
+    return GPT(cfg, TensorTape(grad_dtype=None), device="cpu")
+
+
+def test_decoder_refuses():
+    with pytest.raises(ValueError, match="learned positions"):
+        GPTDecoder(_model(), 2, 33)
+    with pytest.raises(ValueError, match="head size"):
+        GPTDecoder(_model(n_head=4), 2, 16)
+    d = GPTDecoder(_model(), 2, 32, page=16)
+    with pytest.raises(ValueError, match="follows a prefill"):
+        d.step(torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="one token for each"):
+        d.step(torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="for 2 sequences"):
+        d.prefill(torch.zeros(3, 4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="1 to 4 tokens"):
+        d.prefill(torch.zeros(2, 4, dtype=torch.int64), [4, 0])
+    with pytest.raises(ValueError, match="positive"):
+        d.generate(torch.zeros(2, 4, dtype=torch.int64), max_new_tokens=0)
+
+
+def test_rotary_model_has_no_position_table():
+    learned, rotary = _model(), _model(pos="rotary")
+    assert "wpe.weight" in learned.leaf and learned.inv_freq is None and learned.last_embedding == "wpe.weight"
+    assert "wpe.weight" not in rotary.leaf and "wpe.weight" not in rotary.state_dict()
+    assert rotary.inv_freq.shape == (32,) and rotary.inv_freq.dtype == torch.float64
+    assert learned.cfg.param_count() - rotary.cfg.param_count() == 32 * 128
+    assert GPTDecoder(rotary, 1, 1000).cache.table.shape == (1, 16)
+    with pytest.raises(ValueError, match="'learned' or 'rotary'"):
+        _model(pos="none")
+    with pytest.raises(ValueError, match="learned positions only"):
+        rotary.cfg.require_learned_positions("another model")
