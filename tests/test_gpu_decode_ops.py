@@ -181,6 +181,12 @@ def test_append_reports_what_has_no_page(cuda_device):
         for p in good:
             assert torch.equal(kp[table[0][p // 8], :, p % 8], k[0, p - start[0]])
         assert int((~kp.isnan()).sum()) == 64 * (len(good) + 1) and int((~vp.isnan()).sum()) == 64 * (len(good) + 1)
+    for counts, rows in (([5, 1], 5), ([-1, 1], 1)):
+        kp, vp = (torch.full((3, 1, 8, 64), math.nan, dtype=BF, device="cuda") for _ in range(2))
+        D.paged_append(kp, vp, _i32([[1, 2], [0, 0]]), k, v, _i32([0, 0]), _i32(counts))
+        with pytest.raises(K.KernelError, match="BAD_INDEX"):
+            K.check_status()
+        assert int((~kp.isnan()).sum()) == 64 * rows and torch.equal(kp[0, :, 0], k[1, 0])
     K.check_status()
 
 
