@@ -6,12 +6,14 @@
 // What bounds it: each logit is read once and written once, a few operations in between; the copy bandwidth, and for a row or two
 // the latency of two dependent reads.
 //
-// Work.  The vocabulary is cut into slices of up to 24 thousand columns; a unit is a slice of a row, and each CTA (two per SM)
-// takes an equal run of the units.  For a unit it first counts the row's history into shared memory, a word per column -
-// occurrences among the generated tokens in the low 31 bits, "occurred in the prompt" in bit 31; whole numbers, so the order of
-// additions does not matter - and a bit per column that has any.  Then it streams the columns, 16 bytes per thread twice per
-// tile, with the next tile (of the next unit at the end) and the next history already on their way; while one CTA counts the other
-// streams.  Only columns whose bit is set are looked up and cleared.  A history is read once per slice, out of the L2 cache.
+// Work.  The rows' columns behind one another, in blocks of 64, are cut into equal runs, one for each of two CTAs per SM; a run is a
+// few pieces of rows.  For a piece a CTA first counts the row's history into shared memory, 16 bits per column - occurrences
+// among the generated tokens in the low 15, "occurred in the prompt" in the highest; whole numbers, so the order of additions does
+// not matter - and a bit per column that has any.  (Histories of 32768 tokens and more take 32 bits and half the columns.)
+// Then it streams the columns, 16 bytes per thread twice per tile, with the next tile (of the next piece at the end) and the next
+// history already on their way; while one CTA counts the other streams.  Only columns whose bit is set are looked up and cleared.
+// A history is read once per piece, out of the L2 cache: pieces as long as shared memory allows, rather than narrow slices of
+// all rows, are what that costs least with (six slices per row instead of four pieces: 112 us where this takes LARGE_US).
 #include <math.h>
 
 #include "ft_sm100.cuh"
@@ -25,7 +27,7 @@ namespace ftk {
 
 constexpr int LG_THREADS = 512;              // threads of a CTA at most
 constexpr int LG_TOKENS = 4;                 // tokens of a history that a thread requests ahead
-constexpr int LG_SLICE = 24 * 1024;          // columns of a slice at most
+constexpr int LG_BLOCK = 64;                 // columns that stay together
 template <typename T> struct LgCols { static constexpr int value = 16 / (int)sizeof(T); };      // columns of 16 bytes
 
 // A load that stays where it is written: ahead of what waits for others.  (Plain loads of the next tile end up behind the work on
@@ -82,85 +84,102 @@ template <typename T> __device__ __forceinline__ void store1(T* p, float x) { *p
 struct LogitsRow {
   int len, prompt;
   float rep, inv, freq, pres;
-  __device__ __forceinline__ float operator()(float x, unsigned c) const {
-    const unsigned n = c & 0x7fffffffu;
+  __device__ __forceinline__ float operator()(float x, unsigned n) const {
     const float y = x > 0.f ? x * inv : x * rep;
     return n ? y - freq * (float)n - pres : y;
   }
 };
+// Counts of a piece's columns, 16 or 32 bits each in words of shared memory
+template <bool WIDE> struct Counts {
+  static constexpr int COLUMNS = WIDE ? 20 * 1024 : 40 * 1024;      // of a piece at most
+  static constexpr unsigned PROMPT = WIDE ? 0x80000000u : 0x8000u;
+  unsigned* words;
+  __device__ __forceinline__ void add(int at, unsigned n) {
+    if (WIDE) atomicAdd(&words[at], n);
+    else atomicAdd(&words[at >> 1], n << (at & 1) * 16);
+  }
+  __device__ __forceinline__ void mark(int at) {
+    if (WIDE) atomicOr(&words[at], PROMPT);
+    else atomicOr(&words[at >> 1], PROMPT << (at & 1) * 16);
+  }
+  __device__ __forceinline__ unsigned take(int at) {      // the generated tokens' count; by the one thread that has the column
+    if (WIDE) {
+      const unsigned c = words[at];
+      words[at] = 0;
+      return c & (PROMPT - 1);
+    }
+    unsigned short* p = reinterpret_cast<unsigned short*>(words) + at;
+    const unsigned c = *p;
+    *p = 0;
+    return c & (PROMPT - 1);
+  }
+};
 struct LogitsCut {
-  int slice, slices;      // columns of a slice (a multiple of 64), slices of the vocabulary
+  long long blocks;       // of a row
+  int columns;            // of a piece at most
   bool bias16;            // rows of the bias start on 16 bytes
 };
+
 // VEC: rows of logits and results start on 16 bytes
-template <typename T, typename O, bool HISTORY, bool VEC>
+template <typename T, typename O, bool HISTORY, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_constant__ FtkLogitsDesc d, const LogitsCut cut, int* status) {
   constexpr int N = LgCols<T>::value;
-  extern __shared__ __align__(16) unsigned counts[];             // [slice], then a bit per column [slice / 32]
-  unsigned* seen = counts + cut.slice;
-  const int tid = threadIdx.x, bd = blockDim.x, slice = cut.slice, step = bd * N, tile = 2 * step;
-  const long long units = d.R * cut.slices;
-  const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  extern __shared__ __align__(16) unsigned smem[];               // counts, a bit per column, tokens
+  Counts<WIDE> counts = {smem};
+  unsigned* seen = smem + cut.columns / (WIDE ? 1 : 2);
+  long long* ids = reinterpret_cast<long long*>(seen + cut.columns / 32);      // [LG_TOKENS][threads]
+  const int tid = threadIdx.x, bd = blockDim.x, step = bd * N, tile = 2 * step;
+  const long long x0 = d.R * cut.blocks * blockIdx.x / gridDim.x, x1 = d.R * cut.blocks * (blockIdx.x + 1) / gridDim.x;
   if (HISTORY) {
-    for (int i = tid; i < slice / 4; i += bd) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
-    for (int i = tid; i < slice / 32; i += bd) seen[i] = 0;
+    for (int i = tid; i < cut.columns / (WIDE ? 4 : 8); i += bd) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < cut.columns / 32; i += bd) seen[i] = 0;
   }
   pdl_wait();
   pdl_trigger();
 
   struct Unit {
-    long long r, v0;        // row, first column
-    int n, left;            // columns; units of the CTA from this one on
+    int r, v0, left, n;           // row, first column; blocks of the CTA from here on; columns
   };
-  const auto columns_of = [&](long long v0) { return (int)max(0ll, min((long long)slice, d.V - v0)); };
+  const auto unit = [&](int r, int v0, int left) {
+    return Unit{r, v0, left, min(min(left, cut.columns / LG_BLOCK) * LG_BLOCK, (int)d.V - v0)};
+  };
   const auto behind = [&](const Unit& u) {
-    const bool wrap = u.r + 1 == d.R;
-    const long long v0 = wrap ? u.v0 + slice : u.v0;
-    return Unit{wrap ? 0 : u.r + 1, v0, columns_of(v0), u.left - 1};
+    const int v = u.v0 + u.n, left = u.left - (u.n + LG_BLOCK - 1) / LG_BLOCK;
+    return v == (int)d.V ? unit(u.r + 1, 0, left) : unit(u.r, v, left);
   };
-  struct History {
-    LogitsRow w;
-    long long id[LG_TOKENS];
-  };
-  const auto request_history = [&](const Unit& u, History& h) {
+  // a thread's tokens of the next history wait in shared memory, for itself
+  const auto request_history = [&](const Unit& u, LogitsRow& w) {
     if (u.left <= 0) return;
-    if (d.lengths) h.w.len = load_now(d.lengths + u.r);
-    if (d.prompts) h.w.prompt = load_now(d.prompts + u.r);
-    if (d.rep_rows) h.w.rep = load_now(d.rep_rows + u.r);
-    if (d.freq_rows) h.w.freq = load_now(d.freq_rows + u.r);
-    if (d.pres_rows) h.w.pres = load_now(d.pres_rows + u.r);
+    if (d.lengths) w.len = load_now(d.lengths + u.r);
+    if (d.prompts) w.prompt = load_now(d.prompts + u.r);
+    if (d.rep_rows) w.rep = load_now(d.rep_rows + u.r);
+    if (d.freq_rows) w.freq = load_now(d.freq_rows + u.r);
+    if (d.pres_rows) w.pres = load_now(d.pres_rows + u.r);
     const long long* p = d.tokens + u.r * d.ldt + tid;
 #pragma unroll
     for (int i = 0; i < LG_TOKENS; ++i)
-      if (i * bd + tid < d.L) h.id[i] = load_now(p + i * bd);
+      if (i * bd + tid < (int)d.L)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(ids + i * bd + tid)), "l"(p + i * bd) : "memory");
   };
-  const auto count = [&](const Unit& u, const History& h) {
-    if ((h.w.len < 0 || h.w.len > d.L) && tid == 0) ft_index_ok(-1, 1, status);
-    const long long len = min((long long)h.w.len, d.L);
-    const auto one = [&](long long j, long long id) {
+  const auto count = [&](const Unit& u, const LogitsRow& w) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if ((w.len < 0 || w.len > (int)d.L) && tid == 0) ft_index_ok(-1, 1, status);
+    const int len = min(w.len, (int)d.L);
+    const auto one = [&](int j, long long id) {
       if (!ft_index_ok(id, d.V, status)) return;
       const int at = (int)(id - u.v0);
       if ((unsigned)at >= (unsigned)u.n) return;
-      if (j < h.w.prompt) atomicOr(&counts[at], 0x80000000u);
-      else atomicAdd(&counts[at], 1u);
+      if (j < w.prompt) counts.mark(at);
+      else counts.add(at, 1);
       atomicOr(&seen[at >> 5], 1u << (at & 31));
     };
 #pragma unroll
     for (int i = 0; i < LG_TOKENS; ++i)
-      if (i * bd + tid < len) one(i * bd + tid, h.id[i]);
-    for (long long j = (long long)LG_TOKENS * bd + tid; j < len; j += (long long)LG_TOKENS * bd) {
-      long long id[LG_TOKENS];
-#pragma unroll
-      for (int i = 0; i < LG_TOKENS; ++i)
-        if (j + i * bd < len) id[i] = load_now(d.tokens + u.r * d.ldt + j + i * bd);
-#pragma unroll
-      for (int i = 0; i < LG_TOKENS; ++i)
-        if (j + i * bd < len) one(j + i * bd, id[i]);
-    }
+      if (i * bd + tid < len) one(i * bd + tid, ids[i * bd + tid]);
+    for (int j = LG_TOKENS * bd + tid; j < len; j += bd) one(j, d.tokens[u.r * d.ldt + j]);
   };
 
-  Unit u = {u0 % d.R, u0 / d.R * slice, 0, (int)(u1 - u0)};
-  u.n = columns_of(u.v0);
+  Unit u = unit((int)(x0 / cut.blocks), (int)(x0 % cut.blocks) * LG_BLOCK, (int)(x1 - x0));
   // the tile that is requested next: columns and mask bytes of its unit from this thread's on
   struct Tile {
     uint4 x[2];
@@ -189,8 +208,7 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
       aim();
     }
   };
-  History h;
-  h.w = {(int)min(d.L, 0x7fffffffll), 0, (float)d.rep, 1.f, (float)d.freq, (float)d.pres};
+  LogitsRow h = {(int)d.L, 0, (float)d.rep, 1.f, (float)d.freq, (float)d.pres};
   if (HISTORY) request_history(u, h);
   Tile next;
   if (VEC) {
@@ -198,9 +216,9 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
     request(next);
   }
   for (; u.left > 0; u = behind(u)) {
-    const int n = u.n;
-    const long long r = u.r, v0 = u.v0;
-    LogitsRow row = h.w;
+    const int n = u.n, v0 = u.v0;
+    const long long r = u.r;
+    LogitsRow row = h;
     if (HISTORY) {
       __syncthreads();            // the counts and bits of the unit before are read and cleared
       count(u, h);
@@ -248,8 +266,7 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
 #pragma unroll
               for (int e = 0; e < N; ++e)
                 if (k >> e & 1u) {
-                  y[e] = row(y[e], counts[at + e]);
-                  counts[at + e] = 0;
+                  y[e] = row(y[e], counts.take(at + e));
                 }
               if (N == 8) reinterpret_cast<unsigned char*>(seen)[at >> 3] = 0;
               else atomicAnd(&seen[at >> 5], ~(15u << (at & 31)));      // the other half of the byte is a neighbour's
@@ -274,9 +291,9 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
       } else {
         for (int at = t0 + tid; at < min(n, t0 + tile); at += bd) {
           float y = load1((const T*)d.logits + r * d.ld + v0 + at);
-          if (HISTORY && counts[at]) {
-            y = row(y, counts[at]);
-            counts[at] = 0;
+          if (HISTORY && (seen[at >> 5] >> (at & 31) & 1u)) {
+            y = row(y, counts.take(at));
+            atomicAnd(&seen[at >> 5], ~(1u << (at & 31)));
           }
           if (bias) y += bias[at];
           if (d.allowed && !((unsigned)d.allowed[r * d.allowed_rs + ((v0 + at) >> 5)] >> (at & 31) & 1u)) y = -INFINITY;
@@ -287,44 +304,42 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
   }
 }
 
-template <typename T, typename O, bool HISTORY, bool VEC>
+template <typename T, typename O, bool HISTORY, bool VEC, bool WIDE>
 static int launch(const FtkLogitsDesc& d, cudaStream_t s) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const long long places = 2ll * sms;
-  // Slices as wide as a CTA holds, but 2048 columns where that keeps more SMs at work; among so many and a few times as many
-  // the number that leaves the least to the CTA with the most units
-  const long long want = max(2048ll, min((long long)LG_SLICE, (d.V * d.R + places - 1) / places));
-  const long long least = (d.V + want - 1) / want;
-  LogitsCut cut = {0, 0, ((uintptr_t)d.bias | (uintptr_t)(d.bias_rs * 4)) % 16 == 0};
-  long long best = -1;
-  for (long long k = least; k <= 4 * least && k < least + 16; ++k) {
-    const long long slice = ((d.V + k - 1) / k + 63) / 64 * 64, slices = (d.V + slice - 1) / slice;
-    const long long cost = (slices * d.R + places - 1) / places * (slice + (HISTORY ? 4096 : 512));      // a unit's fixed part, in columns
-    if (best < 0 || cost < best) best = cost, cut.slice = (int)slice, cut.slices = (int)slices;
-  }
-  const long long vectors = (cut.slice + 2 * LgCols<T>::value - 1) / (2 * LgCols<T>::value);
+  const long long row = (d.V + LG_BLOCK - 1) / LG_BLOCK;
+  const long long ctas = max(1ll, min(2ll * sms, row * d.R * LG_BLOCK / 2048));      // 2048 columns at least
+  const long long run = (row * d.R + ctas - 1) / ctas * LG_BLOCK;
+  const int columns = (int)min((long long)Counts<WIDE>::COLUMNS, min(run, row * LG_BLOCK));
+  const LogitsCut cut = {row, columns, ((uintptr_t)d.bias | (uintptr_t)(d.bias_rs * 4)) % 16 == 0};
+  // threads for the columns of a short run, or for a long history
+  const long long vectors = max((columns + 2 * LgCols<T>::value - 1) / (2ll * LgCols<T>::value), HISTORY ? d.L / LG_TOKENS : 0ll);
   const int threads = (int)min((long long)LG_THREADS, max(128ll, (vectors + 31) / 32 * 32));
-  const auto kernel = logits_kernel<T, O, HISTORY, VEC>;
-  const auto bytes = [](int slice) { return HISTORY ? slice * 4 + slice / 8 : 0; };
-  int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(LG_SLICE));
+  const auto kernel = logits_kernel<T, O, HISTORY, VEC, WIDE>;
+  const auto bytes = [](int n, int threads) { return HISTORY ? n * (WIDE ? 4 : 2) + n / 8 + LG_TOKENS * threads * 8 : 0; };
+  int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(Counts<WIDE>::COLUMNS, LG_THREADS));
   if (rc) return rc;
-  return launch_pdl(kernel, dim3((unsigned)min(places, cut.slices * d.R)), dim3(threads), bytes(cut.slice), s, d, cut, ftk_status_word());
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(threads), bytes(columns, threads), s, d, cut, ftk_status_word());
+}
+template <typename T, typename O, bool VEC>
+static int launch(const FtkLogitsDesc& d, cudaStream_t s) {
+  if (!d.tokens || d.L == 0) return launch<T, O, false, VEC, false>(d, s);
+  return d.L < 0x8000 ? launch<T, O, true, VEC, false>(d, s) : launch<T, O, true, VEC, true>(d, s);
 }
 template <typename T, typename O>
 static int launch(const FtkLogitsDesc& d, cudaStream_t s) {
   const bool vec = ((uintptr_t)d.logits | (uintptr_t)(d.R > 1 ? d.ld * sizeof(T) : 0)) % 16 == 0 &&
                    ((uintptr_t)d.out | (uintptr_t)(d.R > 1 ? d.ldo * sizeof(O) : 0)) % 16 == 0;
-  if (d.tokens && d.L > 0) return vec ? launch<T, O, true, true>(d, s) : launch<T, O, true, false>(d, s);
-  return vec ? launch<T, O, false, true>(d, s) : launch<T, O, false, false>(d, s);
+  return vec ? launch<T, O, true>(d, s) : launch<T, O, false>(d, s);
 }
 
 }  // namespace ftk
 using namespace ftk;
 
 extern "C" int ftk_logits(const FtkLogitsDesc* d, void* stream) {
-  if (!d || d->R <= 0 || d->R > (1ll << 40) || d->V <= 0 || d->V > 0x7fffffff || !d->logits || !d->out) return -2;
+  if (!d || d->L < 0 || d->L > (1 << 30) || d->R <= 0 || d->R > 0x7fffffff || d->V <= 0 || d->V > 0x7fffffff - (1 << 20) || d->R * ((d->V + 63) / 64) > (1ll << 38) || !d->logits || !d->out) return -2;
   cudaStream_t s = (cudaStream_t)stream;
   if (d->type == FTK_T_FP32 && d->out_type == FTK_T_FP32) return launch<float, float>(*d, s);
   if (d->type == FTK_T_BF16 && d->out_type == FTK_T_FP32) return launch<__nv_bfloat16, float>(*d, s);
