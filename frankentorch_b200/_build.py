@@ -1,6 +1,6 @@
 """In-tree build of the native libraries.
 
-Two shared objects are produced next to the sources (they are git-ignored build
+Three shared objects are produced next to the sources (they are git-ignored build
 artefacts, together with ``lib/build_manifest.json``, which records the sha256 of the
 sources and flags each one was built from; a library is rebuilt when that differs from
 what is on disk now, whatever the modification times say):
@@ -9,6 +9,8 @@ what is on disk now, whatever the modification times say):
   no PyTorch dependency), compiled with ``nvcc -gencode arch=compute_100a,code=sm_100a``.
 * ``lib/libftcore.so``     - the host runtime in C++ (deterministic autograd tape,
   evidence ledger, dispatch key resolution, FNV fingerprints, FTSV codec, PRNGs).
+* ``lib/_ft_decode.so``    - the Python binding of the decoding operators (``csrc/bind``), against
+  PyTorch's C++ headers: argument checks, outputs and launch in one native call.
 
 ``nvcc`` cross-compiles without a GPU, so the build also serves as the
 "does it compile" check on a CPU-only machine.
@@ -160,15 +162,49 @@ def build_core(force: bool = False) -> Path:
     return out
 
 
+def bind_sources():
+    return sorted((CSRC / "bind").glob("*.cpp"))
+
+
+def _bind_digest() -> str:
+    import torch
+    return _digest(bind_sources() + [CSRC / "ftk_api.h"], CXX_FLAGS + [torch.__version__, sys.version])
+
+
+def build_bind(force: bool = False) -> Path:
+    """Compile the Python binding (``csrc/bind/*.cpp``) into ``_ft_decode.so``; it is rebuilt for another PyTorch or Python."""
+    import sysconfig
+
+    import torch
+    LIB.mkdir(exist_ok=True)
+    out = LIB / "_ft_decode.so"
+    d = _bind_digest()
+    if force or _stale(out.name, d, out, _manifest()):
+        with _Lock():
+            if force or _stale(out.name, d, out, _manifest()):
+                root = Path(torch.__file__).resolve().parent
+                cuda = Path(_nvcc()).resolve().parent.parent
+                inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
+                _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                      *(x for i in inc for x in ("-isystem", str(i))), "-I", str(CSRC), "-shared", "-o", str(out),
+                      *map(str, bind_sources()), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch",
+                      "-lc10_cuda", "-lc10"])
+                man = _manifest()
+                man[out.name] = d
+                _save_manifest(man)
+    return out
+
+
 def is_current() -> bool:
-    """True when both libraries exist and were built from the sources now on disk."""
+    """True when all libraries exist and were built from the sources now on disk."""
     man = _manifest()
     headers = list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h"))
     ds = sorted(_digest([s] + headers, NVCC_FLAGS) for s in kernel_sources())
     k_ok = (LIB / "libftk_sm100.so").exists() and man.get("libftk_sm100.so") == _digest([], ds)
     ch = list((CSRC / "core").glob("*.h")) + list((CSRC / "core").glob("*.hpp"))
     c_ok = (LIB / "libftcore.so").exists() and man.get("libftcore.so") == _digest(core_sources() + ch, CXX_FLAGS)
-    return k_ok and c_ok
+    b_ok = (LIB / "_ft_decode.so").exists() and man.get("_ft_decode.so") == _bind_digest()
+    return k_ok and c_ok and b_ok
 
 
 class _Lock:
@@ -186,6 +222,7 @@ class _Lock:
 
 
 def build_all(force: bool = False, verbose: bool = False):
+    build_bind(force)
     return build_kernels(force, verbose), build_core(force)
 
 

@@ -58,10 +58,6 @@ class FtkAttnDesc(C.Structure):
 GEMM_DESC = struct.Struct("@7iP3qP3qP3qPP3qPf5iPqiPPi0q")
 ATTN_DESC = struct.Struct("@5if3P9qP3q3P3P")
 assert GEMM_DESC.size == C.sizeof(FtkGemmDesc) and ATTN_DESC.size == C.sizeof(FtkAttnDesc)
-# FtkRotaryDesc, FtkPagedAttnDesc and FtkLogitsDesc have fields of eight bytes only (flags as whole numbers, scalars as doubles)
-ROTARY_DESC = struct.Struct("@9q20q3q8q5q")
-PAGED_ATTN_DESC = struct.Struct("@5qd3q3qq8q5qq")
-LOGITS_DESC = struct.Struct("@4q4q3q2q3q3d4q")
 
 FTK_MAX_RANKS = 8
 COMM_GATHER_A, COMM_GATHER_B, COMM_SCATTER_D = 1, 2, 3
@@ -168,25 +164,46 @@ def load(build_if_missing: bool = True):
         "ftk_wait_probe": [vp, i, ll, vp, vp],
         "ftk_stream_order": [vp, vp],
     }
-    # descriptors packed by GEMM_DESC / ATTN_DESC and the like (a second function object per entry: argument types are per object)
+    # descriptors packed by GEMM_DESC / ATTN_DESC (a second function object per entry: argument types are per object)
     for name, sym in (("gemm_packed", "ftk_gemm_bf16"), ("attn_fwd_packed", "ftk_attn_fwd"),
-                      ("attn_bwd_packed", "ftk_attn_bwd"), ("rotary_packed", "ftk_rotary"),
-                      ("logits_packed", "ftk_logits")):
+                      ("attn_bwd_packed", "ftk_attn_bwd")):
         fn = lib[sym]
         fn.argtypes, fn.restype = [C.c_char_p, C.c_void_p], C.c_int
         setattr(lib, name, fn)
-    fn = lib["ftk_paged_attn"]
-    fn.argtypes, fn.restype = [C.c_char_p, C.c_void_p, C.c_void_p], C.c_int
-    lib.paged_attn_packed = fn
-    fn = lib["ftk_paged_attn_scratch"]
-    fn.argtypes, fn.restype = [C.c_char_p], C.c_longlong
-    lib.paged_attn_scratch = fn
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = C.c_int
     _LIB = lib
     return lib
+
+
+_BIND = None
+
+
+def bind():
+    """The native binding of the decoding operators (``csrc/bind``), with the library's launchers handed to it."""
+    global _BIND
+    if _BIND is None:
+        import importlib.machinery
+        import importlib.util
+
+        from . import kernels as K
+        path = _LIB_PATH.parent / "_ft_decode.so"
+        if os.environ.get("FT_NO_AUTOBUILD") != "1":
+            from .. import _build
+            _build.build_bind()
+        if not path.exists():
+            raise KernelLibraryMissing(f"{path} is missing; run `python -m frankentorch_b200._build`")
+        lib = load()
+        spec = importlib.util.spec_from_file_location("_ft_decode", path,
+                                                      loader=importlib.machinery.ExtensionFileLoader("_ft_decode", str(path)))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.init(K.KernelError, K._chk, *(C.cast(lib[n], C.c_void_p).value for n in
+                                          ("ftk_rotary", "ftk_paged_attn", "ftk_paged_attn_scratch", "ftk_logits")))
+        _BIND = mod
+    return _BIND
 
 
 def is_loaded() -> bool:
