@@ -11,8 +11,10 @@
 //
 // Work is divided into items of 16 elements of one head of one token: two 16-byte vectors that hold eight whole pairs (the
 // vectors are turn / 2 apart where pairs are (i, i + turn / 2), else neighbours), so an item can be turned in place.  A CTA has some
-// tokens with all their heads: it requests its items, up to four per thread, forms the angles' sines and cosines once per token and
-// pair while they arrive, and turns.
+// tokens with all their heads, a thread the same elements of every so-manieth head of them: it requests its items, up to four,
+// and while they arrive the CTA forms the angles' sines and cosines once per token and pair and looks up the tokens' places.
+// Offsets of tokens are in shared memory: worked out per item they were two thirds of 250 instructions per 64 bytes, and forward and
+// backward of 4 x 2048 tokens of 16 heads of 128 took 59 us instead of ROTARY_US.
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
 #include "launch.cuh"
@@ -30,12 +32,12 @@ __device__ __forceinline__ float2 turn_of(long long position, double inv_freq) {
   return make_float2(c, s);
 }
 
-constexpr int RO_THREADS = 256;
+constexpr int RO_THREADS = 128;
 
-// Where the tokens of a CTA go: page and row in the cache, or page -1 for none.
-struct TokenPlace {
-  long long page;
-  int row, used;
+// A token of a CTA: offsets of its rows in the inputs and outputs, and whether it takes part
+struct Token {
+  long long q, k, v, q_out, k_out, v_out;
+  int used, placed;      // counted among the sequence's tokens; has a place for its key and value
 };
 struct RotaryShape {
   int tokens, heads, hblocks;      // of a CTA; CTAs that share the heads of a token
@@ -43,127 +45,131 @@ struct RotaryShape {
 };
 
 template <typename T, int K, bool INTER>
-__global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constant__ FtkRotaryDesc d, const RotaryShape w, int* status) {
+__global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ RotaryShape w, int* status) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int half = (int)(d.turn >> 1), S = (int)d.S;
-  float2* cs = reinterpret_cast<float2*>(smem);                                 // [tokens][half]
-  TokenPlace* place = reinterpret_cast<TokenPlace*>(cs + w.tokens * half);      // [tokens]
+  float2* cs = reinterpret_cast<float2*>(smem);                       // [tokens][half]
+  Token* tok = reinterpret_cast<Token*>(cs + w.tokens * half);        // [tokens]
   pdl_wait();
   pdl_trigger_work(RO_THREADS * 64 * K);
-  const long long tok0 = (long long)(blockIdx.x / w.hblocks) * w.tokens, all = d.B * d.S;
-  const int h0 = (blockIdx.x % w.hblocks) * w.heads;
-  const int heads = min(w.heads, w.hq + w.hk + (d.k_pages ? w.hk : 0) - h0);
+  const bool append = d.k_pages != nullptr;
+  const long long tok0 = (long long)(blockIdx.x / (unsigned)w.hblocks) * w.tokens, all = d.B * d.S;
+  const int h0 = (int)(blockIdx.x % (unsigned)w.hblocks) * w.heads;
+  const int heads = min(w.heads, w.hq + w.hk + (append ? w.hk : 0) - h0);
   const int tokens = (int)min((long long)w.tokens, all - tok0);
   const long long b0 = tok0 / d.S;
   const unsigned s0 = (unsigned)(tok0 - b0 * d.S);
-  const auto token = [&](int t, long long& b, int& s) {
+  const auto place = [&](int t, long long& b, int& s) {
     const unsigned x = s0 + (unsigned)t;
     b = b0 + x / (unsigned)S, s = (int)(x % (unsigned)S);
   };
-  const int items = tokens * heads * w.chunks;
-  uint4 u0[K], u1[K];
-  const auto item = [&](int i, int& t, int& h, int& o0, int& o1, bool& turn) {
-    const unsigned c = (unsigned)i % (unsigned)w.chunks, r = (unsigned)i / (unsigned)w.chunks;
-    h = h0 + (int)(r % (unsigned)heads), t = (int)(r / (unsigned)heads);
-    turn = (int)c * 16 < (int)d.turn;
-    const bool apart = turn && !INTER;
-    o0 = apart ? c * 8 : c * 16, o1 = apart ? half + c * 8 : c * 16 + 8;
-  };
-  for (int i0 = 0; i0 < items; i0 += K * RO_THREADS) {
+  for (int t = threadIdx.x; t < tokens; t += RO_THREADS) {
+    long long b;
+    int s;
+    place(t, b, s);
+    Token& k = tok[t];
+    k.q = b * d.q_bs + s * d.q_ss, k.k = b * d.k_bs + s * d.k_ss, k.v = b * d.v_bs + s * d.v_ss;
+    k.q_out = b * d.qo_bs + s * d.qo_ss, k.k_out = b * d.ko_bs + s * d.ko_ss;
+    k.used = 1;
+    if (d.counts) {
+      const int n = d.counts[b];
+      k.used = s < n;
+      if (append && s == 0 && (n < 0 || n > S)) ft_index_ok(-1, 1, status);
+    }
+  }
+  __syncthreads();
+  // this thread's elements of a head, and its first head and token
+  const int c = threadIdx.x % (unsigned)w.chunks, step = RO_THREADS / (unsigned)w.chunks, lane = threadIdx.x / (unsigned)w.chunks;
+  const bool turned = c * 16 < (int)d.turn, apart = turned && !INTER;
+  const int o0 = apart ? c * 8 : c * 16, o1 = apart ? half + c * 8 : c * 16 + 8;
+  const int dt = step / heads, dh = step % heads;
+  int t = lane < step ? lane / heads : tokens, h = lane % heads;
+  for (bool first = true; first || t < tokens; first = false) {
+    uint4 u0[K], u1[K];
+    int tt = t, hh = h;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int i = i0 + k * RO_THREADS + threadIdx.x;
-      if (i >= items) break;
-      int t, h, o0, o1, s;
-      bool turn;
-      long long b;
-      item(i, t, h, o0, o1, turn);
-      token(t, b, s);
-      const T* src = h < w.hq ? (const T*)d.q + b * d.q_bs + s * d.q_ss + h * d.q_hs
-                     : h < w.hq + w.hk ? (const T*)d.k + b * d.k_bs + s * d.k_ss + (h - w.hq) * d.k_hs
-                                       : (const T*)d.v + b * d.v_bs + s * d.v_ss + (h - w.hq - w.hk) * d.v_hs;
-      u0[k] = *reinterpret_cast<const uint4*>(src + o0), u1[k] = *reinterpret_cast<const uint4*>(src + o1);
+      if (tt < tokens) {
+        const int g = h0 + hh;
+        const T* src = g < w.hq ? (const T*)d.q + tok[tt].q + g * d.q_hs
+                       : g < w.hq + w.hk ? (const T*)d.k + tok[tt].k + (g - w.hq) * d.k_hs
+                                         : (const T*)d.v + tok[tt].v + (g - w.hq - w.hk) * d.v_hs;
+        if (g < w.hq || !append || tok[tt].used) {
+          u0[k] = *reinterpret_cast<const uint4*>(src + o0), u1[k] = *reinterpret_cast<const uint4*>(src + o1);
+        }
+      }
+      tt += dt, hh += dh;
+      if (hh >= heads) hh -= heads, ++tt;
     }
-    if (i0 == 0) {
-      for (int t = threadIdx.x; t < tokens; t += RO_THREADS) {
+    if (first) {
+      for (int i = threadIdx.x; i < tokens && append; i += RO_THREADS) {
+        Token& k = tok[i];
+        k.placed = 0;
+        if (!k.used) continue;
         long long b;
         int s;
-        token(t, b, s);
-        TokenPlace p = {-1, 0, !d.counts || s < d.counts[b]};
-        if (d.k_pages && p.used) {
-          const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
-          const long long position = (long long)d.start[b] + s;
-          p.page = paged_page(table, b, position);
-          p.row = (int)paged_row(table, position);
-          if (p.page < 0) ft_index_ok(-1, 1, status);
+        place(i, b, s);
+        const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
+        const long long position = (long long)d.start[b] + s, page = paged_page(table, b, position), row = paged_row(table, position);
+        if (page < 0) {
+          ft_index_ok(-1, 1, status);
+          continue;
         }
-        if (d.counts && d.k_pages && s == 0 && (d.counts[b] < 0 || d.counts[b] > S)) ft_index_ok(-1, 1, status);
-        place[t] = p;
+        k.placed = 1;
+        k.k_out = page * d.kp_ps + row * d.kp_rs, k.v_out = page * d.vp_ps + row * d.vp_rs;
       }
       for (int e = threadIdx.x; e < tokens * half; e += RO_THREADS) {
         long long b;
         int s;
-        token((int)((unsigned)e / (unsigned)half), b, s);
-        const float2 c = turn_of((d.start ? d.start[b] : 0) + (long long)s, d.inv_freq[(unsigned)e % (unsigned)half]);
-        cs[e] = make_float2(c.x, d.inverse ? -c.y : c.y);
+        place((int)((unsigned)e / (unsigned)half), b, s);
+        const float2 a = turn_of((d.start ? d.start[b] : 0) + (long long)s, d.inv_freq[(unsigned)e % (unsigned)half]);
+        cs[e] = make_float2(a.x, d.inverse ? -a.y : a.y);
       }
       __syncthreads();
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int i = i0 + k * RO_THREADS + threadIdx.x;
-      if (i >= items) break;
-      int t, h, o0, o1, s;
-      bool turn;
-      long long b;
-      item(i, t, h, o0, o1, turn);
-      token(t, b, s);
-      const TokenPlace p = place[t];
-      T* dst;
-      if (h < w.hq) {
-        dst = (T*)d.q_out + b * d.qo_bs + s * d.qo_ss + h * d.qo_hs;
-        turn = turn && p.used;
-      } else {
-        const bool is_k = h < w.hq + w.hk;
-        const int g = is_k ? h - w.hq : h - w.hq - w.hk;
-        turn = turn && is_k;
-        if (d.k_pages) {
-          if (p.page < 0) continue;
-          dst = is_k ? (T*)d.k_pages + p.page * d.kp_ps + g * d.kp_hs + p.row * d.kp_rs
-                     : (T*)d.v_pages + p.page * d.vp_ps + g * d.vp_hs + p.row * d.vp_rs;
-        } else {
-          dst = (T*)d.k_out + b * d.ko_bs + s * d.ko_ss + g * d.ko_hs;
-        }
-      }
-      if (turn) {
-        float a[16];
-        up8<T>(u0[k], a);
-        up8<T>(u1[k], a + 8);
-        const float4* tc = reinterpret_cast<const float4*>(cs + t * half + (INTER ? o0 >> 1 : o0));      // two pairs each
+      if (t < tokens) {
+        const int g = h0 + h;
+        const bool is_q = g < w.hq, is_k = !is_q && g < w.hq + w.hk;
+        const Token& o = tok[t];
+        T* dst = is_q ? (T*)d.q_out + o.q_out + g * d.qo_hs
+                 : append ? (is_k ? (T*)d.k_pages + o.k_out + (g - w.hq) * d.kp_hs : (T*)d.v_pages + o.v_out + (g - w.hq - w.hk) * d.vp_hs)
+                          : (T*)d.k_out + o.k_out + (g - w.hq) * d.ko_hs;
+        if (turned && (is_q ? o.used : is_k)) {
+          float a[16];
+          up8<T>(u0[k], a);
+          up8<T>(u1[k], a + 8);
+          const float4* tc = reinterpret_cast<const float4*>(cs + t * half + c * 8);      // two pairs each
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float4 f = tc[j >> 1];
+          for (int j = 0; j < 8; j += 2) {
+            const float4 f = tc[j >> 1];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float c = e ? f.z : f.x, sn = e ? f.w : f.y;
-            float& x0 = INTER ? a[2 * (j + e)] : a[j + e];
-            float& x1 = INTER ? a[2 * (j + e) + 1] : a[8 + j + e];
-            const float y0 = x0 * c - x1 * sn, y1 = x1 * c + x0 * sn;
-            x0 = y0, x1 = y1;
+            for (int e = 0; e < 2; ++e) {
+              const float cc = e ? f.z : f.x, sn = e ? f.w : f.y;
+              float& x0 = INTER ? a[2 * (j + e)] : a[j + e];
+              float& x1 = INTER ? a[2 * (j + e) + 1] : a[8 + j + e];
+              const float y0 = x0 * cc - x1 * sn, y1 = x1 * cc + x0 * sn;
+              x0 = y0, x1 = y1;
+            }
           }
+          u0[k] = down8<T>(a);
+          u1[k] = down8<T>(a + 8);
         }
-        u0[k] = down8<T>(a);
-        u1[k] = down8<T>(a + 8);
+        if (is_q || !append || o.placed) {
+          *reinterpret_cast<uint4*>(dst + o0) = u0[k];
+          *reinterpret_cast<uint4*>(dst + o1) = u1[k];
+        }
       }
-      *reinterpret_cast<uint4*>(dst + o0) = u0[k];
-      *reinterpret_cast<uint4*>(dst + o1) = u1[k];
+      t += dt, h += dh;
+      if (h >= heads) h -= heads, ++t;
     }
   }
 }
 
 template <typename T, int K>
 static int launch(const FtkRotaryDesc& d, const RotaryShape& w, long long blocks, cudaStream_t s) {
-  const size_t smem = (size_t)w.tokens * ((d.turn >> 1) * sizeof(float2) + sizeof(TokenPlace));
+  const size_t smem = (size_t)w.tokens * ((d.turn >> 1) * sizeof(float2) + sizeof(Token));
   return d.interleaved ? launch_pdl(rotary_kernel<T, K, true>, dim3((unsigned)blocks), dim3(RO_THREADS), smem, s, d, w, ftk_status_word())
                        : launch_pdl(rotary_kernel<T, K, false>, dim3((unsigned)blocks), dim3(RO_THREADS), smem, s, d, w, ftk_status_word());
 }
@@ -182,8 +188,8 @@ extern "C" int ftk_rotary(const FtkRotaryDesc* d, void* stream) {
   w.hq = d->q ? (int)d->Hq : 0, w.hk = d->k ? (int)d->Hkv : 0, w.chunks = (int)(d->hd >> 4);
   // Four items per thread where that still leaves several CTAs for each SM, fewer for small calls; tokens of a CTA share its
   // table of 4096 sines at most
-  const long long items = d->B * d->S * heads * w.chunks, full = 148ll * 6 * RO_THREADS;
-  const int per = items >= 4 * full ? 4 : (items >= 2 * full ? 2 : 1), most = per * RO_THREADS;
+  const long long items = d->B * d->S * heads * w.chunks, full = 148ll * 8 * RO_THREADS;
+  const int per = items >= 4 * full ? 4 : (items >= 2 * full ? 2 : 1), most = per * (RO_THREADS / w.chunks) * w.chunks;
   w.heads = (int)(heads * w.chunks <= most ? heads : (most / w.chunks > 0 ? most / w.chunks : 1));
   w.hblocks = (int)((heads + w.heads - 1) / w.heads);
   long long tokens = w.hblocks > 1 ? 1 : most / (heads * w.chunks);
