@@ -48,8 +48,9 @@ template <typename T, int K, bool INTER>
 __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ RotaryShape w, int* status) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int half = (int)(d.turn >> 1), S = (int)d.S;
-  float2* cs = reinterpret_cast<float2*>(smem);                       // [tokens][half]
-  Token* tok = reinterpret_cast<Token*>(cs + w.tokens * half);        // [tokens]
+  // Cosines and sines of two pairs, (c, c', s, s'), as [token][two pairs of an item][items]: the items' threads read 16 bytes side by side
+  float4* cs = reinterpret_cast<float4*>(smem);
+  Token* tok = reinterpret_cast<Token*>(cs + w.tokens * half / 2);        // [tokens]
   pdl_wait();
   pdl_trigger_work(RO_THREADS * 64 * K);
   const bool append = d.k_pages != nullptr;
@@ -121,9 +122,11 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constan
       for (int e = threadIdx.x; e < tokens * half; e += RO_THREADS) {
         long long b;
         int s;
-        place((int)((unsigned)e / (unsigned)half), b, s);
-        const float2 a = turn_of((d.start ? d.start[b] : 0) + (long long)s, d.inv_freq[(unsigned)e % (unsigned)half]);
-        cs[e] = make_float2(a.x, d.inverse ? -a.y : a.y);
+        const int i = (int)((unsigned)e % (unsigned)half), t = (int)((unsigned)e / (unsigned)half);
+        place(t, b, s);
+        const float2 a = turn_of((d.start ? d.start[b] : 0) + (long long)s, d.inv_freq[i]);
+        float* to = reinterpret_cast<float*>(cs + t * (half >> 1) + ((i & 7) >> 1) * (half >> 3) + (i >> 3)) + (i & 1);
+        to[0] = a.x, to[2] = d.inverse ? -a.y : a.y;
       }
       __syncthreads();
     }
@@ -137,24 +140,25 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constan
                  : append ? (is_k ? (T*)d.k_pages + o.k_out + (g - w.hq) * d.kp_hs : (T*)d.v_pages + o.v_out + (g - w.hq - w.hk) * d.vp_hs)
                           : (T*)d.k_out + o.k_out + (g - w.hq) * d.ko_hs;
         if (turned && (is_q ? o.used : is_k)) {
-          float a[16];
-          up8<T>(u0[k], a);
-          up8<T>(u1[k], a + 8);
-          const float4* tc = reinterpret_cast<const float4*>(cs + t * half + c * 8);      // two pairs each
+          const float4* tc = cs + t * (half >> 1) + c;
+          uint32_t* x = reinterpret_cast<uint32_t*>(&u0[k]);      // words of two elements
+          uint32_t* y = reinterpret_cast<uint32_t*>(&u1[k]);
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float4 f = tc[j >> 1];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float cc = e ? f.z : f.x, sn = e ? f.w : f.y;
-              float& x0 = INTER ? a[2 * (j + e)] : a[j + e];
-              float& x1 = INTER ? a[2 * (j + e) + 1] : a[8 + j + e];
-              const float y0 = x0 * cc - x1 * sn, y1 = x1 * cc + x0 * sn;
-              x0 = y0, x1 = y1;
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = tc[j * (half >> 3)];
+            if (INTER) {          // words 2 j and 2 j + 1 of the item hold a pair each
+              uint32_t& p = j < 2 ? x[2 * j] : y[2 * j - 4];
+              uint32_t& q = j < 2 ? x[2 * j + 1] : y[2 * j - 3];
+              const float2 a = Half16<T>::up(p), b = Half16<T>::up(q);
+              p = Half16<T>::down(a.x * f.x - a.y * f.z, a.y * f.x + a.x * f.z);
+              q = Half16<T>::down(b.x * f.y - b.y * f.w, b.y * f.y + b.x * f.w);
+            } else {              // the first and second elements of two pairs
+              const float2 a = Half16<T>::up(x[j]), b = Half16<T>::up(y[j]);
+              const f32x2 x0 = pk2(a.x, a.y), x1 = pk2(b.x, b.y), cc = pk2(f.x, f.y), sn = pk2(f.z, f.w);
+              const float2 u = up2(fma2(x0, cc, mul2(x1, pk2(-f.z, -f.w)))), v = up2(fma2(x1, cc, mul2(x0, sn)));
+              x[j] = Half16<T>::down(u.x, u.y), y[j] = Half16<T>::down(v.x, v.y);
             }
           }
-          u0[k] = down8<T>(a);
-          u1[k] = down8<T>(a + 8);
         }
         if (is_q || !append || o.placed) {
           *reinterpret_cast<uint4*>(dst + o0) = u0[k];
