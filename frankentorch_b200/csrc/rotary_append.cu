@@ -11,10 +11,10 @@
 //
 // Work is divided into items of 16 elements of one head of one token: two 16-byte vectors that hold eight whole pairs (the
 // vectors are turn / 2 apart where pairs are (i, i + turn / 2), else neighbours), so an item can be turned in place.  A CTA has some
-// tokens with all their heads, a thread the same elements of every so-manieth head of them: it requests its items, up to four,
+// tokens with all their heads, a thread the same elements of every so-manieth head of them: it requests its items, two at a time,
 // and while they arrive the CTA forms the angles' sines and cosines once per token and pair and looks up the tokens' places.
-// Offsets of tokens are in shared memory: worked out per item they were two thirds of 250 instructions per 64 bytes, and forward and
-// backward of 4 x 2048 tokens of 16 heads of 128 took 59 us instead of ROTARY_US.
+// Offsets of tokens are in shared memory: worked out per item they were the larger part of 250 instructions per 64 bytes.
+// Forward and backward of 4 x 2048 tokens of 16 heads of 128 take 49 us, 5.5 TB/s.
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
 #include "launch.cuh"
@@ -190,10 +190,13 @@ extern "C" int ftk_rotary(const FtkRotaryDesc* d, void* stream) {
   if (d->S > 0x3fffffff || d->B > (1ll << 40)) return -2;
   RotaryShape w = {};
   w.hq = d->q ? (int)d->Hq : 0, w.hk = d->k ? (int)d->Hkv : 0, w.chunks = (int)(d->hd >> 4);
-  // Four items per thread where that still leaves several CTAs for each SM, fewer for small calls; tokens of a CTA share its
-  // table of 4096 sines at most
+  // Two items per thread at a time where that leaves several CTAs for each SM, and up to four rounds of them per CTA in large calls:
+  // what a CTA does once (places, sines, its launch) takes as long as two rounds.  4 x 2048 x 16 x 128 twice / 16 ragged prompts: one
+  // round 52.0 / 87.6 us, two 47.9 / 67.0, four 49.0 / 59.7, eight 51.6 / 63.9; four items at a time, one round 49.2 / 69.2.
+  // Tokens of a CTA share its table of 4096 sines at most.
   const long long items = d->B * d->S * heads * w.chunks, full = 148ll * 8 * RO_THREADS;
-  const int per = items >= 4 * full ? 4 : (items >= 2 * full ? 2 : 1), most = per * (RO_THREADS / w.chunks) * w.chunks;
+  const int per = items >= 2 * full ? 2 : 1, rounds = items >= 16 * full ? 4 : (items >= 8 * full ? 2 : 1);
+  const int most = rounds * per * (RO_THREADS / w.chunks) * w.chunks;
   w.heads = (int)(heads * w.chunks <= most ? heads : (most / w.chunks > 0 ? most / w.chunks : 1));
   w.hblocks = (int)((heads + w.heads - 1) / w.heads);
   long long tokens = w.hblocks > 1 ? 1 : most / (heads * w.chunks);
@@ -204,7 +207,6 @@ extern "C" int ftk_rotary(const FtkRotaryDesc* d, void* stream) {
   const long long blocks = (d->B * d->S + tokens - 1) / tokens * w.hblocks;
   if (blocks > 0x7fffffff) return -2;
   cudaStream_t s = (cudaStream_t)stream;
-  if (d->type == FTK_T_BF16)
-    return per == 4 ? launch<__nv_bfloat16, 4>(*d, w, blocks, s) : per == 2 ? launch<__nv_bfloat16, 2>(*d, w, blocks, s) : launch<__nv_bfloat16, 1>(*d, w, blocks, s);
-  return per == 4 ? launch<__half, 4>(*d, w, blocks, s) : per == 2 ? launch<__half, 2>(*d, w, blocks, s) : launch<__half, 1>(*d, w, blocks, s);
+  if (d->type == FTK_T_BF16) return per == 2 ? launch<__nv_bfloat16, 2>(*d, w, blocks, s) : launch<__nv_bfloat16, 1>(*d, w, blocks, s);
+  return per == 2 ? launch<__half, 2>(*d, w, blocks, s) : launch<__half, 1>(*d, w, blocks, s);
 }
