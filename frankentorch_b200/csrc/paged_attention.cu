@@ -36,12 +36,17 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;
 constexpr int PA_RING = 24 * 1024;           // bytes of a warp's ring: six stages of 16 tokens of 64 elements, three of 128
 constexpr int PA_WHOLE = 8;                  // tiles per head up to which a head is left whole
-constexpr int PA_HEADER = 8;                 // ints per CTA in front of the parts
+constexpr int PA_HEADER = 8;                 // ints of a header
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ float exp2_of(float x) {      // within 2^-22; what is below the normal numbers is 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -67,7 +72,8 @@ template <> struct PaShift<__half> { static constexpr float value = 15.f; };
 struct PagedAttn {
   FtkPagedAttnDesc d;
   int group, subs, sub_heads;      // query heads per head of the cache, parts of a group, heads of a part
-  int* header;                     // [CTAs][PA_HEADER]
+  bool by_head;                    // a header per head rather than per CTA: there are fewer
+  int* header;                     // [heads or CTAs][PA_HEADER]: the first CTA or -1, sequence, head, place of the part, last CTA
   float* parts;                    // [CTAs][2][rows][hd + 2]: accumulators, then maxima and sums
 };
 
@@ -86,6 +92,7 @@ template <typename T, int HD, int ROWS, bool SPLIT>
 __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
   typedef PaSmem<ROWS, HD> SM;
   constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 8, NT = HD / 8, KS = HD / 16;
+  constexpr int RR = ROWS / 8;
   constexpr float SHIFT = PaShift<T>::value;
   extern __shared__ __align__(128) unsigned char smem[];
   const FtkPagedAttnDesc& d = a.d;
@@ -115,12 +122,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
     p.n = length(p.b), p.tiles = (p.n + PA_TILE - 1) / PA_TILE;
     left = p.tiles;
   } else {
-    // tiles in front of each thread's share of the sequences, then the sequence in which the piece begins
-    long long* sums = reinterpret_cast<long long*>(smem);
-    int* found = reinterpret_cast<int*>(sums + PA_WARPS + 1);
-    const int each = ((int)d.B + PA_WARPS * 32 - 1) / (PA_WARPS * 32);
-    const int b0 = min((int)d.B, (int)threadIdx.x * each), b1 = min((int)d.B, b0 + each);
+    // Every warp for itself: tiles in front of each lane's share of the sequences, then the sequence in which the piece begins
+    const int each = ((int)d.B + 31) / 32, b0 = min((int)d.B, lane * each), b1 = min((int)d.B, b0 + each);
     long long mine = 0;
+#pragma unroll 4
     for (int b = b0; b < b1; ++b) mine += (length(b) + PA_TILE - 1) / PA_TILE;
     long long upto = mine;
 #pragma unroll
@@ -128,88 +133,112 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
       const long long v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    long long front = upto - mine;
-    for (int w = 0; w < PA_WARPS; ++w) {
-      if (w < warp) front += sums[w];
-      total += sums[w];
-    }
-    total *= heads;
+    total = __shfl_sync(0xffffffffu, upto, 31) * heads;
     per = max((total + gridDim.x - 1) / gridDim.x, 2ll);      // a part of less than two tiles costs more to join than it saves
     first_unit = per * blockIdx.x;
     left = min(per, total - first_unit);
-    front *= heads;
-    if (left > 0 && front <= first_unit && first_unit < front + mine * heads) {
+    if (!a.by_head && threadIdx.x == 0) a.header[(long long)blockIdx.x * PA_HEADER] = -1;
+    if (left <= 0) return;
+    long long front = (upto - mine) * heads;
+    p = {0, 0, 0, 0, 0};
+    const bool here = front <= first_unit && first_unit < upto * heads;
+    if (here) {
       for (int b = b0; b < b1; ++b) {
         const int n = length(b), tiles = (n + PA_TILE - 1) / PA_TILE;
-        if (first_unit < front + (long long)tiles * heads) {
-          found[0] = b, found[1] = (int)((first_unit - front) / tiles), found[2] = (int)((first_unit - front) % tiles);
-          found[3] = tiles, found[4] = n;
+        const long long in = first_unit - front;
+        if (in < (long long)tiles * heads) {
+          p = {b, (int)(in / tiles), (int)(in % tiles), tiles, n};
           break;
         }
         front += (long long)tiles * heads;
       }
     }
-    __syncthreads();
-    p = {found[0], found[1], found[2], found[3], found[4]};
-    __syncthreads();                    // the ring begins where this was
-    if (threadIdx.x == 0) a.header[(long long)blockIdx.x * PA_HEADER] = -1;
-    // sequences of no tokens are in nobody's piece
-    for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
-      if (length(b) != 0) continue;
-      for (int i = threadIdx.x; i < (int)d.Hq * HD; i += PA_WARPS * 32) ((T*)d.o)[b * d.o_bs + (i / HD) * d.o_hs + i % HD] = Half16<T>::round(0.f);
-      for (int i = threadIdx.x; i < (int)d.Hq; i += PA_WARPS * 32) d.lse[(long long)b * d.Hq + i] = -INFINITY;
-    }
-    if (left <= 0) return;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    p.b = __shfl_sync(0xffffffffu, p.b, owner), p.h = __shfl_sync(0xffffffffu, p.h, owner), p.t = __shfl_sync(0xffffffffu, p.t, owner);
+    p.tiles = __shfl_sync(0xffffffffu, p.tiles, owner), p.n = __shfl_sync(0xffffffffu, p.n, owner);
   }
 
-  // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences
-  Place f = p;
-  long long to_load = left;
-  int next_page = -1;                   // lane j < 16: page of token j of the warp's part of the tile at `f`
-  const auto fetch_page = [&]() {
-    const long long tok = (long long)f.t * PA_TILE + warp * 16 + (lane & 15);
-    next_page = -1;
-    if (to_load > 0 && tok < f.n) {
-      next_page = (int)paged_page(table, f.b, tok);
-      if (next_page < 0) ft_index_ok(-1, 1, status);
+  // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences, and the table is read from
+  // another one as far ahead of that
+  constexpr int AHEAD = STAGES - 1;
+  const auto advance = [&](Place& x, long long& more) {
+    --more;
+    if (++x.t == x.tiles) {
+      x.t = 0;
+      if (++x.h == heads) {
+        x.h = 0;
+        x.tiles = 0;
+        while (more > 0 && x.tiles == 0 && x.b + 1 < (int)d.B) x.n = length(++x.b), x.tiles = (x.n + PA_TILE - 1) / PA_TILE;
+      }
     }
+  };
+  Place f = p, g = p;
+  long long to_load = left, to_look = left;
+  // Pages of the next tiles.  A page of 16 rows or more holds all of a warp's part of a tile; of smaller ones lane j < 16 has token j's.
+  int page_of[AHEAD] = {};
+  const bool one_page = table.shift >= 4;
+  const auto look = [&]() {
+    int page = -1;
+    if (to_look > 0) {
+      const int tok = g.t * PA_TILE + warp * 16 + (one_page ? 0 : lane & 15);
+      if (tok < g.n) {
+        page = (int)paged_page(table, g.b, tok);
+        if (page < 0) ft_index_ok(-1, 1, status);
+      }
+      advance(g, to_look);
+    }
+    return page;
   };
   const uint32_t ring_s = smem_u32(ring);
   const int lrow = lane / CH, lchunk = lane % CH;
+  constexpr int RSTEP = 32 / CH, COPIES = 16 / RSTEP;      // rows of a copy of the warp, copies of 16 rows
+  const uint32_t lane_at = lrow * (HD * 2), lane_sw = lchunk << 4;
+  const long long k_lane = lrow * d.kp_rs + lchunk * 8, v_lane = lrow * d.vp_rs + lchunk * 8;
   const auto load = [&](int stage) {
-    if (to_load > 0) {
-      const unsigned ok = __ballot_sync(0xffffffffu, next_page >= 0) & 0xffffu;
-      if (lane == 0) there[stage] = ok;
-      const int g = f.h / a.subs, tok0 = f.t * PA_TILE + warp * 16;
-      const T* kb = (const T*)d.k_pages + g * d.kp_hs + lchunk * 8;
-      const T* vb = (const T*)d.v_pages + g * d.vp_hs + lchunk * 8;
-      const uint32_t dst = ring_s + stage * STAGE;
+    const int pages = page_of[0];
 #pragma unroll
-      for (int r = 0; r < 16; r += 32 / CH) {
-        const int row = r + lrow;
-        const long long page = __shfl_sync(0xffffffffu, next_page, row);
-        const long long in = paged_row(table, tok0 + row);
-        const bool t = page >= 0;
-        const uint32_t at = dst + row * (HD * 2) + ((lchunk ^ (row & 7)) << 4);
-        copy16(at, t ? kb + page * d.kp_ps + in * d.kp_rs : kb, t);
-        copy16(at + 16 * HD * 2, t ? vb + page * d.vp_ps + in * d.vp_rs : vb, t);
-      }
-      --to_load;
-      if (++f.t == f.tiles) {
-        f.t = 0;
-        if (++f.h == heads) {
-          f.h = 0;
-          f.tiles = 0;
-          while (to_load > 0 && f.tiles == 0 && f.b + 1 < (int)d.B) f.n = length(++f.b), f.tiles = (f.n + PA_TILE - 1) / PA_TILE;
+    for (int i = 0; i + 1 < AHEAD; ++i) page_of[i] = page_of[i + 1];
+    page_of[AHEAD - 1] = look();
+    if (to_load > 0) {
+      const int head = f.h / a.subs, tok0 = f.t * PA_TILE + warp * 16;
+      const T* kb = (const T*)d.k_pages + head * d.kp_hs;
+      const T* vb = (const T*)d.v_pages + head * d.vp_hs;
+      const uint32_t dst = ring_s + stage * STAGE + lane_at;
+      unsigned ok;
+      if (one_page) {
+        const int n = pages < 0 ? 0 : min(16, f.n - tok0);      // rows that are there
+        const long long page = pages < 0 ? 0 : pages, in = paged_row(table, tok0);
+        ok = (1u << n) - 1;
+        const T* k = kb + page * d.kp_ps + in * d.kp_rs + k_lane;
+        const T* v = vb + page * d.vp_ps + in * d.vp_rs + v_lane;
+        const long long k_step = RSTEP * d.kp_rs, v_step = RSTEP * d.vp_rs;
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c) {
+          const bool t = c * RSTEP + lrow < n;
+          const uint32_t at = dst + c * RSTEP * HD * 2 + (lane_sw ^ (((c * RSTEP + lrow) & 7) << 4));
+          copy16(at, t ? k : kb, t);
+          copy16(at + 16 * HD * 2, t ? v : vb, t);
+          k += k_step, v += v_step;
+        }
+      } else {
+        ok = __ballot_sync(0xffffffffu, pages >= 0) & 0xffffu;
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c) {
+          const int row = c * RSTEP + lrow;
+          const long long page = __shfl_sync(0xffffffffu, pages, row), in = paged_row(table, tok0 + row);
+          const bool t = page >= 0;
+          const uint32_t at = dst + c * RSTEP * HD * 2 + (lane_sw ^ ((row & 7) << 4));
+          copy16(at, t ? kb + page * d.kp_ps + in * d.kp_rs + lchunk * 8 : kb, t);
+          copy16(at + 16 * HD * 2, t ? vb + page * d.vp_ps + in * d.vp_rs + lchunk * 8 : vb, t);
         }
       }
-      fetch_page();
+      if (lane == 0) there[stage] = ok;
+      advance(f, to_load);
     }
     copy_commit();
   };
-  fetch_page();
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) page_of[i] = look();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load(s);
 
@@ -238,20 +267,23 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
   bool begun = p.t == 0;                // the piece has the beginning of the head at `p`
   int parts = 0;
   begin();
+  // this lane's rows for ldmatrix: chunk c of row r is at c ^ (r & 7), so the chunks of a step differ by an exclusive or
+  const int k_row = ((lane >> 4) << 3) + (lane & 7), v_row = (((lane >> 3) & 1) << 3) + (lane & 7);
+  const uint32_t k_at = k_row * (HD * 2) + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
+  const uint32_t v_at = 16 * HD * 2 + v_row * (HD * 2) + (((lane >> 4) ^ (v_row & 7)) << 4);
   int stage = 0;
   for (;;) {
     if (left > 0) {
       copy_wait<STAGES - 2>();
       __syncwarp();
-      const uint32_t ks = ring_s + stage * STAGE, vs = ks + 16 * HD * 2;
+      const uint32_t ks = ring_s + stage * STAGE + k_at, vs = ring_s + stage * STAGE + v_at;
       const unsigned ok = there[stage];
       const int refill = stage == 0 ? STAGES - 1 : stage - 1;
       float s[2][4] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t b[4];
-        const int row = ((lane >> 4) << 3) + (lane & 7), ch = 2 * k + ((lane >> 3) & 1);
-        ldm4(ks + row * (HD * 2) + ((ch ^ (row & 7)) << 4), b);
+        ldm4(ks ^ (k << 5), b);
         const uint32_t qa[4] = {q[k][0], ROWS == 16 ? q[k][1] : 0u, ROWS == 16 ? q[k][ROWS == 16 ? 2 : 0] : q[k][1],
                                 ROWS == 16 ? q[k][ROWS == 16 ? 3 : 0] : 0u};
         mma16<T>(s[0], qa, b[0], b[1]);
@@ -263,23 +295,25 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
       float grow[2];
       bool moved = false;
 #pragma unroll
-      for (int r = 0; r < (ROWS == 16 ? 2 : 1); ++r) {
+      for (int r = 0; r < RR; ++r) {
         float x[4], top = m[r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = (i >> 1) * 8 + c0 + (i & 1);
-          x[i] = (ok >> tok) & 1u ? s[i >> 1][2 * r + (i & 1)] * sc : -INFINITY;
-          top = fmaxf(top, x[i]);
+        for (int i = 0; i < 4; ++i) x[i] = s[i >> 1][2 * r + (i & 1)] * sc;
+        if (ok != 0xffffu) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(ok >> ((i >> 1) * 8 + c0 + (i & 1)) & 1u)) x[i] = -INFINITY;
         }
+        top = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float base = top == -INFINITY ? 0.f : top;
         moved |= top != m[r];
-        grow[r] = exp2f(m[r] - base);
+        grow[r] = exp2_of(m[r] - base);
         m[r] = top;
         float e[4], h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = exp2f(x[i] - base + SHIFT);
+        for (int i = 0; i < 4; ++i) e[i] = exp2_of(x[i] - base + SHIFT);
         l[r] = l[r] * grow[r] + ((e[0] + e[1]) + (e[2] + e[3]));
         hi[r] = Half16<T>::down(e[0], e[1]), hi[2 + r] = Half16<T>::down(e[2], e[3]);
         const float2 u = Half16<T>::up(hi[r]), w = Half16<T>::up(hi[2 + r]);
@@ -295,8 +329,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
 #pragma unroll
       for (int i = 0; i < NT; i += 2) {
         uint32_t b[4];
-        const int row = (((lane >> 3) & 1) << 3) + (lane & 7), ch = i + (lane >> 4);
-        ldm4t(vs + row * (HD * 2) + ((ch ^ (row & 7)) << 4), b);
+        ldm4t(vs ^ (i << 4), b);
         mma16<T>(acc[i], hi, b[0], b[1]);
         mma16<T>(acc[i + 1], hi, b[2], b[3]);
         if (ROWS == 16) {
@@ -312,7 +345,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
 
     // ---- the end of a head, or of the piece: the warps' parts become one, over 64 columns at a time
 #pragma unroll
-    for (int r = 0; r < (ROWS == 16 ? 2 : 1); ++r) {
+    for (int r = 0; r < RR; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if ((lane & 3) == 0) {
@@ -323,6 +356,15 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
     const bool whole = begun && p.t == p.tiles;
     const int first = row0(p.h), rows = rows_of(p.h);
     float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * ROWS * (HD + 2) : nullptr;
+    __syncthreads();
+    float scale[RR];                    // of the warp's part: to the maximum of all
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, stat[w * ROWS + r * 8 + r0]);
+      scale[r] = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
+    }
 #pragma unroll
     for (int half = 0; half < HD / 64; ++half) {
 #pragma unroll
@@ -330,41 +372,45 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
         float* to = merge + (warp * ROWS + r0) * 64 + i * 8 + c0;
         const float* c = acc[half * 8 + i];
         if (ROWS == 16) {
-          *reinterpret_cast<float2*>(to) = make_float2(c[0], c[1]);
-          *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(c[2], c[3]);
+          *reinterpret_cast<float2*>(to) = make_float2(c[0] * scale[0], c[1] * scale[0]);
+          *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(c[2] * scale[RR - 1], c[3] * scale[RR - 1]);
         } else {
-          *reinterpret_cast<float2*>(to) = make_float2(c[0] + c[2], c[1] + c[3]);
+          *reinterpret_cast<float2*>(to) = make_float2((c[0] + c[2]) * scale[0], (c[1] + c[3]) * scale[0]);
         }
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < rows * 64; i += PA_WARPS * 32) {
-        const int row = i >> 6, col = half * 64 + (i & 63);
-        float top = stat[row], v = 0.f, sum = 0.f;
+      for (int i = threadIdx.x; i < rows * 32; i += PA_WARPS * 32) {
+        const int row = i >> 5, in = (i & 31) * 2, col = half * 64 + in;
+        float2 v = make_float2(0.f, 0.f);
+        float top = stat[row], sum = 0.f;
 #pragma unroll
         for (int w = 1; w < PA_WARPS; ++w) top = fmaxf(top, stat[w * ROWS + row]);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < PA_WARPS; ++w) {
-          const float e = exp2f(stat[w * ROWS + row] - base);
-          v += e * merge[(w * ROWS + row) * 64 + (i & 63)];
-          sum += e * stat[(PA_WARPS + w) * ROWS + row];
+          const float2 x = *reinterpret_cast<const float2*>(merge + (w * ROWS + row) * 64 + in);
+          v.x += x.x, v.y += x.y;
+          sum += exp2f(stat[w * ROWS + row] - base) * stat[(PA_WARPS + w) * ROWS + row];
         }
         if (!SPLIT || whole) {
-          ((T*)d.o)[p.b * d.o_bs + (first + row) * d.o_hs + col] = Half16<T>::round(sum == 0.f ? 0.f : v / sum);
+          const float by = sum == 0.f ? 0.f : 1.f / sum;
+          T* o = (T*)d.o + p.b * d.o_bs + (first + row) * d.o_hs + col;
+          *reinterpret_cast<uint32_t*>(o) = Half16<T>::down(sum == 0.f ? 0.f : v.x * by, sum == 0.f ? 0.f : v.y * by);
           if (col == 0) d.lse[(long long)p.b * d.Hq + first + row] = sum == 0.f ? -INFINITY : (top + log2f(sum) - SHIFT) * LN2;
         } else {
-          part[row * HD + col] = v;
+          *reinterpret_cast<float2*>(part + row * HD + col) = v;
           if (col == 0) part[ROWS * HD + row] = top, part[ROWS * (HD + 1) + row] = sum;
         }
       }
       __syncthreads();
     }
     if (!SPLIT) return;
-    if (begun && p.t < p.tiles && threadIdx.x == 0) {
-      // the part that has the beginning of its head says who has the rest, up to the CTA of the head's last tile
+    // the part that has the beginning of its head says who has the rest, up to the CTA of the head's last tile
+    if (begun && threadIdx.x == 0 && (a.by_head || !whole)) {
       const long long behind = first_unit + min(per, total - first_unit);
-      int* h = a.header + (long long)blockIdx.x * PA_HEADER;
-      h[0] = 0, h[1] = p.b, h[2] = p.h, h[3] = parts, h[4] = (int)((behind + (p.tiles - p.t) - 1) / per);
+      int* h = a.header + (a.by_head ? (long long)p.b * heads + p.h : (long long)blockIdx.x) * PA_HEADER;
+      h[0] = whole ? -1 : (int)blockIdx.x;
+      h[1] = p.b, h[2] = p.h, h[3] = parts, h[4] = (int)((behind + (p.tiles - p.t) - 1) / per);
     }
     parts = 1;
     if (left <= 0) return;
@@ -380,40 +426,83 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
   }
 }
 
-// Joins the parts of a head that several CTAs had: block (c, row) that whose first part CTA c has.
+// Joins the parts of a head that several CTAs had, if header blockIdx.x is of one: `together` rows from together * blockIdx.y on, and
+// where that leaves threads over, several of them share a row's parts.  Sums are in a fixed order.  And since sequences of no tokens are in
+// nobody's piece, the blocks write them, a sequence each.
 template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(HD) paged_attn_join_kernel(const __grid_constant__ PagedAttn a) {
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
   constexpr float SHIFT = PaShift<T>::value;
+  constexpr int PART = ROWS * (HD + 2), LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
+  extern __shared__ float weight[];      // [parts][together]
+  __shared__ float sums[SLOTS], tops[SLOTS];
+  __shared__ float4 shares[SLOTS][LANES];
+  const FtkPagedAttnDesc& d = a.d;
   pdl_wait();
   pdl_trigger();
-  const FtkPagedAttnDesc& d = a.d;
-  const int c = blockIdx.x, row = blockIdx.y;
-  const int* h = a.header + (long long)c * PA_HEADER;
-  if (h[0] < 0) return;
-  const int b = h[1], hd = h[2], slot = h[3], last = h[4];
-  const int rows = min(a.sub_heads, a.group - (hd % a.subs) * a.sub_heads);
-  if (row >= rows) return;
-  const auto part = [&](int i) { return a.parts + ((long long)i * 2 + (i == c ? slot : 0)) * ROWS * (HD + 2); };
-  float top = -INFINITY;
-  for (int i = c; i <= last; ++i) top = fmaxf(top, part(i)[ROWS * HD + row]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float v = 0.f, sum = 0.f;
-#pragma unroll 4
-  for (int i = c; i <= last; ++i) {
-    const float* f = part(i);
-    const float e = exp2f(f[ROWS * HD + row] - base);
-    v += e * f[row * HD + threadIdx.x];
-    sum += e * f[ROWS * (HD + 1) + row];
+  for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
+    if (d.lengths[b] > 0) continue;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq * LANES; i += gridDim.y * 256)
+      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + (i / LANES) * d.o_hs + (i % LANES) * 4) = make_uint2(0, 0);
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq; i += gridDim.y * 256) d.lse[(long long)b * d.Hq + i] = -INFINITY;
   }
-  const int q = (hd / a.subs) * a.group + (hd % a.subs) * a.sub_heads + row;
-  ((T*)d.o)[b * d.o_bs + q * d.o_hs + threadIdx.x] = Half16<T>::round(sum == 0.f ? 0.f : v / sum);
-  if (threadIdx.x == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (top + log2f(sum) - SHIFT) * LN2;
+  if (a.by_head && d.lengths[blockIdx.x / (d.Hkv * a.subs)] <= 0) return;      // nobody wrote its header
+  const int* h = a.header + (long long)blockIdx.x * PA_HEADER;
+  const int c = h[0];
+  if (c < 0) return;
+  const int b = h[1], head = h[2], slot = h[3], n = h[4] - c + 1;
+  const int rows = min(a.sub_heads, a.group - (head % a.subs) * a.sub_heads);
+  const float* first = a.parts + ((long long)c * 2 + slot) * PART;
+  const float* rest = a.parts + (long long)c * 2 * PART;      // part i > 0 is at rest + 2 i PART
+  const auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * PART; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot_of = threadIdx.x / LANES, quad = threadIdx.x % LANES;
+  const int r0 = blockIdx.y * together, some = min(together, rows - r0);
+  // a warp per row: the largest maximum, every part's factor, the sum
+  for (int j = warp; j < some; j += 8) {
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[ROWS * HD + r0 + j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float* f = part(i);
+      const float e = exp2f(f[ROWS * HD + r0 + j] - base);
+      weight[i * together + j] = e;
+      sum += e * f[ROWS * (HD + 1) + r0 + j];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[j] = sum, tops[j] = top;
+  }
+  __syncthreads();
+  const int j = slot_of % together, share = slot_of / together, sharing = SLOTS / together;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (j < some) {
+#pragma unroll 8
+    for (int i = share; i < n; i += sharing) {
+      const float4 x = *reinterpret_cast<const float4*>(part(i) + (r0 + j) * HD + quad * 4);
+      const float e = weight[i * together + j];
+      v.x += e * x.x, v.y += e * x.y, v.z += e * x.z, v.w += e * x.w;
+    }
+  }
+  shares[slot_of][quad] = v;
+  __syncthreads();
+  if (share != 0 || j >= some) return;
+  for (int k = 1; k < sharing; ++k) {
+    const float4 x = shares[k * together + j][quad];
+    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+  }
+  const float sum = sums[j], by = sum == 0.f ? 0.f : 1.f / sum;
+  const int q = (head / a.subs) * a.group + (head % a.subs) * a.sub_heads + r0 + j;
+  if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+  *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x * by, v.y * by), Half16<T>::down(v.z * by, v.w * by));
+  if (quad == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (tops[j] + log2f(sum) - SHIFT) * LN2;
 }
 
 struct Plan {
   int subs, sub_heads, rows;
   bool split;
-  long long ctas, bytes;
+  long long ctas, heads, headers, bytes;      // heads: of all sequences, a part of a group counting as one
 };
 static Plan plan_of(const FtkPagedAttnDesc& d) {
   Plan p;
@@ -423,22 +512,23 @@ static Plan plan_of(const FtkPagedAttnDesc& d) {
   p.rows = p.sub_heads <= 8 ? 8 : 16;
   const long long tiles = ((d.table_cols << d.page_shift) + PA_TILE - 1) / PA_TILE;
   p.split = tiles > PA_WHOLE;
-  p.ctas = d.B * d.Hkv * p.subs;
-  p.bytes = 0;
+  p.ctas = p.heads = d.B * d.Hkv * p.subs;
+  p.headers = p.bytes = 0;
   if (p.split) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     p.ctas = 2ll * sms;
-    p.bytes = p.ctas * (PA_HEADER * 4 + 2 * p.rows * (d.hd + 2) * 4);
+    p.headers = p.heads < p.ctas ? p.heads : p.ctas;
+    p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * p.rows * (d.hd + 2) * 4;
   }
   return p;
 }
 
 template <typename T, int HD, int ROWS>
 static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaStream_t s) {
-  PagedAttn a = {d, (int)(d.Hq / d.Hkv), p.subs, p.sub_heads, (int*)scratch, nullptr};
-  a.parts = (float*)((char*)scratch + p.ctas * PA_HEADER * 4);
+  PagedAttn a = {d, (int)(d.Hq / d.Hkv), p.subs, p.sub_heads, p.heads < p.ctas, (int*)scratch, nullptr};
+  a.parts = (float*)((char*)scratch + p.headers * PA_HEADER * 4);
   int* status = ftk_status_word();
   const int bytes = PaSmem<ROWS, HD>::BYTES;
   static_assert(2 * (PaSmem<ROWS, HD>::BYTES + 1024) <= 228 * 1024, "two CTAs share an SM");
@@ -448,7 +538,12 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(PA_WARPS * 32), bytes, s, a, status);
   if (rc || !p.split) return rc;
-  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.ctas, (unsigned)p.sub_heads), dim3(HD), 0, s, a);
+  // Few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a head.
+  constexpr int slots = 256 / (HD / 4);
+  int together = 1;
+  while (p.heads > 32 && together < p.sub_heads && together < slots) together *= 2;
+  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.headers, (unsigned)((p.sub_heads + together - 1) / together)), dim3(256),
+                    (size_t)p.ctas * together * 4, s, a, together);
 }
 
 static bool refused(const FtkPagedAttnDesc* d) {
