@@ -34,7 +34,6 @@ namespace ftk {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;
-constexpr int PA_RING = 24 * 1024;           // bytes of a warp's ring: six stages of 16 tokens of 64 elements, three of 128
 constexpr int PA_WHOLE = 8;                  // tiles per head up to which a head is left whole
 constexpr int PA_HEADER = 8;                 // ints of a header
 
@@ -82,14 +81,16 @@ struct Place {
   int b, h, t, tiles, n;
 };
 
+// CTAs of an SM, bytes of a warp's ring (four or six stages of 16 tokens of 64 elements, three of 128)
 template <int ROWS, int HD> struct PaSmem {
-  static constexpr int STAGE = 16 * HD * 4, STAGES = PA_RING / STAGE;
+  static constexpr int CTAS = HD == 64 && ROWS == 8 ? 3 : 2, RING = CTAS == 3 ? 16 * 1024 : 24 * 1024;
+  static constexpr int STAGE = 16 * HD * 4, STAGES = RING / STAGE;
   static constexpr int MERGE = PA_WARPS * ROWS * 64 * 4;      // accumulators of 64 columns of all warps
-  static constexpr int BYTES = PA_WARPS * PA_RING + MERGE + 2 * PA_WARPS * ROWS * 4 + PA_WARPS * STAGES * 4;
+  static constexpr int BYTES = PA_WARPS * RING + MERGE + 2 * PA_WARPS * ROWS * 4 + PA_WARPS * STAGES * 4;
 };
 
 template <typename T, int HD, int ROWS, bool SPLIT>
-__global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
+__global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
   typedef PaSmem<ROWS, HD> SM;
   constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 8, NT = HD / 8, KS = HD / 16;
   constexpr int RR = ROWS / 8;
@@ -97,8 +98,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const __gr
   extern __shared__ __align__(128) unsigned char smem[];
   const FtkPagedAttnDesc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = (int)d.Hkv * a.subs;
-  unsigned char* ring = smem + warp * PA_RING;
-  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * PA_RING);
+  unsigned char* ring = smem + warp * SM::RING;
+  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * SM::RING);
   float* stat = merge + SM::MERGE / 4;                                     // [2][warps][ROWS]
   unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * PA_WARPS * ROWS) + warp * STAGES;
   const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
@@ -518,7 +519,7 @@ static Plan plan_of(const FtkPagedAttnDesc& d) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    p.ctas = 2ll * sms;
+    p.ctas = (d.hd == 64 && p.rows == 8 ? PaSmem<8, 64>::CTAS : 2ll) * sms;
     p.headers = p.heads < p.ctas ? p.heads : p.ctas;
     p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * p.rows * (d.hd + 2) * 4;
   }
@@ -531,7 +532,7 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   a.parts = (float*)((char*)scratch + p.headers * PA_HEADER * 4);
   int* status = ftk_status_word();
   const int bytes = PaSmem<ROWS, HD>::BYTES;
-  static_assert(2 * (PaSmem<ROWS, HD>::BYTES + 1024) <= 228 * 1024, "two CTAs share an SM");
+  static_assert(PaSmem<ROWS, HD>::CTAS * (PaSmem<ROWS, HD>::BYTES + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
   const auto whole = paged_attn_kernel<T, HD, ROWS, false>, split = paged_attn_kernel<T, HD, ROWS, true>;
   const auto kernel = p.split ? split : whole;
   int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
