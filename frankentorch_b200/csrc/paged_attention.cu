@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
   const uint32_t k_at = k_row * (HD * 2) + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
   const uint32_t v_at = 16 * HD * 2 + v_row * (HD * 2) + (((lane >> 4) ^ (v_row & 7)) << 4);
   int stage = 0;
-  for (;;) {
+  for (bool more = true; more; more = left > 0) {
     if (left > 0) {
       copy_wait<STAGES - 2>();
       __syncwarp();
