@@ -6,14 +6,19 @@
 // What bounds it: each logit is read once and written once, a few operations in between; the copy bandwidth, and for a row or two
 // the latency of two dependent reads.
 //
-// Work.  The rows' columns behind one another, in blocks of 64, are cut into equal runs, one for each of two CTAs per SM; a run is a
-// few pieces of rows.  For a piece a CTA first counts the row's history into shared memory, 16 bits per column - occurrences
-// among the generated tokens in the low 15, "occurred in the prompt" in the highest; whole numbers, so the order of additions does
-// not matter - and a bit per column that has any.  (Histories of 32768 tokens and more take 32 bits and half the columns.)
-// Then it streams the columns, 16 bytes per thread twice per tile, with the next tile (of the next piece at the end) and the next
-// history already on their way; while one CTA counts the other streams.  Only columns whose bit is set are looked up and cleared.
-// A history is read once per piece, out of the L2 cache: pieces as long as shared memory allows, rather than narrow slices of
-// all rows, are what that costs least with (six slices per row instead of four pieces: 112 us where this takes LARGE_US).
+// Work.  The rows' columns behind one another, in blocks of 64, are cut into equal runs, one per SM; a run is some pieces of rows.
+// For a piece the CTA first counts the row's history into shared memory, 16 bits per column - occurrences among the generated
+// tokens in the low 15, "occurred in the prompt" in the highest; whole numbers, so the order of additions does not matter - and a bit
+// per column that has any.  (Histories of 32768 tokens and more take 32 bits and half the columns.)  Then it streams the columns, 16
+// bytes per thread twice per tile, with the next tile (of the next piece at the end) and the next history already on their way.
+//
+// What was measured (512 rows of 128003 bf16 columns with bias, mask and 2048 to 4096 tokens / 256 rows of 50257 fp32 columns with
+// mask and 1024 to 2048 tokens; the copy bandwidth gives 43 / 16 us):
+//   * a history is read once per piece and stops the stream, so pieces are as long as shared memory allows: 85 / 20 us with 64
+//     thousand columns, 103 / 24 with two CTAs of 40 thousand, 112 / 33 with six narrow slices of every row; a cluster of CTAs that
+//     share the counts of a row 185 / 50; warps of their own that count ahead of the stream 105 / 27;
+//   * penalties where a column has a history are what the time goes by next: without them the first takes 56 us.  All eight
+//     columns of a vector are done where one of them has its bit set, without a branch per column (that takes 89 / 22).
 #include <math.h>
 
 #include "ft_sm100.cuh"
@@ -25,13 +30,12 @@ extern "C" int* ftk_status_word(void);
 
 namespace ftk {
 
-constexpr int LG_THREADS = 512;              // threads of a CTA at most
+constexpr int LG_THREADS = 896;              // threads of a CTA at most
 constexpr int LG_TOKENS = 4;                 // tokens of a history that a thread requests ahead
 constexpr int LG_BLOCK = 64;                 // columns that stay together
 template <typename T> struct LgCols { static constexpr int value = 16 / (int)sizeof(T); };      // columns of 16 bytes
 
-// A load that stays where it is written: ahead of what waits for others.  (Plain loads of the next tile end up behind the work on
-// this one: 512 x 128003 with a history took 199 us instead.)
+// A load that stays where it is written: ahead of the work on what came before.
 __device__ __forceinline__ uint4 load_now(const uint4* p) {
   uint4 v;
   asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
@@ -42,11 +46,6 @@ __device__ __forceinline__ unsigned load_now(const unsigned char* p) {
   asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ long long load_now(const long long* p) {
-  long long v;
-  asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
 __device__ __forceinline__ int load_now(const int* p) {
   int v;
   asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -55,11 +54,6 @@ __device__ __forceinline__ int load_now(const int* p) {
 __device__ __forceinline__ float load_now(const float* p) {
   float v;
   asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 load_now(const float4* p) {
-  float4 v;
-  asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
   return v;
 }
 template <typename T> __device__ __forceinline__ void floats(const uint4& v, float* f) { up8<T>(v, f); }
@@ -91,7 +85,7 @@ struct LogitsRow {
 };
 // Counts of a piece's columns, 16 or 32 bits each in words of shared memory
 template <bool WIDE> struct Counts {
-  static constexpr int COLUMNS = WIDE ? 20 * 1024 : 40 * 1024;      // of a piece at most
+  static constexpr int COLUMNS = WIDE ? 32 * 1024 : 64 * 1024;      // of a piece at most
   static constexpr unsigned PROMPT = WIDE ? 0x80000000u : 0x8000u;
   unsigned* words;
   __device__ __forceinline__ void add(int at, unsigned n) {
@@ -102,16 +96,18 @@ template <bool WIDE> struct Counts {
     if (WIDE) atomicOr(&words[at], PROMPT);
     else atomicOr(&words[at >> 1], PROMPT << (at & 1) * 16);
   }
-  __device__ __forceinline__ unsigned take(int at) {      // the generated tokens' count; by the one thread that has the column
+  __device__ __forceinline__ unsigned operator[](int at) const {      // of the generated tokens
+    return (WIDE ? words[at] : reinterpret_cast<const unsigned short*>(words)[at]) & (PROMPT - 1);
+  }
+  template <int N> __device__ __forceinline__ void clear(int at) {       // N columns from a multiple of N on
     if (WIDE) {
-      const unsigned c = words[at];
-      words[at] = 0;
-      return c & (PROMPT - 1);
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(words + at + i) = make_uint4(0, 0, 0, 0);
+    } else if (N == 8) {
+      *reinterpret_cast<uint4*>(words + at / 2) = make_uint4(0, 0, 0, 0);
+    } else {
+      *reinterpret_cast<uint2*>(words + at / 2) = make_uint2(0, 0);
     }
-    unsigned short* p = reinterpret_cast<unsigned short*>(words) + at;
-    const unsigned c = *p;
-    *p = 0;
-    return c & (PROMPT - 1);
   }
 };
 struct LogitsCut {
@@ -122,7 +118,7 @@ struct LogitsCut {
 
 // VEC: rows of logits and results start on 16 bytes
 template <typename T, typename O, bool HISTORY, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_constant__ FtkLogitsDesc d, const LogitsCut cut, int* status) {
+__global__ void __launch_bounds__(LG_THREADS, 1) logits_kernel(const __grid_constant__ FtkLogitsDesc d, const LogitsCut cut, int* status) {
   constexpr int N = LgCols<T>::value;
   extern __shared__ __align__(16) unsigned smem[];               // counts, a bit per column, tokens
   Counts<WIDE> counts = {smem};
@@ -229,76 +225,78 @@ __global__ void __launch_bounds__(LG_THREADS, 2) logits_kernel(const __grid_cons
     O* out = (O*)d.out + r * d.ldo + v0;
     const float* bias = d.bias ? d.bias + r * d.bias_rs + v0 : nullptr;
     const unsigned shift = N == 8 ? 0 : (tid & 1) * 4;       // of this thread's bits in their byte
+    // A column as it leaves, with its penalties, bias and mask
+    const auto leave = [&](int at, float x, bool penalised) {
+      if (penalised) x = row(x, counts[at]);
+      if (bias) x += __ldg(bias + at);
+      if (d.allowed && !((unsigned)d.allowed[r * d.allowed_rs + ((v0 + at) >> 5)] >> (at & 31) & 1u)) x = -INFINITY;
+      store1(out + at, x);
+    };
+    // The bits of N columns that have a history; they and the counts are cleared by forget()
+    const auto bits_of = [&](int at) -> unsigned {
+      if (!HISTORY) return 0;
+      return reinterpret_cast<const unsigned char*>(seen)[at >> 3] >> (N == 8 ? 0 : at & 4) & ((1u << N) - 1);
+    };
+    const auto forget = [&](int at) {
+      counts.template clear<N>(at);
+      if (N == 8) reinterpret_cast<unsigned char*>(seen)[at >> 3] = 0;
+      else atomicAnd(&seen[at >> 5], ~(15u << (at & 31)));      // the other half of the byte is a neighbour's
+    };
+    // a vector of columns, all of them there
+    const auto vector = [&](int at, const uint4& x, unsigned bits) {
+      float y[N];
+      floats<T>(x, y);
+      const unsigned k = bits_of(at);
+      if (k) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v = row(y[e], counts[at + e]);
+          y[e] = k >> e & 1u ? v : y[e];
+        }
+        forget(at);
+      }
+      if (bias) {
+        if (cut.bias16) {
+#pragma unroll
+          for (int e = 0; e < N; e += 4) {
+            const float4 p = __ldg(reinterpret_cast<const float4*>(bias + at + e));
+            y[e] += p.x, y[e + 1] += p.y, y[e + 2] += p.z, y[e + 3] += p.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) y[e] += __ldg(bias + at + e);
+        }
+      }
+      if (d.allowed) {
+        bits >>= shift;
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = bits >> e & 1u ? y[e] : -INFINITY;
+      }
+      write<N>(out + at, y);
+    };
+    const auto few = [&](int from) {      // up to N columns, one by one
+      const unsigned k = bits_of(from);
+      for (int e = 0; e < N && from + e < n; ++e) leave(from + e, load1((const T*)d.logits + r * d.ld + v0 + from + e), k >> e & 1u);
+      if (k) forget(from);
+    };
     for (int t0 = 0; t0 < n; t0 += tile) {
+      const int at = t0 + tid * N;
       if (VEC) {
         const Tile x = next;
         request(next);
+        if (t0 + tile <= n) {
+          vector(at, x.x[0], x.bits[0]);
+          vector(at + step, x.x[1], x.bits[1]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int at = t0 + i * step + tid * N;
-          if (at >= n) continue;
-          const bool full = at + N <= n;
-          float y[N], b[N];
-          unsigned bits = ~0u;
-          if (full) {
-            floats<T>(x.x[i], y);
-            if (d.allowed) bits = x.bits[i] >> shift;
-          } else {                // the vocabulary's last columns
-            if (d.allowed) bits = (unsigned)d.allowed[r * d.allowed_rs + ((v0 + at) >> 5)] >> (at & 31);
-#pragma unroll
-            for (int e = 0; e < N; ++e) y[e] = at + e < n ? load1((const T*)d.logits + r * d.ld + v0 + at + e) : 0.f;
-          }
-          if (bias) {
-            if (full && cut.bias16) {
-#pragma unroll
-              for (int e = 0; e < N; e += 4) {
-                const float4 p = __ldg(reinterpret_cast<const float4*>(bias + at + e));
-                b[e] = p.x, b[e + 1] = p.y, b[e + 2] = p.z, b[e + 3] = p.w;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < N; ++e) b[e] = at + e < n ? __ldg(bias + at + e) : 0.f;
-            }
-          }
-          if (HISTORY) {
-            const unsigned k = seen[at >> 5] >> (at & 31) & ((1u << N) - 1);
-            if (k) {
-#pragma unroll
-              for (int e = 0; e < N; ++e)
-                if (k >> e & 1u) {
-                  y[e] = row(y[e], counts.take(at + e));
-                }
-              if (N == 8) reinterpret_cast<unsigned char*>(seen)[at >> 3] = 0;
-              else atomicAnd(&seen[at >> 5], ~(15u << (at & 31)));      // the other half of the byte is a neighbour's
-            }
-          }
-          if (bias) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) y[e] += b[e];
-          }
-          if (d.allowed) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) y[e] = bits >> e & 1u ? y[e] : -INFINITY;
-          }
-          if (full) {
-            write<N>(out + at, y);
-          } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (at + e < n) store1(out + at + e, y[e]);
+          for (int i = 0; i < 2; ++i) {
+            const int from = at + i * step;
+            if (from + N <= n) vector(from, x.x[i], x.bits[i]);
+            else if (from < n) few(from);      // the vocabulary's last columns
           }
         }
       } else {
-        for (int at = t0 + tid; at < min(n, t0 + tile); at += bd) {
-          float y = load1((const T*)d.logits + r * d.ld + v0 + at);
-          if (HISTORY && (seen[at >> 5] >> (at & 31) & 1u)) {
-            y = row(y, counts.take(at));
-            atomicAnd(&seen[at >> 5], ~(1u << (at & 31)));
-          }
-          if (bias) y += bias[at];
-          if (d.allowed && !((unsigned)d.allowed[r * d.allowed_rs + ((v0 + at) >> 5)] >> (at & 31) & 1u)) y = -INFINITY;
-          store1(out + at, y);
-        }
+        for (int from = at; from < min(n, t0 + tile); from += step) few(from);
       }
     }
   }
@@ -310,7 +308,7 @@ static int launch(const FtkLogitsDesc& d, cudaStream_t s) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const long long row = (d.V + LG_BLOCK - 1) / LG_BLOCK;
-  const long long ctas = max(1ll, min(2ll * sms, row * d.R * LG_BLOCK / 2048));      // 2048 columns at least
+  const long long ctas = max(1ll, min((long long)sms, row * d.R * LG_BLOCK / 2048));      // 2048 columns at least
   const long long run = (row * d.R + ctas - 1) / ctas * LG_BLOCK;
   const int columns = (int)min((long long)Counts<WIDE>::COLUMNS, min(run, row * LG_BLOCK));
   const LogitsCut cut = {row, columns, ((uintptr_t)d.bias | (uintptr_t)(d.bias_rs * 4)) % 16 == 0};

@@ -417,6 +417,42 @@ def test_logits_of_values_that_are_not_finite(cuda_device):
     assert got[0, 3] == inf and got[0, 5] == -inf and got[0, 6] == 1.0 and got[0, 7] == -inf
 
 
+@pytest.mark.parametrize("R,V,L,dtype", [
+    (3, 200003, 700, BF),             # a row in several pieces, runs that end inside a row
+    (300, 5001, 90, torch.float32),   # a run of several rows
+    (37, 70000, 5000, HF),            # more tokens than are requested ahead
+    (2, 70001, 40000, BF),            # counts of 32 bits
+    (149, 2048, 10, BF),
+])
+def test_logits_of_many_pieces(cuda_device, R, V, L, dtype):
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    g = _gen(R)
+    x = (3 * torch.randn(R, V + 5, generator=g, device="cuda")).to(dtype)
+    tokens = (torch.rand(R, L, generator=g, device="cuda", dtype=torch.float64) ** 2 * V).long()
+    lengths = torch.randint(L // 2, L + 1, (R,), generator=g, device="cuda", dtype=torch.int32)
+    prompts = lengths // 3
+    rep, freq, pres = (0.5 + torch.rand(R, generator=g, device="cuda") for _ in range(3))
+    bias = torch.randn(V, generator=g, device="cuda")
+    words = torch.randint(-2 ** 31, 2 ** 31 - 1, (R, (V + 31) // 32), generator=g, device="cuda").to(torch.int32)
+    got = D.logits_process(x, vocab=V, tokens=tokens, lengths=lengths, prompt_lengths=prompts, repetition=rep, frequency=freq,
+                           presence=pres, bias=bias, allowed=words, out_dtype=torch.float32)
+    K.check_status()
+    ids = torch.arange(V, device="cuda")
+    for r in range(R):
+        n, m = int(lengths[r]), int(prompts[r])
+        y = x[r, :V].double()
+        seen = torch.bincount(tokens[r, :n], minlength=V) > 0
+        made = torch.bincount(tokens[r, m:n], minlength=V)
+        y = torch.where(seen, torch.where(y > 0, y / rep[r].double(), y * rep[r].double()), y)
+        size = y.abs() + freq[r] * made + pres[r] * (made > 0) + bias.abs()
+        y = y - freq[r].double() * made - pres[r].double() * (made > 0) + bias.double()
+        allowed = words[r][ids // 32] >> (ids % 32) & 1 == 1
+        assert torch.equal(got[r].isinf(), ~allowed)
+        # six roundings of fp32 on what was added up, as above
+        assert bool(((got[r].double() - y).abs() <= 6 * 2.0 ** -24 * size.double())[allowed].all())
+
+
 def test_logits_count_far(cuda_device):
     """One token a hundred thousand times, and every history's place used."""
     from frankentorch_b200.ops import decode as D
