@@ -104,11 +104,13 @@ void frequencies(const Arg& a, FtkRotaryDesc& d) {
   d.inv_freq = (const double*)a.ptr();
   d.turn = 2 * n;
 }
+// Positions are counted in 32 bits, which `d`'s pages times the table's columns must not pass.
 template <typename D> void page_table(const Arg& a, int64_t B, D& d) {
   if (a->scalar_type() != at::kInt || a->dim() != 2 || a->size(0) != B || a->size(1) < 1 || (a->size(1) > 1 && a->stride(1) != 1))
     refuse("the page table must be int32 [" + std::to_string(B) + ", columns] with unit inner stride, got " + text(a->scalar_type()) + " " + text(a->sizes()));
   d.table = (const int*)a.ptr();
   d.table_stride = a->stride(0), d.table_cols = a->size(1);
+  if (d.table_cols > (0x7fffff00ll >> d.page_shift)) refuse("the page table has more than 2^31 - 256 positions");
 }
 template <typename D> void pages(const Arg& k, const Arg& v, int64_t heads, int64_t hd, at::ScalarType type, bool out, D& d) {
   long long s[3];
@@ -121,6 +123,7 @@ template <typename D> void pages(const Arg& k, const Arg& v, int64_t heads, int6
   const int64_t page = n[2];
   if (n[1] != heads || n[3] != hd || page < 1 || (page & (page - 1)))
     refuse("pages must be [pages, " + std::to_string(heads) + ", page, " + std::to_string(hd) + "] with a power of two of rows, got " + text(n));
+  if (n[0] == 0) refuse("the cache has no pages");
   d.k_pages = k.ptr(), d.v_pages = v.ptr();
   d.n_pages = n[0];
   for (d.page_shift = 0; (int64_t(1) << d.page_shift) < page;) ++d.page_shift;
@@ -294,7 +297,6 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else if (qo) {
       refuse("q_out without q");
     }
-    if (d.n_pages == 0) refuse("the cache has no pages");
     same_device(k, {&v, &kp, &vp, &table, &start, &counts, &w, &q, &qo});
     const On on(k);
     at::Tensor a;

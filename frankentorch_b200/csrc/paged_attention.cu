@@ -549,8 +549,8 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
 
 static bool refused(const FtkPagedAttnDesc* d) {
   return !d || d->B <= 0 || d->B > (1 << 30) || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > (1 << 20) || (d->hd != 64 && d->hd != 128) ||
-         (d->type != FTK_T_BF16 && d->type != FTK_T_FP16) || d->page_shift < 0 || d->page_shift > 30 || d->table_cols <= 0 || d->n_pages < 0 ||
-         d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff;
+         (d->type != FTK_T_BF16 && d->type != FTK_T_FP16) || d->page_shift < 0 || d->page_shift > 30 || d->table_cols <= 0 ||
+         d->table_cols > (0x7fffff00ll >> d->page_shift) || d->n_pages <= 0 || d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff;
 }
 
 }  // namespace ftk

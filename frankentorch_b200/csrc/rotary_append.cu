@@ -3,7 +3,7 @@
 //
 // Mathematics.  A pair (x0, x1) of a token at position p is turned by a = p w: (x0 cos a - x1 sin a, x1 cos a + x0 sin a).  The
 // backward pass is the inverse rotation of the gradient.  Far positions turn thousands of times, so the angle is formed and
-// reduced to a fraction of a turn in 64 bits (2^31 turns leave 2^-22 of a turn); sine and cosine of the fraction and the products
+// reduced to a fraction of a turn in 64 bits (2^28 turns at position 2^31 leave 2^-24 of a turn); sine and cosine of the fraction and the products
 // are fp32, each output is rounded once.
 //
 // What bounds it: each element is read once and written once; the copy bandwidth, and for a handful of tokens the latency of a

@@ -109,6 +109,8 @@ ATTEND = dict(q=lambda: _z(3, 4, 64), k_pages=lambda: _z(5, 2, 16, 64), v_pages=
     ("differ", {"k_pages": lambda: _z(5, 2, 8, 64)}),
     ("power of two", {"k_pages": lambda: _z(5, 2, 24, 64), "v_pages": lambda: _z(5, 2, 24, 64)}),
     ("16 bytes", {"q": lambda: _z(3, 4, 65)[..., :64]}),
+    ("no pages", {"k_pages": lambda: _z(0, 2, 16, 64), "v_pages": lambda: _z(0, 2, 16, 64)}),
+    ("2.31 - 256 positions", {"table": lambda: torch.empty(1, 2 ** 27, dtype=torch.int32).expand(3, -1)}),
     ("lengths must be", {"lengths": lambda: torch.ones(3, dtype=torch.int64)}),
     ("lengths must be", {"lengths": lambda: _i(1, 1, 1, 1, 1, 1)[::2]}),
     ("page table", {"table": lambda: torch.zeros(12, dtype=torch.int32)}),

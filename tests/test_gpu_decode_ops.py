@@ -544,6 +544,56 @@ def test_captured_steps_follow_their_lengths(cuda_device):
     K.check_status()
 
 
+FIRST_CALLS = """
+import sys
+sys.path[:0] = ["tests", "."]
+import torch
+import test_gpu_decode_ops as T
+from frankentorch_b200.ops import decode as D
+s = T._state(D, 3, [700, 1, 2048])
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    got = T._step(D, s)
+graph.replay()
+torch.cuda.synchronize()
+held = [t.clone() for t in got]
+want = T._step(D, s)
+from frankentorch_b200.ops import kernels as K
+K.check_status()
+assert all(torch.equal(a, b) for a, b in zip(held, want))
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_are_captured(cuda_device):
+    import subprocess
+    import sys
+    from pathlib import Path
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parent.parent)
+    assert out.returncode == 0 and "the same" in out.stdout, out.stderr[-2000:]
+
+
+def test_tables_that_share(cuda_device):
+    """Sequences with the same pages, a table that is a view into a wider one, or one row for all sequences."""
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    g = _gen(12)
+    n = [700, 130, 1, 699]
+    q, kp, vp, table = _attend(g, 1, 8, 2, 64, 16, [700], BF)
+    q = _rnd(g, 4, 8, 64)
+    wide = torch.full((4, table.shape[1] + 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, 3: 3 + table.shape[1]] = table
+    for t in (table.expand(4, -1), wide[:, 3: 3 + table.shape[1]]):
+        o, lse = D.paged_attention(q, kp, vp, t, _i32(n))
+        wo, wl, to, tl = attention64(q, kp, vp, t, n)
+        close(o, wo, to, "o")
+        close(lse, wl, tl, "lse")
+    K.check_status()
+
+
 def test_calls_of_two_streams_and_threads(cuda_device):
     import threading
 
