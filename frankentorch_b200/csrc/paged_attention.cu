@@ -434,70 +434,86 @@ template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
   constexpr float SHIFT = PaShift<T>::value;
   constexpr int PART = ROWS * (HD + 2), LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
-  extern __shared__ float weight[];      // [parts][together]
+  constexpr int FIRST = 4;               // parts whose accumulators a thread requests along with the statistics
+  extern __shared__ float2 part_ml[];    // [parts][together]: maximum and sum, then (factor, -)
   __shared__ float sums[SLOTS], tops[SLOTS];
   __shared__ float4 shares[SLOTS][LANES];
   const FtkPagedAttnDesc& d = a.d;
   pdl_wait();
   pdl_trigger();
+  const int* h = a.header + (long long)blockIdx.x * PA_HEADER;
+  const int4 head4 = *reinterpret_cast<const int4*>(h);
+  const int last = h[4], own = a.by_head ? d.lengths[blockIdx.x / (unsigned)(d.Hkv * a.subs)] : 1;
+  const int c = own > 0 ? head4.x : -1;      // (nobody writes the header of a head without tokens)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot_of = threadIdx.x / LANES, quad = threadIdx.x % LANES;
+  if (c >= 0) {
+    const int b = head4.y, head = head4.z, slot = head4.w, n = last - c + 1;
+    const int rows = min(a.sub_heads, a.group - (head % a.subs) * a.sub_heads);
+    const float* first = a.parts + ((long long)c * 2 + slot) * PART;
+    const float* rest = a.parts + (long long)c * 2 * PART;      // part i > 0 is at rest + 2 i PART
+    const auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * PART; };
+    const int r0 = blockIdx.y * together, some = min(together, rows - r0);
+    const int j = slot_of % together, share = slot_of / together, sharing = SLOTS / together;
+    const auto acc_of = [&](int i) { return *reinterpret_cast<const float4*>(part(i) + (r0 + j) * HD + quad * 4); };
+    float4 x[FIRST];
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k)
+      if (j < some && share + k * sharing < n) x[k] = acc_of(share + k * sharing);
+    for (int i = threadIdx.x; i < n * together; i += 256) {
+      const int p = i / together, row = i % together;
+      if (row < some) part_ml[i] = make_float2(part(p)[ROWS * HD + r0 + row], part(p)[ROWS * (HD + 1) + r0 + row]);
+    }
+    __syncthreads();
+    // a warp per row: the largest maximum, every part's factor, the sum
+    for (int row = warp; row < some; row += 8) {
+      float top = -INFINITY;
+      for (int i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i * together + row].x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      for (int i = lane; i < n; i += 32) {
+        float2& ml = part_ml[i * together + row];
+        ml.x = exp2f(ml.x - base);
+        sum += ml.x * ml.y;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) sums[row] = sum, tops[row] = top;
+    }
+    __syncthreads();
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](int i, const float4& y) {
+      const float e = part_ml[i * together + j].x;
+      v.x += e * y.x, v.y += e * y.y, v.z += e * y.z, v.w += e * y.w;
+    };
+    if (j < some) {
+#pragma unroll
+      for (int k = 0; k < FIRST; ++k)
+        if (share + k * sharing < n) add(share + k * sharing, x[k]);
+#pragma unroll 8
+      for (int i = share + FIRST * sharing; i < n; i += sharing) add(i, acc_of(i));
+    }
+    shares[slot_of][quad] = v;
+    __syncthreads();
+    if (share == 0 && j < some) {
+      for (int k = 1; k < sharing; ++k) {
+        const float4 y = shares[k * together + j][quad];
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+      }
+      const float sum = sums[j], by = sum == 0.f ? 0.f : 1.f / sum;
+      const int q = (head / a.subs) * a.group + (head % a.subs) * a.sub_heads + r0 + j;
+      if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x * by, v.y * by), Half16<T>::down(v.z * by, v.w * by));
+      if (quad == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (tops[j] + log2f(sum) - SHIFT) * LN2;
+    }
+  }
   for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
     if (d.lengths[b] > 0) continue;
     for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq * LANES; i += gridDim.y * 256)
       *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + (i / LANES) * d.o_hs + (i % LANES) * 4) = make_uint2(0, 0);
     for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq; i += gridDim.y * 256) d.lse[(long long)b * d.Hq + i] = -INFINITY;
   }
-  if (a.by_head && d.lengths[blockIdx.x / (d.Hkv * a.subs)] <= 0) return;      // nobody wrote its header
-  const int* h = a.header + (long long)blockIdx.x * PA_HEADER;
-  const int c = h[0];
-  if (c < 0) return;
-  const int b = h[1], head = h[2], slot = h[3], n = h[4] - c + 1;
-  const int rows = min(a.sub_heads, a.group - (head % a.subs) * a.sub_heads);
-  const float* first = a.parts + ((long long)c * 2 + slot) * PART;
-  const float* rest = a.parts + (long long)c * 2 * PART;      // part i > 0 is at rest + 2 i PART
-  const auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * PART; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot_of = threadIdx.x / LANES, quad = threadIdx.x % LANES;
-  const int r0 = blockIdx.y * together, some = min(together, rows - r0);
-  // a warp per row: the largest maximum, every part's factor, the sum
-  for (int j = warp; j < some; j += 8) {
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[ROWS * HD + r0 + j]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const float* f = part(i);
-      const float e = exp2f(f[ROWS * HD + r0 + j] - base);
-      weight[i * together + j] = e;
-      sum += e * f[ROWS * (HD + 1) + r0 + j];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[j] = sum, tops[j] = top;
-  }
-  __syncthreads();
-  const int j = slot_of % together, share = slot_of / together, sharing = SLOTS / together;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (j < some) {
-#pragma unroll 8
-    for (int i = share; i < n; i += sharing) {
-      const float4 x = *reinterpret_cast<const float4*>(part(i) + (r0 + j) * HD + quad * 4);
-      const float e = weight[i * together + j];
-      v.x += e * x.x, v.y += e * x.y, v.z += e * x.z, v.w += e * x.w;
-    }
-  }
-  shares[slot_of][quad] = v;
-  __syncthreads();
-  if (share != 0 || j >= some) return;
-  for (int k = 1; k < sharing; ++k) {
-    const float4 x = shares[k * together + j][quad];
-    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-  }
-  const float sum = sums[j], by = sum == 0.f ? 0.f : 1.f / sum;
-  const int q = (head / a.subs) * a.group + (head % a.subs) * a.sub_heads + r0 + j;
-  if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-  *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x * by, v.y * by), Half16<T>::down(v.z * by, v.w * by));
-  if (quad == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (tops[j] + log2f(sum) - SHIFT) * LN2;
 }
 
 struct Plan {
@@ -542,9 +558,9 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   // Few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a head.
   constexpr int slots = 256 / (HD / 4);
   int together = 1;
-  while (p.heads > 32 && together < p.sub_heads && together < slots) together *= 2;
+  while (p.heads > 32 && together < p.sub_heads && together < slots && p.ctas * together * 2 * sizeof(float2) <= 48 * 1024) together *= 2;
   return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.headers, (unsigned)((p.sub_heads + together - 1) / together)), dim3(256),
-                    (size_t)p.ctas * together * 4, s, a, together);
+                    (size_t)p.ctas * together * sizeof(float2), s, a, together);
 }
 
 static bool refused(const FtkPagedAttnDesc* d) {
