@@ -34,7 +34,10 @@ namespace ftk {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;
-constexpr int PA_WHOLE = 8;                  // tiles per head up to which a head is left whole
+// Tiles per head up to which a head is left whole: a second launch and the join cost 3 - 4 us, a tile of a head on its own 0.4 - 0.8.  Whole
+// and split: 12 heads of 8 tiles 8.2 and 8.5 us, of 16 14.1 and 8.6; 32 heads of up to 9 9.7 and 10.7, of up to 17 16.7 and 10.5; with a
+// head for every SM the others fill the time: 256 heads of up to 9 13.0 and 17.7, of up to 17 21.7 and 26.4, of up to 33 38.0 and 36.9.
+constexpr int PA_WHOLE = 9, PA_WHOLE_MANY = 20;
 constexpr int PA_HEADER = 8;                 // ints of a header
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -527,14 +530,14 @@ static Plan plan_of(const FtkPagedAttnDesc& d) {
   p.subs = (int)((group + 15) / 16);
   p.sub_heads = (int)((group + p.subs - 1) / p.subs);
   p.rows = p.sub_heads <= 8 ? 8 : 16;
-  const long long tiles = ((d.table_cols << d.page_shift) + PA_TILE - 1) / PA_TILE;
-  p.split = tiles > PA_WHOLE;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   p.ctas = p.heads = d.B * d.Hkv * p.subs;
   p.headers = p.bytes = 0;
+  const long long tiles = ((d.table_cols << d.page_shift) + PA_TILE - 1) / PA_TILE;
+  p.split = tiles > (p.heads >= sms ? PA_WHOLE_MANY : PA_WHOLE);
   if (p.split) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     p.ctas = (d.hd == 64 && p.rows == 8 ? PaSmem<8, 64>::CTAS : 2ll) * sms;
     p.headers = p.heads < p.ctas ? p.heads : p.ctas;
     p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * p.rows * (d.hd + 2) * 4;

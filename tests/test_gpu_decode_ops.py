@@ -216,6 +216,12 @@ def test_attention(cuda_device, H, Hk, page, hd, dtype):
     close(o, wo, to, "o")
     close(lse, wl, tl, "lse")
     assert bool((o[0] == 0).all())
+    # a table for longer sequences: the heads are cut into pieces
+    wide = torch.full((len(EDGES), 21 * 64 // page + 1), -7, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table[:, : wide.shape[1]]
+    o2, lse2 = D.paged_attention(q, kp, vp, wide, _i32(EDGES))
+    close(o2, wo, to, "o in pieces")
+    close(lse2, wl, tl, "lse in pieces")
     out = torch.full((len(EDGES), H + 2, hd), 7.0, dtype=dtype, device="cuda")
     o2, lse2 = D.paged_attention(q, kp, vp, table, _i32(EDGES), out=out[:, 1:-1])
     assert torch.equal(o2, o) and torch.equal(lse2, lse)
