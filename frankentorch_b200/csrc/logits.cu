@@ -337,7 +337,9 @@ static int launch(const FtkLogitsDesc& d, cudaStream_t s) {
 using namespace ftk;
 
 extern "C" int ftk_logits(const FtkLogitsDesc* d, void* stream) {
-  if (!d || d->L < 0 || d->L > (1 << 30) || d->R <= 0 || d->R > 0x7fffffff || d->V <= 0 || d->V > 0x7fffffff - (1 << 20) || d->R * ((d->V + 63) / 64) > (1ll << 38) || !d->logits || !d->out) return -2;
+  if (!d || !d->logits || !d->out || d->L < 0 || d->L > (1 << 30) || d->R <= 0 || d->R > 0x7fffffff || d->V <= 0 || d->V > 0x7fffffff - (1 << 20) ||
+      d->R * ((d->V + 63) / 64) > (1ll << 38))
+    return -2;
   cudaStream_t s = (cudaStream_t)stream;
   if (d->type == FTK_T_FP32 && d->out_type == FTK_T_FP32) return launch<float, float>(*d, s);
   if (d->type == FTK_T_BF16 && d->out_type == FTK_T_FP32) return launch<__nv_bfloat16, float>(*d, s);

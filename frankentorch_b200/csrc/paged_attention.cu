@@ -7,8 +7,8 @@
 // What bounds it: every key and value is read once, 1 to 16 flops a byte, so it is the copy bandwidth.
 //
 // Work.  A unit is a tile of 64 tokens of one head of the cache with the (up to 16) query heads that share it, so keys and values
-// are read once for the group.  The units of all sequences and heads are one list, of which each of the (two per SM) CTAs takes an
-// equal piece: ragged batches, few long sequences and many short ones all keep every SM busy to the end.  The list is made from
+// are read once for the group.  The units of all sequences and heads are one list, of which each of the CTAs (two or three per SM)
+// takes an equal piece: ragged batches, few long sequences and many short ones all keep every SM busy to the end.  The list is made from
 // the lengths on the device, so a captured launch follows them.  A CTA that has a whole head writes the output; pieces of one are
 // left as (m, l, a) in the call's scratch and joined by a second kernel, always in the order of the tokens.  Where the table is so
 // short that nothing is worth splitting a CTA takes one head and there is no second kernel.
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
   constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 8, NT = HD / 8, KS = HD / 16;
   constexpr int RR = ROWS / 8;
   constexpr float SHIFT = PaShift<T>::value;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(256) unsigned char smem[];      // rows of 256 bytes are addressed by exclusive or
   const FtkPagedAttnDesc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = (int)d.Hkv * a.subs;
   unsigned char* ring = smem + warp * SM::RING;
@@ -558,10 +558,12 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(PA_WARPS * 32), bytes, s, a, status);
   if (rc || !p.split) return rc;
-  // Few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a head.
+  // Few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a head, as far as
+  // shared memory goes.
   constexpr int slots = 256 / (HD / 4);
   int together = 1;
-  while (p.heads > 32 && together < p.sub_heads && together < slots && p.ctas * together * 2 * sizeof(float2) <= 48 * 1024) together *= 2;
+  while (p.heads > 32 && together < p.sub_heads && together < slots && p.ctas * together * 2 * sizeof(float2) <= 40 * 1024)
+    together *= 2;
   return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.headers, (unsigned)((p.sub_heads + together - 1) / together)), dim3(256),
                     (size_t)p.ctas * together * sizeof(float2), s, a, together);
 }

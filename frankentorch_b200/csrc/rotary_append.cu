@@ -45,7 +45,8 @@ struct RotaryShape {
 };
 
 template <typename T, int K, bool INTER>
-__global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ RotaryShape w, int* status) {
+__global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ RotaryShape w,
+                                                            int* status) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int half = (int)(d.turn >> 1), S = (int)d.S;
   // Cosines and sines of two pairs, (c, c', s, s'), as [token][two pairs of an item][items]: the items' threads read 16 bytes side by side

@@ -120,7 +120,8 @@ class GPTDecoder:
             raise ValueError(f"prompts have 1 to {S} tokens, not {lengths}")
         if S > cfg.max_seq and cfg.pos == "learned":
             raise ValueError(f"{S} tokens, the model has {cfg.max_seq} learned positions")
-        for b, n in enumerate(lengths):
+        self._host_lengths = [0] * B            # until the prompts are in
+        for b in range(B):
             cache.release(b)
         for b, n in enumerate(lengths):
             cache.reserve(b, n)
@@ -209,7 +210,7 @@ class GPTDecoder:
         Row ``b`` holds its prompt and what was generated behind it, ``totals[b]`` tokens; the rest of the row is 0.  The penalties,
         ``bias`` and ``allowed`` are those of :func:`~frankentorch_b200.ops.decode.logits_process`; ``allowed`` may be a function of the
         tokens and totals so far.  ``choose`` takes the processed logits ``[batch, vocabulary]`` to the next ids (default: the
-        highest).  A row ends behind ``eos``."""
+        highest).  A row ends behind ``eos``, and where mask and bias leave it no token."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens is positive")
         B, S = ids.shape
@@ -229,13 +230,15 @@ class GPTDecoder:
                                  lengths=totals if penalised else None, prompt_lengths=prompt if penalised else None,
                                  repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=words)
             new = x.argmax(-1) if choose is None else choose(x)
+            if words is not None or bias is not None:
+                live &= x.amax(-1) != float("-inf")
             place = totals.to(torch.int64)[:, None]
             tokens.scatter_(1, place, torch.where(live[:, None], new[:, None], tokens.gather(1, place)))
             totals += live
             if eos is not None:
                 live &= new != eos
-                if i % 32 == 31 and not bool(live.any()):
-                    break
+            if i % 32 == 31 and (eos is not None or words is not None) and not bool(live.any()):
+                break
             if i + 1 < max_new_tokens:
                 logits = self.step(new)
         K.check_status()

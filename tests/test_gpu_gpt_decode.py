@@ -145,17 +145,18 @@ def test_rotary_step_in_a_graph_beside_an_eager_one(cuda_device):
 
 
 @pytest.mark.parametrize("graph", [True, False])
-@pytest.mark.parametrize("pos,heads,page", [("learned", 2, 16), ("rotary", 2, 8), ("rotary", 1, 64)])
-def test_steps_give_the_logits_of_the_whole_sequence(cuda_device, pos, heads, page, graph):
+@pytest.mark.parametrize("pos,heads,page,lengths", [("learned", 2, 16, [1, 17, 40]), ("rotary", 2, 8, [1, 17, 40]),
+                                                    ("rotary", 1, 64, [40, 39, 2]), ("rotary", 2, 32, [40]), ("learned", 1, 4, [1])])
+def test_steps_give_the_logits_of_the_whole_sequence(cuda_device, pos, heads, page, lengths, graph):
     """Ragged prompts, then tokens one by one: at every length the logits of the model over all tokens so far."""
     from frankentorch_b200.models.gpt_decode import GPTDecoder
     from frankentorch_b200.ops import kernels as K
     cfg, _, model = _build(cuda_device, pos, n_head=heads)
     P = _params64(cfg, model)
     g = torch.Generator().manual_seed(4)
-    lengths, new = [1, 17, 40], 12
-    tok = torch.randint(0, cfg.vocab_size, (3, 60), generator=g).to(cuda_device)
-    dec = GPTDecoder(model, 3, 64, page=page, use_cuda_graph=graph)
+    new, B = 12, len(lengths)
+    tok = torch.randint(0, cfg.vocab_size, (B, 60), generator=g).to(cuda_device)
+    dec = GPTDecoder(model, B, 64, page=page, use_cuda_graph=graph)
     for again in range(2):                       # a second batch of prompts takes the pages of the first
         got = [dec.prefill(tok[:, :40], lengths)]
         for i in range(new):
@@ -208,9 +209,35 @@ def test_generation(cuda_device):
         one = tok[:, :1]
         w.scatter_(1, one // 32, torch.ones_like(one) << (one % 32))
         return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
+    # a mask that leaves a row nothing ends it
+    none = words.expand(4, -1).clone()
+    none[2] = 0
+    stuck, totals = dec.generate(ids, lengths, max_new_tokens=6, allowed=none)
+    assert totals.tolist() == [26, 9, 11, 7] and not bool(stuck[2, 11:].any()) and bool((stuck[0, 20:26] % 2 == 1).all())
     same, _ = dec.generate(ids, lengths, max_new_tokens=5, allowed=first_only, bias=torch.zeros(333, device=cuda_device))
     for b, n in enumerate(lengths):
         assert bool((same[b, n: n + 5] == ids[b, 0]).all())
+
+
+def test_a_cache_that_is_too_small(cuda_device):
+    """Pages run out: the call is refused, a smaller one works, and what a refused prefill left is not stepped on."""
+    from frankentorch_b200.models.gpt_decode import CacheFull, GPTDecoder
+    cfg, _, model = _build(cuda_device)
+    ids = torch.zeros(2, 40, dtype=torch.int64, device=cuda_device)
+    dec = GPTDecoder(model, 2, 64, page=8, pages=6)
+    with pytest.raises(CacheFull):
+        dec.prefill(ids)
+    with pytest.raises(ValueError, match="follows a prefill"):
+        dec.step(ids[:, 0])
+    dec.prefill(ids, [16, 20])                   # two and three pages of six
+    for _ in range(4):                           # three each, up to 20 and 24 tokens
+        dec.step(ids[:, 0])
+    with pytest.raises(CacheFull):
+        dec.step(ids[:, 0])
+    with pytest.raises(ValueError, match="made for 64"):
+        dec.generate(ids[:, :8], max_new_tokens=60)
+    tokens, totals = dec.generate(ids[:, :8], max_new_tokens=10)
+    assert totals.tolist() == [18, 18]
 
 
 def test_two_decoders_of_one_model(cuda_device):
