@@ -11,9 +11,10 @@
 // takes an equal piece: ragged batches, few long sequences and many short ones all keep every SM busy to the end.  The list is made from
 // the lengths on the device, so a captured launch follows them.  A CTA that has a whole head writes the output; pieces of one are
 // left as (m, l, a) in the call's scratch and joined by a second kernel, always in the order of the tokens.  Where the table is so
-// short that nothing is worth splitting a CTA takes one head and there is no second kernel.
+// short that nothing is worth splitting a CTA takes one head and there is no second kernel; with an SM for each head it has 8 or 16
+// warps instead of four, since one warp per scheduler needs 1400 cycles for 16 tokens (12 heads of 64, 500 tokens: 5.3 us, 8.1 with four).
 //
-// Inside a CTA each of four warps takes 16 tokens of the tile on its own, through a ring of stages in shared memory that it fills
+// Inside a CTA each of the warps takes 16 tokens of the tile on its own, through a ring of stages in shared memory that it fills
 // with 16-byte asynchronous copies several tiles (and heads, and sequences) ahead: no barrier but the warp's own until the end of a
 // head.  Scores and the product with V are 16 x 8 x 16 matrix instructions of the warp (mma.sync): rows of a tile are the query
 // heads of the group, of which there are too few for a tile of the tensor memory's 128 rows, and a quarter of the warp
@@ -33,11 +34,12 @@ extern "C" int* ftk_status_word(void);
 namespace ftk {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;
-// Tiles per head up to which a head is left whole: a second launch and the join cost 3 - 4 us, a tile of a head on its own 0.4 - 0.8.  Whole
-// and split: 12 heads of 8 tiles 8.2 and 8.5 us, of 16 14.1 and 8.6; 32 heads of up to 9 9.7 and 10.7, of up to 17 16.7 and 10.5; with a
-// head for every SM the others fill the time: 256 heads of up to 9 13.0 and 17.7, of up to 17 21.7 and 26.4, of up to 33 38.0 and 36.9.
-constexpr int PA_WHOLE = 9, PA_WHOLE_MANY = 20;
+constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;      // of a CTA that shares its SM
+// Tiles of 64 tokens up to which a head is left whole: a second launch and the join cost 3 - 4 us, so few heads are cut late, and heads for all
+// SMs fill the time among themselves.  Whole and cut (us), with an SM for each head: 12 heads of 64, 16 tiles 8.1 and 8.6, 32 tiles 13.7
+// and 9.2; 32 heads of 128, up to 17 tiles 13.1 and 10.7; 128 heads of 128, up to 17 13.7 and 16.4, up to 33 22.4 and 25.0; with several
+// heads per SM, 256 of 128, up to 17 21.7 and 26.4, up to 33 38.0 and 36.9.
+__host__ inline long long pa_whole(long long heads, long long sms) { return heads <= sms ? 9 + 28 * heads / sms : 20; }
 constexpr int PA_HEADER = 8;                 // ints of a header
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -84,17 +86,25 @@ struct Place {
   int b, h, t, tiles, n;
 };
 
-// CTAs of an SM, bytes of a warp's ring (four or six stages of 16 tokens of 64 elements, three of 128)
-template <int ROWS, int HD> struct PaSmem {
-  static constexpr int CTAS = HD == 64 && ROWS == 8 ? 3 : 2, RING = CTAS == 3 ? 16 * 1024 : 24 * 1024;
+// W warps of a CTA: CTAs of an SM, bytes of a warp's ring (three to six stages of 16 tokens)
+template <int ROWS, int HD, int W> struct PaSmem {
+  static constexpr int CTAS = W > PA_WARPS ? 1 : (HD == 64 && ROWS == 8 ? 3 : 2);
+  static constexpr int RING = W == 16 ? 12 * 1024 : (CTAS == 3 ? 16 * 1024 : 24 * 1024);
   static constexpr int STAGE = 16 * HD * 4, STAGES = RING / STAGE;
-  static constexpr int MERGE = PA_WARPS * ROWS * 64 * 4;      // accumulators of 64 columns of all warps
-  static constexpr int BYTES = PA_WARPS * RING + MERGE + 2 * PA_WARPS * ROWS * 4 + PA_WARPS * STAGES * 4;
+  static constexpr int MERGE = W * ROWS * 64 * 4;             // accumulators of 64 columns of all warps
+  static constexpr bool OWN = W <= PA_WARPS;                  // in memory of their own, or in the rings of a head that is through
+  static constexpr int BYTES = W * RING + (OWN ? MERGE : 0) + 2 * W * ROWS * 4 + W * STAGES * 4;
+  static_assert(OWN || MERGE <= W * RING, "the accumulators fit the rings");
+  static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
 };
+// Warps of a CTA that has its SM and one head for itself: as many as registers and rings allow
+template <int ROWS, int HD> constexpr int PA_ALONE = HD == 64 && ROWS == 8 ? 16 : 8;
 
-template <typename T, int HD, int ROWS, bool SPLIT>
-__global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
-  typedef PaSmem<ROWS, HD> SM;
+template <typename T, int HD, int ROWS, bool SPLIT, int W>
+__global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
+  typedef PaSmem<ROWS, HD, W> SM;
+  static_assert(!SPLIT || SM::OWN, "a piece goes on while the parts are joined");
+  constexpr int TILE = 16 * W;
   constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 8, NT = HD / 8, KS = HD / 16;
   constexpr int RR = ROWS / 8;
   constexpr float SHIFT = PaShift<T>::value;
@@ -102,9 +112,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
   const FtkPagedAttnDesc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = (int)d.Hkv * a.subs;
   unsigned char* ring = smem + warp * SM::RING;
-  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * SM::RING);
-  float* stat = merge + SM::MERGE / 4;                                     // [2][warps][ROWS]
-  unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * PA_WARPS * ROWS) + warp * STAGES;
+  float* merge = reinterpret_cast<float*>(smem + (SM::OWN ? W * SM::RING : 0));
+  float* stat = reinterpret_cast<float*>(smem + W * SM::RING + (SM::OWN ? SM::MERGE : 0));                                     // [2][warps][ROWS]
+  unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * W * ROWS) + warp * STAGES;
   const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
   const auto length = [&](int b) {
     bool bad;
@@ -117,20 +127,31 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
   pdl_wait();
   pdl_trigger();
 
+  constexpr int AHEAD = STAGES - 1;     // tiles whose pages are known before they are asked for
+  const bool one_page = table.shift >= 4;
+  const int tok_of = warp * 16 + (one_page ? 0 : lane & 15);      // of a tile: the token whose page this lane looks up
+
   // ---- this CTA's piece of the list
   Place p;
   long long left;                       // tiles of the piece
   long long first_unit = 0, total = 0, per = 0;
+  int entry[AHEAD];
   if (!SPLIT) {
     p.b = blockIdx.x / heads, p.h = blockIdx.x % heads, p.t = 0;
-    p.n = length(p.b), p.tiles = (p.n + PA_TILE - 1) / PA_TILE;
+    // the first entries of the table along with the length that says whether they count
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const long long col = (i * TILE + tok_of) >> table.shift;
+      entry[i] = col < table.cols ? table.table[p.b * table.stride + col] : -1;
+    }
+    p.n = length(p.b), p.tiles = (p.n + TILE - 1) / TILE;
     left = p.tiles;
   } else {
     // Every warp for itself: tiles in front of each lane's share of the sequences, then the sequence in which the piece begins
     const int each = ((int)d.B + 31) / 32, b0 = min((int)d.B, lane * each), b1 = min((int)d.B, b0 + each);
     long long mine = 0;
 #pragma unroll 4
-    for (int b = b0; b < b1; ++b) mine += (length(b) + PA_TILE - 1) / PA_TILE;
+    for (int b = b0; b < b1; ++b) mine += (length(b) + TILE - 1) / TILE;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -148,7 +169,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
     const bool here = front <= first_unit && first_unit < upto * heads;
     if (here) {
       for (int b = b0; b < b1; ++b) {
-        const int n = length(b), tiles = (n + PA_TILE - 1) / PA_TILE;
+        const int n = length(b), tiles = (n + TILE - 1) / TILE;
         const long long in = first_unit - front;
         if (in < (long long)tiles * heads) {
           p = {b, (int)(in / tiles), (int)(in % tiles), tiles, n};
@@ -164,7 +185,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
 
   // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences, and the table is read from
   // another one as far ahead of that
-  constexpr int AHEAD = STAGES - 1;
   const auto advance = [&](Place& x, long long& more) {
     --more;
     if (++x.t == x.tiles) {
@@ -172,7 +192,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
       if (++x.h == heads) {
         x.h = 0;
         x.tiles = 0;
-        while (more > 0 && x.tiles == 0 && x.b + 1 < (int)d.B) x.n = length(++x.b), x.tiles = (x.n + PA_TILE - 1) / PA_TILE;
+        while (more > 0 && x.tiles == 0 && x.b + 1 < (int)d.B) x.n = length(++x.b), x.tiles = (x.n + TILE - 1) / TILE;
       }
     }
   };
@@ -180,15 +200,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
   long long to_load = left, to_look = left;
   // Pages of the next tiles.  A page of 16 rows or more holds all of a warp's part of a tile; of smaller ones lane j < 16 has token j's.
   int page_of[AHEAD] = {};
-  const bool one_page = table.shift >= 4;
+  const auto checked = [&](long long page) {
+    if (page >= 0 && page < table.n_pages) return (int)page;
+    ft_index_ok(-1, 1, status);
+    return -1;
+  };
   const auto look = [&]() {
     int page = -1;
     if (to_look > 0) {
-      const int tok = g.t * PA_TILE + warp * 16 + (one_page ? 0 : lane & 15);
-      if (tok < g.n) {
-        page = (int)paged_page(table, g.b, tok);
-        if (page < 0) ft_index_ok(-1, 1, status);
-      }
+      const int tok = g.t * TILE + tok_of;
+      if (tok < g.n) page = checked(paged_page(table, g.b, tok));
       advance(g, to_look);
     }
     return page;
@@ -204,7 +225,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
     for (int i = 0; i + 1 < AHEAD; ++i) page_of[i] = page_of[i + 1];
     page_of[AHEAD - 1] = look();
     if (to_load > 0) {
-      const int head = f.h / a.subs, tok0 = f.t * PA_TILE + warp * 16;
+      const int head = f.h / a.subs, tok0 = f.t * TILE + warp * 16;
       const T* kb = (const T*)d.k_pages + head * d.kp_hs;
       const T* vb = (const T*)d.v_pages + head * d.vp_hs;
       const uint32_t dst = ring_s + stage * STAGE + lane_at;
@@ -242,7 +263,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
     copy_commit();
   };
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) page_of[i] = look();
+  for (int i = 0; i < AHEAD; ++i) {
+    if (SPLIT) {
+      page_of[i] = look();
+    } else {
+      page_of[i] = to_look > 0 && g.t * TILE + tok_of < g.n ? checked(entry[i]) : -1;
+      if (to_look > 0) advance(g, to_look);
+    }
+  }
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load(s);
 
@@ -354,7 +382,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if ((lane & 3) == 0) {
         stat[warp * ROWS + r * 8 + r0] = m[r];
-        stat[(PA_WARPS + warp) * ROWS + r * 8 + r0] = l[r];
+        stat[(W + warp) * ROWS + r * 8 + r0] = l[r];
       }
     }
     const bool whole = begun && p.t == p.tiles;
@@ -366,7 +394,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
     for (int r = 0; r < RR; ++r) {
       float top = m[r];
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, stat[w * ROWS + r * 8 + r0]);
+      for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w * ROWS + r * 8 + r0]);
       scale[r] = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
     }
 #pragma unroll
@@ -383,18 +411,18 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
         }
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < rows * 32; i += PA_WARPS * 32) {
+      for (int i = threadIdx.x; i < rows * 32; i += W * 32) {
         const int row = i >> 5, in = (i & 31) * 2, col = half * 64 + in;
         float2 v = make_float2(0.f, 0.f);
         float top = stat[row], sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < PA_WARPS; ++w) top = fmaxf(top, stat[w * ROWS + row]);
+        for (int w = 1; w < W; ++w) top = fmaxf(top, stat[w * ROWS + row]);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
+        for (int w = 0; w < W; ++w) {
           const float2 x = *reinterpret_cast<const float2*>(merge + (w * ROWS + row) * 64 + in);
           v.x += x.x, v.y += x.y;
-          sum += exp2f(stat[w * ROWS + row] - base) * stat[(PA_WARPS + w) * ROWS + row];
+          sum += exp2f(stat[w * ROWS + row] - base) * stat[(W + w) * ROWS + row];
         }
         if (!SPLIT || whole) {
           const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -424,7 +452,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaSmem<ROWS, HD>::CTAS) paged_a
     if (++p.h == heads) {
       p.h = 0;
       p.tiles = 0;
-      while (p.tiles == 0 && p.b + 1 < (int)d.B) p.n = length(++p.b), p.tiles = (p.n + PA_TILE - 1) / PA_TILE;
+      while (p.tiles == 0 && p.b + 1 < (int)d.B) p.n = length(++p.b), p.tiles = (p.n + TILE - 1) / TILE;
     }
     begin();
   }
@@ -521,7 +549,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
 
 struct Plan {
   int subs, sub_heads, rows;
-  bool split;
+  bool split, alone;               // heads cut into pieces; a CTA per SM, for few heads
   long long ctas, heads, headers, bytes;      // heads: of all sequences, a part of a group counting as one
 };
 static Plan plan_of(const FtkPagedAttnDesc& d) {
@@ -536,9 +564,10 @@ static Plan plan_of(const FtkPagedAttnDesc& d) {
   p.ctas = p.heads = d.B * d.Hkv * p.subs;
   p.headers = p.bytes = 0;
   const long long tiles = ((d.table_cols << d.page_shift) + PA_TILE - 1) / PA_TILE;
-  p.split = tiles > (p.heads >= sms ? PA_WHOLE_MANY : PA_WHOLE);
+  p.alone = p.heads <= sms;
+  p.split = tiles > pa_whole(p.heads, sms);
   if (p.split) {
-    p.ctas = (d.hd == 64 && p.rows == 8 ? PaSmem<8, 64>::CTAS : 2ll) * sms;
+    p.ctas = (d.hd == 64 && p.rows == 8 ? PaSmem<8, 64, PA_WARPS>::CTAS : 2ll) * sms;
     p.headers = p.heads < p.ctas ? p.heads : p.ctas;
     p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * p.rows * (d.hd + 2) * 4;
   }
@@ -550,9 +579,14 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   PagedAttn a = {d, (int)(d.Hq / d.Hkv), p.subs, p.sub_heads, p.heads < p.ctas, (int*)scratch, nullptr};
   a.parts = (float*)((char*)scratch + p.headers * PA_HEADER * 4);
   int* status = ftk_status_word();
-  const int bytes = PaSmem<ROWS, HD>::BYTES;
-  static_assert(PaSmem<ROWS, HD>::CTAS * (PaSmem<ROWS, HD>::BYTES + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
-  const auto whole = paged_attn_kernel<T, HD, ROWS, false>, split = paged_attn_kernel<T, HD, ROWS, true>;
+  if (!p.split && p.alone) {
+    constexpr int W = PA_ALONE<ROWS, HD>, bytes = PaSmem<ROWS, HD, W>::BYTES;
+    const auto kernel = paged_attn_kernel<T, HD, ROWS, false, W>;
+    const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return rc ? rc : launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(W * 32), bytes, s, a, status);
+  }
+  constexpr int bytes = PaSmem<ROWS, HD, PA_WARPS>::BYTES;
+  const auto whole = paged_attn_kernel<T, HD, ROWS, false, PA_WARPS>, split = paged_attn_kernel<T, HD, ROWS, true, PA_WARPS>;
   const auto kernel = p.split ? split : whole;
   int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (rc) return rc;

@@ -10,7 +10,7 @@ and no logits processing; shapes, masks and empty rows follow its attention (ft-
 
 A paged cache is two tensors of pages, ``[pages, heads, page, hd]`` (``page`` a power of two), and a table ``[B, columns]`` of
 page numbers (int32): position ``p`` of sequence ``b`` is row ``p % page`` of page ``table[b, p // page]``.  Table entries behind the
-last position that a call touches are not read.  Rows of ``hd`` elements are contiguous and start on 16 bytes; everything else
+last position that a call touches have no meaning for it.  Rows of ``hd`` elements are contiguous and start on 16 bytes; everything else
 may be strided.  Lengths, positions and counts are int32 on the device, so a captured graph follows them.
 
 As everywhere in :mod:`~frankentorch_b200.ops.kernels`, a call enqueues on the current stream of its tensors' device and
