@@ -14,7 +14,7 @@ last position that a call touches have no meaning for it.  Rows of ``hd`` elemen
 may be strided.  Lengths, positions and counts are int32 on the device, so a captured graph follows them.
 
 As everywhere in :mod:`~frankentorch_b200.ops.kernels`, a call enqueues on the current stream of its tensors' device and
-returns; arguments that the host can judge are refused with :class:`~.kernels.KernelError`; a page, token or length out of range
+returns; arguments that the host can check are refused with :class:`~.kernels.KernelError`; a page, token or length out of range
 on the device is reported by :func:`~.kernels.check_status`, and what it leads to is not read and not written.  A call keeps
 nothing: its scratch is its own, so calls of several streams, threads and captured graphs do not meet, and the same call gives
 the same bits.  (The attention cuts a sequence's heads by the work of the whole call: beside other sequences its last bits may
