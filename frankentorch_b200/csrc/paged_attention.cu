@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
 
   // ---- this CTA's piece of the list
   Place p;
-  long long left;                       // tiles of the piece
+  int left;                             // tiles of the piece (counters of 64 bits took 5 % more for heads of 64)
   long long first_unit = 0, total = 0, per = 0;
   int entry[AHEAD];
   if (!SPLIT) {
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
     total = __shfl_sync(0xffffffffu, upto, 31) * heads;
     per = max((total + gridDim.x - 1) / gridDim.x, 2ll);      // a part of less than two tiles costs more to join than it saves
     first_unit = per * blockIdx.x;
-    left = min(per, total - first_unit);
+    left = (int)min(per, total - first_unit);
     if (!a.by_head && threadIdx.x == 0) a.header[(long long)blockIdx.x * PA_HEADER] = -1;
     if (left <= 0) return;
     long long front = (upto - mine) * heads;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
 
   // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences, and the table is read from
   // another one as far ahead of that
-  const auto advance = [&](Place& x, long long& more) {
+  const auto advance = [&](Place& x, int& more) {
     --more;
     if (++x.t == x.tiles) {
       x.t = 0;
@@ -197,19 +197,17 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
     }
   };
   Place f = p, g = p;
-  long long to_load = left, to_look = left;
+  int to_load = left, to_look = left;
   // Pages of the next tiles.  A page of 16 rows or more holds all of a warp's part of a tile; of smaller ones lane j < 16 has token j's.
   int page_of[AHEAD] = {};
-  const auto checked = [&](long long page) {
-    if (page >= 0 && page < table.n_pages) return (int)page;
-    ft_index_ok(-1, 1, status);
-    return -1;
-  };
   const auto look = [&]() {
     int page = -1;
     if (to_look > 0) {
       const int tok = g.t * TILE + tok_of;
-      if (tok < g.n) page = checked(paged_page(table, g.b, tok));
+      if (tok < g.n) {
+        page = (int)paged_page(table, g.b, tok);
+        if (page < 0) ft_index_ok(-1, 1, status);
+      }
       advance(g, to_look);
     }
     return page;
@@ -267,7 +265,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
     if (SPLIT) {
       page_of[i] = look();
     } else {
-      page_of[i] = to_look > 0 && g.t * TILE + tok_of < g.n ? checked(entry[i]) : -1;
+      page_of[i] = to_look > 0 && g.t * TILE + tok_of < g.n && ft_index_ok(entry[i], table.n_pages, status) ? entry[i] : -1;
       if (to_look > 0) advance(g, to_look);
     }
   }
@@ -397,22 +395,24 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
       for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w * ROWS + r * 8 + r0]);
       scale[r] = exp2f(m[r] - (top == -INFINITY ? 0.f : top));
     }
+    // all columns of a few rows at once, else 64 of all rows
+    const int cols = rows * HD <= ROWS * 64 ? HD : 64;
+    for (int from = 0; from < HD; from += cols) {
 #pragma unroll
-    for (int half = 0; half < HD / 64; ++half) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float* to = merge + (warp * ROWS + r0) * 64 + i * 8 + c0;
-        const float* c = acc[half * 8 + i];
+      for (int i = 0; i < NT; ++i) {
+        if (i * 8 < from || i * 8 >= from + cols) continue;
+        float* to = merge + (warp * rows + r0) * cols + i * 8 - from + c0;
+        const float* c = acc[i];
         if (ROWS == 16) {
-          *reinterpret_cast<float2*>(to) = make_float2(c[0] * scale[0], c[1] * scale[0]);
-          *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(c[2] * scale[RR - 1], c[3] * scale[RR - 1]);
+          if (r0 < rows) *reinterpret_cast<float2*>(to) = make_float2(c[0] * scale[0], c[1] * scale[0]);
+          if (r0 + 8 < rows) *reinterpret_cast<float2*>(to + 8 * cols) = make_float2(c[2] * scale[RR - 1], c[3] * scale[RR - 1]);
         } else {
-          *reinterpret_cast<float2*>(to) = make_float2((c[0] + c[2]) * scale[0], (c[1] + c[3]) * scale[0]);
+          if (r0 < rows) *reinterpret_cast<float2*>(to) = make_float2((c[0] + c[2]) * scale[0], (c[1] + c[3]) * scale[0]);
         }
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < rows * 32; i += W * 32) {
-        const int row = i >> 5, in = (i & 31) * 2, col = half * 64 + in;
+      for (int i = threadIdx.x; i < rows * cols / 2; i += W * 32) {
+        const int row = i / (cols / 2), in = (i % (cols / 2)) * 2, col = from + in;
         float2 v = make_float2(0.f, 0.f);
         float top = stat[row], sum = 0.f;
 #pragma unroll
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float2 x = *reinterpret_cast<const float2*>(merge + (w * ROWS + row) * 64 + in);
+          const float2 x = *reinterpret_cast<const float2*>(merge + (w * rows + row) * cols + in);
           v.x += x.x, v.y += x.y;
           sum += exp2f(stat[w * ROWS + row] - base) * stat[(W + w) * ROWS + row];
         }
@@ -605,7 +605,8 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
 static bool refused(const FtkPagedAttnDesc* d) {
   return !d || d->B <= 0 || d->B > (1 << 30) || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > (1 << 20) || (d->hd != 64 && d->hd != 128) ||
          (d->type != FTK_T_BF16 && d->type != FTK_T_FP16) || d->page_shift < 0 || d->page_shift > 30 || d->table_cols <= 0 ||
-         d->table_cols > (0x7fffff00ll >> d->page_shift) || d->n_pages <= 0 || d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff;
+         d->table_cols > (0x7fffff00ll >> d->page_shift) || d->n_pages <= 0 || d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff ||
+         d->B * d->Hq * (((d->table_cols << d->page_shift) >> 6) + 1) > (1ll << 38);      // a CTA counts its tiles in 32 bits
 }
 
 }  // namespace ftk
