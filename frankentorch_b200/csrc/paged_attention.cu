@@ -20,7 +20,8 @@
 // heads of the group, of which there are too few for a tile of the tensor memory's 128 rows, and a quarter of the warp
 // instructions' rate is enough to keep up with the memory.  Probabilities are needed in 16 bits there; rounding them once would
 // cost as much accuracy as the rounding of the output, so each is split into two 16-bit halves, p = hi + lo with an error of
-// 2^-17: for groups of up to 8 heads the lo halves are the rows 8 to 15 of the same instruction, which are idle otherwise.
+// 2^-17: for groups of up to 8 heads the lo halves are the rows 8 to 15 of the same instruction, which are idle otherwise.  A lo of
+// 0 makes NaN of an infinite value, so elements that end as NaN are added up again with undivided probabilities (pa_infinite()).
 #include <math.h>
 
 #include "ft_sm100.cuh"
@@ -99,6 +100,42 @@ template <int ROWS, int HD, int W> struct PaSmem {
 };
 // Warps of a CTA that has its SM and one head for itself: as many as registers and rings allow
 template <int ROWS, int HD> constexpr int PA_ALONE = HD == 64 && ROWS == 8 ? 16 : 8;
+
+// An element of the output whose column has infinities or NaN among the values of tokens [t, end), as a sum of those alone with their
+// whole probabilities: exp2(x - base), positive for every score that fp32 can tell from the maximum.  `was` where there are none: NaN
+// came from elsewhere.  `q`: the query; `k`, `v`: the head's first row of the cache, `v` from the element's column on.  Nobody comes here
+// but with NaN.
+template <typename T, int HD>
+__device__ __forceinline__ float pa_infinite(const FtkPagedAttnDesc& d, const int b, const T* q, const T* k, const T* v, const int t, const int end,
+                                          const float base, const float was) {
+  constexpr int AT_ONCE = 8;
+  const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
+  const float sc = (float)d.scale * LOG2E;
+  float sum = 0.f;
+  bool some = false;
+#pragma unroll 1
+  for (int from = t; from < end; from += AT_ONCE) {
+    unsigned odd = 0;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const long long page = from + i < end ? paged_page(table, b, from + i) : -1;
+      const float y = page < 0 ? 0.f : Half16<T>::one(v[page * d.vp_ps + paged_row(table, from + i) * d.vp_rs]);
+      odd |= isfinite(y) ? 0u : 1u << i;
+    }
+#pragma unroll 1
+    for (; odd; odd &= odd - 1) {
+      const int at = from + __ffs(odd) - 1;
+      const long long page = paged_page(table, b, at), row = paged_row(table, at);
+      const T* key = k + page * d.kp_ps + row * d.kp_rs;
+      float x = 0.f;
+#pragma unroll 1
+      for (int e = 0; e < HD; ++e) x += Half16<T>::one(q[e]) * Half16<T>::one(key[e]);
+      sum += exp2f(x * sc - base + PaShift<T>::value) * Half16<T>::one(v[page * d.vp_ps + row * d.vp_rs]);
+      some = true;
+    }
+  }
+  return some ? sum : was;
+}
 
 template <typename T, int HD, int ROWS, bool SPLIT, int W>
 __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttn a, int* status) {
@@ -423,6 +460,15 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
           const float2 x = *reinterpret_cast<const float2*>(merge + (w * rows + row) * cols + in);
           v.x += x.x, v.y += x.y;
           sum += exp2f(stat[w * ROWS + row] - base) * stat[(W + w) * ROWS + row];
+        }
+        if (sum == sum && (v.x != v.x || v.y != v.y)) {
+          const int kv = p.h / a.subs, start = begun ? 0 : p.t - ((int)min(per, total - first_unit) - left);      // the piece's first tile
+          const T* qr = (const T*)d.q + p.b * d.q_bs + (first + row) * d.q_hs;
+          const T* kr = (const T*)d.k_pages + kv * d.kp_hs;
+          const T* vr = (const T*)d.v_pages + kv * d.vp_hs + col;
+          const int end = min(p.n, p.t * TILE);
+          if (v.x != v.x) v.x = pa_infinite<T, HD>(d, p.b, qr, kr, vr, start * TILE, end, base, v.x);
+          if (v.y != v.y) v.y = pa_infinite<T, HD>(d, p.b, qr, kr, vr + 1, start * TILE, end, base, v.y);
         }
         if (!SPLIT || whole) {
           const float by = sum == 0.f ? 0.f : 1.f / sum;

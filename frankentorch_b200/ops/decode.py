@@ -72,7 +72,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q`` is ``[B, H, hd]`` (bf16 or fp16, ``hd`` 64 or 128), ``H`` a multiple of the cache's heads, which groups of ``H / Hkv``
     neighbouring query heads share.  ``o`` is ``[B, H, hd]``, ``lse`` fp32 ``[B, H]`` (natural logarithm).  A sequence of no tokens
     has ``o = 0`` and ``lse = -inf``.  ``scale`` is ``1 / sqrt(hd)`` where it is not given.  What stands in the cache behind
-    ``lengths[b]`` has no influence, NaN included."""
+    ``lengths[b]`` has no influence, NaN included; an infinite value before it is infinity in its element of ``o``, NaN beside one of
+    the other sign or where its token has no weight (a score of ``-inf``, or so far below the largest that fp32 has 0 for it)."""
     return _lib.bind().paged_attention(q, k_pages, v_pages, table, lengths, scale, out)
 
 
