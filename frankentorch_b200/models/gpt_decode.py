@@ -109,8 +109,8 @@ class GPTDecoder:
 
     # ------------------------------------------------------------------ prompts
     def prefill(self, ids: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
-        """Take the prompts ``ids`` (int64 ``[batch, S]``, the first ``lengths[b]`` of row ``b``) into an empty cache; returns the
-        logits behind each prompt's last token, fp32 ``[batch, padded vocabulary]``."""
+        """Take the prompts ``ids`` (int64 ``[batch, S]``, the first ``lengths[b]`` of row ``b``; what stands behind them need not be a
+        token) into an empty cache; returns the logits behind each prompt's last token, fp32 ``[batch, padded vocabulary]``."""
         cfg, cache = self.cfg, self.cache
         B, S = ids.shape
         lengths = [S] * B if lengths is None else [int(n) for n in lengths]
@@ -125,8 +125,9 @@ class GPTDecoder:
             cache.release(b)
         for b, n in enumerate(lengths):
             cache.reserve(b, n)
-        ids = ids.to(self.device, torch.int64).contiguous()
         counts = torch.tensor(lengths, dtype=torch.int32, device=self.device)
+        ids = ids.to(self.device, torch.int64)
+        ids = torch.where(torch.arange(S, device=self.device)[None, :] < counts[:, None], ids, 0)
         start = torch.zeros_like(counts)
         H, hd, d = cfg.n_head, self.hd, cfg.d_model
         x = K.embedding_fwd(ids, self._w("wte.weight"), self._w("wpe.weight") if cfg.pos == "learned" else None, S)

@@ -77,3 +77,26 @@ def test_rotary_model_has_no_position_table():
         _model(pos="none")
     with pytest.raises(ValueError, match="learned positions only"):
         rotary.cfg.require_learned_positions("another model")
+
+
+class _Seen(Exception):
+    pass
+
+
+@pytest.mark.parametrize("padding", [-1, -100, 100, 2 ** 40])
+def test_prompts_are_embedded_without_their_padding(monkeypatch, padding):
+    """What stands behind a prompt's tokens need not be a token: the model sees 0 there, the caller's tensor stays."""
+    from frankentorch_b200.models import gpt_decode
+
+    def embedding(ids, *a):
+        raise _Seen(ids.clone())
+    monkeypatch.setattr(gpt_decode.K, "embedding_fwd", embedding)
+    ids = torch.tensor([[5, 6, 7, 8], [9, padding, padding, padding], [1, 2, padding, padding]])
+    held = ids.clone()
+    d = GPTDecoder(_model(), 3, 32, page=16)
+    with pytest.raises(_Seen) as e:
+        d.prefill(ids, [4, 1, 2])
+    assert e.value.args[0].tolist() == [[5, 6, 7, 8], [9, 0, 0, 0], [1, 2, 0, 0]] and torch.equal(ids, held)
+    with pytest.raises(_Seen) as e:
+        d.prefill(ids.clamp(0, 9).to(torch.int32))                     # no lengths: all of them are tokens
+    assert e.value.args[0].tolist() == ids.clamp(0, 9).tolist() and e.value.args[0].dtype == torch.int64

@@ -259,3 +259,23 @@ def test_two_decoders_of_one_model(cuda_device):
     for a, b in zip(alone, both):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("pos", ["learned", "rotary"])
+@pytest.mark.parametrize("padding", [-1, -100, 10 ** 12])
+def test_padding_that_is_no_token(cuda_device, pos, padding):
+    """Ragged prompts padded with what is in no vocabulary: the tokens of the same prompts padded with 0, and nothing reported."""
+    from frankentorch_b200.models.gpt_decode import GPTDecoder
+    from frankentorch_b200.ops import kernels as K
+    cfg, _, model = _build(cuda_device, pos)
+    g = torch.Generator().manual_seed(11)
+    lengths = [9, 1, 4]
+    ids = torch.randint(0, cfg.vocab_size, (3, 9), generator=g).to(cuda_device)
+    behind = torch.arange(9, device=cuda_device)[None, :] >= torch.tensor(lengths, device=cuda_device)[:, None]
+    dec = GPTDecoder(model, 3, 40, page=8)
+    want = dec.generate(ids.masked_fill(behind, 0), lengths, max_new_tokens=12, repetition=1.2)
+    got = dec.generate(ids.masked_fill(behind, padding), lengths, max_new_tokens=12, repetition=1.2)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    first = dec.prefill(ids.masked_fill(behind, padding), lengths)
+    K.check_status()
+    assert torch.equal(first, dec.prefill(ids.masked_fill(behind, 0), lengths))
