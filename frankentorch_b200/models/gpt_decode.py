@@ -127,7 +127,7 @@ class GPTDecoder:
             cache.reserve(b, n)
         counts = torch.tensor(lengths, dtype=torch.int32, device=self.device)
         ids = ids.to(self.device, torch.int64)
-        ids = torch.where(torch.arange(S, device=self.device)[None, :] < counts[:, None], ids, 0)
+        ids = torch.where(torch.arange(S, device=self.device)[None, :] < counts[:, None], ids, 0).contiguous()
         start = torch.zeros_like(counts)
         H, hd, d = cfg.n_head, self.hd, cfg.d_model
         x = K.embedding_fwd(ids, self._w("wte.weight"), self._w("wpe.weight") if cfg.pos == "learned" else None, S)

@@ -100,3 +100,19 @@ def test_prompts_are_embedded_without_their_padding(monkeypatch, padding):
     with pytest.raises(_Seen) as e:
         d.prefill(ids.clamp(0, 9).to(torch.int32))                     # no lengths: all of them are tokens
     assert e.value.args[0].tolist() == ids.clamp(0, 9).tolist() and e.value.args[0].dtype == torch.int64
+
+
+def test_prompts_of_any_layout(monkeypatch):
+    """The embedding reads ids one after the other: transposed, strided and broadcast prompts arrive in that order."""
+    from frankentorch_b200.models import gpt_decode
+
+    def embedding(ids, *a):
+        raise _Seen(ids)
+    monkeypatch.setattr(gpt_decode.K, "embedding_fwd", embedding)
+    d = GPTDecoder(_model(), 3, 32, page=16)
+    for ids in (torch.arange(12).view(4, 3).t(), torch.arange(24).view(3, 8)[:, ::2], torch.arange(4).expand(3, 4)):
+        for lengths in (None, [4, 1, 2]):
+            with pytest.raises(_Seen) as e:
+                d.prefill(ids, lengths)
+            got = e.value.args[0]
+            assert got.is_contiguous() and [r[:1] for r in got.tolist()] == [r[:1] for r in ids.tolist()]
