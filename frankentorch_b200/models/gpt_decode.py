@@ -211,7 +211,8 @@ class GPTDecoder:
         Row ``b`` holds its prompt and what was generated behind it, ``totals[b]`` tokens; the rest of the row is 0.  The penalties,
         ``bias`` and ``allowed`` are those of :func:`~frankentorch_b200.ops.decode.logits_process`; ``allowed`` may be a function of the
         tokens and totals so far.  ``choose`` takes the processed logits ``[batch, vocabulary]`` to the next ids (default: the
-        highest).  A row ends behind ``eos``, and where mask and bias leave it no token."""
+        highest).  A row ends behind ``eos``, and where mask and bias leave it no token; with a mask or a bias ``choose`` gets
+        zeros for the rows that have ended, and what it returns for them is not used."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens is positive")
         B, S = ids.shape
@@ -230,15 +231,17 @@ class GPTDecoder:
             x = D.logits_process(logits, vocab=self.cfg.vocab_size, tokens=tokens if penalised else None,
                                  lengths=totals if penalised else None, prompt_lengths=prompt if penalised else None,
                                  repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=words)
-            new = x.argmax(-1) if choose is None else choose(x)
             if words is not None or bias is not None:
                 live &= x.amax(-1) != float("-inf")
+                if choose is not None:          # a sampler would make NaN of a row of -inf
+                    x = torch.where(live[:, None], x, 0.0)
+            new = torch.where(live, x.argmax(-1) if choose is None else choose(x), 0)
             place = totals.to(torch.int64)[:, None]
             tokens.scatter_(1, place, torch.where(live[:, None], new[:, None], tokens.gather(1, place)))
             totals += live
             if eos is not None:
                 live &= new != eos
-            if i % 32 == 31 and (eos is not None or words is not None) and not bool(live.any()):
+            if i % 32 == 31 and (eos is not None or words is not None or bias is not None) and not bool(live.any()):
                 break
             if i + 1 < max_new_tokens:
                 logits = self.step(new)

@@ -116,3 +116,90 @@ def test_prompts_of_any_layout(monkeypatch):
                 d.prefill(ids, lengths)
             got = e.value.args[0]
             assert got.is_contiguous() and [r[:1] for r in got.tolist()] == [r[:1] for r in ids.tolist()]
+
+
+def _stub_decoder(monkeypatch, logits):
+    """A decoder whose model gives the same ``logits`` at every step, and the ids that its steps get."""
+    from frankentorch_b200.models import gpt_decode
+    B, V = logits.shape
+    d = GPTDecoder(_model(vocab_size=V), B, 200, page=16, use_cuda_graph=False) if V > 32 else \
+        GPTDecoder(_model(vocab_size=V, pos="rotary"), B, 200, page=16, use_cuda_graph=False)
+    steps = []
+
+    def prefill(ids, lengths=None):
+        n = [ids.shape[1]] * B if lengths is None else list(lengths)
+        d._host_lengths = n
+        d.lengths.copy_(torch.tensor(n))
+        return logits.clone()
+
+    def step(ids):
+        steps.append(ids.clone())
+        return logits.clone()
+
+    def process(x, *, vocab, bias=None, allowed=None, **kw):
+        x = x[:, :vocab].clone() if bias is None else x[:, :vocab] + bias
+        if allowed is not None:
+            c = torch.arange(vocab)
+            x = x.masked_fill(((allowed.expand(B, -1)[:, c // 32] >> (c % 32)) & 1) == 0, float("-inf"))
+        return x
+    monkeypatch.setattr(d, "prefill", prefill)
+    monkeypatch.setattr(d, "step", step)
+    monkeypatch.setattr(gpt_decode.D, "logits_process", process)
+    monkeypatch.setattr(gpt_decode.K, "check_status", lambda: None)
+    return d, steps
+
+
+def _sampler(seen):
+    def choose(x):
+        assert bool(x.isfinite().any(-1).all()) and not bool(x.isnan().any()), "a row without a choice"
+        seen.append(x.clone())
+        return torch.multinomial(torch.softmax(x, -1), 1)[:, 0]
+    return choose
+
+
+def test_rows_without_a_choice_are_not_sampled(monkeypatch):
+    """``choose`` gets rows that have something to choose from: a sampler would turn the others into NaN.  What it returns for a
+    row that has ended goes nowhere."""
+    V, S = 20, 3
+    logits = torch.randn(4, V, generator=torch.Generator().manual_seed(0))
+    words = torch.full((4, 1), (1 << V) - 1, dtype=torch.int32)
+    words[2] = 0                                           # nothing, from the first token on
+    seen = []
+    d, steps = _stub_decoder(monkeypatch, logits)
+    tokens, totals = d.generate(torch.ones(4, S, dtype=torch.int64), max_new_tokens=5, allowed=words, choose=_sampler(seen))
+    assert totals.tolist() == [8, 8, 3, 8] and not bool(tokens[2, S:].any())
+    assert len(seen) == 5 and torch.equal(seen[0][[0, 1, 3]], logits[[0, 1, 3]])
+    assert all(0 <= int(i) < V for s in steps for i in s) and all(int(s[2]) == 0 for s in steps)
+    # a bias that leaves nothing
+    bias = torch.zeros(4, V)
+    bias[1] = float("-inf")
+    d, _ = _stub_decoder(monkeypatch, logits)
+    tokens, totals = d.generate(torch.ones(4, S, dtype=torch.int64), max_new_tokens=5, bias=bias, choose=_sampler([]))
+    assert totals.tolist() == [8, 3, 8, 8]
+    # a function that allows nothing from a row's fifth token on: it ended there, and stays so
+    def grammar(tok, tot):
+        return torch.where(tot[:, None] < torch.tensor([[9], [5], [9], [4]]), (1 << V) - 1, 0).to(torch.int32)
+    d, steps = _stub_decoder(monkeypatch, logits)
+    tokens, totals = d.generate(torch.ones(4, S, dtype=torch.int64), max_new_tokens=5, allowed=grammar, choose=_sampler([]))
+    assert totals.tolist() == [8, 5, 8, 4]
+    # a choice for an ended row that is no token: not fed, not kept
+    def wild(x):
+        return torch.where(x.abs().sum(-1) == 0, 10 ** 9, 7)
+    d, steps = _stub_decoder(monkeypatch, logits)
+    tokens, totals = d.generate(torch.ones(4, S, dtype=torch.int64), max_new_tokens=5, allowed=words, choose=wild)
+    assert all(s.tolist() == [7, 7, 0, 7] for s in steps) and totals.tolist() == [8, 8, 3, 8]
+    # behind the end token as well
+    d, steps = _stub_decoder(monkeypatch, logits)
+    tokens, totals = d.generate(torch.ones(4, S, dtype=torch.int64), max_new_tokens=5, eos=7, choose=lambda x: torch.tensor([7, 3, 7, 3]))
+    assert totals.tolist() == [4, 8, 4, 8] and all(s.tolist()[1::2] == [3, 3] and s[0] in (0, 7) for s in steps)
+
+
+@pytest.mark.parametrize("how", ["bias", "allowed", "eos"])
+def test_generation_stops_when_all_rows_have_ended(monkeypatch, how):
+    V = 20
+    logits = torch.randn(2, V, generator=torch.Generator().manual_seed(1))
+    kw = {"bias": dict(bias=torch.full((V,), float("-inf"))), "allowed": dict(allowed=torch.zeros(1, dtype=torch.int32)),
+          "eos": dict(eos=int(logits[0].argmax()), bias=torch.zeros(V).index_fill(0, logits[0].argmax(), 99.0))}[how]
+    d, steps = _stub_decoder(monkeypatch, logits)
+    _, totals = d.generate(torch.ones(2, 3, dtype=torch.int64), max_new_tokens=150, **kw)
+    assert totals.tolist() == ([4, 4] if how == "eos" else [3, 3]) and len(steps) < 40

@@ -279,3 +279,33 @@ def test_padding_that_is_no_token(cuda_device, pos, padding):
     first = dec.prefill(ids.masked_fill(behind, padding), lengths)
     K.check_status()
     assert torch.equal(first, dec.prefill(ids.masked_fill(behind, 0), lengths))
+
+
+def test_sampling_beside_rows_without_a_choice(cuda_device):
+    """A sampler under masks and biases that end some rows early: it gets finite rows only, and the others go on."""
+    from frankentorch_b200.models.gpt_decode import GPTDecoder
+    cfg, _, model = _build(cuda_device, "rotary", vocab_size=333)
+    g = torch.Generator().manual_seed(12)
+    ids = torch.randint(0, 333, (4, 6), generator=g).to(cuda_device)
+    dec = GPTDecoder(model, 4, 40, page=16)
+    draws = torch.Generator(device=cuda_device).manual_seed(0)
+    finite = []
+
+    def sample(x):
+        finite.append(x.isfinite().any(-1).all() & ~x.isnan().any())
+        p = torch.softmax(torch.where(finite[-1], x, torch.zeros_like(x)), -1)       # never NaN in multinomial
+        return torch.multinomial(p, 1, generator=draws)[:, 0]
+    words = torch.full((4, 11), -0x55555556, dtype=torch.int32, device=cuda_device)
+    words[1] = 0
+    tokens, totals = dec.generate(ids, [6, 2, 3, 1], max_new_tokens=8, allowed=words, choose=sample)
+    assert totals.tolist() == [14, 2, 11, 9] and bool(torch.stack(finite).all())
+    assert bool((tokens[0, 6:14] % 2 == 1).all()) and not bool(tokens[1, 2:].any())
+
+    def until(tok, tot):                       # nothing from a length on
+        return torch.where(tot[:, None] < torch.tensor([[99], [5], [99], [4]], device=cuda_device), words[:1], 0)
+    tokens, totals = dec.generate(ids, [6, 2, 3, 1], max_new_tokens=8, allowed=until, choose=sample, repetition=1.1)
+    assert totals.tolist() == [14, 5, 11, 4] and bool(torch.stack(finite).all())
+    bias = torch.zeros(4, 333, device=cuda_device)
+    bias[3] = -math.inf
+    tokens, totals = dec.generate(ids, [6, 2, 3, 1], max_new_tokens=8, bias=bias, choose=sample)
+    assert totals.tolist() == [14, 10, 11, 1] and bool(torch.stack(finite).all())
