@@ -10,6 +10,8 @@ sequences grow.
 """
 from __future__ import annotations
 
+import contextlib
+import functools
 from typing import Callable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -19,6 +21,15 @@ from ..ops import kernels as K
 from .gpt import GPT
 
 _EPI = {"gelu_tanh": K.EPI_GELU_TANH, "gelu_erf": K.EPI_GELU_ERF, "relu": K.EPI_RELU}
+
+
+def _on_its_device(method):
+    """The kernels of :mod:`..ops.kernels` run on the current device: here that is the model's, whichever the caller's is."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        with self._on():
+            return method(self, *args, **kw)
+    return call
 
 
 class CacheFull(RuntimeError):
@@ -74,7 +85,7 @@ class GPTDecoder:
         cfg = model.cfg
         if cfg.pos == "learned" and max_tokens > cfg.max_seq:
             raise ValueError(f"{max_tokens} tokens, the model has {cfg.max_seq} learned positions")
-        self.model, self.cfg, self.device = model, cfg, model.device
+        self.model, self.cfg, self.device = model, cfg, model.arena.params.device
         self.batch = batch
         self.hd = cfg.d_model // cfg.n_head
         if self.hd not in D.HEAD_SIZES:
@@ -89,6 +100,9 @@ class GPTDecoder:
         self.use_graph = use_cuda_graph
         self._graph: Optional[torch.cuda.CUDAGraph] = None
         self._logits: Optional[torch.Tensor] = None
+
+    def _on(self):
+        return torch.cuda.device(self.device) if self.device.type == "cuda" else contextlib.nullcontext()
 
     def _w(self, name: str) -> torch.Tensor:
         return self.model.arena.view(self.model.arena.params, name)
@@ -108,6 +122,7 @@ class GPTDecoder:
         return K.gemm(h, self._w("wte.weight" if self.cfg.tie_lm_head else "lm_head.weight"), out_dtype=torch.float32)
 
     # ------------------------------------------------------------------ prompts
+    @_on_its_device
     def prefill(self, ids: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Take the prompts ``ids`` (int64 ``[batch, S]``, the first ``lengths[b]`` of row ``b``; what stands behind them need not be a
         token) into an empty cache; returns the logits behind each prompt's last token, fp32 ``[batch, padded vocabulary]``."""
@@ -166,6 +181,7 @@ class GPTDecoder:
         self.lengths.copy_(reach)
         return out
 
+    @_on_its_device
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """Append one token per sequence (int64 ``[batch]``); returns the logits behind it, fp32 ``[batch, padded vocabulary]``.
         With a CUDA graph the logits are one buffer, which the next step writes again."""
@@ -196,11 +212,12 @@ class GPTDecoder:
         self.lengths.copy_(held)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, stream=side):      # (the default capture stream is of the device that captured first)
             self._logits = self._step_body()
         self._graph = graph
 
     # ------------------------------------------------------------------ generation
+    @_on_its_device
     def generate(self, ids: torch.Tensor, lengths: Optional[Sequence[int]] = None, *, max_new_tokens: int,
                  eos: Optional[int] = None, repetition=None, frequency=None, presence=None,
                  bias: Optional[torch.Tensor] = None,

@@ -203,3 +203,41 @@ def test_generation_stops_when_all_rows_have_ended(monkeypatch, how):
     d, steps = _stub_decoder(monkeypatch, logits)
     _, totals = d.generate(torch.ones(2, 3, dtype=torch.int64), max_new_tokens=150, **kw)
     assert totals.tolist() == ([4, 4] if how == "eos" else [3, 3]) and len(steps) < 40
+
+
+def test_calls_run_on_the_device_of_the_model(monkeypatch):
+    """The kernels take the current device's stream: prefill, step and generate make the model's device current, with its index."""
+    import contextlib
+
+    from frankentorch_b200.models import gpt_decode
+    d = GPTDecoder(_model(), 2, 32, page=16, use_cuda_graph=False)
+    assert d.device == torch.device("cpu")
+    inside = []
+
+    @contextlib.contextmanager
+    def on():
+        inside.append(True)
+        try:
+            yield
+        finally:
+            inside.pop()
+
+    def body(*a):
+        raise _Seen(bool(inside))
+    monkeypatch.setattr(d, "_on", on)
+    monkeypatch.setattr(gpt_decode.K, "embedding_fwd", body)
+    ids = torch.ones(2, 4, dtype=torch.int64)
+    for call in (lambda: d.prefill(ids), lambda: d.generate(ids, max_new_tokens=2)):
+        with pytest.raises(_Seen) as e:
+            call()
+        assert e.value.args[0]
+    d._host_lengths = [4, 4]
+    with pytest.raises(_Seen) as e:
+        d.step(ids[:, 0])
+    assert e.value.args[0] and not inside
+    monkeypatch.undo()
+    asked = []
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: asked.append(dev) or contextlib.nullcontext())
+    d.device = torch.device("cuda", 1)
+    with d._on():
+        assert asked == [torch.device("cuda", 1)]
