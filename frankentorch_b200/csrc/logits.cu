@@ -74,12 +74,18 @@ __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 template <typename T> __device__ __forceinline__ void store1(T* p, float x) { *p = Half16<T>::round(x); }
 
 // A row's history and what it costs.  x / r is x times the rounded 1 / r: off by one unit of fp32 more than a division, which
-// would take as long as all the rest of a column.
+// would take as long as all the rest of a column.  Beyond 2^126 or below 2^-126 the normal numbers do not hold 1 / r: there x and r are
+// multiplied by 2^-64 or 2^64 first, which is exact for every x whose quotient is neither 0 nor infinite.
 struct LogitsRow {
   int len, prompt;
-  float rep, inv, freq, pres;
+  float rep, up, inv, freq, pres;
+  __device__ __forceinline__ void invert() {
+    const float r = fabsf(rep);
+    up = r < 0x1p-126f ? 0x1p64f : (r > 0x1p126f ? 0x1p-64f : 1.f);
+    inv = 1.f / (rep * up);
+  }
   __device__ __forceinline__ float operator()(float x, unsigned n) const {
-    const float y = x > 0.f ? x * inv : x * rep;
+    const float y = x > 0.f ? x * up * inv : x * rep;
     return n ? y - freq * (float)n - pres : y;
   }
 };
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) logits_kernel(const __grid_cons
       aim();
     }
   };
-  LogitsRow h = {(int)d.L, 0, (float)d.rep, 1.f, (float)d.freq, (float)d.pres};
+  LogitsRow h = {(int)d.L, 0, (float)d.rep, 1.f, 1.f, (float)d.freq, (float)d.pres};
   if (HISTORY) request_history(u, h);
   Tile next;
   if (VEC) {
@@ -218,7 +224,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1) logits_kernel(const __grid_cons
     if (HISTORY) {
       __syncthreads();            // the counts and bits of the unit before are read and cleared
       count(u, h);
-      row.inv = 1.f / row.rep;
+      row.invert();
       request_history(behind(u), h);
       __syncthreads();
     }

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _decode_oracle import attention as attention64
+from _decode_oracle import attention as attention64, logits as logits64
 from test_gpu_decode_forms import _sms, _widened, form
 from test_gpu_decode_ops import BF, HF, _attend, _gen, _i32
 
@@ -64,3 +64,30 @@ def test_attention_of_infinite_values(cuda_device, B, H, Hk, hd, page, tiles, ki
     _same(lse, wl, tl, "lse")
     again = D.paged_attention(q, kp, vp, table, _i32(lengths))[0]
     assert torch.equal(again.nan_to_num(), o.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, torch.float32])
+@pytest.mark.parametrize("columns", [512, 501])
+def test_logits_of_extreme_repetitions(cuda_device, columns, dtype):
+    """Factors whose reciprocal fp32 does not hold, or holds in fewer bits: per row and as a number."""
+    from frankentorch_b200.ops import decode as D
+    V, big = 501, torch.finfo(torch.float32).max
+    reps = [1e-45, 1e-40, 2.0 ** -128, 2.0 ** -127, 1.17e-38, 2.0 ** -64, 1.0, 1.5, 2.0 ** 64, 2.0 ** 126, 1e38, 3e38, big]
+    R = len(reps)
+    g = _gen(columns)
+    x = torch.randn(R, columns, generator=g, device="cuda")
+    # from the smallest numbers of fp32 to the largest, and zeros
+    x = x * torch.exp2(torch.rand(R, columns, generator=g, device="cuda") * 250 - 125)
+    x[:, ::50] = 0.0
+    x = x.to(dtype)
+    tokens = torch.arange(V, device="cuda").expand(R, -1)[:, ::2].contiguous()
+    rep = torch.tensor(reps, dtype=torch.float32, device="cuda")
+    want, tol = logits64(x, V, torch.float32, tokens.cpu(), None, None, rep.double().tolist(), None, None)
+    # what leaves fp32's range is infinite there (from half a step above its largest number on)
+    want = torch.where(want.abs() >= big * (1 + 2.0 ** -25), want.sign() * INF, want)
+    near = want.isfinite() & (want.abs() > big * (1 - 2.0 ** -21))      # what six roundings may carry over the border
+    tol = torch.where(want.isfinite(), tol, torch.zeros_like(tol))
+    for got in (D.logits_process(x, vocab=V, tokens=tokens, repetition=rep, out_dtype=torch.float32),
+                torch.cat([D.logits_process(x[r: r + 1], vocab=V, tokens=tokens[r: r + 1], repetition=float(rep[r]),
+                                            out_dtype=torch.float32) for r in range(R)])):
+        _same(torch.where(near.cuda(), want.float().cuda(), got), want, tol, "logits")
