@@ -423,7 +423,7 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Arg rep, freq, pres;
     d.rep = 1.0;
     per_row(args[5], "repetition", d.R, rep, d.rep_rows, d.rep);
-    if (d.rep <= 0) refuse("repetition must be positive, got " + std::to_string(d.rep));
+    if ((float)d.rep <= 0 || !std::isfinite((float)d.rep)) refuse("repetition must be positive and finite in fp32, got " + std::to_string(d.rep));
     per_row(args[6], "frequency", d.R, freq, d.freq_rows, d.freq);
     per_row(args[7], "presence", d.R, pres, d.pres_rows, d.pres);
     const void* p = nullptr;

@@ -211,3 +211,12 @@ def test_refusals_leave_the_references_of_their_arguments():
     for _ in range(50):
         _refused("CUDA tensors", D.paged_attention, **kw)
     assert {n: sys.getrefcount(t) for n, t in kw.items()} == before
+
+
+@pytest.mark.parametrize("value", [0, -0.0, -1.5, 1e-60, 7e-46, 3.4028236e38, 1e39, 1e300])
+def test_repetitions_that_fp32_does_not_hold(value):
+    """The factor is handed on in fp32: as 0 it would make infinity of every logit, as infinity NaN of a logit of 0."""
+    tokens = torch.zeros(2, 3, dtype=torch.int64)
+    _refused("repetition must be positive", D.logits_process, _z(2, 40), tokens=tokens, repetition=value)
+    for good in (1e-45, 3.4028234e38):
+        _refused("CUDA tensors", D.logits_process, _z(2, 40), tokens=tokens, repetition=good)
