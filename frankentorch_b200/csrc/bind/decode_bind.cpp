@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -72,7 +73,8 @@ Arg arg(PyObject* o, const char* name, bool needed) {
   return a;
 }
 
-// Strides of a [..., heads, hd] operand but the last: rows of whole 16 bytes, every row on a 16-byte boundary.
+// Strides of a [..., heads, hd] operand but the last: rows of whole 16 bytes, every row on a 16-byte boundary; rows of an output (`out`)
+// one behind the other in some order of the dimensions.
 void rows16(const Arg& a, int64_t ndim, at::ScalarType type, bool out, long long* strides) {
   const at::Tensor& t = *a.t;
   if (t.dim() != ndim) refuse(std::string(a.name) + " must have " + std::to_string(ndim) + " dimensions, got shape " + text(t.sizes()));
@@ -83,7 +85,16 @@ void rows16(const Arg& a, int64_t ndim, at::ScalarType type, bool out, long long
     strides[i] = s[i];
     if (n[i] > 1) {
       bits |= (uintptr_t)(2 * s[i]);
-      if (out && s[i] == 0) refuse(std::string(a.name) + " is written: its elements must not share memory");
+    }
+  }
+  if (out && t.numel() > 0) {       // each stride passes what the smaller ones span: no element is two rows'
+    int64_t order[4], m = 0, span = n[ndim - 1];
+    for (int64_t i = 0; i + 1 < ndim; ++i)
+      if (n[i] > 1) order[m++] = i;
+    std::sort(order, order + m, [&](int64_t x, int64_t y) { return s[x] < s[y]; });
+    for (int64_t k = 0; k < m; ++k) {
+      if (s[order[k]] < span) refuse(std::string(a.name) + " is written: its elements must not share memory");
+      span += s[order[k]] * (n[order[k]] - 1);
     }
   }
   if (s[ndim - 1] != 1 || bits % 16) refuse(std::string(a.name) + " needs contiguous rows that start on 16 bytes, got strides " + text(s));

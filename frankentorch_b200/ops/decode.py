@@ -19,7 +19,7 @@ on the device is reported by :func:`~.kernels.check_status`, and what it leads t
 nothing: its scratch is its own, so calls of several streams, threads and captured graphs do not meet, and the same call gives
 the same bits.  (The attention cuts a sequence's heads by the work of the whole call: beside other sequences its last bits may
 be others.)  Two tokens of one append must not have the same place, and an output must not overlap an input other than where
-the function says so.
+the function says so; one whose own rows overlap is refused.
 """
 from __future__ import annotations
 

@@ -220,3 +220,31 @@ def test_repetitions_that_fp32_does_not_hold(value):
     _refused("repetition must be positive", D.logits_process, _z(2, 40), tokens=tokens, repetition=value)
     for good in (1e-45, 3.4028234e38):
         _refused("CUDA tensors", D.logits_process, _z(2, 40), tokens=tokens, repetition=good)
+
+
+def _strided(size, stride, dtype=BF):
+    return torch.zeros(1 + sum((n - 1) * s for n, s in zip(size, stride)), dtype=dtype).as_strided(size, stride)
+
+
+def test_outputs_whose_rows_overlap():
+    """Rows, heads or sequences that share elements are written by several threads: refused whatever the stride."""
+    def base(kw):
+        return {n: f() for n, f in kw.items()}
+    for stride in ((128, 32, 1), (64, 64, 1), (64, 128, 1), (8, 64, 1), (256, 56, 1), (192, 64, 1)):
+        _refused("must not share memory", D.paged_attention, **base(ATTEND), out=_strided((3, 4, 64), stride))
+    for stride in ((256, 64, 1), (64, 192, 1), (264, 64, 1), (1000, 72, 1), (64, 208, 1)):
+        _refused("CUDA tensors", D.paged_attention, **base(ATTEND), out=_strided((3, 4, 64), stride))
+    size = (5, 2, 16, 64)
+    for stride in ((2048, 512, 64, 1), (1024, 1024, 64, 1), (2048, 1024, 32, 1), (2048, 64, 64, 1), (64, 2048, 64, 1), (2048, 32, 128, 1)):
+        for name in ("k_pages", "v_pages"):
+            _refused("%s is written" % name, D.paged_append, **{**base(APPEND), name: _strided(size, stride)})
+        _refused("CUDA tensors", D.paged_attention, **{**base(ATTEND), "k_pages": _strided(size, stride)})      # read, that is well
+    for stride in ((2048, 1024, 64, 1), (2048, 64, 128, 1), (1024, 5 * 1024, 64, 1), (64, 320, 640, 1), (4096, 1024, 64, 1)):
+        _refused("CUDA tensors", D.paged_append, **{**base(APPEND), "k_pages": _strided(size, stride)})
+    kw = base(ROTARY)
+    q, k, w = kw.pop("q"), kw.pop("k"), kw.pop("inv_freq")
+    for stride in ((768, 128, 64, 1), (768, 256, 48, 1), (256, 256, 64, 1), (0, 256, 64, 1)):
+        _refused("q_out is written", D.rotary, q, k, w, q_out=_strided((2, 3, 4, 64), stride))
+    _refused("CUDA tensors", D.rotary, q, k, w, q_out=_strided((2, 3, 4, 64), (64, 512, 128, 1)))
+    # what has one sequence, page or head may have any stride there
+    _refused("CUDA tensors", D.rotary, q[:1], None, w, q_out=_strided((1, 3, 4, 64), (0, 256, 64, 1)))
