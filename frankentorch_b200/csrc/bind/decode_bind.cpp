@@ -343,6 +343,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     page_table(table, d.B, d);
     d.lengths = ints(lengths, d.B);
     d.scale = number(args[5], "scale", 1.0 / std::sqrt((double)d.hd));
+    if (!std::isfinite((float)(d.scale * 1.5))) refuse("scale must be finite in fp32, times log2(e) too, got " + std::to_string(d.scale));
     if (out) like(out, q), rows16(out, 3, type, true, s);
     else s[1] = d.hd, s[0] = d.Hq * d.hd;
     d.o_bs = s[0], d.o_hs = s[1];

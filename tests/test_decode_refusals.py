@@ -248,3 +248,12 @@ def test_outputs_whose_rows_overlap():
     _refused("CUDA tensors", D.rotary, q, k, w, q_out=_strided((2, 3, 4, 64), (64, 512, 128, 1)))
     # what has one sequence, page or head may have any stride there
     _refused("CUDA tensors", D.rotary, q[:1], None, w, q_out=_strided((1, 3, 4, 64), (0, 256, 64, 1)))
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 3e38])
+def test_scales_that_fp32_does_not_hold(scale):
+    """The kernel multiplies by scale log2(e) in fp32: as infinity it would make NaN of a score of 0."""
+    kw = {n: f() for n, f in ATTEND.items()}
+    _refused("scale must be finite", D.paged_attention, **kw, scale=scale)
+    _refused("CUDA tensors", D.paged_attention, **kw, scale=scale / 1e270)
+    _refused("CUDA tensors", D.paged_attention, **kw, scale=2e38)
