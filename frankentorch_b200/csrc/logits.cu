@@ -14,7 +14,7 @@
 //
 // What was measured (512 rows of 128003 bf16 columns with bias, mask and 2048 to 4096 tokens / 256 rows of 50257 fp32 columns with
 // mask and 1024 to 2048 tokens; the copy bandwidth gives 43 / 16 us):
-//   * a history is read once per piece and stops the stream, so pieces are as long as shared memory allows: 85 / 20 us with 64
+//   * a history is read once per piece and stops the stream, so pieces are as long as shared memory allows: 85 / 20.5 us with 64
 //     thousand columns, 103 / 24 with two CTAs of 40 thousand, 112 / 33 with six narrow slices of every row; a cluster of CTAs that
 //     share the counts of a row 185 / 50; warps of their own that count ahead of the stream 105 / 27;
 //   * penalties where a column has a history are what the time goes by next: without them the first takes 56 us.  All eight

@@ -36,10 +36,12 @@ namespace ftk {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;      // of a CTA that shares its SM
-// Tiles of 64 tokens up to which a head is left whole: a second launch and the join cost 3 - 4 us, so few heads are cut late, and heads for all
-// SMs fill the time among themselves.  Whole and cut (us), with an SM for each head: 12 heads of 64, 16 tiles 8.1 and 8.6, 32 tiles 13.7
-// and 9.2; 32 heads of 128, up to 17 tiles 13.1 and 10.7; 128 heads of 128, up to 17 13.7 and 16.4, up to 33 22.4 and 25.0; with several
-// heads per SM, 256 of 128, up to 17 21.7 and 26.4, up to 33 38.0 and 36.9.
+// Tiles of 64 tokens, by the width of the table, up to which a head is left whole: a second launch and the join cost 3 - 4 us, so few heads
+// are cut late, and heads for all SMs fill the time among themselves.  Whole and cut (us) with all positions in use, an SM for each head:
+// 12 heads of 64, 16 tiles 8.1 and 8.6, 32 tiles 13.7 and 9.2; 32 heads of 128, up to 17 tiles 13.1 and 10.7; 128 heads of 128, up to 17
+// 13.7 and 16.4, up to 33 22.4 and 25.0; with several heads per SM, 256 of 128, up to 17 21.7 and 26.4, up to 33 38.0 and 36.9.  A straight
+// line below these borders: for a dozen heads it cuts from 12 tiles on where 17 would do, and the width stands for lengths that only the
+// device knows, so few tokens under a wide table are cut too (12 heads of 64, 301 tokens: 4.8 us under 5 tiles, 8.9 under 16).
 __host__ inline long long pa_whole(long long heads, long long sms) { return heads <= sms ? 9 + 28 * heads / sms : 20; }
 constexpr int PA_HEADER = 8;                 // ints of a header
 

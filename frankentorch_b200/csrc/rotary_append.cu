@@ -14,7 +14,7 @@
 // tokens with all their heads, a thread the same elements of every so-manieth head of them: it requests its items, two at a time,
 // and while they arrive the CTA forms the angles' sines and cosines once per token and pair and looks up the tokens' places.
 // Offsets of tokens are in shared memory: worked out per item they were the larger part of 250 instructions per 64 bytes.
-// Forward and backward of 4 x 2048 tokens of 16 heads of 128 take 49 us, 5.5 TB/s.
+// Forward and backward of 4 x 2048 tokens of 16 heads of 128 take 48 us, 5.6 TB/s.
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
 #include "launch.cuh"
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const __grid_constan
   float4* cs = reinterpret_cast<float4*>(smem);
   Token* tok = reinterpret_cast<Token*>(cs + w.tokens * half / 2);        // [tokens]
   pdl_wait();
-  pdl_trigger_work(RO_THREADS * 64 * K);
+  pdl_trigger();      // a CTA has 8 KB and more to move
   const bool append = d.k_pages != nullptr;
   const long long tok0 = (long long)(blockIdx.x / (unsigned)w.hblocks) * w.tokens, all = d.B * d.S;
   const int h0 = (int)(blockIdx.x % (unsigned)w.hblocks) * w.heads;
@@ -195,7 +195,10 @@ extern "C" int ftk_rotary(const FtkRotaryDesc* d, void* stream) {
   // what a CTA does once (places, sines, its launch) takes as long as two rounds.  4 x 2048 x 16 x 128 twice / 16 ragged prompts: one
   // round 52.0 / 87.6 us, two 47.9 / 67.0, four 49.0 / 59.7, eight 51.6 / 63.9; four items at a time, one round 49.2 / 69.2.
   // Tokens of a CTA share its table of 4096 sines at most.
-  const long long items = d->B * d->S * heads * w.chunks, full = 148ll * 8 * RO_THREADS;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const long long items = d->B * d->S * heads * w.chunks, full = 8ll * sms * RO_THREADS;
   const int per = items >= 2 * full ? 2 : 1, rounds = items >= 16 * full ? 4 : (items >= 8 * full ? 2 : 1);
   const int most = rounds * per * (RO_THREADS / w.chunks) * w.chunks;
   w.heads = (int)(heads * w.chunks <= most ? heads : (most / w.chunks > 0 ? most / w.chunks : 1));

@@ -13,9 +13,9 @@ page numbers (int32): position ``p`` of sequence ``b`` is row ``p % page`` of pa
 last position that a call touches have no meaning for it.  Rows of ``hd`` elements are contiguous and start on 16 bytes; everything else
 may be strided.  Lengths, positions and counts are int32 on the device, so a captured graph follows them.
 
-As everywhere in :mod:`~frankentorch_b200.ops.kernels`, a call enqueues on the current stream of its tensors' device and
-returns; arguments that the host can check are refused with :class:`~.kernels.KernelError`; a page, token or length out of range
-on the device is reported by :func:`~.kernels.check_status`, and what it leads to is not read and not written.  A call keeps
+A call enqueues on the current stream of its tensors' device, also where another device is the current one, and returns.
+Arguments that the host can check are refused with :class:`~.kernels.KernelError`; a page, token or length out of range on the
+device is reported by that device's :func:`~.kernels.check_status`, and what it leads to is not read and not written.  A call keeps
 nothing: its scratch is its own, so calls of several streams, threads and captured graphs do not meet, and the same call gives
 the same bits.  (The attention cuts a sequence's heads by the work of the whole call: beside other sequences its last bits may
 be others.)  Two tokens of one append must not have the same place, and an output must not overlap an input other than where
