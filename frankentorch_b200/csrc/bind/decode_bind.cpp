@@ -28,6 +28,10 @@ int (*g_rotary)(const FtkRotaryDesc*, void*) = nullptr;
 int (*g_attn)(const FtkPagedAttnDesc*, void*, void*) = nullptr;
 long long (*g_attn_scratch)(const FtkPagedAttnDesc*) = nullptr;
 int (*g_logits)(const FtkLogitsDesc*, void*) = nullptr;
+int (*g_append8)(const FtkRotaryDesc*, void*) = nullptr;
+int (*g_attn8)(const FtkPagedAttnDesc*, void*, void*) = nullptr;
+long long (*g_attn8_scratch)(const FtkPagedAttnDesc*) = nullptr;
+int (*g_sample)(const FtkSampleDesc*, void*) = nullptr;
 
 struct Refused {
   std::string why;
@@ -48,6 +52,7 @@ std::string text(at::ScalarType t) {
     case at::kDouble: return "torch.float64";
     case at::kInt: return "torch.int32";
     case at::kLong: return "torch.int64";
+    case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
     default: return std::string("torch type ") + c10::toString(t);
   }
 }
@@ -73,6 +78,21 @@ Arg arg(PyObject* o, const char* name, bool needed) {
   return a;
 }
 
+// Of an operand that is written: each stride passes what the smaller ones span, so that no element is two of its places.
+void apart(const Arg& a) {
+  const at::Tensor& t = *a.t;
+  if (t.numel() == 0) return;
+  const at::IntArrayRef n = t.sizes(), s = t.strides();
+  const int64_t ndim = t.dim();
+  int64_t order[4], m = 0, span = n[ndim - 1];
+  for (int64_t i = 0; i + 1 < ndim; ++i)
+    if (n[i] > 1) order[m++] = i;
+  std::sort(order, order + m, [&](int64_t x, int64_t y) { return s[x] < s[y]; });
+  for (int64_t k = 0; k < m; ++k) {
+    if (s[order[k]] < span) refuse(std::string(a.name) + " is written: its elements must not share memory");
+    span += s[order[k]] * (n[order[k]] - 1);
+  }
+}
 // Strides of a [..., heads, hd] operand but the last: rows of whole 16 bytes, every row on a 16-byte boundary; rows of an output (`out`)
 // one behind the other in some order of the dimensions.
 void rows16(const Arg& a, int64_t ndim, at::ScalarType type, bool out, long long* strides) {
@@ -80,23 +100,15 @@ void rows16(const Arg& a, int64_t ndim, at::ScalarType type, bool out, long long
   if (t.dim() != ndim) refuse(std::string(a.name) + " must have " + std::to_string(ndim) + " dimensions, got shape " + text(t.sizes()));
   if (t.scalar_type() != type) refuse(std::string(a.name) + " is " + text(t.scalar_type()) + ", expected " + text(type));
   const at::IntArrayRef n = t.sizes(), s = t.strides();
+  const int64_t size = type == at::kFloat8_e4m3fn ? 1 : 2;
   uintptr_t bits = (uintptr_t)t.data_ptr();
   for (int64_t i = 0; i + 1 < ndim; ++i) {
     strides[i] = s[i];
     if (n[i] > 1) {
-      bits |= (uintptr_t)(2 * s[i]);
+      bits |= (uintptr_t)(size * s[i]);
     }
   }
-  if (out && t.numel() > 0) {       // each stride passes what the smaller ones span: no element is two rows'
-    int64_t order[4], m = 0, span = n[ndim - 1];
-    for (int64_t i = 0; i + 1 < ndim; ++i)
-      if (n[i] > 1) order[m++] = i;
-    std::sort(order, order + m, [&](int64_t x, int64_t y) { return s[x] < s[y]; });
-    for (int64_t k = 0; k < m; ++k) {
-      if (s[order[k]] < span) refuse(std::string(a.name) + " is written: its elements must not share memory");
-      span += s[order[k]] * (n[order[k]] - 1);
-    }
-  }
+  if (out) apart(a);
   if (s[ndim - 1] != 1 || bits % 16) refuse(std::string(a.name) + " needs contiguous rows that start on 16 bytes, got strides " + text(s));
 }
 const int* ints(const Arg& a, int64_t n) {
@@ -138,6 +150,32 @@ template <typename D> void pages(const Arg& k, const Arg& v, int64_t heads, int6
   d.k_pages = k.ptr(), d.v_pages = v.ptr();
   d.n_pages = n[0];
   for (d.page_shift = 0; (int64_t(1) << d.page_shift) < page;) ++d.page_shift;
+}
+// The type of a cache's pages: that of the other operands, or 8 bits with scales for keys and values.
+at::ScalarType cache_type(const Arg& k, const Arg& ks, const Arg& vs, at::ScalarType type) {
+  const bool eight = k->scalar_type() == at::kFloat8_e4m3fn;
+  if (eight && !(ks && vs)) refuse("pages of torch.float8_e4m3fn need k_scales and v_scales");
+  if (!eight && (ks || vs)) refuse("k_scales and v_scales belong to pages of torch.float8_e4m3fn, k_pages is " + text(k->scalar_type()));
+  return eight ? at::kFloat8_e4m3fn : type;
+}
+// Scales of a cache in 8 bits: a number for each block of rows of a page and head
+template <typename D> void block_scales(const Arg& pages, const Arg& k, const Arg& v, bool out, D& d) {
+  if (!k) return;
+  const at::IntArrayRef n = pages->sizes();
+  for (const Arg* a : {&k, &v}) {
+    const at::Tensor& t = *a->t;
+    if (t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(0) != n[0] || t.size(1) != n[1] || (t.size(2) > 1 && t.stride(2) != 1))
+      refuse(std::string(a->name) + " must be fp32 [" + std::to_string(n[0]) + ", " + std::to_string(n[1]) + ", blocks of a page] with unit inner stride, got " +
+             text(t.scalar_type()) + " " + text(t.sizes()));
+    const int64_t blocks = t.size(2);
+    if (blocks < 1 || (blocks & (blocks - 1)) || blocks > n[2] || n[2] / blocks > 64)
+      refuse(std::string(a->name) + " has " + std::to_string(blocks) + " blocks for a page of " + std::to_string(n[2]) + " rows: a block is a power of two of rows, 64 at most");
+    if (out) apart(*a);
+  }
+  if (k->sizes() != v->sizes()) refuse("k_scales " + text(k->sizes()) + " and v_scales " + text(v->sizes()) + " differ");
+  d.k_scales = (float*)k.ptr(), d.ks_ps = k->stride(0), d.ks_hs = k->stride(1);
+  d.v_scales = (float*)v.ptr(), d.vs_ps = v->stride(0), d.vs_hs = v->stride(1);
+  for (d.block_shift = 0; (k->size(2) << d.block_shift) < n[2];) ++d.block_shift;
 }
 void same_device(const Arg& ref, std::initializer_list<const Arg*> others) {
   if (!ref->is_cuda()) refuse("operands must be CUDA tensors");
@@ -274,13 +312,14 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out) -> q_out or None
+// paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out, k_scales, v_scales) -> q_out or None
 PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    expect(nargs, 11, "paged_append");
+    expect(nargs, 13, "paged_append");
     const Arg kp = arg(args[0], "k_pages", true), vp = arg(args[1], "v_pages", true), table = arg(args[2], "the page table", true);
     const Arg k = arg(args[3], "k", true), v = arg(args[4], "v", true), start = arg(args[5], "start", true), counts = arg(args[6], "counts", false);
     const Arg q = arg(args[7], "q", false), w = arg(args[8], "inv_freq", false), qo = arg(args[10], "q_out", false);
+    const Arg ks = arg(args[11], "k_scales", false), vs = arg(args[12], "v_scales", false);
     FtkRotaryDesc d = {};
     d.type = type16(k, "paged_append");
     const at::ScalarType type = k->scalar_type();
@@ -292,7 +331,9 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     rows16(v, 4, type, false, s);
     d.v_bs = s[0], d.v_ss = s[1], d.v_hs = s[2];
     if (v->sizes() != k->sizes()) refuse("k " + text(k->sizes()) + " and v " + text(v->sizes()) + " differ");
-    pages(kp, vp, d.Hkv, d.hd, type, true, d);
+    const at::ScalarType held = cache_type(kp, ks, vs, type);
+    pages(kp, vp, d.Hkv, d.hd, held, true, d);
+    block_scales(kp, ks, vs, true, d);
     page_table(table, d.B, d);
     d.start = ints(start, d.B), d.counts = ints(counts, d.B);
     frequencies(w, d);
@@ -308,26 +349,28 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else if (qo) {
       refuse("q_out without q");
     }
-    same_device(k, {&v, &kp, &vp, &table, &start, &counts, &w, &q, &qo});
+    same_device(k, {&v, &kp, &vp, &ks, &vs, &table, &start, &counts, &w, &q, &qo});
     const On on(k);
     at::Tensor a;
     if (q && !qo) a = on.empty(q->sizes(), type);
     if (d.B * d.S * (d.Hq + d.Hkv) != 0) {
       d.k = k.ptr(), d.v = v.ptr();
       if (q) d.q = q.ptr(), d.q_out = qo ? qo.ptr() : a.data_ptr();
-      launched(g_rotary(&d, on.stream()), "ftk_rotary");
+      if (ks) launched(g_append8(&d, on.stream()), "ftk_append_e4m3");
+      else launched(g_rotary(&d, on.stream()), "ftk_rotary");
     }
     if (!q) Py_RETURN_NONE;
     return result(args[10], a);
   });
 }
 
-// paged_attention(q, k_pages, v_pages, table, lengths, scale, out) -> (o, lse)
+// paged_attention(q, k_pages, v_pages, table, lengths, scale, out, k_scales, v_scales) -> (o, lse)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    expect(nargs, 7, "paged_attention");
+    expect(nargs, 9, "paged_attention");
     const Arg q = arg(args[0], "q", true), kp = arg(args[1], "k_pages", true), vp = arg(args[2], "v_pages", true);
     const Arg table = arg(args[3], "the page table", true), lengths = arg(args[4], "lengths", true), out = arg(args[6], "out", false);
+    const Arg ks = arg(args[7], "k_scales", false), vs = arg(args[8], "v_scales", false);
     FtkPagedAttnDesc d = {};
     d.type = type16(q, "paged_attention");
     const at::ScalarType type = q->scalar_type();
@@ -337,7 +380,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     d.B = q->size(0), d.Hq = q->size(1), d.hd = q->size(2);
     if (d.hd != 64 && d.hd != 128) refuse("head size " + std::to_string(d.hd) + " is none of (64, 128)");
     d.Hkv = kp->dim() == 4 ? kp->size(1) : 0;
-    pages(kp, vp, d.Hkv, d.hd, type, false, d);
+    const at::ScalarType held = cache_type(kp, ks, vs, type);
+    pages(kp, vp, d.Hkv, d.hd, held, false, d);
+    block_scales(kp, ks, vs, false, d);
     if (d.Hkv < 1 || d.Hq % d.Hkv)
       refuse(std::to_string(d.Hq) + " query heads do not divide into groups over " + std::to_string(d.Hkv) + " heads of the cache");
     page_table(table, d.B, d);
@@ -347,16 +392,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (out) like(out, q), rows16(out, 3, type, true, s);
     else s[1] = d.hd, s[0] = d.Hq * d.hd;
     d.o_bs = s[0], d.o_hs = s[1];
-    same_device(q, {&kp, &vp, &table, &lengths, &out});
+    same_device(q, {&kp, &vp, &ks, &vs, &table, &lengths, &out});
     const On on(q);
     at::Tensor o, scratch;
     if (!out) o = on.empty({d.B, d.Hq, d.hd}, type);
     at::Tensor lse = on.empty({d.B, d.Hq}, at::kFloat);
     if (d.B * d.Hq != 0) {
       d.q = q.ptr(), d.o = out ? out.ptr() : o.data_ptr(), d.lse = (float*)lse.data_ptr();
-      const long long need = g_attn_scratch(&d);
+      const long long need = ks ? g_attn8_scratch(&d) : g_attn_scratch(&d);
       if (need > 0) scratch = on.empty({need}, at::kByte);
-      launched(need < 0 ? (int)need : g_attn(&d, need > 0 ? scratch.data_ptr() : nullptr, on.stream()), "ftk_paged_attn");
+      launched(need < 0 ? (int)need : (ks ? g_attn8 : g_attn)(&d, need > 0 ? scratch.data_ptr() : nullptr, on.stream()),
+               ks ? "ftk_paged_attn_e4m3" : "ftk_paged_attn");
     }
     PyObject* first = result(args[6], o);
     return pair(first, wrapped(lse));
@@ -388,6 +434,17 @@ void per_column(const Arg& a, at::ScalarType type, int64_t R, int64_t n, const v
 }
 int type32(at::ScalarType t) { return t == at::kBFloat16 ? FTK_T_BF16 : t == at::kHalf ? FTK_T_FP16 : t == at::kFloat ? FTK_T_FP32 : -1; }
 
+// Tokens of the vocabulary: `o`, or all columns for None
+int64_t vocabulary(PyObject* o, int64_t columns) {
+  int64_t V = columns;
+  if (o != Py_None) {
+    V = PyLong_AsLongLong(o);
+    if (V == -1 && PyErr_Occurred()) throw PythonError{};
+  }
+  if (V <= 0 || V > columns) refuse("vocab " + std::to_string(V) + " does not fit " + std::to_string(columns) + " columns");
+  return V;
+}
+
 // logits_process(logits, vocab, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed, out, out_dtype) -> out
 PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
@@ -402,12 +459,7 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (x->dim() != 2 || (x->size(1) > 1 && x->stride(1) != 1)) refuse("logits must be [rows, columns] with unit inner stride, got " + text(x->sizes()));
     d.R = x->size(0);
     const int64_t columns = x->size(1);
-    d.V = columns;
-    if (args[1] != Py_None) {
-      d.V = PyLong_AsLongLong(args[1]);
-      if (d.V == -1 && PyErr_Occurred()) throw PythonError{};
-    }
-    if (d.V <= 0 || d.V > columns) refuse("vocab " + std::to_string(d.V) + " does not fit " + std::to_string(columns) + " columns");
+    d.V = vocabulary(args[1], columns);
     at::ScalarType kind = type;
     if (args[11] != Py_None) {
       if (!THPDtype_Check(args[11])) refuse("out_dtype must be a type");
@@ -459,12 +511,58 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// init(KernelError, launched, rotary, attention, attention scratch, logits): the last four are addresses
+// sample(logits, uniform, vocab, temperature, top_k, top_p, min_p) -> (token, logprob)
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    expect(nargs, 7, "sample");
+    const Arg x = arg(args[0], "logits", true), u = arg(args[1], "uniform", true);
+    FtkSampleDesc d = {};
+    d.type = type32(x->scalar_type());
+    if (d.type < 0) refuse("logits must be bf16, fp16 or fp32, got " + text(x->scalar_type()));
+    if (x->dim() != 2 || (x->size(1) > 1 && x->stride(1) != 1)) refuse("logits must be [rows, columns] with unit inner stride, got " + text(x->sizes()));
+    d.R = x->size(0);
+    d.V = vocabulary(args[2], x->size(1));
+    if (d.V > (1 << 20)) refuse("a vocabulary of " + std::to_string(d.V) + " tokens: 2^20 are the most");
+    if (u->scalar_type() != at::kFloat || u->dim() != 1 || u->size(0) != d.R || (d.R > 1 && u->stride(0) != 1))
+      refuse("uniform must be contiguous fp32 [" + std::to_string(d.R) + "], got " + text(u->scalar_type()) + " " + text(u->sizes()));
+    Arg temp, k, p, least;
+    d.temp = 1.0, d.p = 1.0;
+    per_row(args[3], "temperature", d.R, temp, d.temp_rows, d.temp);
+    if (!((float)d.temp >= 0.f) || !std::isfinite((float)d.temp)) refuse("temperature must be 0 or positive, and finite in fp32, got " + std::to_string(d.temp));
+    if ((float)d.temp == 0.f && d.temp > 0.0) refuse("temperature must be 0 or positive in fp32, got " + std::to_string(d.temp));
+    k.name = "top_k";
+    if (THPVariable_Check(args[4])) {
+      k = arg(args[4], "top_k", true);
+      d.k_rows = ints(k, d.R);
+    } else if (args[4] != Py_None) {
+      d.k = PyLong_AsLongLong(args[4]);
+      if (d.k == -1 && PyErr_Occurred()) throw PythonError{};
+      if (d.k < 0) refuse("top_k must not be negative, got " + std::to_string(d.k));
+    }
+    per_row(args[5], "top_p", d.R, p, d.p_rows, d.p);
+    if (!(d.p > 0.0 && d.p <= 1.0)) refuse("top_p must be above 0 and 1 at most, got " + std::to_string(d.p));
+    per_row(args[6], "min_p", d.R, least, d.min_rows, d.min_p);
+    if (!(d.min_p >= 0.0 && d.min_p <= 1.0)) refuse("min_p must be from 0 to 1, got " + std::to_string(d.min_p));
+    same_device(x, {&u, &temp, &k, &p, &least});
+    const On on(x);
+    at::Tensor token = on.empty({d.R}, at::kLong), logprob = on.empty({d.R}, at::kFloat);
+    if (d.R != 0) {
+      d.logits = x.ptr(), d.ld = x->stride(0), d.uniform = (const float*)u.ptr();
+      d.token = (long long*)token.data_ptr(), d.logprob = (float*)logprob.data_ptr();
+      launched(g_sample(&d, on.stream()), "ftk_sample");
+    }
+    PyObject* first = wrapped(token);
+    return pair(first, wrapped(logprob));
+  });
+}
+
+// init(KernelError, launched, rotary, attention, attention scratch, logits, the append and attention over 8 bits, the scratch of that,
+// sample): all but the first two are addresses
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    expect(nargs, 6, "init");
-    void* p[4];
-    for (int i = 0; i < 4; ++i) {
+    expect(nargs, 10, "init");
+    void* p[8];
+    for (int i = 0; i < 8; ++i) {
       p[i] = PyLong_AsVoidPtr(args[2 + i]);
       if (!p[i]) {
         if (PyErr_Occurred()) throw PythonError{};
@@ -479,12 +577,17 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     g_attn = reinterpret_cast<decltype(g_attn)>(p[1]);
     g_attn_scratch = reinterpret_cast<decltype(g_attn_scratch)>(p[2]);
     g_logits = reinterpret_cast<decltype(g_logits)>(p[3]);
+    g_append8 = reinterpret_cast<decltype(g_append8)>(p[4]);
+    g_attn8 = reinterpret_cast<decltype(g_attn8)>(p[5]);
+    g_attn8_scratch = reinterpret_cast<decltype(g_attn8_scratch)>(p[6]);
+    g_sample = reinterpret_cast<decltype(g_sample)>(p[7]);
     Py_RETURN_NONE;
   });
 }
 
 #define FT_FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FT_FN(init), FT_FN(rotary), FT_FN(paged_append), FT_FN(paged_attention), FT_FN(logits_process), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FT_FN(init), FT_FN(rotary), FT_FN(paged_append), FT_FN(paged_attention), FT_FN(logits_process), FT_FN(sample),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ft_decode", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -375,8 +375,18 @@ typedef struct FtkRotaryDesc {
   long long vp_ps, vp_hs, vp_rs;
   const int* table;
   long long table_stride, table_cols, n_pages, page_shift;
+  // Of a cache in 8 bits: a scale for each block of 1 << block_shift (64 at most) rows of a page and head, unit inner stride
+  float* k_scales;
+  long long ks_ps, ks_hs;
+  float* v_scales;
+  long long vs_ps, vs_hs;
+  long long block_shift;
 } FtkRotaryDesc;
 int ftk_rotary(const FtkRotaryDesc* d, void* stream);
+// The same into a cache of e4m3 (pages counted in bytes): an element y of a block stands for y times the block's scale.  The scale of
+// a block is the smallest power of two (2^-100 at least) of which 448 times reaches its finite elements; a block whose first rows lie
+// in front of start[b] keeps at least its own, and when it grows those rows are rounded anew.  Infinities and NaN are held as NaN.
+int ftk_append_e4m3(const FtkRotaryDesc* d, void* stream);
 
 // One new token per sequence: o[b, h] = sum over t < lengths[b] of softmax_t(scale q[b, h] . k[t]) v[t], keys and values of head
 // h / (Hq / Hkv); lse[b, h] the natural log of the softmax's sum.  A sequence of no tokens: o = 0, lse = -inf.
@@ -395,10 +405,19 @@ typedef struct FtkPagedAttnDesc {
   const int* table;
   long long table_stride, table_cols, n_pages, page_shift;
   const int* lengths;       // [B]
+  // Of a cache in 8 bits (e4m3, strides of the pages in bytes), else NULL: scales of blocks of 1 << block_shift rows
+  const float* k_scales;
+  long long ks_ps, ks_hs;
+  const float* v_scales;
+  long long vs_ps, vs_hs;
+  long long block_shift;
 } FtkPagedAttnDesc;
 // Scratch of one call in bytes (0: none), or a negative value for rejected arguments.  Its contents do not outlive the call.
 long long ftk_paged_attn_scratch(const FtkPagedAttnDesc* d);
 int ftk_paged_attn(const FtkPagedAttnDesc* d, void* scratch, void* stream);
+// The same over a cache in 8 bits
+long long ftk_paged_attn_e4m3_scratch(const FtkPagedAttnDesc* d);
+int ftk_paged_attn_e4m3(const FtkPagedAttnDesc* d, void* scratch, void* stream);
 
 // Per row r and column c < V: x = logits; x = x > 0 ? x / rep : x * rep where c is among tokens[r, 0:lengths[r]];
 // x -= freq * n + pres * (n > 0) with n the count of c among tokens[r, prompts[r]:lengths[r]]; x += bias; -inf where bit c % 32
@@ -421,6 +440,25 @@ typedef struct FtkLogitsDesc {
   long long allowed_rs;
 } FtkLogitsDesc;
 int ftk_logits(const FtkLogitsDesc* d, void* stream);
+
+// Row r: token i < V weighs w_i = round(2^43 exp((x_i - max x) / T)), nothing where x_i is -inf.  In the order of x, equal ones by
+// their ids, are kept the first k (k <= 0: all), of those the ones before which less than p of their sum lies (p >= 1: all; the first
+// always), of those the ones of at least min_p of the largest; T = 0 keeps the first.  token[r] is the first kept one by id with
+// sum_{j <= i} w_j > floor(u sum_j w_j), logprob[r] = log(w_i / sum_j w_j).  A row of nothing but -inf: -1, -inf; with a NaN among its
+// logits or settings, or T < 0: -1, NaN.  Settings: per row where the pointer is given, else the value.
+typedef struct FtkSampleDesc {
+  long long type, R, V;     // V <= 2^20: the sums are 63 bits
+  const void* logits;
+  long long ld;
+  const float* uniform;     // [R]
+  const float *temp_rows, *p_rows, *min_rows;
+  const int* k_rows;
+  double temp, p, min_p;
+  long long k;
+  long long* token;         // [R]
+  float* logprob;           // [R]
+} FtkSampleDesc;
+int ftk_sample(const FtkSampleDesc* d, void* stream);
 #ifdef __cplusplus
 }
 #endif

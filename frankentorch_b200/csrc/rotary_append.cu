@@ -20,17 +20,11 @@
 #include "launch.cuh"
 #include "ftk_api.h"
 #include "paged_cache.h"
+#include "rotary.cuh"
 
 extern "C" int* ftk_status_word(void);
 
 namespace ftk {
-
-__device__ __forceinline__ float2 turn_of(long long position, double inv_freq) {
-  const double turns = (double)position * inv_freq * 0.15915494309189533577;      // 1 / (2 pi)
-  float s, c;
-  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-  return make_float2(c, s);
-}
 
 constexpr int RO_THREADS = 128;
 

@@ -201,7 +201,8 @@ def bind():
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         mod.init(K.KernelError, K._chk, *(C.cast(lib[n], C.c_void_p).value for n in
-                                          ("ftk_rotary", "ftk_paged_attn", "ftk_paged_attn_scratch", "ftk_logits")))
+                                          ("ftk_rotary", "ftk_paged_attn", "ftk_paged_attn_scratch", "ftk_logits", "ftk_append_e4m3",
+                                           "ftk_paged_attn_e4m3", "ftk_paged_attn_e4m3_scratch", "ftk_sample")))
         _BIND = mod
     return _BIND
 

@@ -3,22 +3,28 @@
 * :func:`rotary`: queries and keys turned by position, forward and backward (training);
 * :func:`paged_append`: keys and values of new tokens into a paged cache, turned on the way;
 * :func:`paged_attention`: one new token per sequence over the cache;
-* :func:`logits_process`: penalties for repeated tokens, biases and a grammar's mask on the logits of a step.
+* :func:`logits_process`: penalties for repeated tokens, biases and a grammar's mask on the logits of a step;
+* :func:`sample`: the next token from them and given random numbers (temperature, top-k, top-p, min-p).
 
-The reference composes the rotation from tensor operators (``apply_rotary_pos_emb``) and has no cache, no decoding attention
-and no logits processing; shapes, masks and empty rows follow its attention (ft-nn/src/lib.rs:5145-5184) where they overlap.
+The reference composes the rotation from tensor operators (``apply_rotary_pos_emb``) and has no cache, no decoding attention,
+no logits processing and no sampling; shapes, masks and empty rows follow its attention (ft-nn/src/lib.rs:5145-5184) where they overlap.
 
 A paged cache is two tensors of pages, ``[pages, heads, page, hd]`` (``page`` a power of two), and a table ``[B, columns]`` of
 page numbers (int32): position ``p`` of sequence ``b`` is row ``p % page`` of page ``table[b, p // page]``.  Table entries behind the
 last position that a call touches have no meaning for it.  Rows of ``hd`` elements are contiguous and start on 16 bytes; everything else
 may be strided.  Lengths, positions and counts are int32 on the device, so a captured graph follows them.
 
+The cache may be held in 8 bits: pages of ``torch.float8_e4m3fn`` with fp32 scales, ``[pages, heads, blocks]`` with unit inner stride,
+for keys (``k_scales``) and for values (``v_scales``).  A block is ``page / blocks`` neighbouring rows of a page and head (a power of two,
+64 at most), and an element stands for its 8 bits times its block's scale.  :func:`paged_append` makes the scales, powers of two;
+:func:`paged_attention` takes any from 2^-100 to 2^100, or 0.
+
 A call enqueues on the current stream of its tensors' device, also where another device is the current one, and returns.
 Arguments that the host can check are refused with :class:`~.kernels.KernelError`; a page, token or length out of range on the
 device is reported by that device's :func:`~.kernels.check_status`, and what it leads to is not read and not written.  A call keeps
 nothing: its scratch is its own, so calls of several streams, threads and captured graphs do not meet, and the same call gives
 the same bits.  (The attention cuts a sequence's heads by the work of the whole call: beside other sequences its last bits may
-be others.)  Two tokens of one append must not have the same place, and an output must not overlap an input other than where
+be others.)  Two tokens of one append must not have the same place (over 8 bits: two sequences no common block), and an output must not overlap an input other than where
 the function says so; one whose own rows overlap is refused.
 """
 from __future__ import annotations
@@ -55,18 +61,25 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
 def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                  start: torch.Tensor, counts: Optional[torch.Tensor] = None, *, q: Optional[torch.Tensor] = None,
                  inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
-                 q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                 q_out: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                 v_scales: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Put ``k`` and ``v`` (``[B, S, Hkv, hd]``) at positions ``start[b] + s`` of the cache, for ``s < counts[b]`` (all ``S`` tokens
     where ``counts`` is not given); the rest of the cache stays as it was.
 
     With ``inv_freq`` the keys are turned by position as in :func:`rotary`, and ``q`` (``[B, S, H, hd]``), where given, is
-    returned turned; queries behind ``counts[b]`` are copied as they are.  ``q_out`` may be ``q`` itself."""
-    return _lib.bind().paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out)
+    returned turned; queries behind ``counts[b]`` are copied as they are.  ``q_out`` may be ``q`` itself.
+
+    Into a cache in 8 bits a block's new elements (keys in fp32 behind their rotation) get the smallest power of two, 2^-100 at least, of
+    which 448 times reaches the largest finite one, and each is rounded once to a multiple of it; infinities and NaN are held as NaN.
+    A block that has rows in front of ``start[b]`` keeps at least its own scale; where it grows, those rows are rounded anew (exact but
+    for the smallest ones).  What stands in a block behind the last new token has no meaning any more."""
+    return _lib.bind().paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out, k_scales, v_scales)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                     lengths: torch.Tensor, *, scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                    out: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Attention of one token per sequence over the first ``lengths[b]`` positions of the cache; returns ``(o, lse)``.
 
     ``q`` is ``[B, H, hd]`` (bf16 or fp16, ``hd`` 64 or 128), ``H`` a multiple of the cache's heads, which groups of ``H / Hkv``
@@ -74,7 +87,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     has ``o = 0`` and ``lse = -inf``.  ``scale`` is ``1 / sqrt(hd)`` where it is not given.  What stands in the cache behind
     ``lengths[b]`` has no influence, NaN included; an infinite value before it is infinity in its element of ``o``, NaN beside one of
     the other sign or where its token has no weight (a score of ``-inf``, or so far below the largest that fp32 has 0 for it)."""
-    return _lib.bind().paged_attention(q, k_pages, v_pages, table, lengths, scale, out)
+    return _lib.bind().paged_attention(q, k_pages, v_pages, table, lengths, scale, out, k_scales, v_scales)
 
 
 def logits_process(logits: torch.Tensor, *, vocab: Optional[int] = None, tokens: Optional[torch.Tensor] = None,
@@ -98,3 +111,25 @@ def logits_process(logits: torch.Tensor, *, vocab: Optional[int] = None, tokens:
     on 16 bytes, so a new one is a view of wider rows.  ``out`` may be ``logits[:, :vocab]`` itself."""
     return _lib.bind().logits_process(logits, vocab, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed,
                                       out, out_dtype)
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, *, vocab: Optional[int] = None, temperature=None, top_k=None, top_p=None,
+           min_p=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A token for each row of ``logits`` (the first ``vocab`` columns, 2^20 at most, of ``[R, columns]``; bf16, fp16 or fp32) from
+    ``uniform`` (fp32 ``[R]``, in [0, 1)); returns ``(token int64 [R], logprob fp32 [R])``.
+
+    Token ``i`` weighs ``w_i = round(2^43 exp((x_i - max x) / temperature))``.  In the order of the logits, equal ones by their ids, are kept
+
+    * ``top_k``: the first ``top_k`` (0: all);
+    * ``top_p``: of those the ones before which less than ``top_p`` of their sum lies (1: all; the first always);
+    * ``min_p``: of those the ones that weigh at least ``min_p`` of the largest (0: all).
+
+    The token is the first by id with ``sum_{j <= i} w_j > floor(uniform sum_j w_j)`` over what is kept, ``logprob`` is
+    ``log(w_i / sum_j w_j)``.  ``temperature`` 0 is the highest logit, the first of equal ones.  Sums are whole numbers: the same row, settings
+    and random number give the same token in any batch.
+
+    Settings are numbers, or tensors ``[R]``: fp32, ``top_k`` int32.  Of a tensor's rows, ``top_k`` below 0 is 0, ``top_p`` and ``min_p``
+    beyond their range count as its ends, an infinite temperature makes all tokens equal, and ``uniform`` beyond its range takes the first or
+    last kept token that weighs anything.  Tokens at ``inf`` leave the others nothing.  A row of nothing but ``-inf`` has token -1 and
+    ``logprob`` ``-inf``; one with NaN among its logits, settings or ``uniform``, or with a negative temperature, -1 and NaN."""
+    return _lib.bind().sample(logits, uniform, vocab, temperature, top_k, top_p, min_p)
