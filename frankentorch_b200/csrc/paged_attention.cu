@@ -22,19 +22,12 @@
 // cost as much accuracy as the rounding of the output, so each is split into two 16-bit halves, p = hi + lo with an error of
 // 2^-17: for groups of up to 8 heads the lo halves are the rows 8 to 15 of the same instruction, which are idle otherwise.  A lo of
 // 0 makes NaN of an infinite value, so elements that end as NaN are added up again with undivided probabilities (pa_infinite()).
-#include <math.h>
-
-#include "ft_sm100.cuh"
-#include "half_types.cuh"
-#include "launch.cuh"
-#include "ftk_api.h"
-#include "paged_cache.h"
+#include "paged_attn.cuh"
 
 extern "C" int* ftk_status_word(void);
 
 namespace ftk {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;      // of a CTA that shares its SM
 // Tiles of 64 tokens, by the width of the table, up to which a head is left whole: a second launch and the join cost 3 - 4 us, so few heads
 // are cut late, and heads for all SMs fill the time among themselves.  Whole and cut (us) with all positions in use, an SM for each head:
@@ -43,51 +36,10 @@ constexpr int PA_WARPS = 4, PA_TILE = 16 * PA_WARPS;      // of a CTA that share
 // line below these borders: for a dozen heads it cuts from 12 tiles on where 17 would do, and the width stands for lengths that only the
 // device knows, so few tokens under a wide table are cut too (12 heads of 64, 301 tokens: 4.8 us under 5 tiles, 8.9 under 16).
 __host__ inline long long pa_whole(long long heads, long long sms) { return heads <= sms ? 9 + 28 * heads / sms : 20; }
-constexpr int PA_HEADER = 8;                 // ints of a header
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ float exp2_of(float x) {      // within 2^-22; what is below the normal numbers is 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <> __device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // fp16 has five bits of exponent: probabilities are carried times 2^15, so that what underflows is 2^-39 of the largest.
-template <typename T> struct PaShift { static constexpr float value = 0.f; };
-template <> struct PaShift<__half> { static constexpr float value = 15.f; };
-
-struct PagedAttn {
-  FtkPagedAttnDesc d;
-  int group, subs, sub_heads;      // query heads per head of the cache, parts of a group, heads of a part
-  bool by_head;                    // a header per head rather than per CTA: there are fewer
-  int* header;                     // [heads or CTAs][PA_HEADER]: the first CTA or -1, sequence, head, place of the part, last CTA
-  float* parts;                    // [CTAs][2][rows][hd + 2]: accumulators, then maxima and sums
-};
-
-// A place in the list of tiles: tile `t` of `tiles` of unit head `h` (head of the cache times part of the group) of sequence `b`.
-struct Place {
-  int b, h, t, tiles, n;
-};
+template <typename T> struct PaShift { static constexpr int value = 0; };
+template <> struct PaShift<__half> { static constexpr int value = 15; };
 
 // W warps of a CTA: CTAs of an SM, bytes of a warp's ring (three to six stages of 16 tokens)
 template <int ROWS, int HD, int W> struct PaSmem {
@@ -186,40 +138,11 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
     p.n = length(p.b), p.tiles = (p.n + TILE - 1) / TILE;
     left = p.tiles;
   } else {
-    // Every warp for itself: tiles in front of each lane's share of the sequences, then the sequence in which the piece begins
-    const int each = ((int)d.B + 31) / 32, b0 = min((int)d.B, lane * each), b1 = min((int)d.B, b0 + each);
-    long long mine = 0;
-#pragma unroll 4
-    for (int b = b0; b < b1; ++b) mine += (length(b) + TILE - 1) / TILE;
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    total = __shfl_sync(0xffffffffu, upto, 31) * heads;
-    per = max((total + gridDim.x - 1) / gridDim.x, 2ll);      // a part of less than two tiles costs more to join than it saves
-    first_unit = per * blockIdx.x;
-    left = (int)min(per, total - first_unit);
+    Piece piece;
+    p = first_place<TILE>((int)d.B, heads, length, piece);
+    total = piece.total, per = piece.per, first_unit = piece.first, left = piece.left;
     if (!a.by_head && threadIdx.x == 0) a.header[(long long)blockIdx.x * PA_HEADER] = -1;
     if (left <= 0) return;
-    long long front = (upto - mine) * heads;
-    p = {0, 0, 0, 0, 0};
-    const bool here = front <= first_unit && first_unit < upto * heads;
-    if (here) {
-      for (int b = b0; b < b1; ++b) {
-        const int n = length(b), tiles = (n + TILE - 1) / TILE;
-        const long long in = first_unit - front;
-        if (in < (long long)tiles * heads) {
-          p = {b, (int)(in / tiles), (int)(in % tiles), tiles, n};
-          break;
-        }
-        front += (long long)tiles * heads;
-      }
-    }
-    const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-    p.b = __shfl_sync(0xffffffffu, p.b, owner), p.h = __shfl_sync(0xffffffffu, p.h, owner), p.t = __shfl_sync(0xffffffffu, p.t, owner);
-    p.tiles = __shfl_sync(0xffffffffu, p.tiles, owner), p.n = __shfl_sync(0xffffffffu, p.n, owner);
   }
 
   // ---- loads: the ring is filled from a place of its own, which runs ahead over heads and sequences, and the table is read from
@@ -506,95 +429,6 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
   }
 }
 
-// Joins the parts of a head that several CTAs had, if header blockIdx.x is of one: `together` rows from together * blockIdx.y on, and
-// where that leaves threads over, several of them share a row's parts.  Sums are in a fixed order.  And since sequences of no tokens are in
-// nobody's piece, the blocks write them, a sequence each.
-template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
-  constexpr float SHIFT = PaShift<T>::value;
-  constexpr int PART = ROWS * (HD + 2), LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
-  constexpr int FIRST = 4;               // parts whose accumulators a thread requests along with the statistics
-  extern __shared__ float2 part_ml[];    // [parts][together]: maximum and sum, then (factor, -)
-  __shared__ float sums[SLOTS], tops[SLOTS];
-  __shared__ float4 shares[SLOTS][LANES];
-  const FtkPagedAttnDesc& d = a.d;
-  pdl_wait();
-  pdl_trigger();
-  const int* h = a.header + (long long)blockIdx.x * PA_HEADER;
-  const int4 head4 = *reinterpret_cast<const int4*>(h);
-  const int last = h[4], own = a.by_head ? d.lengths[blockIdx.x / (unsigned)(d.Hkv * a.subs)] : 1;
-  const int c = own > 0 ? head4.x : -1;      // (nobody writes the header of a head without tokens)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot_of = threadIdx.x / LANES, quad = threadIdx.x % LANES;
-  if (c >= 0) {
-    const int b = head4.y, head = head4.z, slot = head4.w, n = last - c + 1;
-    const int rows = min(a.sub_heads, a.group - (head % a.subs) * a.sub_heads);
-    const float* first = a.parts + ((long long)c * 2 + slot) * PART;
-    const float* rest = a.parts + (long long)c * 2 * PART;      // part i > 0 is at rest + 2 i PART
-    const auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * PART; };
-    const int r0 = blockIdx.y * together, some = min(together, rows - r0);
-    const int j = slot_of % together, share = slot_of / together, sharing = SLOTS / together;
-    const auto acc_of = [&](int i) { return *reinterpret_cast<const float4*>(part(i) + (r0 + j) * HD + quad * 4); };
-    float4 x[FIRST];
-#pragma unroll
-    for (int k = 0; k < FIRST; ++k)
-      if (j < some && share + k * sharing < n) x[k] = acc_of(share + k * sharing);
-    for (int i = threadIdx.x; i < n * together; i += 256) {
-      const int p = i / together, row = i % together;
-      if (row < some) part_ml[i] = make_float2(part(p)[ROWS * HD + r0 + row], part(p)[ROWS * (HD + 1) + r0 + row]);
-    }
-    __syncthreads();
-    // a warp per row: the largest maximum, every part's factor, the sum
-    for (int row = warp; row < some; row += 8) {
-      float top = -INFINITY;
-      for (int i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i * together + row].x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      for (int i = lane; i < n; i += 32) {
-        float2& ml = part_ml[i * together + row];
-        ml.x = exp2f(ml.x - base);
-        sum += ml.x * ml.y;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) sums[row] = sum, tops[row] = top;
-    }
-    __syncthreads();
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    const auto add = [&](int i, const float4& y) {
-      const float e = part_ml[i * together + j].x;
-      v.x += e * y.x, v.y += e * y.y, v.z += e * y.z, v.w += e * y.w;
-    };
-    if (j < some) {
-#pragma unroll
-      for (int k = 0; k < FIRST; ++k)
-        if (share + k * sharing < n) add(share + k * sharing, x[k]);
-#pragma unroll 8
-      for (int i = share + FIRST * sharing; i < n; i += sharing) add(i, acc_of(i));
-    }
-    shares[slot_of][quad] = v;
-    __syncthreads();
-    if (share == 0 && j < some) {
-      for (int k = 1; k < sharing; ++k) {
-        const float4 y = shares[k * together + j][quad];
-        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-      }
-      const float sum = sums[j], by = sum == 0.f ? 0.f : 1.f / sum;
-      const int q = (head / a.subs) * a.group + (head % a.subs) * a.sub_heads + r0 + j;
-      if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x * by, v.y * by), Half16<T>::down(v.z * by, v.w * by));
-      if (quad == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (tops[j] + log2f(sum) - SHIFT) * LN2;
-    }
-  }
-  for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
-    if (d.lengths[b] > 0) continue;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq * LANES; i += gridDim.y * 256)
-      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + (i / LANES) * d.o_hs + (i % LANES) * 4) = make_uint2(0, 0);
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq; i += gridDim.y * 256) d.lse[(long long)b * d.Hq + i] = -INFINITY;
-  }
-}
-
 struct Plan {
   int subs, sub_heads, rows;
   bool split, alone;               // heads cut into pieces; a CTA per SM, for few heads
@@ -640,14 +474,7 @@ static int launch(const FtkPagedAttnDesc& d, const Plan& p, void* scratch, cudaS
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(PA_WARPS * 32), bytes, s, a, status);
   if (rc || !p.split) return rc;
-  // Few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a head, as far as
-  // shared memory goes.
-  constexpr int slots = 256 / (HD / 4);
-  int together = 1;
-  while (p.heads > 32 && together < p.sub_heads && together < slots && p.ctas * together * 2 * sizeof(float2) <= 40 * 1024)
-    together *= 2;
-  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS>, dim3((unsigned)p.headers, (unsigned)((p.sub_heads + together - 1) / together)), dim3(256),
-                    (size_t)p.ctas * together * sizeof(float2), s, a, together);
+  return launch_join<T, HD, ROWS, PaShift<T>::value>(a, p.heads, p.ctas, p.headers, s);
 }
 
 static bool refused(const FtkPagedAttnDesc* d) {
