@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(W * 32, PaSmem<ROWS, HD, W>::CTAS) paged_attn_
     }
     const bool whole = begun && p.t == p.tiles;
     const int first = row0(p.h), rows = rows_of(p.h);
-    float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * ROWS * (HD + 2) : nullptr;
+    float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * PA_PART<ROWS, HD> : nullptr;
     __syncthreads();
     float scale[RR];                    // of the warp's part: to the maximum of all
 #pragma unroll

@@ -21,41 +21,64 @@ extern "C" int* ftk_status_word(void);
 
 namespace ftk {
 
-constexpr int A8_WARPS = 4, A8_TOKENS = 32;      // of a CTA that shares its SM; tokens that a warp takes at a time
+constexpr int A8_WARPS = 2, A8_TOKENS = 32;      // of a CTA that shares its SM; tokens that a warp takes at a time
 constexpr float A8_SHIFT = 16384.f;
 __host__ inline long long a8_whole(long long heads, long long sms) { return heads <= sms ? 9 + 28 * heads / sms : 20; }
 
+// ROWS query heads of a head of the cache: 1, up to 8 or up to 16
 template <int ROWS, int HD, int W> struct A8Smem {
-  static constexpr int CTAS = W > A8_WARPS ? 1 : (HD == 64 ? 3 : 2);
+  static constexpr bool ONE = ROWS == 1, OWN = W <= A8_WARPS;      // OWN: what is joined in memory of its own, or in the rings of a head that is through
+  static constexpr int CTAS = !OWN ? 1 : (HD == 64 ? (ROWS == 16 ? 6 : 8) : (ROWS == 16 ? 4 : 6));
   static constexpr int DATA = A8_TOKENS * HD * 2, STAGE = DATA + A8_TOKENS * 8;      // keys, values, scales
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = OWN ? 2 : 3;
+  static constexpr int WEIGHT_ROW = 80, TURN = ONE ? A8_TOKENS * 4 + 16 * WEIGHT_ROW : A8_TOKENS * 16;      // of a warp, for what goes from lane to lane
   static constexpr int RING = STAGES * STAGE;
-  static constexpr int COLS = ROWS == 16 && HD == 128 ? 32 : 64;      // columns of the accumulators of all warps that are joined at a time
+  static constexpr int COLS = ONE ? HD : (HD == 128 ? 32 : 64);      // columns of the accumulators of all warps that are joined at a time
   static constexpr int MERGE = W * ROWS * COLS * 4;
-  static constexpr bool OWN = W <= A8_WARPS;                  // in memory of their own, or in the rings of a head that is through
-  static constexpr int BYTES = W * RING + (OWN ? MERGE : 0) + 2 * W * ROWS * 4 + W * STAGES * 4;
+  static constexpr int BYTES = W * (RING + TURN) + (OWN ? MERGE : 0) + 2 * W * ROWS * 4 + W * STAGES * 4;
   static_assert(OWN || MERGE <= W * RING, "the accumulators fit the rings");
+  static_assert(STAGE % 128 == 0, "chunks of a row are exchanged by address bits");
   static_assert(CTAS * (BYTES + 1024) <= 228 * 1024 && BYTES <= 227 * 1024, "the CTAs of an SM share its memory");
 };
-template <int ROWS, int HD> constexpr int A8_ALONE = HD == 64 && ROWS == 8 ? 16 : 8;
+template <int ROWS, int HD> constexpr int A8_ALONE = HD == 64 && ROWS <= 8 ? 16 : 8;
 
+__device__ __forceinline__ uint32_t transposed(uint32_t pair) {      // of 8 x 8 values of 16 bits, two of row lane / 4 in each lane
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(pair));
+  return r;
+}
+__device__ __forceinline__ float max_of(float x) {      // over the warp; NaN is not counted
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 
+// What the loads of a tile take, in 32 bits: with 64 bits of everything and a division for the head they were 100 of 770 instructions
+struct Strides8 {
+  unsigned k_page, k_head, k_row, v_page, v_head, v_row;      // of pages, in 16 bytes
+  unsigned ks_page, ks_head, vs_page, vs_head;                // of scales
+  unsigned n_pages, cols, table_row;
+  int page_shift, block_shift;
+};
+
 template <typename T, int HD, int ROWS, bool SPLIT, int W>
-__global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_e4m3_kernel(const __grid_constant__ PagedAttn a, int* status) {
+__global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_e4m3_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ Strides8 by, int* status) {
   typedef A8Smem<ROWS, HD, W> SM;
   static_assert(!SPLIT || SM::OWN, "a piece goes on while the parts are joined");
   constexpr int N = A8_TOKENS, TILE = N * W;
   constexpr int STAGES = SM::STAGES, STAGE = SM::STAGE, CH = HD / 16, NT = HD / 8;      // CH: 16-byte chunks of a row
-  constexpr int RR = ROWS / 8;
+  constexpr int RR = ROWS == 16 ? 2 : 1;      // eights of query heads
+  constexpr bool ONE = SM::ONE;
   extern __shared__ __align__(256) unsigned char smem[];
   const FtkPagedAttnDesc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = (int)d.Hkv * a.subs;
   unsigned char* ring = smem + warp * SM::RING;
-  float* merge = reinterpret_cast<float*>(smem + (SM::OWN ? W * SM::RING : 0));
-  float* stat = reinterpret_cast<float*>(smem + W * SM::RING + (SM::OWN ? SM::MERGE : 0));                                     // [2][warps][ROWS]
+  unsigned char* turn = smem + W * SM::RING + warp * SM::TURN;      // ONE: scores, then 16 rows of weights; else the scales of each token
+  float* merge = reinterpret_cast<float*>(smem + (SM::OWN ? W * (SM::RING + SM::TURN) : 0));
+  float* stat = reinterpret_cast<float*>(smem + W * (SM::RING + SM::TURN) + (SM::OWN ? SM::MERGE : 0));      // [2][warps][ROWS]
   unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * W * ROWS) + warp * STAGES;
   const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
   const auto length = [&](int b) {
@@ -116,8 +139,9 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
     if (to_look > 0) {
       const int tok = g.t * TILE + tok_of;
       if (tok < g.n) {
-        page = (int)paged_page(table, g.b, tok);
-        if (page < 0) ft_index_ok(-1, 1, status);
+        const unsigned col = (unsigned)tok >> by.page_shift;
+        page = col < by.cols ? d.table[(unsigned long long)(unsigned)g.b * by.table_row + col] : -1;
+        if ((unsigned)page >= by.n_pages) page = -1, ft_index_ok(-1, 1, status);
       }
       advance(g, to_look);
     }
@@ -129,53 +153,62 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
   const int lrow = lane / CH, lchunk = lane % CH;
   constexpr int RSTEP = 32 / CH, COPIES = N / RSTEP;      // rows of a copy of the warp, copies of 32 rows
   const uint32_t lane_at = lrow * HD, lane_sw = lchunk << 4;
-  const long long k_lane = lrow * d.kp_rs + lchunk * 16, v_lane = lrow * d.vp_rs + lchunk * 16;
+  const bool packed = by.k_row == HD / 16 && by.v_row == HD / 16;
+  const auto offset = [](unsigned page, unsigned s_page, unsigned head, unsigned s_head, unsigned row, unsigned s_row) {
+    return (unsigned long long)page * s_page + (unsigned long long)head * s_head + (unsigned long long)row * s_row;
+  };
   const auto load = [&](int stage) {
     const int pages = page_of[0];
 #pragma unroll
     for (int i = 0; i + 1 < AHEAD; ++i) page_of[i] = page_of[i + 1];
     page_of[AHEAD - 1] = look();
     if (to_load > 0) {
-      const int head = f.h / a.subs, tok0 = f.t * TILE + warp * N;
-      const unsigned char* kb = (const unsigned char*)d.k_pages + head * d.kp_hs;
-      const unsigned char* vb = (const unsigned char*)d.v_pages + head * d.vp_hs;
+      const int tok0 = f.t * TILE + warp * N;
+      const unsigned f_kv = a.subs == 1 ? f.h : f.h / a.subs;      // head of the cache
+      const uint4 *const keys = (const uint4*)d.k_pages + lchunk, *const values = (const uint4*)d.v_pages + lchunk;
+      const unsigned in_page = (1u << by.page_shift) - 1;
       const uint32_t dst = ring_s + stage * STAGE + lane_at, sdst = ring_s + stage * STAGE + SM::DATA + lane * 4;
-      unsigned ok;
+      unsigned ok, own_row;             // this lane's own token: its row in its page, its page
+      int own_page;
       if (one_page) {
         const int n = pages < 0 ? 0 : min(N, f.n - tok0);      // rows that are there
-        const long long page = pages < 0 ? 0 : pages, in = paged_row(table, tok0);
-        ok = n >= N ? 0xffffffffu : (1u << n) - 1;
-        const unsigned char* k = kb + page * d.kp_ps + in * d.kp_rs + k_lane;
-        const unsigned char* v = vb + page * d.vp_ps + in * d.vp_rs + v_lane;
-        const long long k_step = RSTEP * d.kp_rs, v_step = RSTEP * d.vp_rs;
+        const unsigned page = pages < 0 ? 0u : (unsigned)pages, in = (unsigned)tok0 & in_page;
+        ok = n >= N ? 0xffffffffu : (1u << max(n, 0)) - 1;
+        const uint4* k = keys + offset(page, by.k_page, f_kv, by.k_head, in + lrow, by.k_row);
+        const uint4* v = values + offset(page, by.v_page, f_kv, by.v_head, in + lrow, by.v_row);
+        if (packed && n >= N) {         // one run of bytes, all of it there
 #pragma unroll
-        for (int c = 0; c < COPIES; ++c) {
-          const bool t = c * RSTEP + lrow < n;
-          const uint32_t at = dst + c * RSTEP * HD + (lane_sw ^ (swizzle(c * RSTEP + lrow) << 4));
-          copy16(at, t ? k : kb, t);
-          copy16(at + N * HD, t ? v : vb, t);
-          k += k_step, v += v_step;
+          for (int c = 0; c < COPIES; ++c) {
+            const uint32_t at = dst + c * RSTEP * HD + (lane_sw ^ (swizzle(c * RSTEP + lrow) << 4));
+            copy16(at, k + c * 32, true);
+            copy16(at + N * HD, v + c * 32, true);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < COPIES; ++c) {
+            const bool t = c * RSTEP + lrow < n;
+            const uint32_t at = dst + c * RSTEP * HD + (lane_sw ^ (swizzle(c * RSTEP + lrow) << 4));
+            copy16(at, t ? k + (unsigned long long)(c * RSTEP) * by.k_row : keys, t);
+            copy16(at + N * HD, t ? v + (unsigned long long)(c * RSTEP) * by.v_row : values, t);
+          }
         }
-        const bool t = lane < n;
-        const long long block = t ? (in + lane) >> d.block_shift : 0;
-        copy4(sdst, d.k_scales + page * d.ks_ps + head * d.ks_hs + block, t);
-        copy4(sdst + N * 4, d.v_scales + page * d.vs_ps + head * d.vs_hs + block, t);
+        own_page = lane < n ? (int)page : -1, own_row = in + lane;
       } else {
         ok = __ballot_sync(0xffffffffu, pages >= 0);
 #pragma unroll
         for (int c = 0; c < COPIES; ++c) {
-          const int row = c * RSTEP + lrow;
-          const long long page = __shfl_sync(0xffffffffu, pages, row), in = paged_row(table, tok0 + row);
+          const int row = c * RSTEP + lrow, page = __shfl_sync(0xffffffffu, pages, row);
+          const unsigned in = (unsigned)(tok0 + row) & in_page;
           const bool t = page >= 0;
           const uint32_t at = dst + c * RSTEP * HD + (lane_sw ^ (swizzle(row) << 4));
-          copy16(at, t ? kb + page * d.kp_ps + in * d.kp_rs + lchunk * 16 : kb, t);
-          copy16(at + N * HD, t ? vb + page * d.vp_ps + in * d.vp_rs + lchunk * 16 : vb, t);
+          copy16(at, t ? keys + offset(page, by.k_page, f_kv, by.k_head, in, by.k_row) : keys, t);
+          copy16(at + N * HD, t ? values + offset(page, by.v_page, f_kv, by.v_head, in, by.v_row) : values, t);
         }
-        const bool t = pages >= 0;
-        const long long page = t ? pages : 0, block = t ? paged_row(table, tok0 + lane) >> d.block_shift : 0;
-        copy4(sdst, d.k_scales + page * d.ks_ps + head * d.ks_hs + block, t);
-        copy4(sdst + N * 4, d.v_scales + page * d.vs_ps + head * d.vs_hs + block, t);
+        own_page = pages, own_row = (unsigned)(tok0 + lane) & in_page;
       }
+      const bool t = own_page >= 0;
+      copy4(sdst, t ? d.k_scales + offset(own_page, by.ks_page, f_kv, by.ks_head, own_row >> by.block_shift, 1) : d.k_scales, t);
+      copy4(sdst + N * 4, t ? d.v_scales + offset(own_page, by.vs_page, f_kv, by.vs_head, own_row >> by.block_shift, 1) : d.v_scales, t);
       if (lane == 0) there[stage] = ok;
       advance(f, to_load);
     }
@@ -194,8 +227,8 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
   for (int s = 0; s < STAGES - 1; ++s) load(s);
 
   // ---- tiles
-  uint32_t q[CH][2 * RR];               // of chunk c: elements 4 c0' .. + 3 of row r0, then of row r0 + 8
-  float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, sc[2] = {0.f, 0.f};
+  uint32_t q[CH][2 * RR];               // of chunk c: elements 2 c0 .. + 3 of head r0, then of head r0 + 8
+  float acc[NT][4], m[2 * RR], l[2 * RR], sc[2 * RR];      // of heads c0, c0 + 1, c0 + 8, c0 + 9; ONE: [0], of all lanes
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
   const auto begin = [&]() {            // queries of the head at `p`; rows beyond the group are zero
     const int first = row0(p.h), rows = rows_of(p.h);
@@ -215,7 +248,9 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
       const float by = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-      sc[r] = (float)d.scale * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      const float own = (float)d.scale * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      sc[2 * r] = __shfl_sync(0xffffffffu, own, ONE ? 0 : c0 * 4);
+      sc[2 * r + 1] = __shfl_sync(0xffffffffu, own, c0 * 4 + 4);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const float2 x = Half16<T>::up(u[c].x), y = Half16<T>::up(u[c].y);
@@ -226,90 +261,129 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int r = 0; r < 2 * RR; ++r) m[r] = -INFINITY, l[r] = 0.f;
   };
   bool begun = p.t == 0;                // the piece has the beginning of the head at `p`
   int parts = 0;
   begin();
   // this lane's row for ldmatrix: of four groups of eight tokens at one chunk
   const uint32_t l_at = lane * HD + (swizzle(lane) << 4);
+  // ONE: the row of weights that this lane addresses, of 16 rows at the first eight tokens and 16 at the next; all but two rows stay 0
+  const uint32_t weights_at = smem_u32(turn) + N * 4 + (lane & 15) * SM::WEIGHT_ROW + (lane >> 4) * 16;
+  if (ONE) {
+    for (int i = lane; i < SM::TURN / 4; i += 32) reinterpret_cast<uint32_t*>(turn)[i] = 0;
+  }
   int stage = 0;
   for (bool more = true; more; more = left > 0) {
     if (left > 0) {
       copy_wait<STAGES - 2>();
       __syncwarp();
       const uint32_t ks = ring_s + stage * STAGE + l_at, vs = ks + N * HD;
-      const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);
       const unsigned ok = there[stage];
-      const int refill = stage == 0 ? STAGES - 1 : stage - 1;
-      float s[4][4] = {};
+      load(stage == 0 ? STAGES - 1 : stage - 1);      // the stage that the tile before left: its reads are behind the warp's barrier
+      const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);      // keys', values', the values' exponents
+      const float k_scale = scales[lane], v_scale = scales[N + lane], v_exp = (float)max((int)(__float_as_uint(v_scale) >> 23 & 255) - 127, -100);
+      if (!ONE) reinterpret_cast<float4*>(turn)[lane] = make_float4(k_scale, v_exp, v_scale * A8_SHIFT, 0.f);
+      // Scores with the tokens as rows: s[2 r + t] of tokens 16 t and on, the r-th eight heads
+      float s[2 * RR][4] = {};
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        uint32_t b[4];
+        uint32_t b[4], lower[4], upper[4];
         ldm4(ks ^ (c << 4), b);
-        const uint32_t qa[4] = {q[c][0], ROWS == 16 ? q[c][2 * RR - 2] : 0u, q[c][1], ROWS == 16 ? q[c][2 * RR - 1] : 0u};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma16<__half>(s[j], qa, e4m3_up(b[j] & 0xffffu), e4m3_up(b[j] >> 16));
-      }
-      load(refill);                     // the stage that the tile before left: its reads are behind the warp's barrier
-      // masked scores, and the larger maximum of the row's tokens and what was there
-      float kf[8], vf[8], lv[8];        // of this thread's tokens: 8 j + c0, + 1
+        for (int j = 0; j < 4; ++j) lower[j] = e4m3_up(b[j] & 0xffffu), upper[j] = e4m3_up(b[j] >> 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = *reinterpret_cast<const float2*>(scales + j * 8 + c0), y = *reinterpret_cast<const float2*>(scales + N + j * 8 + c0);
-        kf[2 * j] = x.x, kf[2 * j + 1] = x.y, vf[2 * j] = y.x, vf[2 * j + 1] = y.y;
-      }
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t k[4] = {lower[2 * u], lower[2 * u + 1], upper[2 * u], upper[2 * u + 1]};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lv[i] = (float)max((int)(__float_as_uint(vf[i]) >> 23 & 255) - 127, -100);
-        vf[i] *= A8_SHIFT;
-      }
-      uint32_t hi[2][4] = {}, lo[2][4] = {};      // of two steps of 16 tokens
-      float grow[2];
-      bool moved = false;
-#pragma unroll
-      for (int r = 0; r < RR; ++r) {
-        float x[8], top = m[r];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[i >> 1][2 * r + (i & 1)] * (kf[i] * sc[r]);
-        if (ok != 0xffffffffu) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (!(ok >> ((i >> 1) * 8 + c0 + (i & 1)) & 1u)) x[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i] + lv[i]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float base = top == -INFINITY ? 0.f : top;
-        moved |= top != m[r];
-        grow[r] = exp2_of(m[r] - base);
-        m[r] = top;
-        float e[8], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          e[i] = exp2_of(x[i] - base), e[i + 1] = exp2_of(x[i + 1] - base);
-          sum += e[i] + e[i + 1];
-          e[i] *= vf[i], e[i + 1] *= vf[i + 1];
-        }
-        l[r] = l[r] * grow[r] + sum;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {      // tokens 8 j and on: step j / 2, its first or second half
-          const uint32_t h = Half16<__half>::down(e[2 * j], e[2 * j + 1]);
-          const float2 u = Half16<__half>::up(h);
-          hi[j >> 1][(j & 1) * 2 + r] = h;
-          lo[j >> 1][(j & 1) * 2 + r] = Half16<__half>::down(e[2 * j] - u.x, e[2 * j + 1] - u.y);
+          for (int r = 0; r < RR; ++r) mma16<__half>(s[2 * r + u], k, q[c][2 * r], q[c][2 * r + 1]);
         }
       }
-      if (__any_sync(0xffffffffu, moved)) {
-        const float g0 = grow[0], g1 = ROWS == 16 ? grow[RR - 1] : grow[0];
+      uint32_t hi[2][4] = {}, lo[2][4] = {};      // weights of two steps of 16 tokens
+      if constexpr (ONE) {
+        // the one head's scores, in every fourth lane, go to a token per lane, their weights to the rows 0 (hi) and 8 (lo) of an operand
+        float* score = reinterpret_cast<float*>(turn);
+        unsigned short* weight = reinterpret_cast<unsigned short*>(turn + N * 4);
+        if (c0 == 0) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i][0] *= g0, acc[i][1] *= g0, acc[i][2] *= g1, acc[i][3] *= g1;
-      }
-      if (ROWS != 16) {
+          for (int u = 0; u < 2; ++u) score[16 * u + r0] = s[u][0], score[16 * u + 8 + r0] = s[u][2];
+        }
+        __syncwarp();
+        const float x = ok >> lane & 1u ? score[lane] * (k_scale * sc[0]) : -INFINITY;
+        const float top = fmaxf(m[0], max_of(x + v_exp)), base = top == -INFINITY ? 0.f : top, e = exp2_of(x - base), w = e * (v_scale * A8_SHIFT);
+        if (top != m[0]) {
+          const float grow = exp2_of(m[0] - base);
+          l[0] *= grow;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) hi[t][1] = lo[t][0], hi[t][3] = lo[t][2];
+          for (int i = 0; i < NT; ++i) acc[i][0] *= grow, acc[i][1] *= grow, acc[i][2] *= grow, acc[i][3] *= grow;
+          m[0] = top;
+        }
+        l[0] += e;
+        const __half h = __float2half_rn(w);
+        weight[lane] = __half_as_ushort(h);
+        weight[8 * (SM::WEIGHT_ROW / 2) + lane] = __half_as_ushort(__float2half_rn(w - __half2float(h)));
+        __syncwarp();
+        ldm4(weights_at, hi[0]);
+        ldm4(weights_at + 32, hi[1]);
+      } else {
+        // masked scores of heads c0, c0 + 1 at tokens r0, r0 + 8 .., and the larger maximum of the head's tokens and what was there
+        __syncwarp();
+        float grow[2 * RR], v14[4];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+          float x[4][2], top[2] = {m[2 * r], m[2 * r + 1]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {        // token 8 i + r0: key's scale, exponent of the value's, that times 2^14
+            const float4 f = reinterpret_cast<const float4*>(turn)[8 * i + r0];
+            v14[i] = f.z;
+            const bool there = ok >> (8 * i + r0) & 1u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              x[i][e] = there ? s[2 * r + (i >> 1)][(i & 1) * 2 + e] * (f.x * sc[2 * r + e]) : -INFINITY;
+              top[e] = fmaxf(top[e], x[i][e] + f.y);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
+            const float base = top[e] == -INFINITY ? 0.f : top[e];
+            moved |= top[e] != m[2 * r + e];
+            grow[2 * r + e] = exp2_of(m[2 * r + e] - base);
+            m[2 * r + e] = top[e];
+            l[2 * r + e] *= grow[2 * r + e];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[i][e] = exp2_of(x[i][e] - base);
+              l[2 * r + e] += x[i][e];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {        // to rows of heads: step i / 2, its first or second eight tokens
+            const float w0 = x[i][0] * v14[i], w1 = x[i][1] * v14[i];
+            const uint32_t h = Half16<__half>::down(w0, w1);
+            const float2 u = Half16<__half>::up(h);
+            hi[i >> 1][(i & 1) * 2 + r] = transposed(h);
+            lo[i >> 1][(i & 1) * 2 + r] = transposed(Half16<__half>::down(w0 - u.x, w1 - u.y));
+          }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+          float g[2];                          // of the accumulators' rows r0 and r0 + 8
+#pragma unroll
+          for (int r = 0; r < RR; ++r) {
+            const float even = __shfl_sync(0xffffffffu, grow[2 * r], r0 >> 1), odd = __shfl_sync(0xffffffffu, grow[2 * r + 1], r0 >> 1);
+            g[r] = r0 & 1 ? odd : even;
+          }
+          if (RR == 1) g[1] = g[0];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) acc[i][0] *= g[0], acc[i][1] *= g[0], acc[i][2] *= g[1], acc[i][3] *= g[1];
+        }
+        if (RR == 1) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) hi[u][1] = lo[u][0], hi[u][3] = lo[u][2];
+        }
       }
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -336,25 +410,28 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
 
     // ---- the end of a head, or of the piece: the warps' parts become one
 #pragma unroll
-    for (int r = 0; r < RR; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if ((lane & 3) == 0) {
-        stat[warp * ROWS + r * 8 + r0] = m[r];
-        stat[(W + warp) * ROWS + r * 8 + r0] = l[r];
+    for (int r = 0; r < (ONE ? 1 : 2 * RR); ++r) {
+#pragma unroll
+      for (int o = ONE ? 1 : 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+      if (r0 == 0 && (!ONE || c0 == 0)) {
+        const int head = ONE ? 0 : (r >> 1) * 8 + c0 + (r & 1);
+        stat[warp * ROWS + head] = m[r];
+        stat[(W + warp) * ROWS + head] = l[r];
       }
     }
     const bool whole = begun && p.t == p.tiles;
     const int first = row0(p.h), rows = rows_of(p.h);
-    float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * ROWS * (HD + 2) : nullptr;
+    float* part = SPLIT ? a.parts + ((long long)blockIdx.x * 2 + parts) * PA_PART<ROWS, HD> : nullptr;
     __syncthreads();
     float scale[RR];                    // of the warp's part: to the maximum of all, without the 2^14
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      float top = m[r];
+      const int head = ONE ? 0 : r * 8 + r0;
+      const float own = stat[warp * ROWS + head];
+      float top = own;
 #pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w * ROWS + r * 8 + r0]);
-      scale[r] = exp2f(m[r] - (top == -INFINITY ? 0.f : top)) * (1.f / A8_SHIFT);
+      for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w * ROWS + head]);
+      scale[r] = exp2f(own - (top == -INFINITY ? 0.f : top)) * (1.f / A8_SHIFT);
     }
     // all columns of a few rows at once, else some of all rows
     const int cols = rows * HD <= ROWS * SM::COLS ? HD : SM::COLS;
@@ -431,7 +508,7 @@ static Plan8 plan_of(const FtkPagedAttnDesc& d) {
   const long long group = d.Hq / d.Hkv;
   p.subs = (int)((group + 15) / 16);
   p.sub_heads = (int)((group + p.subs - 1) / p.subs);
-  p.rows = p.sub_heads <= 8 ? 8 : 16;
+  p.rows = p.sub_heads == 1 ? 1 : (p.sub_heads <= 8 ? 8 : 16);
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -441,9 +518,10 @@ static Plan8 plan_of(const FtkPagedAttnDesc& d) {
   p.alone = p.heads <= sms;
   p.split = tiles > a8_whole(p.heads, sms);
   if (p.split) {
-    p.ctas = (d.hd == 64 ? (p.rows == 8 ? A8_CTAS<8, 64> : A8_CTAS<16, 64>) : (p.rows == 8 ? A8_CTAS<8, 128> : A8_CTAS<16, 128>)) * (long long)sms;
+    p.ctas = (d.hd == 64 ? (p.rows == 1 ? A8_CTAS<1, 64> : p.rows == 8 ? A8_CTAS<8, 64> : A8_CTAS<16, 64>)
+                         : (p.rows == 1 ? A8_CTAS<1, 128> : p.rows == 8 ? A8_CTAS<8, 128> : A8_CTAS<16, 128>)) * (long long)sms;
     p.headers = p.heads < p.ctas ? p.heads : p.ctas;
-    p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * p.rows * (d.hd + 2) * 4;
+    p.bytes = p.headers * PA_HEADER * 4 + p.ctas * 2 * (p.rows * (d.hd + 2) + 2) * 4;
   }
   return p;
 }
@@ -452,25 +530,37 @@ template <typename T, int HD, int ROWS>
 static int launch(const FtkPagedAttnDesc& d, const Plan8& p, void* scratch, cudaStream_t s) {
   PagedAttn a = {d, (int)(d.Hq / d.Hkv), p.subs, p.sub_heads, p.heads < p.ctas, (int*)scratch, nullptr};
   a.parts = (float*)((char*)scratch + p.headers * PA_HEADER * 4);
+  const Strides8 by = {(unsigned)(d.kp_ps >> 4), (unsigned)(d.kp_hs >> 4), (unsigned)(d.kp_rs >> 4), (unsigned)(d.vp_ps >> 4), (unsigned)(d.vp_hs >> 4),
+                       (unsigned)(d.vp_rs >> 4), (unsigned)d.ks_ps, (unsigned)d.ks_hs, (unsigned)d.vs_ps, (unsigned)d.vs_hs, (unsigned)d.n_pages,
+                       (unsigned)d.table_cols, (unsigned)d.table_stride, (int)d.page_shift, (int)d.block_shift};
   int* status = ftk_status_word();
   if (!p.split && p.alone) {
     constexpr int W = A8_ALONE<ROWS, HD>, bytes = A8Smem<ROWS, HD, W>::BYTES;
     const auto kernel = paged_attn_e4m3_kernel<T, HD, ROWS, false, W>;
     const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return rc ? rc : launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(W * 32), bytes, s, a, status);
+    return rc ? rc : launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(W * 32), bytes, s, a, by, status);
   }
   constexpr int bytes = A8Smem<ROWS, HD, A8_WARPS>::BYTES;
   const auto whole = paged_attn_e4m3_kernel<T, HD, ROWS, false, A8_WARPS>, split = paged_attn_e4m3_kernel<T, HD, ROWS, true, A8_WARPS>;
   const auto kernel = p.split ? split : whole;
   int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (rc) return rc;
-  rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(A8_WARPS * 32), bytes, s, a, status);
+  rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(A8_WARPS * 32), bytes, s, a, by, status);
   if (rc || !p.split) return rc;
   return launch_join<T, HD, ROWS, 0>(a, p.heads, p.ctas, p.headers, s);
 }
 
+// Strides of 64 GB and more are refused: offsets are 32 bits times 16 bytes (4 of scales and of the table) of each kind, added up in 64
+static bool wide(const FtkPagedAttnDesc* d) {
+  const long long most = 0xffffffffll;
+  for (long long s : {d->kp_ps, d->kp_hs, d->kp_rs, d->vp_ps, d->vp_hs, d->vp_rs})
+    if (s < 0 || s >> 4 > most) return true;
+  for (long long s : {d->ks_ps, d->ks_hs, d->vs_ps, d->vs_hs, d->table_stride})
+    if (s < 0 || s > most) return true;
+  return false;
+}
 static bool refused(const FtkPagedAttnDesc* d) {
-  return !d || d->B <= 0 || d->B > (1 << 30) || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > (1 << 20) || (d->hd != 64 && d->hd != 128) ||
+  return !d || wide(d) || d->B <= 0 || d->B > (1 << 30) || d->Hkv <= 0 || d->Hq <= 0 || d->Hq % d->Hkv || d->Hq > (1 << 20) || (d->hd != 64 && d->hd != 128) ||
          (d->type != FTK_T_BF16 && d->type != FTK_T_FP16) || d->page_shift < 0 || d->page_shift > 30 || d->table_cols <= 0 ||
          d->table_cols > (0x7fffff00ll >> d->page_shift) || d->n_pages <= 0 || d->n_pages > 0x7fffffff || d->B * d->Hq > 0x7fffffff ||
          d->B * d->Hq * (((d->table_cols << d->page_shift) >> 6) + 1) > (1ll << 38) ||      // a CTA counts its tiles in 32 bits
@@ -488,6 +578,10 @@ extern "C" int ftk_paged_attn_e4m3(const FtkPagedAttnDesc* d, void* scratch, voi
   if (p.split && !scratch) return -2;
   cudaStream_t s = (cudaStream_t)stream;
   const bool bf = d->type == FTK_T_BF16;
+  if (p.rows == 1) {
+    if (d->hd == 64) return bf ? launch<__nv_bfloat16, 64, 1>(*d, p, scratch, s) : launch<__half, 64, 1>(*d, p, scratch, s);
+    return bf ? launch<__nv_bfloat16, 128, 1>(*d, p, scratch, s) : launch<__half, 128, 1>(*d, p, scratch, s);
+  }
   if (p.rows == 8) {
     if (d->hd == 64) return bf ? launch<__nv_bfloat16, 64, 8>(*d, p, scratch, s) : launch<__half, 64, 8>(*d, p, scratch, s);
     return bf ? launch<__nv_bfloat16, 128, 8>(*d, p, scratch, s) : launch<__half, 128, 8>(*d, p, scratch, s);

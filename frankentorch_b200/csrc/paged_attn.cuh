@@ -47,8 +47,9 @@ struct PagedAttn {
   int group, subs, sub_heads;      // query heads per head of the cache, parts of a group, heads of a part
   bool by_head;                    // a header per head rather than per CTA: there are fewer
   int* header;                     // [heads or CTAs][PA_HEADER]: the first CTA or -1, sequence, head, place of the part, last CTA
-  float* parts;                    // [CTAs][2][rows][hd + 2]: accumulators, then maxima and sums
+  float* parts;                    // [CTAs][2][PA_PART]: accumulators, then maxima and sums
 };
+template <int ROWS, int HD> constexpr int PA_PART = (ROWS * (HD + 2) + 3) / 4 * 4;      // floats of a part: the next one starts on 16 bytes
 
 // A place in the list of tiles: tile `t` of `tiles` of unit head `h` (head of the cache times part of the group) of sequence `b`.
 struct Place {
@@ -103,7 +104,7 @@ __device__ __forceinline__ Place first_place(const int B, const int heads, const
 // nobody's piece, the blocks write them, a sequence each.  Sums and accumulators are carried times 2^SHIFT.
 template <typename T, int HD, int ROWS, int SHIFT>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
-  constexpr int PART = ROWS * (HD + 2), LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
+  constexpr int PART = PA_PART<ROWS, HD>, LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
   constexpr int FIRST = 4;               // parts whose accumulators a thread requests along with the statistics
   extern __shared__ float2 part_ml[];    // [parts][together]: maximum and sum, then (factor, -)
   __shared__ float sums[SLOTS], tops[SLOTS];
