@@ -457,6 +457,7 @@ typedef struct FtkSampleDesc {
   long long k;
   long long* token;         // [R]
   float* logprob;           // [R]
+  long long cluster;        // set by the launcher
 } FtkSampleDesc;
 int ftk_sample(const FtkSampleDesc* d, void* stream);
 #ifdef __cplusplus
