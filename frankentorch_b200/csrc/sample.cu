@@ -5,16 +5,20 @@
 // order of their logits (equal ones by their ids): the first k; of those the ones before which less than p of the sum lies; of those the
 // ones of at least min_p of the largest; then the first by id whose running sum passes u times the sum.
 //
-// What bounds it: each logit is read once.  Weights take 9 operations in 64 bits, half the rate of fp32.
+// What bounds it: each logit is read once.  A weight takes 9 operations in 64 bits, at half the rate of fp32, so where all are needed they are
+// next: with what is around them 6 to 7 cycles of an SM for 32.
 //
 // Work.  A cluster of CTAs has a row, each an equal run of its columns, which it keeps in shared memory (rows of more than that are read
-// again from L2): everything behind the first pass works there.  Sums, histograms and lists of the CTAs are read by all of them over
-// distributed shared memory, and all come to the same conclusions.
-//   * The k largest of a small k are among the elements that reach the k-th largest of the threads' own maxima: hardly more than k.
-//     They become a list, ordered by counting, and the rest is done on it.
-//   * Else the border of top-k and of top-p is found by counts of 2048 equal steps of the logits' range: the step with the border is
-//     looked into, with the sums of weights in it and above it, until it is one value or a short list.  Its equal elements are taken by id.
+// again from L2): everything behind the first pass works there.  The CTAs read one another's sums, histograms and lists over
+// distributed shared memory, a warp of each for all of it, and come to the same conclusions.
+//   * The k largest of a small k are among the elements that reach the k-th largest of 512 maxima, of as many parts of the row: hardly more
+//     than k.  They become a list, ordered by counting, and the rest is done on it by one CTA.
+//   * Else the border of top-k and of top-p is looked for in two steps: counts of 2048 equal steps of the logits' range say between which
+//     two logits it is, and the elements between them are set aside.  For top-p the same pass has the sum of all weights and of those
+//     above, the only time that all weights are formed.  What is set aside is divided further until it is one value, whose elements are
+//     taken by their ids, or a short list.
 //   * The choice: sums per warp in the order of the ids, the warp with the target, the 32 vectors, the lane.
+// The random sums of shared memory's counters take 10 cycles of an SM for 32 elements; collectives of a cluster 1500 cycles each.
 #include <math.h>
 
 #include "ft_sm100.cuh"
@@ -26,11 +30,13 @@ namespace ftk {
 
 typedef unsigned long long u64;
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
-constexpr int SA_BINS = 2048;          // steps of a histogram
-constexpr int SA_LIST = 512;           // elements of a list
+constexpr int SA_BINS = 2048;          // steps of a histogram of counts
+constexpr int SA_FINE = 1024;          // steps among the elements set aside
+constexpr int SA_ASIDE = 2048;         // elements that a CTA can set aside
+constexpr int SA_LIST = 512;           // elements of a list: one per thread
 constexpr int SA_CLUSTER = 8;          // CTAs of a row at most
-constexpr int SA_STEPS = 512;          // vectors of a lane at most
-constexpr int SA_SHARE = 72 * 1024;    // bytes of a row that a CTA keeps at most: two CTAs share an SM
+constexpr int SA_STEPS = 64;           // vectors of a lane at most
+constexpr int SA_SHARE = 64 * 1024;    // bytes of a row that a CTA keeps at most: two CTAs share an SM
 
 template <typename T> __device__ __forceinline__ void logits_of(const uint4& v, float (&x)[8]) { up8<T>(v, x); }
 template <typename T> __device__ __forceinline__ void logits_of(const uint4& v, float (&x)[4]) {
@@ -97,17 +103,31 @@ template <typename V> __device__ __forceinline__ V warp_upto(V v) {      // runn
   }
   return v;
 }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 struct SampleShared {
-  u64 sums[2][SA_WARPS + 8];           // per warp, published; then the CTA's
-  u64 steps[SA_STEPS];
+  u64 aside[SA_ASIDE];                 // order and inverted id, as in a list
+  union {
+    u64 mass[SA_FINE];                 // published: sums of weights per step
+    struct {
+      u64 sorted[SA_LIST], value[SA_LIST];
+    };
+  };
+  u64 list[SA_LIST];                   // published
   double table[256];                   // 2^(i / 256)
-  u64 list[SA_LIST], all[SA_LIST], sorted[SA_LIST], weights[SA_LIST];
-  uint32_t hist[SA_BINS], total[SA_BINS];
-  u64 found[4], mass[SA_WARPS];
-  uint32_t words[2][4];                // published: minima and maxima of the CTA
-  uint32_t part[SA_WARPS];
-  uint32_t count[2];                   // of the list
+  u64 steps[SA_STEPS];
+  u64 sums[2][SA_WARPS];               // published: per warp, in the order of the ids
+  u64 words[2][4];                     // published: of the CTA
+  u64 record[2][2];                    // published: what the CTA with it has found
+  u64 part[SA_WARPS][4];               // of the CTA's warps
+  u64 got[8];                          // what all threads learn
+  uint32_t hist[SA_BINS];              // published: counts per step
+  uint32_t maxima[SA_THREADS];         // published: of parts of the row
+  uint32_t n_list, n_aside;
 };
 
 // A row's settings.  2^43 exp((x - top) / T): 2^(k / 256) out of the table, the rest by three terms of the exponential series (relative
@@ -116,7 +136,7 @@ struct Weigh {
   const double* table;
   double top, by;                      // 256 log2(e) / T
   float floor;                         // what is below weighs less than half a unit
-  __device__ __forceinline__ u64 operator()(float x) const {
+  __device__ __forceinline__ u64 operator()(float x) const {      // x >= floor
     constexpr double MAGIC = 6755399441055744.0;      // 1.5 2^52
     const double d = (double)x - top, kd = fma(d, by, MAGIC), r = fma(d, by, MAGIC - kd);
     const int k = __double2loint(kd);
@@ -124,8 +144,7 @@ struct Weigh {
     const double p = r * fma(r, fma(r, C * C * C / 6, C * C / 2), C), t = table[k & 255];
     double v = fma(t, p, t);
     v = __hiloint2double(__double2hiint(v) + (k >> 8) * (1 << 20), __double2loint(v));
-    const u64 w = (u64)__double_as_longlong(v + 512.0) - 0x4080000000000000ull;
-    return x >= floor ? w : 0;
+    return (u64)__double_as_longlong(v + 512.0) - 0x4080000000000000ull;
   }
 };
 
@@ -136,13 +155,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
   uint4* kept_row = reinterpret_cast<uint4*>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = (int)d.V;
-  const int rank = (int)cluster_rank(), C = (int)d.cluster;
-  const long long r = blockIdx.x / C;
+  const int rank = (int)cluster_rank(), C = (int)d.cluster;      // C: a power of two
+  const long long r = blockIdx.x / (unsigned)C;
   const int begin = (rank * SA_WARPS + warp) * its * STEP;      // this warp's run of columns
   const int mine = max(0, min(its, (V - begin + STEP - 1) / STEP));
   if (tid < 256) s.table[tid] = exp2(tid * (1.0 / 256));
   for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
-  if (tid < 2) s.count[tid] = 0;
+  if (tid == 0) s.n_list = s.n_aside = 0;
   pdl_wait();
   pdl_trigger();
   const T* row = (const T*)d.logits + r * d.ld;
@@ -161,19 +180,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       if (first + i < V) e[i] = row[first + i];
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  // ---- the row comes in: largest and smallest finite elements
+  // ---- the row comes in: its largest element, and about its smallest finite one
   float most = -INFINITY, fewest = INFINITY;
-  bool odd = !(t >= 0.f) || p != p || least != least || u != u;
   const auto take = [&](const uint4& v, int it) {
     if (RES) kept_row[(warp * its + it) * 32 + lane] = v;
     float x[N];
     logits_of<T>(v, x);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      odd |= x[e] != x[e];
-      most = fmaxf(most, x[e]);
-      if (x[e] > -INFINITY) fewest = fminf(fewest, x[e]);
-    }
+    for (int e = 0; e < N; ++e) most = max_or_nan(most, x[e]);
+    fewest = x[0] > -INFINITY ? fminf(fewest, x[0]) : fewest;
   };
   int it0 = 0;
   for (; it0 + 4 <= mine; it0 += 4) {
@@ -184,27 +199,40 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     for (int j = 0; j < 4; ++j) take(v[j], it0 + j);
   }
   for (; it0 < mine; ++it0) take(fetch(begin + (it0 * 32 + lane) * N), it0);
+  bool odd = most != most || !(t >= 0.f) || p != p || least != least || u != u;
 
-  // ---- what all CTAs of the row agree on.  Two sets of published words take turns: between two uses of one lies a barrier of the cluster.
+  // ---- what all CTAs of the row agree on.  Published words take turns: between two uses of a set lies a barrier of the cluster.
   int turn = 0;
-  const auto extremes = [&](uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t flag, uint32_t (&out)[4]) {      // smallest, largest, smallest, any
-    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), lo2 = __reduce_min_sync(0xffffffffu, lo2);
-    flag = __reduce_or_sync(0xffffffffu, flag);
-    uint32_t* w = s.words[turn];
-    if (tid == 0) w[0] = 0xffffffffu, w[1] = 0, w[2] = 0xffffffffu, w[3] = 0;
+  // The 512 parts of the row are C neighbouring lanes each; a thread learns one of their maxima (as `order`, 0 for none)
+  uint32_t best = most > -INFINITY ? order_of(most) : 0;
+  for (int o = 1; o < C; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (tid % (unsigned)C == 0) s.maxima[tid / (unsigned)C] = best;
+  {
+    const uint32_t lo = __reduce_min_sync(0xffffffffu, order_of(fewest)), flag = __any_sync(0xffffffffu, odd);
+    if (lane == 0) s.part[warp][0] = lo, s.part[warp][1] = flag;
     __syncthreads();
-    if (lane == 0) atomicMin(&w[0], lo), atomicMax(&w[1], hi), atomicMin(&w[2], lo2), atomicOr(&w[3], flag);
+    if (warp == 0) {
+      const uint32_t a = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][0]), b = __any_sync(0xffffffffu, s.part[lane & 15][1] != 0);
+      if (lane == 0) s.words[0][0] = a, s.words[0][1] = b;
+    }
+  }
+  cluster_sync();
+  const uint32_t part_max = peek(&s.maxima[tid % (unsigned)(SA_THREADS / C)], tid / (SA_THREADS / C));
+  {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, part_max), lo = __reduce_min_sync(0xffffffffu, part_max ? part_max : 0xffffffffu);
+    if (lane == 0) s.part[warp][2] = hi, s.part[warp][3] = lo;
+    if (warp == 0) {
+      const uint32_t a = lane < C ? (uint32_t)peek(&s.words[0][0], lane) : 0xffffffffu, b = lane < C ? (uint32_t)peek(&s.words[0][1], lane) : 0;
+      const uint32_t all = __reduce_min_sync(0xffffffffu, a), any = __reduce_or_sync(0xffffffffu, b);
+      if (lane == 0) s.got[0] = all, s.got[1] = any;
+    }
     __syncthreads();
-    cluster_sync();
-    out[0] = 0xffffffffu, out[1] = 0, out[2] = 0xffffffffu, out[3] = 0;
-    for (int c = 0; c < C; ++c)
-      out[0] = min(out[0], peek(&w[0], c)), out[1] = max(out[1], peek(&w[1], c)), out[2] = min(out[2], peek(&w[2], c)), out[3] |= peek(&w[3], c);
-    turn ^= 1;
-  };
-  uint32_t e4[4];
-  extremes(order_of(fewest), order_of(most), most > -INFINITY ? order_of(most) : 0xffffffffu, odd, e4);
-  const float top = ordered(e4[1]), lowest = ordered(e4[0]), least_top = ordered(e4[2]);      // least_top: the smallest of the threads' maxima
-  odd = e4[3] != 0;
+  }
+  turn = 1;
+  uint32_t hi32 = (uint32_t)s.part[lane & 15][2], lo32 = (uint32_t)s.part[lane & 15][3];
+  hi32 = __reduce_max_sync(0xffffffffu, hi32), lo32 = __reduce_min_sync(0xffffffffu, lo32);
+  const float top = hi32 ? ordered(hi32) : -INFINITY, least_top = ordered(lo32), lowest = ordered((uint32_t)s.got[0]);
+  odd = s.got[1] != 0;
   const auto leave = [&](long long token, float logprob) { d.token[r] = token, d.logprob[r] = logprob; };
   if (odd || top == -INFINITY) {
     if (rank == 0 && tid == 0) leave(-1, odd ? NAN : -INFINITY);
@@ -212,9 +240,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     return;
   }
   const double floor_d = t > 0.f ? (double)top - 31.0 * (double)t : (double)top;      // exp(-31) is below 2^-44
-  const Weigh weigh = {s.table, (double)top, t > 0.f ? 369.32993046757463 / (double)t : 0.0,
-                       top == INFINITY ? INFINITY : __double2float_ru(fmax(floor_d, -3.4028234663852886e38))};
-  const auto weight = [&](float x) -> u64 { return x == top ? 1ull << 43 : weigh(x); };
+  const Weigh weigh = {s.table, (double)top, t > 0.f ? 369.32993046757463 / (double)t : 0.0, __double2float_ru(fmax(floor_d, -3.4028234663852886e38))};
 
   const auto each = [&](const auto& fn) {      // over this thread's elements: fn(id, logit), in the order of the ids per warp
     for (int it = 0; it < mine; ++it) {
@@ -224,66 +250,77 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       for (int e = 0; e < N; ++e) fn(begin + (it * 32 + lane) * N + e, x[e]);
     }
   };
-  const auto sums = [&](u64 a, u64 b, u64 c, u64 (&out)[3]) {      // of the whole row
-    a = warp_sum(a), b = warp_sum(b), c = warp_sum(c);
-    u64* w = s.sums[turn] + SA_WARPS;
-    if (tid < 3) w[tid] = 0;
+  // Sums of two numbers over the row
+  const auto all_of = [&](u64 a, u64 b, u64& sum_a, u64& sum_b) {
+    a = warp_sum(a), b = warp_sum(b);
+    if (lane == 0) s.part[warp][0] = a, s.part[warp][1] = b;
     __syncthreads();
-    if (lane == 0) atomicAdd(&w[0], a), atomicAdd(&w[1], b), atomicAdd(&w[2], c);
-    __syncthreads();
+    if (warp == 0) {
+      u64 v = s.part[lane & 15][lane >> 4];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if ((lane & 15) == 0) s.words[turn][lane >> 4] = v;
+    }
     cluster_sync();
-    out[0] = out[1] = out[2] = 0;
-    for (int q = 0; q < C; ++q) out[0] += peek(&w[0], q), out[1] += peek(&w[1], q), out[2] += peek(&w[2], q);
+    if (warp == 0) {
+      u64 v = lane < 2 * C ? peek(&s.words[turn][lane & 1], lane >> 1) : 0;
+#pragma unroll
+      for (int o = 2; o < 2 * SA_CLUSTER; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane < 2) s.got[lane] = v;
+    }
+    __syncthreads();
+    sum_a = s.got[0], sum_b = s.got[1];
     turn ^= 1;
   };
-  // The first element by id whose running sum of value(id, logit) passes aim(sum of all)
+  // The first element by id whose running sum of value(id, logit) passes aim(sum of all).  `sum`: of this thread's elements
   struct Place {
     int id;
     u64 value, total;
   };
-  const auto locate = [&](const auto& value, const auto& aim) -> Place {
-    u64 sum = 0;
-    each([&](int i, float x) { sum += value(i, x); });
-    sum = warp_sum(sum);
+  const auto locate_from = [&](u64 warps_sum, const auto& value, const auto& aim) -> Place {
     u64* w = s.sums[turn];
-    if (lane == 0) w[warp] = sum;
+    if (lane == 0) w[warp] = warps_sum;
     cluster_sync();
-    // every warp for itself: four warps' sums of the row per lane
-    u64 v[4], four = 0;
+    if (warp == 0) {      // four warps' sums of the row per lane
+      u64 v[4], four = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = lane * 4 + j;
-      v[j] = at < C * SA_WARPS ? peek(&w[at % SA_WARPS], at / SA_WARPS) : 0;
-      four += v[j];
+      for (int j = 0; j < 4; ++j) {
+        const int at = lane * 4 + j;
+        v[j] = at < C * SA_WARPS ? peek(&w[at % SA_WARPS], at / SA_WARPS) : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) four += v[j];
+      const u64 upto = warp_upto(four), total = __shfl_sync(0xffffffffu, upto, 31), target = aim(total);
+      u64 front = upto - four;
+      const bool here = front <= target && target < upto;
+      int owner = 0;
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (owner == j && target >= front + v[j]) front += v[j], ++owner;
+      if (here || (lane == 0 && target >= total)) s.got[2] = lane * 4 + owner, s.got[3] = front, s.got[4] = target, s.got[5] = total;
     }
-    const u64 upto = warp_upto(four), total = __shfl_sync(0xffffffffu, upto, 31), target = aim(total);
-    u64 front = upto - four;
-    int owner = 0;
-    const bool here = front <= target && target < upto;
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (owner == j && target >= front + v[j]) front += v[j], ++owner;
-    const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-    owner = __shfl_sync(0xffffffffu, lane * 4 + owner, max(who, 0));
-    front = __shfl_sync(0xffffffffu, front, max(who, 0));
+    __syncthreads();
+    const int owner = (int)s.got[2];
+    const u64 target = s.got[4], total = s.got[5];
     if (owner / SA_WARPS == rank) {      // its CTA: the steps of that warp's run, then the lanes of one step
       const int wo = owner % SA_WARPS, first = (rank * SA_WARPS + wo) * its * STEP, n = max(0, min(its, (V - first + STEP - 1) / STEP));
-      const auto lane_of = [&](int it, float (&x)[N], u64 (&y)[N]) {
+      const auto lane_of = [&](int it, u64 (&y)[N]) {
+        float x[N];
         logits_of<T>(RES ? kept_row[(wo * its + it) * 32 + lane] : fetch(first + (it * 32 + lane) * N), x);
         u64 q = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) y[e] = value(first + (it * 32 + lane) * N + e, x[e]), q += y[e];
         return q;
       };
-      float x[N];
       u64 y[N];
       for (int it = warp; it < n; it += SA_WARPS) {
-        const u64 q = warp_sum(lane_of(it, x, y));
+        const u64 q = warp_sum(lane_of(it, y));
         if (lane == 0) s.steps[it] = q;
       }
       __syncthreads();
       if (warp == 0) {
         int it = 0;
+        u64 front = s.got[3];
         for (int i0 = 0; i0 < n; i0 += 32) {
           const u64 q = i0 + lane < n ? s.steps[i0 + lane] : 0, up = warp_upto(q);
           const unsigned hit = __ballot_sync(0xffffffffu, front + up > target);
@@ -294,13 +331,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
           }
           front += __shfl_sync(0xffffffffu, up, 31);
         }
-        const u64 q = lane_of(it, x, y), up = warp_upto(q);
+        const u64 q = lane_of(it, y), up = warp_upto(q);
         u64 at = front + up - q;
         bool done = !(at <= target && target < front + up);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           if (!done && target < at + y[e]) {
-            s.found[0] = (u64)(first + (it * 32 + lane) * N + e), s.found[1] = y[e];
+            s.record[turn][0] = (u64)(first + (it * 32 + lane) * N + e), s.record[turn][1] = y[e];
             done = true;
           }
           at += y[e];
@@ -308,292 +345,435 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       }
     }
     cluster_sync();
-    const Place got = {(int)peek(&s.found[0], owner / SA_WARPS), peek(&s.found[1], owner / SA_WARPS), total};
+    if (tid < 2) s.got[6 + tid] = peek(&s.record[turn][tid], owner / SA_WARPS);
+    __syncthreads();
+    const Place got = {(int)s.got[6], s.got[7], total};
     turn ^= 1;
     return got;
   };
+  const auto locate = [&](const auto& value, const auto& aim) -> Place {
+    u64 sum = 0;
+    each([&](int i, float x) { sum += value(i, x); });
+    return locate_from(warp_sum(sum), value, aim);
+  };
   const auto finish = [&](const Place& x) {
     if (rank == 0 && tid == 0) leave(x.id, (float)log((double)x.value / (double)x.total));
+    cluster_sync();      // nobody leaves while its words are read
   };
   const auto at_random = [&](u64 total) { return u >= 1.f ? total - 1 : min(share_of<false>(total, u), total - 1); };
 
   const long long k = t == 0.f ? 1 : (k0 <= 0 || k0 > V ? V : k0);
   const u64 low = least >= 1.f ? 1ull << 43 : (u64)ceil(fmax((double)least, 0.0) * 0x1p43);
-  if (k == 1) {
-    finish(locate([&](int, float x) -> u64 { return x == top; }, [](u64) -> u64 { return 0; }));
-    // (a sum of one for each of the largest: what is drawn is certain)
-    if (rank == 0 && tid == 0) d.logprob[r] = 0.f;
+  if (k == 1 || top == INFINITY) {      // of the largest the first, or the first few: they weigh the same
+    u64 kept_ones = 1;
+    const Place at = locate([&](int, float x) -> u64 { return x == top; }, [&](u64 total) {
+      kept_ones = min(total, (u64)k);
+      if (p < 1.f) kept_ones = max((share_of<true>(kept_ones << 43, p) + (1ull << 43) - 1) >> 43, 1ull);
+      return at_random(kept_ones << 43) >> 43;
+    });
+    if (rank == 0 && warp == 0) {
+      kept_ones = __shfl_sync(0xffffffffu, kept_ones, 0);
+      if (lane == 0) leave(at.id, kept_ones == 1 ? 0.f : (float)-log((double)kept_ones));
+    }
     cluster_sync();
     return;
   }
 
-  // ---- lists: `order` (32 bits) and id of elements, the same in all CTAs, the largest first.  Returns how many, or more than SA_LIST.
-  const auto collect = [&](const auto& belongs) {
-    each([&](int i, float x) {
-      if (belongs(i, x)) {
-        const uint32_t at = atomicAdd(&s.count[0], 1);
-        if (at < SA_LIST) s.list[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
-      }
-    });
+  // ---- lists: `order` and inverted id of elements, the largest first: sorted[] of the CTAs that sort.  Returns how many there are.
+  // Elements have been put into list[], n_list of them by this CTA (more than SA_LIST: not all).
+  const auto sort_list = [&](bool here) {
     cluster_sync();
-    int n = 0, before[SA_CLUSTER + 1];
-#pragma unroll
-    for (int c = 0; c < SA_CLUSTER; ++c) {
-      before[c] = n;
-      if (c < C) n += (int)min(peek(&s.count[0], c), 1u << 21);
+    if (warp == 0) {
+      const uint32_t n = lane < C ? min(peek(&s.n_list, lane), 1u << 21) : 0, upto = warp_upto(n);
+      if (lane < SA_CLUSTER) s.part[lane][0] = upto;      // (behind the last CTA: all)
     }
-    before[SA_CLUSTER] = n;
-    if (n <= SA_LIST) {
+    __syncthreads();
+    const int n = (int)s.part[SA_CLUSTER - 1][0];
+    if (here && n <= SA_LIST) {
       u64 v = 0;
       if (tid < n) {
-#pragma unroll
-        for (int c = 0; c < SA_CLUSTER; ++c)
-          if (before[c] <= tid && tid < before[c + 1]) v = peek(&s.list[tid - before[c]], c);
-        s.all[tid] = v;
+        int c = 0, before = 0;
+        while (tid >= (int)s.part[c][0]) before = (int)s.part[c++][0];
+        v = peek(&s.list[tid - before], c);
+        s.value[tid] = v;
       }
       __syncthreads();
       if (tid < n) {
         int above = 0;
-        for (int j = 0; j < n; ++j) above += s.all[j] > v;
+        for (int j = 0; j < n; ++j) above += s.value[j] > v;
         s.sorted[above] = v;
       }
+      __syncthreads();
     }
-    cluster_sync();      // the counts have been read
-    if (tid == 0) s.count[0] = 0;
-    __syncthreads();
     return n;
   };
-  // Running sums of a value per element of the sorted list, into weights[]; returns the sum
-  const auto run = [&](int n, u64 v) {
-    const u64 up = warp_upto(tid < n ? v : 0);
-    if (lane == 31) s.mass[warp] = up;
-    __syncthreads();
-    u64 front = 0, all = 0;
-    for (int w = 0; w < SA_WARPS; ++w) {
-      if (w < warp) front += s.mass[w];
-      all += s.mass[w];
-    }
-    if (tid < n) s.weights[tid] = front + up;
-    __syncthreads();
-    return all;
+  const auto to_list = [&](int i, float x) {
+    const uint32_t at = atomicAdd(&s.n_list, 1);
+    if (at < SA_LIST) s.list[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
   };
-  const auto step_of = [&](float x, float scale) { return (int)fminf((top - x) * scale, (float)(SA_BINS - 1)); };
+  // Running sum of a number per thread, and the sum of all
+  const auto run = [&](u64 v, u64& all) {
+    const u64 up = warp_upto(v);
+    if (lane == 31) s.part[warp][1] = up;
+    __syncthreads();
+    u64 front = up;
+    all = 0;
+    for (int w = 0; w < SA_WARPS; ++w) {
+      const u64 q = s.part[w][1];
+      if (w < warp) front += q;
+      all += q;
+    }
+    __syncthreads();
+    return front;
+  };
+  // Equal steps of the logits from the top down, to the nearest: no less for a smaller logit
+  const auto step_of = [&](float x, float scale) {
+    const float y = fminf((top - x) * scale, (float)(SA_BINS - 1));
+    return __float_as_int(y + 12582912.f) - 0x4b400000;      // 1.5 2^23
+  };
   const auto scale_of = [&](float lo) {
     const float range = top - lo;
-    return range > 0.f && range < INFINITY ? (float)(SA_BINS - 1) / range : 0.f;
-  };
-  // Adds the CTAs' histograms up and clears them; every thread has four neighbouring bins, from the largest elements on
-  const auto add_up = [&]() {
-    cluster_sync();
-    for (int i = tid; i < SA_BINS; i += SA_THREADS) {
-      uint32_t n = 0;
-      for (int c = 0; c < C; ++c) n += peek(&s.hist[i], c);
-      s.total[i] = n;
-    }
-    cluster_sync();
-    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
-    __syncthreads();
-  };
-  // The first bin at which the running sum of value(bin) reaches `limit` (the last one if none does), and the sum in front of it
-  const auto crossing = [&](const auto& value, auto limit, auto& front) {
-    typedef decltype(limit) S;
-    S v[SA_BINS / SA_THREADS], four = 0;
-#pragma unroll
-    for (int j = 0; j < SA_BINS / SA_THREADS; ++j) v[j] = value(tid * (SA_BINS / SA_THREADS) + j), four += v[j];
-    const S up = warp_upto(four);
-    S* part = reinterpret_cast<S*>(s.mass);
-    if (lane == 31) part[warp] = up;
-    if (tid == 0) s.found[2] = SA_BINS;
-    __syncthreads();
-    S at = up - four;
-    for (int w = 0; w < warp; ++w) at += part[w];
-    int hit = SA_BINS;
-    S before = 0;
-#pragma unroll
-    for (int j = 0; j < SA_BINS / SA_THREADS; ++j) {
-      if (hit == SA_BINS && at + v[j] >= limit) hit = tid * (SA_BINS / SA_THREADS) + j, before = at;
-      at += v[j];
-    }
-    if (hit < SA_BINS) atomicMin(&s.found[2], (u64)hit);
-    __syncthreads();
-    const int bin = (int)s.found[2];
-    if (hit == bin) *reinterpret_cast<S*>(&s.found[3]) = before;
-    __syncthreads();
-    front = bin == SA_BINS ? S(0) : *reinterpret_cast<S*>(&s.found[3]);
-    __syncthreads();
-    return bin == SA_BINS ? SA_BINS - 1 : bin;
+    const float per = (float)(SA_BINS - 1) / range;
+    return range > 0.f && per < INFINITY ? per : 0.f;
   };
 
-  // ---- a small k: the elements that reach the k-th largest of the threads' maxima
+  // ---- a small k: the elements that reach the k-th largest of the parts' maxima
   if (k <= SA_LIST / 2) {
-    float reach = -INFINITY;
     const float scale = scale_of(least_top);
-    if (most > -INFINITY) atomicAdd(&s.hist[step_of(most, scale)], 1);
-    add_up();
-    uint32_t front;
-    const int bin = crossing([&](int b) { return s.total[b]; }, (uint32_t)k, front);
-    if (front + s.total[bin] >= (uint32_t)k) {
-      uint32_t m4[4];
-      extremes(most > -INFINITY && step_of(most, scale) <= bin ? order_of(most) : 0xffffffffu, 0, 0xffffffffu, 0, m4);
-      reach = ordered(m4[0]);
+    const int bin = part_max ? step_of(ordered(part_max), scale) : SA_BINS;
+    if (part_max) atomicAdd(&s.hist[bin], 1);
+    __syncthreads();
+    u64 all;
+    uint32_t four = 0, v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = s.hist[tid * 4 + j], four += v[j];
+    const u64 upto = run(four, all);
+    if (tid == 0) s.got[0] = SA_BINS;
+    __syncthreads();
+    if (upto - four < (u64)k && (u64)k <= upto) {
+      u64 at = upto - four;
+      int j = 0;
+      while (at + v[j] < (u64)k) at += v[j++];
+      s.got[0] = tid * 4 + j;
     }
-    const int n = collect([&](int, float x) { return x >= reach && x > -INFINITY; });
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.hist[tid * 4 + j] = 0;
+    __syncthreads();
+    const int border = (int)s.got[0];
+    const uint32_t low_max = __reduce_min_sync(0xffffffffu, part_max && bin <= border ? part_max : 0xffffffffu);
+    if (lane == 0) s.part[warp][2] = low_max;
+    __syncthreads();
+    const uint32_t reach32 = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][2]);
+    const float reach = border == SA_BINS ? -3.402823466e38f : ordered(reach32);      // fewer maxima than k: all finite ones
+    each([&](int i, float x) {
+      if (x >= reach) to_list(i, x);
+    });
+    const int n = sort_list(rank == 0);
     if (n <= SA_LIST) {
-      const u64 key = tid < n ? s.sorted[tid] : 0;
-      const u64 w = tid < min((long long)n, k) ? weight(ordered((uint32_t)(key >> 32))) : 0;
-      const u64 total = run(n, w);
-      const u64 limit = p < 1.f ? share_of<true>(total, p) : ~0ull, front_w = tid < n ? s.weights[tid] - w : 0;
-      const u64 stays = tid < n && tid < k && (tid == 0 || front_w < limit) && w >= low ? w : 0;
-      const u64 sum = run(n, stays), target = at_random(sum);
-      // what is kept by the order of the ids: the sum in front of each
-      __syncthreads();
-      if (tid < n) s.all[tid] = stays;
-      __syncthreads();
-      if (rank == 0 && stays) {
-        u64 before = 0;
-        for (int j = 0; j < n; ++j)
-          if ((uint32_t)s.sorted[j] > (uint32_t)key) before += s.all[j];      // ids are held inverted
-        if (before <= target && target < before + stays) leave((long long)(uint32_t)~(uint32_t)key, (float)log((double)stays / (double)sum));
+      if (rank == 0) {
+        const u64 key = tid < n ? s.sorted[tid] : 0;
+        const float x = ordered((uint32_t)(key >> 32));
+        const u64 w = tid < n && tid < k && x >= weigh.floor ? weigh(x) : 0;
+        u64 total, sum;
+        const u64 before = run(w, total) - w, limit = p < 1.f ? share_of<true>(total, p) : ~0ull;
+        const u64 stays = (tid == 0 || before < limit) && w >= low ? w : 0;
+        run(stays, sum);
+        const u64 target = at_random(sum);
+        s.value[tid] = stays;
+        __syncthreads();
+        if (stays) {      // the sum in front of it in the order of the ids, which are held inverted
+          u64 front = 0;
+          for (int j = 0; j < n; ++j)
+            if ((uint32_t)s.sorted[j] > (uint32_t)key) front += s.value[j];
+          if (front <= target && target < front + stays) leave((long long)(uint32_t)~(uint32_t)key, (float)log((double)stays / (double)sum));
+        }
       }
       cluster_sync();
       return;
     }
+    cluster_sync();      // the lists have been looked at
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
   }
 
   // ---- borders: kept is what is larger than `edge`, and equal ones up to id `last`
   float edge = -INFINITY;
   int last = V;
   const auto kept = [&](int i, float x) { return x > edge || (x == edge && i <= last); };
-  // Inside the elements of `belongs`, of which there are n, the border is where the running count (or sum of weights) reaches `need`
-  const auto inside = [&](const auto& belongs, uint32_t n, bool mass, u64 need) {
-    uint32_t lo = 0xffffffffu, hi = 0, m4[4];
-    each([&](int i, float x) {
-      if (belongs(i, x)) lo = min(lo, order_of(x)), hi = max(hi, order_of(x));
-    });
-    extremes(lo, hi, 0xffffffffu, 0, m4);
-    lo = m4[0], hi = m4[1];
+  // Up to two steps of a histogram of the row at which the running sum of value(step, count) reaches aim(sum of all, ..): each CTA adds up
+  // its part of the steps.  The sums are fp32 in a fixed order, exact for counts.  got[]: two steps, the sums in front of them (as fp32).
+  const auto find = [&](const auto& value, const auto& aim) {
+    const int nb = SA_BINS / C, per = nb >= SA_THREADS ? nb / SA_THREADS : 1, b0 = rank * nb + tid * per;
+    cluster_sync();
+    float v[4], four = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t n = 0;
+      if (j < per && tid * per < nb)
+        for (int c = 0; c < C; ++c) n += peek(&s.hist[b0 + j], c);
+      v[j] = n ? value(b0 + j, n) : 0.f;
+      four += v[j];
+    }
+    const float up = warp_upto(four);
+    float* part = reinterpret_cast<float*>(s.part);
+    if (lane == 31) part[warp] = up;
+    __syncthreads();
+    float front = up - four, mine_all = 0.f;
+    for (int w = 0; w < SA_WARPS; ++w) {
+      if (w < warp) front += part[w];
+      mine_all += part[w];
+    }
+    if (tid == 0) s.words[turn][0] = __float_as_uint(mine_all);
+    if (tid < 2) s.record[turn][tid] = ~0ull;
+    cluster_sync();
+    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
+    if (warp == 0) {
+      const float q = lane < C ? __uint_as_float((uint32_t)peek(&s.words[turn][0], lane)) : 0.f, upto = warp_upto(q);
+      const float all = __shfl_sync(0xffffffffu, upto, 31), before = __shfl_sync(0xffffffffu, upto - q, rank);
+      if (lane == 0) s.got[0] = __float_as_uint(all), s.got[1] = __float_as_uint(before);
+    }
+    __syncthreads();
+    const float all = __uint_as_float((uint32_t)s.got[0]);
+    front += __uint_as_float((uint32_t)s.got[1]);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const float want = aim(all, a);
+      float at = front;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (v[j] > 0.f && at + v[j] >= want) {
+          atomicMin(&s.record[turn][a], (u64)(b0 + j) << 32 | __float_as_uint(at));
+          break;
+        }
+        at += v[j];
+      }
+    }
+    cluster_sync();
+    if (warp == 0) {
+      u64 q = lane < 2 * C ? peek(&s.record[turn][lane & 1], lane >> 1) : ~0ull;
+#pragma unroll
+      for (int o = 2; o < 2 * SA_CLUSTER; o <<= 1) q = min(q, __shfl_xor_sync(0xffffffffu, q, o));
+      if (lane < 2) s.got[lane] = q;
+    }
+    __syncthreads();
+    turn ^= 1;
+  };
+  // The smallest logit (as `order`) of step `b` or one further up, found by all lanes of a warp
+  const auto first_of = [&](int b, float scale) {
+    uint32_t lo = 0x00800000u, hi = order_of(top);      // the lowest finite number; step_of(top) = 0
+    while (lo < hi) {      // 31 points between them
+      const u64 span = (u64)hi - lo;
+      const uint32_t at = lo + (uint32_t)(span * (u64)lane >> 5);
+      const unsigned yes = __ballot_sync(0xffffffffu, step_of(ordered(at), scale) <= b);
+      const int f = yes ? __ffs(yes) - 1 : 32;
+      const uint32_t new_hi = f < 32 ? lo + (uint32_t)(span * (u64)f >> 5) : hi;
+      const uint32_t new_lo = f > 0 ? lo + (uint32_t)(span * (u64)(f - 1) >> 5) + 1 : lo;
+      lo = min(new_lo, new_hi), hi = new_hi;
+    }
+    return lo;
+  };
+  // The logits of steps b1 to b2: got[0] the smallest, got[1] the largest (as `order`)
+  const auto between = [&](int b1, int b2, float scale) {
+    if (warp < 2) {
+      const int b = warp == 0 ? b2 : b1 - 1;
+      const uint32_t o = b >= SA_BINS - 1 ? 0x00800000u : b < 0 ? order_of(top) + 1 : first_of(b, scale);
+      if (lane == 0) s.got[warp] = warp == 0 ? o : o - 1;
+    }
+    __syncthreads();
+  };
+  const auto set_aside = [&](int i, float x) {
+    const uint32_t at = atomicAdd(&s.n_aside, 1);
+    if (at < SA_ASIDE) s.aside[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
+  };
+  // The border among the elements set aside, kept ones of logits lo .. hi, is where the running count or sum of weights reaches `need`
+  const auto inside = [&](uint32_t lo, uint32_t hi, bool mass, u64 need) {
+    const float lo0 = ordered(lo), hi0 = ordered(hi);
+    u64 n, over;
+    __syncthreads();
+    {
+      const uint32_t own = s.n_aside;
+      all_of(tid == 0 ? own : 0, tid == 0 && own > SA_ASIDE, n, over);
+    }
+    const int own = min((int)s.n_aside, SA_ASIDE);
+    const auto members = [&](const auto& fn) {      // fn(order, inverted id); where a CTA had no room all look at the whole row
+      if (!over) {
+        for (int j = tid; j < own; j += SA_THREADS) {
+          const u64 v = s.aside[j];
+          if (lo <= (uint32_t)(v >> 32) && (uint32_t)(v >> 32) <= hi) fn((uint32_t)(v >> 32), (uint32_t)v);
+        }
+      } else {
+        each([&](int i, float x) {
+          if (lo0 <= x && x <= hi0 && kept(i, x) && lo <= order_of(x) && order_of(x) <= hi) fn(order_of(x), (uint32_t)~i);
+        });
+      }
+    };
+    const auto weight_of = [&](uint32_t o) -> u64 { return mass ? (ordered(o) >= weigh.floor ? weigh(ordered(o)) : 0) : 1; };
+    {      // their extremes
+      uint32_t a = 0xffffffffu, b = 0;
+      members([&](uint32_t o, uint32_t) { a = min(a, o), b = max(b, o); });
+      a = __reduce_min_sync(0xffffffffu, a), b = __reduce_max_sync(0xffffffffu, b);
+      if (lane == 0) s.part[warp][0] = a, s.part[warp][1] = b;
+      __syncthreads();
+      if (warp == 0) {
+        a = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][0]), b = __reduce_max_sync(0xffffffffu, (uint32_t)s.part[lane & 15][1]);
+        if (lane == 0) s.words[turn][0] = (u64)b << 32 | a;
+      }
+      cluster_sync();
+      if (warp == 0) {
+        const u64 q = lane < C ? peek(&s.words[turn][0], lane) : 0xffffffffull;
+        a = __reduce_min_sync(0xffffffffu, (uint32_t)q), b = __reduce_max_sync(0xffffffffu, (uint32_t)(q >> 32));
+        if (lane == 0) s.got[0] = a, s.got[1] = b;
+      }
+      __syncthreads();
+      turn ^= 1;
+      lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
+    }
     while (lo < hi && n > SA_LIST) {      // steps of the order itself
       int shift = 0;
-      while ((hi - lo) >> shift >= SA_BINS) ++shift;
-      uint32_t above = 0;
-      u64 above_w = 0;
-      each([&](int i, float x) {
-        const uint32_t o = order_of(x);
-        if (belongs(i, x) && lo <= o && o <= hi) atomicAdd(&s.hist[(hi - o) >> shift], 1);
+      while ((hi - lo) >> shift >= SA_FINE) ++shift;
+      for (int i = tid; i < SA_FINE; i += SA_THREADS) s.mass[i] = 0, s.hist[i] = 0;
+      __syncthreads();
+      members([&](uint32_t o, uint32_t) {
+        const uint32_t b = (hi - o) >> shift;
+        atomicAdd(&s.hist[b], 1);
+        if (mass) atomicAdd(&s.mass[b], weight_of(o));
       });
-      add_up();
-      int bin;
-      if (!mass) {
-        bin = crossing([&](int b) { return s.total[b]; }, (uint32_t)need, above);
-        need -= above;
-      } else {
-        // sums of weights by halving: the first bin up to which they reach what is needed
-        int b0 = 0, b1 = (int)((hi - lo) >> shift);
-        while (b0 < b1) {
-          const int mid = (b0 + b1) >> 1;
-          u64 sum = 0, s3[3];
-          each([&](int i, float x) {
-            const uint32_t o = order_of(x);
-            if (belongs(i, x) && lo <= o && o <= hi) {
-              const int b = (int)((hi - o) >> shift);
-              if (b0 <= b && b <= mid) sum += weight(x);
-            }
-          });
-          sums(sum, 0, 0, s3);
-          if (above_w + s3[0] >= need) b1 = mid;
-          else above_w += s3[0], b0 = mid + 1;
+      cluster_sync();
+      // two steps per thread, all of them in each CTA
+      u64 v[2];
+      uint32_t m[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        v[j] = m[j] = 0;
+        for (int c = 0; c < C; ++c) {
+          m[j] += peek(&s.hist[tid * 2 + j], c);
+          if (mass) v[j] += peek(&s.mass[tid * 2 + j], c);
         }
-        bin = b0;
-        need -= above_w;
+        if (!mass) v[j] = m[j];
       }
-      const uint32_t start = hi - ((uint32_t)bin << shift);
-      n = s.total[bin];
-      lo = max(lo, shift ? start - ((1u << shift) - 1) : start);
-      hi = start;
+      u64 sum;
+      const u64 upto = run(v[0] + v[1], sum), front = upto - v[0] - v[1];
+      if (front < need && (need <= upto || (upto == sum && v[0] + v[1]))) {      // (the last one that has anything, if they do not reach it)
+        const int j = need > front + v[0] && v[1] ? 1 : 0;
+        s.got[0] = tid * 2 + j, s.got[1] = j ? front + v[0] : front, s.got[2] = m[j];
+      }
+      cluster_sync();
+      const uint32_t start = hi - ((uint32_t)s.got[0] << shift);
+      need -= s.got[1], n = s.got[2];
+      lo = max(lo, shift ? start - ((1u << shift) - 1) : start), hi = start;
     }
+    for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0;
     if (lo < hi) {
-      const int m = collect([&](int i, float x) { return belongs(i, x) && lo <= order_of(x) && order_of(x) <= hi; });
-      const u64 key = tid < m ? s.sorted[tid] : 0;
-      const u64 w = tid < m ? (mass ? weight(ordered((uint32_t)(key >> 32))) : 1) : 0;
-      run(m, w);
-      if (tid == 0) s.found[2] = (u64)(m - 1);
-      __syncthreads();
-      if (tid < m && s.weights[tid] >= need) atomicMin(&s.found[2], (u64)tid);
-      __syncthreads();
-      const u64 border = s.sorted[s.found[2]];
-      __syncthreads();
-      edge = ordered((uint32_t)(border >> 32)), last = (int)(uint32_t)~(uint32_t)border;
-      return;
+      members([&](uint32_t o, uint32_t inverted) { to_list((int)~inverted, ordered(o)); });
+      const int m = sort_list(true);
+      const u64 key = tid < m ? s.sorted[tid] : 0, w = tid < m ? weight_of((uint32_t)(key >> 32)) : 0;
+      u64 sum;
+      const u64 upto = run(w, sum);
+      if (tid < m && upto - w < need && (need <= upto || tid == m - 1)) s.got[0] = key;
+      cluster_sync();      // the lists have been read
+      edge = ordered((uint32_t)(s.got[0] >> 32)), last = (int)(uint32_t)~(uint32_t)s.got[0];
+      if (tid == 0) s.n_list = 0;
+    } else {
+      // equal ones: as many as are needed, by their ids
+      const float value = ordered(lo);
+      const u64 one = weight_of(lo), many = one ? (need + one - 1) / one : n;
+      const Place at = locate([&](int i, float x) -> u64 { return x == value && kept(i, x); }, [&](u64 total) { return min(max(many, 1ull), total) - 1; });
+      edge = value, last = at.id;
     }
-    // equal ones: as many as are needed, by their ids
-    const float value = ordered(lo);
-    const u64 one = mass ? weight(value) : 1, many = one ? (need + one - 1) / one : n;
-    const Place at = locate([&](int i, float x) -> u64 { return x == value && belongs(i, x); }, [&](u64 total) { return min(max(many, 1ull), total) - 1; });
-    edge = value, last = at.id;
+    __syncthreads();
+    if (tid == 0) s.n_aside = 0;
+    __syncthreads();
   };
   if (k < V) {
-    const float lo = fmaxf(lowest, top - 48.f), scale = scale_of(lo);
+    const float scale = scale_of(fmaxf(lowest, top - 48.f));
     each([&](int, float x) {
       if (x > -INFINITY) atomicAdd(&s.hist[step_of(x, scale)], 1);
     });
-    add_up();
-    uint32_t above;
-    const int bin = crossing([&](int b) { return s.total[b]; }, (uint32_t)k, above);
-    if (above + s.total[bin] >= (uint32_t)k)      // else there are not so many
-      inside([&](int, float x) { return x > -INFINITY && step_of(x, scale) == bin; }, s.total[bin], false, (u64)k - above);
+    find([](int, uint32_t n) { return (float)n; }, [&](float, int) { return (float)k; });
+    if (s.got[0] != ~0ull) {      // else there are not so many
+      const int bin = (int)(s.got[0] >> 32);
+      const u64 above = (u64)__uint_as_float((uint32_t)s.got[0]);
+      __syncthreads();
+      between(bin, bin, scale);
+      const uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
+      const float lo_x = ordered(lo), hi_x = ordered(hi);
+      each([&](int i, float x) {
+        if (lo_x <= x && x <= hi_x) set_aside(i, x);
+      });
+      inside(lo, hi, false, (u64)k - above);
+    }
   }
+  // What counts of each element: from what on it weighs anything, and whether it is kept
+  const auto final = [&](int i, float x) -> u64 {
+    if (!(x >= weigh.floor) || !kept(i, x)) return 0;
+    const u64 w = weigh(x);
+    return w >= low ? w : 0;
+  };
   if (p < 1.f) {
-    const float lo = fmaxf(fmaxf(lowest, weigh.floor), edge), scale = scale_of(lo);
-    each([&](int i, float x) {
-      if (x > -INFINITY && kept(i, x)) atomicAdd(&s.hist[step_of(x, scale)], 1);
+    const float from = fmaxf(weigh.floor, edge), scale = scale_of(fmaxf(lowest, from));
+    const bool ties = edge >= from;
+    each([&](int, float x) {
+      if (x >= from) atomicAdd(&s.hist[step_of(x, scale)], 1);
     });
-    add_up();
-    // by counts and the weight at the middle of a bin, about where the border is
-    const float per_bin = scale > 0.f && t > 0.f ? 1.4426950f / (scale * t) : 0.f;
-    const auto about = [&](int b) { return (float)s.total[b] * exp2f(-((float)b + 0.5f) * per_bin); };
-    float before;
-    crossing(about, INFINITY, before);
-    float sum = 0.f;
-    for (int w = 0; w < SA_WARPS; ++w) sum += reinterpret_cast<float*>(s.mass)[w];
+    // A step's elements by the weight of its middle, within a factor of exp(1 / 2 scale T): the border is between the two steps where their
+    // sums pass p of it all, less and more 1/4 of that
+    const float per_bin = scale > 0.f ? 1.4426950f / (scale * t) : 0.f, slack = fminf(0.25f * per_bin, 0.5f) + 1e-5f;
+    find([&](int b, uint32_t n) { return (float)n * exp2f(-(float)b * per_bin); }, [&](float all, int a) { return p * all * (a ? 1.f + slack : 1.f - slack); });
+    const int b1 = s.got[0] == ~0ull ? 0 : (int)(s.got[0] >> 32), b2 = s.got[1] == ~0ull ? SA_BINS - 1 : (int)(s.got[1] >> 32);
     __syncthreads();
-    int bin = crossing(about, p * sum, before);
-    while (bin > 0 && s.total[bin] == 0) --bin;
-    u64 all = 0, above = 0, in = 0, s3[3];
+    between(b1, b2, scale);
+    uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
+    const float lo_x = fmaxf(ordered(lo), from), hi_x = ordered(hi);
+    u64 all = 0, above = 0, all_sum, above_sum;
     each([&](int i, float x) {
-      if (x > -INFINITY && kept(i, x)) {
-        const u64 w = weight(x);
-        const int b = step_of(x, scale);
+      if (x >= from && !(ties && x == edge && i > last)) {
+        const u64 w = weigh(x);
         all += w;
-        if (b < bin) above += w;
-        if (b == bin) in += w;
+        if (x > hi_x) above += w;
+        else if (x >= lo_x) set_aside(i, x);
       }
     });
-    sums(all, above, in, s3);
-    const u64 limit = max(share_of<true>(s3[0], p), 1ull);
-    above = s3[1], in = s3[2];
-    while (above >= limit || above + in < limit) {      // a bin further up or down
-      const bool down = above + in < limit;
-      int next = bin;
-      do next += down ? 1 : -1;
-      while (next > 0 && next < SA_BINS - 1 && s.total[next] == 0);
-      u64 got = 0;
+    above = warp_sum(above);
+    all_of(all, lane == 0 ? above : 0, all_sum, above_sum);
+    const u64 limit = max(share_of<true>(all_sum, p), 1ull);
+    u64 in = 0, in_sum, over;
+    __syncthreads();
+    const int own = min((int)s.n_aside, SA_ASIDE);
+    for (int j = tid; j < own; j += SA_THREADS) in += weigh(ordered((uint32_t)(s.aside[j] >> 32)));
+    all_of(in, tid == 0 && s.n_aside > SA_ASIDE, in_sum, over);
+    if (over) {      // no room for them all
+      in = 0;
       each([&](int i, float x) {
-        if (x > -INFINITY && kept(i, x) && step_of(x, scale) == next) got += weight(x);
+        if (lo_x <= x && x <= hi_x && !(ties && x == edge && i > last)) in += weigh(x);
       });
-      sums(got, 0, 0, s3);
-      if (down) above += in;
-      else above -= s3[0];
-      in = s3[0], bin = next;
-      if (next <= 0 || next >= SA_BINS - 1) break;
+      u64 none;
+      all_of(in, 0, in_sum, none);
     }
-    inside([&](int i, float x) { return x > -INFINITY && kept(i, x) && step_of(x, scale) == bin; }, s.total[bin], true, limit > above ? limit - above : 1);
+    if (above_sum >= limit || above_sum + in_sum < limit) {      // not between those two: among all
+      __syncthreads();
+      if (tid == 0) s.n_aside = SA_ASIDE + 1;
+      over = 1, above_sum = 0;
+      lo = 0, hi = order_of(top);
+    }
+    inside(max(lo, order_of(from)), hi, true, limit - above_sum);
+    // the warps' sums: what was above, and of what was set aside the kept ones
+    if (low == 0 && !over) {
+      if (lane == 0) s.sums[turn][warp] = above;
+      __syncthreads();
+      for (int j = tid; j < own; j += SA_THREADS) {
+        const u64 v = s.aside[j];
+        const int i = (int)(uint32_t)~(uint32_t)v;
+        const float x = ordered((uint32_t)(v >> 32));
+        if (kept(i, x)) atomicAdd(&s.sums[turn][i / (its * STEP) % SA_WARPS], weigh(x));
+      }
+      __syncthreads();
+      const u64 sum = s.sums[turn][warp];
+      __syncthreads();
+      finish(locate_from(sum, final, at_random));
+      return;
+    }
   }
-  finish(locate([&](int i, float x) -> u64 {
-    if (!(x >= weigh.floor) || !kept(i, x)) return 0;
-    const u64 w = weight(x);
-    return w >= low ? w : 0;
-  }, at_random));
-  cluster_sync();
+  finish(locate(final, at_random));
 }
 
 template <typename T, bool RES, bool VEC>
