@@ -457,7 +457,7 @@ typedef struct FtkSampleDesc {
   long long k;
   long long* token;         // [R]
   float* logprob;           // [R]
-  long long cluster;        // set by the launcher
+  long long cluster;        // set by the launcher: CTAs of a row, as a power of two
 } FtkSampleDesc;
 int ftk_sample(const FtkSampleDesc* d, void* stream);
 #ifdef __cplusplus

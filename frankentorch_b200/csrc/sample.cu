@@ -21,6 +21,8 @@
 // The random sums of shared memory's counters take 10 cycles of an SM for 32 elements; collectives of a cluster 1500 cycles each.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
 #include "launch.cuh"
@@ -67,8 +69,13 @@ template <bool UP> __device__ __forceinline__ u64 share_of(u64 n, float f) {
   const bool rest = s < 64 ? (lo << (64 - s)) != 0 : lo != 0 || (s > 64 && (hi << (128 - s)) != 0);
   return down + rest;
 }
+// All threads of the row's CTAs have come here, and what they wrote to shared memory is seen by all: one fence for a CTA's threads, which
+// its own barrier has put in front of it (a fence of each warp takes three times as long)
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -155,8 +162,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
   uint4* kept_row = reinterpret_cast<uint4*>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = (int)d.V;
-  const int rank = (int)cluster_rank(), C = (int)d.cluster;      // C: a power of two
-  const long long r = blockIdx.x / (unsigned)C;
+  const int rank = (int)cluster_rank(), lc = (int)d.cluster, C = 1 << lc;
+  const long long r = blockIdx.x >> lc;
   const int begin = (rank * SA_WARPS + warp) * its * STEP;      // this warp's run of columns
   const int mine = max(0, min(its, (V - begin + STEP - 1) / STEP));
   if (tid < 256) s.table[tid] = exp2(tid * (1.0 / 256));
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   // The 512 parts of the row are C neighbouring lanes each; a thread learns one of their maxima (as `order`, 0 for none)
   uint32_t best = most > -INFINITY ? order_of(most) : 0;
   for (int o = 1; o < C; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (tid % (unsigned)C == 0) s.maxima[tid / (unsigned)C] = best;
+  if ((tid & (C - 1)) == 0) s.maxima[tid >> lc] = best;
   {
     const uint32_t lo = __reduce_min_sync(0xffffffffu, order_of(fewest)), flag = __any_sync(0xffffffffu, odd);
     if (lane == 0) s.part[warp][0] = lo, s.part[warp][1] = flag;
@@ -217,13 +224,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     }
   }
   cluster_sync();
-  const uint32_t part_max = peek(&s.maxima[tid % (unsigned)(SA_THREADS / C)], tid / (SA_THREADS / C));
+  const uint32_t part_max = peek(&s.maxima[tid & ((SA_THREADS >> lc) - 1)], tid >> (9 - lc));
   {
+    const u64 own = lane < 2 * C ? peek(&s.words[0][lane & 1], lane >> 1) : (lane & 1 ? 0 : 0xffffffffu);
     const uint32_t hi = __reduce_max_sync(0xffffffffu, part_max), lo = __reduce_min_sync(0xffffffffu, part_max ? part_max : 0xffffffffu);
     if (lane == 0) s.part[warp][2] = hi, s.part[warp][3] = lo;
     if (warp == 0) {
-      const uint32_t a = lane < C ? (uint32_t)peek(&s.words[0][0], lane) : 0xffffffffu, b = lane < C ? (uint32_t)peek(&s.words[0][1], lane) : 0;
-      const uint32_t all = __reduce_min_sync(0xffffffffu, a), any = __reduce_or_sync(0xffffffffu, b);
+      const uint32_t all = __reduce_min_sync(0xffffffffu, lane & 1 ? 0xffffffffu : (uint32_t)own), any = __reduce_or_sync(0xffffffffu, lane & 1 ? (uint32_t)own : 0);
       if (lane == 0) s.got[0] = all, s.got[1] = any;
     }
     __syncthreads();
@@ -250,26 +257,30 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       for (int e = 0; e < N; ++e) fn(begin + (it * 32 + lane) * N + e, x[e]);
     }
   };
-  // Sums of two numbers over the row
-  const auto all_of = [&](u64 a, u64 b, u64& sum_a, u64& sum_b) {
-    a = warp_sum(a), b = warp_sum(b);
-    if (lane == 0) s.part[warp][0] = a, s.part[warp][1] = b;
+  // Sums of up to four numbers over the row
+  const auto all_of = [&](u64 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = warp_sum(v[j]);
+      if (lane == 0) s.part[warp][j] = v[j];
+    }
     __syncthreads();
     if (warp == 0) {
-      u64 v = s.part[lane & 15][lane >> 4];
+      u64 a = s.part[lane & 15][lane >> 4], b = s.part[lane & 15][2 + (lane >> 4)];
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if ((lane & 15) == 0) s.words[turn][lane >> 4] = v;
+      for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o), b += __shfl_xor_sync(0xffffffffu, b, o);
+      if ((lane & 15) == 0) s.words[turn][lane >> 4] = a, s.words[turn][2 + (lane >> 4)] = b;
     }
     cluster_sync();
     if (warp == 0) {
-      u64 v = lane < 2 * C ? peek(&s.words[turn][lane & 1], lane >> 1) : 0;
+      u64 a = lane < 4 * C ? peek(&s.words[turn][lane & 3], lane >> 2) : 0;
 #pragma unroll
-      for (int o = 2; o < 2 * SA_CLUSTER; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane < 2) s.got[lane] = v;
+      for (int o = 4; o < 4 * SA_CLUSTER; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (lane < 4) s.got[lane] = a;
     }
     __syncthreads();
-    sum_a = s.got[0], sum_b = s.got[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = s.got[j];
     turn ^= 1;
   };
   // The first element by id whose running sum of value(id, logit) passes aim(sum of all).  `sum`: of this thread's elements
@@ -503,14 +514,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   // Up to two steps of a histogram of the row at which the running sum of value(step, count) reaches aim(sum of all, ..): each CTA adds up
   // its part of the steps.  The sums are fp32 in a fixed order, exact for counts.  got[]: two steps, the sums in front of them (as fp32).
   const auto find = [&](const auto& value, const auto& aim) {
-    const int nb = SA_BINS / C, per = nb >= SA_THREADS ? nb / SA_THREADS : 1, b0 = rank * nb + tid * per;
+    const int nb = SA_BINS >> lc, per = max(nb / SA_THREADS, 1), b0 = rank * nb + tid * per;
     cluster_sync();
     float v[4], four = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t n = 0;
-      if (j < per && tid * per < nb)
-        for (int c = 0; c < C; ++c) n += peek(&s.hist[b0 + j], c);
+      if (j < per && tid * per < nb) {
+#pragma unroll
+        for (int c = 0; c < SA_CLUSTER; ++c) n += c < C ? peek(&s.hist[b0 + j], c) : 0;
+      }
       v[j] = n ? value(b0 + j, n) : 0.f;
       four += v[j];
     }
@@ -585,17 +598,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const uint32_t at = atomicAdd(&s.n_aside, 1);
     if (at < SA_ASIDE) s.aside[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
   };
-  // The border among the elements set aside, kept ones of logits lo .. hi, is where the running count or sum of weights reaches `need`
-  const auto inside = [&](uint32_t lo, uint32_t hi, bool mass, u64 need) {
+  // The border among n kept elements of logits lo .. hi (as `order`) is where the running count or sum of weights reaches `need`.  They have
+  // been set aside, or where there was no room all look at the whole row for them.
+  const auto inside = [&](uint32_t lo, uint32_t hi, u64 n, bool over, bool mass, u64 need) {
+    constexpr int GRAIN = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);      // two logits are 2^GRAIN apart, at least
     const float lo0 = ordered(lo), hi0 = ordered(hi);
-    u64 n, over;
-    __syncthreads();
-    {
-      const uint32_t own = s.n_aside;
-      all_of(tid == 0 ? own : 0, tid == 0 && own > SA_ASIDE, n, over);
-    }
     const int own = min((int)s.n_aside, SA_ASIDE);
-    const auto members = [&](const auto& fn) {      // fn(order, inverted id); where a CTA had no room all look at the whole row
+    const auto members = [&](const auto& fn) {      // fn(order, inverted id)
       if (!over) {
         for (int j = tid; j < own; j += SA_THREADS) {
           const u64 v = s.aside[j];
@@ -608,35 +617,25 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       }
     };
     const auto weight_of = [&](uint32_t o) -> u64 { return mass ? (ordered(o) >= weigh.floor ? weigh(ordered(o)) : 0) : 1; };
-    {      // their extremes
-      uint32_t a = 0xffffffffu, b = 0;
-      members([&](uint32_t o, uint32_t) { a = min(a, o), b = max(b, o); });
-      a = __reduce_min_sync(0xffffffffu, a), b = __reduce_max_sync(0xffffffffu, b);
-      if (lane == 0) s.part[warp][0] = a, s.part[warp][1] = b;
-      __syncthreads();
-      if (warp == 0) {
-        a = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][0]), b = __reduce_max_sync(0xffffffffu, (uint32_t)s.part[lane & 15][1]);
-        if (lane == 0) s.words[turn][0] = (u64)b << 32 | a;
-      }
-      cluster_sync();
-      if (warp == 0) {
-        const u64 q = lane < C ? peek(&s.words[turn][0], lane) : 0xffffffffull;
-        a = __reduce_min_sync(0xffffffffu, (uint32_t)q), b = __reduce_max_sync(0xffffffffu, (uint32_t)(q >> 32));
-        if (lane == 0) s.got[0] = a, s.got[1] = b;
-      }
-      __syncthreads();
-      turn ^= 1;
-      lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
-    }
+    uint32_t* const mass32 = reinterpret_cast<uint32_t*>(s.mass);      // the low halves of all steps, then the high ones
     while (lo < hi && n > SA_LIST) {      // steps of the order itself
-      int shift = 0;
+      int shift = GRAIN;
       while ((hi - lo) >> shift >= SA_FINE) ++shift;
-      for (int i = tid; i < SA_FINE; i += SA_THREADS) s.mass[i] = 0, s.hist[i] = 0;
+      const bool one_value = shift == GRAIN;      // in each step: its sum of weights is a product
+      const auto value_of = [&](int b) {          // the logit that a step of one value has
+        const uint32_t start = hi - ((uint32_t)b << shift), c = start & ~((1u << GRAIN) - 1);
+        return c >= 0x80000000u ? c : ((start + 1) & ~((1u << GRAIN) - 1)) - 1;
+      };
+      for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0, s.mass[i] = 0;
       __syncthreads();
       members([&](uint32_t o, uint32_t) {
         const uint32_t b = (hi - o) >> shift;
         atomicAdd(&s.hist[b], 1);
-        if (mass) atomicAdd(&s.mass[b], weight_of(o));
+        if (mass && !one_value) {      // (64 bits by two counters of 32)
+          const u64 w = weight_of(o);
+          const uint32_t was = atomicAdd(&mass32[b], (uint32_t)w);
+          atomicAdd(&mass32[SA_FINE + b], (uint32_t)(w >> 32) + (was + (uint32_t)w < was));
+        }
       });
       cluster_sync();
       // two steps per thread, all of them in each CTA
@@ -645,11 +644,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         v[j] = m[j] = 0;
-        for (int c = 0; c < C; ++c) {
-          m[j] += peek(&s.hist[tid * 2 + j], c);
-          if (mass) v[j] += peek(&s.mass[tid * 2 + j], c);
+#pragma unroll
+        for (int c = 0; c < SA_CLUSTER; ++c) m[j] += c < C ? peek(&s.hist[tid * 2 + j], c) : 0;
+        if (mass && !one_value) {
+#pragma unroll
+          for (int c = 0; c < SA_CLUSTER; ++c)
+            if (c < C) v[j] += (u64)peek(&mass32[SA_FINE + tid * 2 + j], c) << 32 | peek(&mass32[tid * 2 + j], c);
+        } else {
+          v[j] = m[j] ? m[j] * weight_of(value_of(tid * 2 + j)) : 0;
         }
-        if (!mass) v[j] = m[j];
       }
       u64 sum;
       const u64 upto = run(v[0] + v[1], sum), front = upto - v[0] - v[1];
@@ -658,9 +661,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         s.got[0] = tid * 2 + j, s.got[1] = j ? front + v[0] : front, s.got[2] = m[j];
       }
       cluster_sync();
-      const uint32_t start = hi - ((uint32_t)s.got[0] << shift);
+      const int bin = (int)s.got[0];
       need -= s.got[1], n = s.got[2];
-      lo = max(lo, shift ? start - ((1u << shift) - 1) : start), hi = start;
+      if (one_value) {
+        lo = hi = value_of(bin);
+      } else {
+        const uint32_t start = hi - ((uint32_t)bin << shift);
+        lo = max(lo, start - ((1u << shift) - 1)), hi = start;
+      }
     }
     for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0;
     if (lo < hi) {
@@ -684,6 +692,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     if (tid == 0) s.n_aside = 0;
     __syncthreads();
   };
+  // The kept elements of logits lo .. hi are set aside; of 16-bit logits there are few values in between, of many elements each
+  constexpr bool ASIDE = sizeof(T) == 4;
+  const auto put_aside = [&](float lo_x, float hi_x) {
+    each([&](int i, float x) {
+      if (lo_x <= x && x <= hi_x && kept(i, x)) set_aside(i, x);
+    });
+    __syncthreads();
+  };
   if (k < V) {
     const float scale = scale_of(fmaxf(lowest, top - 48.f));
     each([&](int, float x) {
@@ -696,11 +712,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       __syncthreads();
       between(bin, bin, scale);
       const uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
-      const float lo_x = ordered(lo), hi_x = ordered(hi);
-      each([&](int i, float x) {
-        if (lo_x <= x && x <= hi_x) set_aside(i, x);
-      });
-      inside(lo, hi, false, (u64)k - above);
+      u64 v[4] = {0, 0, 0, 0};
+      if (ASIDE) {
+        put_aside(ordered(lo), ordered(hi));
+        v[0] = tid == 0 ? s.n_aside : 0, v[1] = tid == 0 && s.n_aside > SA_ASIDE;
+        all_of(v);
+      }
+      inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - above);
     }
   }
   // What counts of each element: from what on it weighs anything, and whether it is kept
@@ -724,47 +742,57 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     between(b1, b2, scale);
     uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
     const float lo_x = fmaxf(ordered(lo), from), hi_x = ordered(hi);
-    u64 all = 0, above = 0, all_sum, above_sum;
+    u64 all = 0, above = 0;
     each([&](int i, float x) {
-      if (x >= from && !(ties && x == edge && i > last)) {
-        const u64 w = weigh(x);
-        all += w;
-        if (x > hi_x) above += w;
-        else if (x >= lo_x) set_aside(i, x);
-      }
+      u64 w = weigh(x);
+      w = x >= from ? w : 0;
+      if (ties) w = x == edge && i > last ? 0 : w;
+      all += w;
+      above += x > hi_x ? w : 0;
     });
-    above = warp_sum(above);
-    all_of(all, lane == 0 ? above : 0, all_sum, above_sum);
-    const u64 limit = max(share_of<true>(all_sum, p), 1ull);
-    u64 in = 0, in_sum, over;
-    __syncthreads();
-    const int own = min((int)s.n_aside, SA_ASIDE);
-    for (int j = tid; j < own; j += SA_THREADS) in += weigh(ordered((uint32_t)(s.aside[j] >> 32)));
-    all_of(in, tid == 0 && s.n_aside > SA_ASIDE, in_sum, over);
-    if (over) {      // no room for them all
-      in = 0;
+    u64 v[4] = {all, above, 0, 0}, in = 0;
+    bool over = !ASIDE;
+    int own = 0;
+    if (ASIDE) {
+      put_aside(lo_x, hi_x);
+      own = min((int)s.n_aside, SA_ASIDE);
+      for (int j = tid; j < own; j += SA_THREADS) v[2] += weigh(ordered((uint32_t)(s.aside[j] >> 32)));
+      v[3] = tid == 0 ? (u64)(s.n_aside > SA_ASIDE) << 32 | s.n_aside : 0;
+    }
+    const u64 warps_above = warp_sum(above);
+    all_of(v);
+    const u64 limit = max(share_of<true>(v[0], p), 1ull);
+    u64 above_sum = v[1], n = (uint32_t)v[3];
+    over |= v[3] >> 32 != 0;
+    in = v[2];
+    if (over) {      // the row has them
+      u64 q[4] = {0, 0, 0, 0};
       each([&](int i, float x) {
-        if (lo_x <= x && x <= hi_x && !(ties && x == edge && i > last)) in += weigh(x);
+        if (lo_x <= x && x <= hi_x && kept(i, x)) q[0] += weigh(x), ++q[1];
       });
-      u64 none;
-      all_of(in, 0, in_sum, none);
+      all_of(q);
+      in = q[0], n = q[1];
     }
-    if (above_sum >= limit || above_sum + in_sum < limit) {      // not between those two: among all
+    const bool guessed = above_sum < limit && limit <= above_sum + in;
+    if (!guessed) over = true, n = V, lo = 0, hi = order_of(top);      // not between those two: among all
+    inside(max(lo, order_of(from)), hi, n, over, true, guessed ? limit - above_sum : limit);
+    if (low == 0 && guessed) {      // the warps' sums: what was above, and the kept ones between the two
+      if (lane == 0) s.sums[turn][warp] = warps_above;
       __syncthreads();
-      if (tid == 0) s.n_aside = SA_ASIDE + 1;
-      over = 1, above_sum = 0;
-      lo = 0, hi = order_of(top);
-    }
-    inside(max(lo, order_of(from)), hi, true, limit - above_sum);
-    // the warps' sums: what was above, and of what was set aside the kept ones
-    if (low == 0 && !over) {
-      if (lane == 0) s.sums[turn][warp] = above;
-      __syncthreads();
-      for (int j = tid; j < own; j += SA_THREADS) {
-        const u64 v = s.aside[j];
-        const int i = (int)(uint32_t)~(uint32_t)v;
-        const float x = ordered((uint32_t)(v >> 32));
-        if (kept(i, x)) atomicAdd(&s.sums[turn][i / (its * STEP) % SA_WARPS], weigh(x));
+      if (!over) {
+        for (int j = tid; j < own; j += SA_THREADS) {
+          const u64 e = s.aside[j];
+          const int i = (int)(uint32_t)~(uint32_t)e;
+          const float x = ordered((uint32_t)(e >> 32));
+          if (kept(i, x)) atomicAdd(&s.sums[turn][i / (its * STEP) % SA_WARPS], weigh(x));
+        }
+      } else {
+        u64 rest = 0;
+        each([&](int i, float x) {
+          if (lo_x <= x && x <= hi_x && kept(i, x)) rest += weigh(x);
+        });
+        rest = warp_sum(rest);
+        if (lane == 0) s.sums[turn][warp] += rest;
       }
       __syncthreads();
       const u64 sum = s.sums[turn][warp];
@@ -783,7 +811,7 @@ static int launch(const FtkSampleDesc& d, int its, cudaStream_t s) {
   int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(d.R * d.cluster));
+  cfg.gridDim = dim3((unsigned)(d.R << d.cluster));
   cfg.blockDim = dim3(SA_THREADS);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
@@ -791,7 +819,7 @@ static int launch(const FtkSampleDesc& d, int its, cudaStream_t s) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)d.cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  at[1].val.clusterDim.x = 1u << d.cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
   return (int)cudaLaunchKernelEx(&cfg, kernel, d, its);
@@ -806,7 +834,9 @@ template <typename T> static int launch(FtkSampleDesc d, cudaStream_t s) {
   // As many CTAs for a row as fill the SMs twice, with two steps each at least, and as many as it takes to keep the row
   int c = 1;
   while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 2ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > SA_SHARE)) c *= 2;
-  d.cluster = c;
+  int lc = 0;
+  while ((1 << lc) < c) ++lc;
+  d.cluster = lc;
   const int its = its_of(c);
   if (its > SA_STEPS || d.R * c > 0x7fffffff) return -2;
   const bool res = its * SA_THREADS * 16 <= SA_SHARE;
