@@ -77,6 +77,15 @@ __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// In two halves, for the end of a kernel: nobody leaves while its words are read
+__device__ __forceinline__ void leave_arrive() {
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void leave_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -285,10 +294,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   };
   // The first element by id whose running sum of value(id, logit) passes aim(sum of all).  `sum`: of this thread's elements
   struct Place {
-    int id;
-    u64 value, total;
+    int id, owner;                     // id; warp of the row
+    u64 front, target;                 // sum in front of that warp's run, and what was looked for
   };
-  const auto locate_from = [&](u64 warps_sum, const auto& value, const auto& aim) -> Place {
+  // `leaves`: the answer of the row, written by who finds it; the CTAs end with it
+  const auto locate_from = [&](u64 warps_sum, bool leaves, const auto& value, const auto& aim) -> Place {
     u64* w = s.sums[turn];
     if (lane == 0) w[warp] = warps_sum;
     cluster_sync();
@@ -310,7 +320,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
         if (owner == j && target >= front + v[j]) front += v[j], ++owner;
       if (here || (lane == 0 && target >= total)) s.got[2] = lane * 4 + owner, s.got[3] = front, s.got[4] = target, s.got[5] = total;
     }
-    __syncthreads();
+    if (leaves) leave_arrive();
+    else __syncthreads();
     const int owner = (int)s.got[2];
     const u64 target = s.got[4], total = s.got[5];
     if (owner / SA_WARPS == rank) {      // its CTA: the steps of that warp's run, then the lanes of one step
@@ -348,28 +359,31 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           if (!done && target < at + y[e]) {
-            s.record[turn][0] = (u64)(first + (it * 32 + lane) * N + e), s.record[turn][1] = y[e];
+            const int id = first + (it * 32 + lane) * N + e;
+            if (leaves) d.token[r] = id, d.logprob[r] = (float)log((double)y[e] / (double)total);
+            else s.record[turn][0] = (u64)id;
             done = true;
           }
           at += y[e];
         }
       }
     }
+    Place got = {0, owner, s.got[3], target};
+    if (leaves) {
+      leave_wait();
+      return got;
+    }
     cluster_sync();
-    if (tid < 2) s.got[6 + tid] = peek(&s.record[turn][tid], owner / SA_WARPS);
+    if (tid == 0) s.got[6] = peek(&s.record[turn][0], owner / SA_WARPS);
     __syncthreads();
-    const Place got = {(int)s.got[6], s.got[7], total};
+    got.id = (int)s.got[6];
     turn ^= 1;
     return got;
   };
-  const auto locate = [&](const auto& value, const auto& aim) -> Place {
-    u64 sum = 0;
+  const auto sum_of = [&](const auto& value) {      // of this warp's elements
+    decltype(value(0, 0.f)) sum = 0;
     each([&](int i, float x) { sum += value(i, x); });
-    return locate_from(warp_sum(sum), value, aim);
-  };
-  const auto finish = [&](const Place& x) {
-    if (rank == 0 && tid == 0) leave(x.id, (float)log((double)x.value / (double)x.total));
-    cluster_sync();      // nobody leaves while its words are read
+    return (u64)warp_sum(sum);
   };
   const auto at_random = [&](u64 total) { return u >= 1.f ? total - 1 : min(share_of<false>(total, u), total - 1); };
 
@@ -377,15 +391,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   const u64 low = least >= 1.f ? 1ull << 43 : (u64)ceil(fmax((double)least, 0.0) * 0x1p43);
   if (k == 1 || top == INFINITY) {      // of the largest the first, or the first few: they weigh the same
     u64 kept_ones = 1;
-    const Place at = locate([&](int, float x) -> u64 { return x == top; }, [&](u64 total) {
+    const auto largest = [&](int, float x) -> uint32_t { return x == top; };
+    const Place at = locate_from(sum_of(largest), false, largest, [&](u64 total) {
       kept_ones = min(total, (u64)k);
       if (p < 1.f) kept_ones = max((share_of<true>(kept_ones << 43, p) + (1ull << 43) - 1) >> 43, 1ull);
       return at_random(kept_ones << 43) >> 43;
     });
-    if (rank == 0 && warp == 0) {
-      kept_ones = __shfl_sync(0xffffffffu, kept_ones, 0);
-      if (lane == 0) leave(at.id, kept_ones == 1 ? 0.f : (float)-log((double)kept_ones));
-    }
+    if (rank == 0 && tid == 0) leave(at.id, kept_ones == 1 ? 0.f : (float)-log((double)kept_ones));
     cluster_sync();
     return;
   }
@@ -511,69 +523,67 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   float edge = -INFINITY;
   int last = V;
   const auto kept = [&](int i, float x) { return x > edge || (x == edge && i <= last); };
-  // Up to two steps of a histogram of the row at which the running sum of value(step, count) reaches aim(sum of all, ..): each CTA adds up
-  // its part of the steps.  The sums are fp32 in a fixed order, exact for counts.  got[]: two steps, the sums in front of them (as fp32).
+  // Two steps of a histogram of the row at which the running sum of value(step) per element reaches aim(sum of all, of squares, ..), in fp32 (exact for
+  // counts) and a fixed order, all of it in each CTA.  got[]: the steps in the upper halves, the sums in front of them in the lower; ~0
+  // where it is not reached.  The histogram may be cleared behind the next barrier of the cluster.
   const auto find = [&](const auto& value, const auto& aim) {
-    const int nb = SA_BINS >> lc, per = max(nb / SA_THREADS, 1), b0 = rank * nb + tid * per;
     cluster_sync();
-    float v[4], four = 0.f;
+    float v[4], four = 0.f, square = 0.f;      // square: of what one element of a step counts, over all
+    uint32_t n[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < SA_CLUSTER; ++c) {
+      if (c < C) {
+        uint4 q;
+        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(there(&s.hist[tid * 4], c)) : "memory");
+        n[0] += q.x, n[1] += q.y, n[2] += q.z, n[3] += q.w;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint32_t n = 0;
-      if (j < per && tid * per < nb) {
-#pragma unroll
-        for (int c = 0; c < SA_CLUSTER; ++c) n += c < C ? peek(&s.hist[b0 + j], c) : 0;
-      }
-      v[j] = n ? value(b0 + j, n) : 0.f;
+      const float one = n[j] ? value(tid * 4 + j) : 0.f;
+      v[j] = (float)n[j] * one, square += v[j] * one;
       four += v[j];
     }
     const float up = warp_upto(four);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
     float* part = reinterpret_cast<float*>(s.part);
-    if (lane == 31) part[warp] = up;
+    if (lane == 31) part[warp] = up, part[SA_WARPS + warp] = square;
+    if (tid < 2) s.got[tid] = ~0ull;
     __syncthreads();
-    float front = up - four, mine_all = 0.f;
+    float front = up - four, all = 0.f, squares = 0.f;
+#pragma unroll
     for (int w = 0; w < SA_WARPS; ++w) {
-      if (w < warp) front += part[w];
-      mine_all += part[w];
+      const float q = part[w];
+      squares += part[SA_WARPS + w];
+      front += w < warp ? q : 0.f;
+      all += q;
     }
-    if (tid == 0) s.words[turn][0] = __float_as_uint(mine_all);
-    if (tid < 2) s.record[turn][tid] = ~0ull;
-    cluster_sync();
-    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
-    if (warp == 0) {
-      const float q = lane < C ? __uint_as_float((uint32_t)peek(&s.words[turn][0], lane)) : 0.f, upto = warp_upto(q);
-      const float all = __shfl_sync(0xffffffffu, upto, 31), before = __shfl_sync(0xffffffffu, upto - q, rank);
-      if (lane == 0) s.got[0] = __float_as_uint(all), s.got[1] = __float_as_uint(before);
-    }
-    __syncthreads();
-    const float all = __uint_as_float((uint32_t)s.got[0]);
-    front += __uint_as_float((uint32_t)s.got[1]);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const float want = aim(all, a);
+      const float want = aim(all, squares, a);
       float at = front;
+      if (front < want && front + four >= want) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (v[j] > 0.f && at + v[j] >= want) {
-          atomicMin(&s.record[turn][a], (u64)(b0 + j) << 32 | __float_as_uint(at));
-          break;
+        for (int j = 0; j < 4; ++j) {
+          if (v[j] > 0.f && at + v[j] >= want) {
+            atomicMin(&s.got[a], (u64)(tid * 4 + j) << 32 | __float_as_uint(at));
+            break;
+          }
+          at += v[j];
         }
-        at += v[j];
       }
     }
-    cluster_sync();
-    if (warp == 0) {
-      u64 q = lane < 2 * C ? peek(&s.record[turn][lane & 1], lane >> 1) : ~0ull;
-#pragma unroll
-      for (int o = 2; o < 2 * SA_CLUSTER; o <<= 1) q = min(q, __shfl_xor_sync(0xffffffffu, q, o));
-      if (lane < 2) s.got[lane] = q;
-    }
     __syncthreads();
-    turn ^= 1;
   };
   // The smallest logit (as `order`) of step `b` or one further up, found by all lanes of a warp
   const auto first_of = [&](int b, float scale) {
     uint32_t lo = 0x00800000u, hi = order_of(top);      // the lowest finite number; step_of(top) = 0
+    {      // about there
+      const uint32_t at = order_of(fmaxf(top - ((float)b + 0.5f) / scale, -3.4e38f)) - 16 + lane;
+      const unsigned yes = __ballot_sync(0xffffffffu, lo <= at && at <= hi && step_of(ordered(at), scale) <= b), in = __ballot_sync(0xffffffffu, lo <= at && at <= hi);
+      if (in == 0xffffffffu && yes && !(yes & 1u)) return __shfl_sync(0xffffffffu, at, __ffs(yes) - 1);
+    }
     while (lo < hi) {      // 31 points between them
       const u64 span = (u64)hi - lo;
       const uint32_t at = lo + (uint32_t)(span * (u64)lane >> 5);
@@ -598,10 +608,32 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const uint32_t at = atomicAdd(&s.n_aside, 1);
     if (at < SA_ASIDE) s.aside[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
   };
+  constexpr int GRAIN = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);      // two logits are 2^GRAIN apart, at least
+  const auto logit_below = [&](uint32_t o) {      // the largest logit up to `o`
+    const uint32_t c = o & ~((1u << GRAIN) - 1);
+    return c >= 0x80000000u ? c : ((o + 1) & ~((1u << GRAIN) - 1)) - 1;
+  };
+  // The border among the kept elements of one value, of which this warp has `many`: it has as many of them as are needed, by their ids.
+  // Sets how many of the warp's own that are.  False where there are not so many.
+  const auto among_equal = [&](uint32_t o, u64 one, u64 many, u64 need, u64& stay) {
+    const float value = ordered(o);
+    const int until = value == edge ? last : V;
+    const u64 take = (need + one - 1) / max(one, 1ull);
+    __syncthreads();
+    if (tid == 0) s.got[0] = 0;
+    const Place at = locate_from(many, false, [&](int i, float x) -> uint32_t { return x == value && i <= until; }, [&](u64 total) {
+      if (take > total) s.got[0] = 1;
+      return min(take, total) - 1;
+    });
+    if (s.got[0]) return false;
+    const int own = rank * SA_WARPS + warp;
+    stay = own < at.owner ? many : own == at.owner ? at.target - at.front + 1 : 0;
+    edge = value, last = at.id;
+    return true;
+  };
   // The border among n kept elements of logits lo .. hi (as `order`) is where the running count or sum of weights reaches `need`.  They have
-  // been set aside, or where there was no room all look at the whole row for them.
+  // been set aside, or where there was no room all look at the whole row for them.  False where they do not reach it.
   const auto inside = [&](uint32_t lo, uint32_t hi, u64 n, bool over, bool mass, u64 need) {
-    constexpr int GRAIN = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);      // two logits are 2^GRAIN apart, at least
     const float lo0 = ordered(lo), hi0 = ordered(hi);
     const int own = min((int)s.n_aside, SA_ASIDE);
     const auto members = [&](const auto& fn) {      // fn(order, inverted id)
@@ -622,10 +654,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       int shift = GRAIN;
       while ((hi - lo) >> shift >= SA_FINE) ++shift;
       const bool one_value = shift == GRAIN;      // in each step: its sum of weights is a product
-      const auto value_of = [&](int b) {          // the logit that a step of one value has
-        const uint32_t start = hi - ((uint32_t)b << shift), c = start & ~((1u << GRAIN) - 1);
-        return c >= 0x80000000u ? c : ((start + 1) & ~((1u << GRAIN) - 1)) - 1;
-      };
+      const auto value_of = [&](int b) { return logit_below(hi - ((uint32_t)b << shift)); };
       for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0, s.mass[i] = 0;
       __syncthreads();
       members([&](uint32_t o, uint32_t) {
@@ -656,11 +685,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       }
       u64 sum;
       const u64 upto = run(v[0] + v[1], sum), front = upto - v[0] - v[1];
-      if (front < need && (need <= upto || (upto == sum && v[0] + v[1]))) {      // (the last one that has anything, if they do not reach it)
+      if (front < need && need <= upto) {
         const int j = need > front + v[0] && v[1] ? 1 : 0;
         s.got[0] = tid * 2 + j, s.got[1] = j ? front + v[0] : front, s.got[2] = m[j];
       }
       cluster_sync();
+      if (need > sum) {
+        for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0;
+        __syncthreads();
+        return false;
+      }
       const int bin = (int)s.got[0];
       need -= s.got[1], n = s.got[2];
       if (one_value) {
@@ -677,19 +711,25 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       const u64 key = tid < m ? s.sorted[tid] : 0, w = tid < m ? weight_of((uint32_t)(key >> 32)) : 0;
       u64 sum;
       const u64 upto = run(w, sum);
-      if (tid < m && upto - w < need && (need <= upto || tid == m - 1)) s.got[0] = key;
+      if (upto - w < need && need <= upto) s.got[0] = key;
       cluster_sync();      // the lists have been read
+      if (need > sum) {
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        return false;
+      }
       edge = ordered((uint32_t)(s.got[0] >> 32)), last = (int)(uint32_t)~(uint32_t)s.got[0];
       if (tid == 0) s.n_list = 0;
     } else {
-      // equal ones: as many as are needed, by their ids
       const float value = ordered(lo);
-      const u64 one = weight_of(lo), many = one ? (need + one - 1) / one : n;
-      const Place at = locate([&](int i, float x) -> u64 { return x == value && kept(i, x); }, [&](u64 total) { return min(max(many, 1ull), total) - 1; });
-      edge = value, last = at.id;
+      const int until = value == edge ? last : V;
+      u64 stay;
+      return among_equal(lo, weight_of(lo), sum_of([&](int i, float x) -> uint32_t { return x == value && i <= until; }), need, stay);
     }
-    __syncthreads();
-    if (tid == 0) s.n_aside = 0;
+    return true;
+  };
+  const auto clear_hist = [&]() {
+    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
     __syncthreads();
   };
   // The kept elements of logits lo .. hi are set aside; of 16-bit logits there are few values in between, of many elements each
@@ -705,27 +745,32 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     each([&](int, float x) {
       if (x > -INFINITY) atomicAdd(&s.hist[step_of(x, scale)], 1);
     });
-    find([](int, uint32_t n) { return (float)n; }, [&](float, int) { return (float)k; });
-    if (s.got[0] != ~0ull) {      // else there are not so many
-      const int bin = (int)(s.got[0] >> 32);
-      const u64 above = (u64)__uint_as_float((uint32_t)s.got[0]);
-      __syncthreads();
-      between(bin, bin, scale);
+    find([](int) { return 1.f; }, [&](float, float, int) { return (float)k; });
+    const u64 got = s.got[0];
+    __syncthreads();
+    if (got != ~0ull) {      // else there are not so many
+      between((int)(got >> 32), (int)(got >> 32), scale);
       const uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
       u64 v[4] = {0, 0, 0, 0};
-      if (ASIDE) {
-        put_aside(ordered(lo), ordered(hi));
-        v[0] = tid == 0 ? s.n_aside : 0, v[1] = tid == 0 && s.n_aside > SA_ASIDE;
-        all_of(v);
-      }
-      inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - above);
+      if (ASIDE) put_aside(ordered(lo), ordered(hi));
+      v[0] = tid == 0 ? s.n_aside : 0, v[1] = tid == 0 && s.n_aside > SA_ASIDE;
+      all_of(v);
+      clear_hist();
+      inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - (u64)__uint_as_float((uint32_t)got));
+      if (tid == 0) s.n_aside = 0;
+      __syncthreads();
+    } else {
+      cluster_sync();
+      clear_hist();
     }
   }
   // What counts of each element: from what on it weighs anything, and whether it is kept
   const auto final = [&](int i, float x) -> u64 {
-    if (!(x >= weigh.floor) || !kept(i, x)) return 0;
-    const u64 w = weigh(x);
-    return w >= low ? w : 0;
+    u64 w = weigh(x);
+    w = x >= weigh.floor && x >= edge ? w : 0;
+    if (last < V) w = x == edge && i > last ? 0 : w;
+    if (low) w = w >= low ? w : 0;
+    return w;
   };
   if (p < 1.f) {
     const float from = fmaxf(weigh.floor, edge), scale = scale_of(fmaxf(lowest, from));
@@ -733,53 +778,56 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     each([&](int, float x) {
       if (x >= from) atomicAdd(&s.hist[step_of(x, scale)], 1);
     });
-    // A step's elements by the weight of its middle, within a factor of exp(1 / 2 scale T): the border is between the two steps where their
-    // sums pass p of it all, less and more 1/4 of that
-    const float per_bin = scale > 0.f ? 1.4426950f / (scale * t) : 0.f, slack = fminf(0.25f * per_bin, 0.5f) + 1e-5f;
-    find([&](int b, uint32_t n) { return (float)n * exp2f(-(float)b * per_bin); }, [&](float all, int a) { return p * all * (a ? 1.f + slack : 1.f - slack); });
+    // A step's elements by the weight of its middle: each is off by up to half a step's factor, 1/sqrt(12) of a step on average and either
+    // way, so that the border is between the two steps where their sums pass p of it all less and more four times that in the square mean
+    const float per_bin = scale > 0.f ? 1.f / (scale * t) : 0.f;
+    find([&](int b) { return exp2f(-1.4426950f * (float)b * per_bin); }, [&](float all, float squares, int a) {
+      const float off = 1.2f * fminf(per_bin, 1.f) * sqrtf(squares) + 1e-5f * all;
+      return p * all + (a ? off : -off);
+    });
     const int b1 = s.got[0] == ~0ull ? 0 : (int)(s.got[0] >> 32), b2 = s.got[1] == ~0ull ? SA_BINS - 1 : (int)(s.got[1] >> 32);
     __syncthreads();
     between(b1, b2, scale);
     uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
     const float lo_x = fmaxf(ordered(lo), from), hi_x = ordered(hi);
+    const uint32_t one = logit_below(hi);
+    const bool single = one >= lo && (one == 0 || logit_below(one - 1) < lo);      // one value: its elements need not be looked at
     u64 all = 0, above = 0;
     each([&](int i, float x) {
-      u64 w = weigh(x);
-      w = x >= from ? w : 0;
-      if (ties) w = x == edge && i > last ? 0 : w;
+      const bool in = x >= from && !(ties && x == edge && i > last), up = x > hi_x;
+      const u64 w = in ? weigh(x) : 0;
       all += w;
-      above += x > hi_x ? w : 0;
+      above += up ? w : 0;
     });
-    u64 v[4] = {all, above, 0, 0}, in = 0;
-    bool over = !ASIDE;
-    int own = 0;
-    if (ASIDE) {
+    u64 v[4] = {all, above, 0, 0};
+    if (ASIDE && !single) {
       put_aside(lo_x, hi_x);
-      own = min((int)s.n_aside, SA_ASIDE);
-      for (int j = tid; j < own; j += SA_THREADS) v[2] += weigh(ordered((uint32_t)(s.aside[j] >> 32)));
-      v[3] = tid == 0 ? (u64)(s.n_aside > SA_ASIDE) << 32 | s.n_aside : 0;
+      v[2] = tid == 0 ? s.n_aside : 0, v[3] = tid == 0 && s.n_aside > SA_ASIDE;
     }
+    const int own = min((int)s.n_aside, SA_ASIDE);
     const u64 warps_above = warp_sum(above);
     all_of(v);
+    clear_hist();
     const u64 limit = max(share_of<true>(v[0], p), 1ull);
-    u64 above_sum = v[1], n = (uint32_t)v[3];
-    over |= v[3] >> 32 != 0;
-    in = v[2];
-    if (over) {      // the row has them
-      u64 q[4] = {0, 0, 0, 0};
-      each([&](int i, float x) {
-        if (lo_x <= x && x <= hi_x && kept(i, x)) q[0] += weigh(x), ++q[1];
-      });
-      all_of(q);
-      in = q[0], n = q[1];
+    const bool over = !ASIDE || v[3];
+    lo = max(lo, order_of(from));
+    u64 stay = 0;
+    bool guessed = v[1] < limit;
+    if (guessed) {
+      if (single) {
+        const float value = ordered(one);
+        const int until = value == edge ? last : V;
+        guessed = value >= from && among_equal(one, weigh(value), sum_of([&](int i, float x) -> uint32_t { return x == value && i <= until; }), limit - v[1], stay);
+      } else {
+        guessed = inside(lo, hi, over ? SA_LIST + 1 : v[2], over, true, limit - v[1]);
+      }
     }
-    const bool guessed = above_sum < limit && limit <= above_sum + in;
-    if (!guessed) over = true, n = V, lo = 0, hi = order_of(top);      // not between those two: among all
-    inside(max(lo, order_of(from)), hi, n, over, true, guessed ? limit - above_sum : limit);
+    if (!guessed) inside(order_of(from), order_of(top), V, true, true, limit);      // not between those two: among all
     if (low == 0 && guessed) {      // the warps' sums: what was above, and the kept ones between the two
-      if (lane == 0) s.sums[turn][warp] = warps_above;
+      if (lane == 0) s.sums[turn][warp] = warps_above + stay * (single ? weigh(ordered(one)) : 0);
       __syncthreads();
-      if (!over) {
+      if (single) {
+      } else if (!over) {
         for (int j = tid; j < own; j += SA_THREADS) {
           const u64 e = s.aside[j];
           const int i = (int)(uint32_t)~(uint32_t)e;
@@ -797,11 +845,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
       __syncthreads();
       const u64 sum = s.sums[turn][warp];
       __syncthreads();
-      finish(locate_from(sum, final, at_random));
+      locate_from(sum, true, final, at_random);
       return;
     }
   }
-  finish(locate(final, at_random));
+  locate_from(sum_of(final), true, final, at_random);
 }
 
 template <typename T, bool RES, bool VEC>
