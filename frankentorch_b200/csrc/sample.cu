@@ -11,9 +11,9 @@
 // Work.  A cluster of CTAs has a row, each an equal run of its columns, which it keeps in shared memory (rows of more than that are read
 // again from L2): everything behind the first pass works there.  The CTAs read one another's sums, histograms and lists over
 // distributed shared memory, a warp of each for all of it, and come to the same conclusions.
-//   * The k largest of a small k are among the elements that reach the k-th largest of 512 maxima, of as many parts of the row: hardly more
+//   * The k largest of a small k are among the elements that reach the k-th largest of 256 maxima, of as many parts of the row: hardly more
 //     than k.  They become a list, ordered by counting, and the rest is done on it by one CTA.
-//   * Else the border of top-k and of top-p is looked for in two steps: counts of 2048 equal steps of the logits' range say between which
+//   * Else the border of top-k and of top-p is looked for in two steps: counts of 1024 equal steps of the logits' range say between which
 //     two logits it is, and the elements between them are set aside.  For top-p the same pass has the sum of all weights and of those
 //     above, the only time that all weights are formed.  What is set aside is divided further until it is one value, whose elements are
 //     taken by their ids, or a short list.
@@ -31,14 +31,15 @@
 namespace ftk {
 
 typedef unsigned long long u64;
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
-constexpr int SA_BINS = 2048;          // steps of a histogram of counts
-constexpr int SA_FINE = 1024;          // steps among the elements set aside
-constexpr int SA_ASIDE = 2048;         // elements that a CTA can set aside
-constexpr int SA_LIST = 512;           // elements of a list: one per thread
+constexpr int SA_LOG = 8, SA_THREADS = 1 << SA_LOG, SA_WARPS = SA_THREADS / 32;
+constexpr int SA_BINS = 4 * SA_THREADS;      // steps of a histogram of counts
+constexpr int SA_FINE = 2 * SA_THREADS;      // steps among the elements set aside
+constexpr int SA_ASIDE = 1024;         // elements that a CTA can set aside
+constexpr int SA_LIST = SA_THREADS;    // elements of a list: one per thread
 constexpr int SA_CLUSTER = 8;          // CTAs of a row at most
-constexpr int SA_STEPS = 64;           // vectors of a lane at most
-constexpr int SA_SHARE = 64 * 1024;    // bytes of a row that a CTA keeps at most: two CTAs share an SM
+constexpr int SA_STEPS = 128;          // vectors of a lane at most
+constexpr int SA_SHARE = 176 * 1024;   // bytes of a row that a CTA keeps at most
+static_assert(SA_WARPS == 8, "a lane for each of four sums of the warps");
 
 template <typename T> __device__ __forceinline__ void logits_of(const uint4& v, float (&x)[8]) { up8<T>(v, x); }
 template <typename T> __device__ __forceinline__ void logits_of(const uint4& v, float (&x)[4]) {
@@ -159,13 +160,13 @@ struct Weigh {
     constexpr double C = 0.0027076061740622863;       // ln(2) / 256
     const double p = r * fma(r, fma(r, C * C * C / 6, C * C / 2), C), t = table[k & 255];
     double v = fma(t, p, t);
-    v = __hiloint2double(__double2hiint(v) + (k >> 8) * (1 << 20), __double2loint(v));
-    return (u64)__double_as_longlong(v + 512.0) - 0x4080000000000000ull;
+    v = __hiloint2double(__double2hiint(v) + (int)((uint32_t)(k & ~255) << 12), __double2loint(v)) + 512.0;
+    return (u64)(uint32_t)(__double2hiint(v) - 0x40800000) << 32 | (uint32_t)__double2loint(v);
   }
 };
 
 template <typename T, bool RES, bool VEC>
-__global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_constant__ FtkSampleDesc d, const int its) {
+__global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_constant__ FtkSampleDesc d, const int its) {
   constexpr int N = 16 / (int)sizeof(T), STEP = 32 * N;      // elements of a vector, of a warp's step
   extern __shared__ __align__(16) unsigned char smem[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
 
   // ---- what all CTAs of the row agree on.  Published words take turns: between two uses of a set lies a barrier of the cluster.
   int turn = 0;
-  // The 512 parts of the row are C neighbouring lanes each; a thread learns one of their maxima (as `order`, 0 for none)
+  // The 256 parts of the row are C neighbouring lanes each; a thread learns one of their maxima (as `order`, 0 for none)
   uint32_t best = most > -INFINITY ? order_of(most) : 0;
   for (int o = 1; o < C; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & (C - 1)) == 0) s.maxima[tid >> lc] = best;
@@ -228,12 +229,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     if (lane == 0) s.part[warp][0] = lo, s.part[warp][1] = flag;
     __syncthreads();
     if (warp == 0) {
-      const uint32_t a = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][0]), b = __any_sync(0xffffffffu, s.part[lane & 15][1] != 0);
+      const uint32_t a = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 7][0]), b = __any_sync(0xffffffffu, s.part[lane & 7][1] != 0);
       if (lane == 0) s.words[0][0] = a, s.words[0][1] = b;
     }
   }
   cluster_sync();
-  const uint32_t part_max = peek(&s.maxima[tid & ((SA_THREADS >> lc) - 1)], tid >> (9 - lc));
+  const uint32_t part_max = peek(&s.maxima[tid & ((SA_THREADS >> lc) - 1)], tid >> (SA_LOG - lc));
   {
     const u64 own = lane < 2 * C ? peek(&s.words[0][lane & 1], lane >> 1) : (lane & 1 ? 0 : 0xffffffffu);
     const uint32_t hi = __reduce_max_sync(0xffffffffu, part_max), lo = __reduce_min_sync(0xffffffffu, part_max ? part_max : 0xffffffffu);
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     __syncthreads();
   }
   turn = 1;
-  uint32_t hi32 = (uint32_t)s.part[lane & 15][2], lo32 = (uint32_t)s.part[lane & 15][3];
+  uint32_t hi32 = (uint32_t)s.part[lane & 7][2], lo32 = (uint32_t)s.part[lane & 7][3];
   hi32 = __reduce_max_sync(0xffffffffu, hi32), lo32 = __reduce_min_sync(0xffffffffu, lo32);
   const float top = hi32 ? ordered(hi32) : -INFINITY, least_top = ordered(lo32), lowest = ordered((uint32_t)s.got[0]);
   odd = s.got[1] != 0;
@@ -275,10 +276,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     }
     __syncthreads();
     if (warp == 0) {
-      u64 a = s.part[lane & 15][lane >> 4], b = s.part[lane & 15][2 + (lane >> 4)];
+      u64 a = s.part[lane & 7][lane >> 3];
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o), b += __shfl_xor_sync(0xffffffffu, b, o);
-      if ((lane & 15) == 0) s.words[turn][lane >> 4] = a, s.words[turn][2 + (lane >> 4)] = b;
+      for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if ((lane & 7) == 0) s.words[turn][lane >> 3] = a;
     }
     cluster_sync();
     if (warp == 0) {
@@ -302,23 +303,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     u64* w = s.sums[turn];
     if (lane == 0) w[warp] = warps_sum;
     cluster_sync();
-    if (warp == 0) {      // four warps' sums of the row per lane
-      u64 v[4], four = 0;
+    if (warp == 0) {      // two warps' sums of the row per lane
+      u64 v[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = lane * 4 + j;
+      for (int j = 0; j < 2; ++j) {
+        const int at = lane * 2 + j;
         v[j] = at < C * SA_WARPS ? peek(&w[at % SA_WARPS], at / SA_WARPS) : 0;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) four += v[j];
-      const u64 upto = warp_upto(four), total = __shfl_sync(0xffffffffu, upto, 31), target = aim(total);
-      u64 front = upto - four;
-      const bool here = front <= target && target < upto;
-      int owner = 0;
-#pragma unroll
-      for (int j = 0; j < 3; ++j)
-        if (owner == j && target >= front + v[j]) front += v[j], ++owner;
-      if (here || (lane == 0 && target >= total)) s.got[2] = lane * 4 + owner, s.got[3] = front, s.got[4] = target, s.got[5] = total;
+      const u64 upto = warp_upto(v[0] + v[1]), total = __shfl_sync(0xffffffffu, upto, 31), target = aim(total), front = upto - v[0] - v[1];
+      const bool here = front <= target && target < upto, second = target >= front + v[0];
+      if (here || (lane == 0 && target >= total))
+        s.got[2] = lane * 2 + second, s.got[3] = second ? front + v[0] : front, s.got[4] = target, s.got[5] = total;
     }
     if (leaves) leave_arrive();
     else __syncthreads();
@@ -454,6 +449,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const float y = fminf((top - x) * scale, (float)(SA_BINS - 1));
     return __float_as_int(y + 12582912.f) - 0x4b400000;      // 1.5 2^23
   };
+  const uint32_t hist_s = smem_u32(s.hist);
+  const auto count_step = [&](float x, float scale) {
+    asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(hist_s + (uint32_t)step_of(x, scale) * 4) : "memory");
+  };
   const auto scale_of = [&](float lo) {
     const float range = top - lo;
     const float per = (float)(SA_BINS - 1) / range;
@@ -486,7 +485,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const uint32_t low_max = __reduce_min_sync(0xffffffffu, part_max && bin <= border ? part_max : 0xffffffffu);
     if (lane == 0) s.part[warp][2] = low_max;
     __syncthreads();
-    const uint32_t reach32 = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 15][2]);
+    const uint32_t reach32 = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[lane & 7][2]);
     const float reach = border == SA_BINS ? -3.402823466e38f : ordered(reach32);      // fewer maxima than k: all finite ones
     each([&](int i, float x) {
       if (x >= reach) to_list(i, x);
@@ -743,7 +742,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
   if (k < V) {
     const float scale = scale_of(fmaxf(lowest, top - 48.f));
     each([&](int, float x) {
-      if (x > -INFINITY) atomicAdd(&s.hist[step_of(x, scale)], 1);
+      if (x > -INFINITY) count_step(x, scale);
     });
     find([](int) { return 1.f; }, [&](float, float, int) { return (float)k; });
     const u64 got = s.got[0];
@@ -776,7 +775,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const float from = fmaxf(weigh.floor, edge), scale = scale_of(fmaxf(lowest, from));
     const bool ties = edge >= from;
     each([&](int, float x) {
-      if (x >= from) atomicAdd(&s.hist[step_of(x, scale)], 1);
+      if (x >= from) count_step(x, scale);
     });
     // A step's elements by the weight of its middle: each is off by up to half a step's factor, 1/sqrt(12) of a step on average and either
     // way, so that the border is between the two steps where their sums pass p of it all less and more four times that in the square mean
@@ -793,12 +792,16 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const __grid_cons
     const uint32_t one = logit_below(hi);
     const bool single = one >= lo && (one == 0 || logit_below(one - 1) < lo);      // one value: its elements need not be looked at
     u64 all = 0, above = 0;
-    each([&](int i, float x) {
-      const bool in = x >= from && !(ties && x == edge && i > last), up = x > hi_x;
-      const u64 w = in ? weigh(x) : 0;
-      all += w;
-      above += up ? w : 0;
+    each([&](int, float x) {
+      const u64 w = weigh(x);
+      if (x >= from) all += w;
+      if (x > hi_x) above += w;
     });
+    if (ties) {      // equal ones that top-k has not kept
+      uint32_t out = 0;
+      each([&](int i, float x) { out += x == edge && i > last; });
+      all -= out * weigh(edge);
+    }
     u64 v[4] = {all, above, 0, 0};
     if (ASIDE && !single) {
       put_aside(lo_x, hi_x);
@@ -879,9 +882,10 @@ template <typename T> static int launch(FtkSampleDesc d, cudaStream_t s) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const auto its_of = [&](int c) { return (int)((d.V + (long long)STEP * c - 1) / ((long long)STEP * c)); };
-  // As many CTAs for a row as fill the SMs twice, with two steps each at least, and as many as it takes to keep the row
+  // As many CTAs for a row as fill the SMs four times, with two steps each at least, and as many as it takes to keep 32 KB each: four
+  // CTAs share an SM then, and one works while others wait
   int c = 1;
-  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 2ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > SA_SHARE)) c *= 2;
+  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 4ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > 32 * 1024)) c *= 2;
   int lc = 0;
   while ((1 << lc) < c) ++lc;
   d.cluster = lc;
