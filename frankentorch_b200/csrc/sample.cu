@@ -13,7 +13,7 @@
 // distributed shared memory, a warp of each for all of it, and come to the same conclusions.
 //   * The k largest of a small k are among the elements that reach the k-th largest of 256 maxima, of as many parts of the row: hardly more
 //     than k.  They become a list, ordered by counting, and the rest is done on it by one CTA.
-//   * Else the border of top-k and of top-p is looked for in two steps: counts of 1024 equal steps of the logits' range say between which
+//   * Else the border of top-k and of top-p is looked for in two steps: counts of 2048 equal steps of the logits' range say between which
 //     two logits it is, and the elements between them are set aside.  For top-p the same pass has the sum of all weights and of those
 //     above, the only time that all weights are formed.  What is set aside is divided further until it is one value, whose elements are
 //     taken by their ids, or a short list.
@@ -32,9 +32,9 @@ namespace ftk {
 
 typedef unsigned long long u64;
 constexpr int SA_LOG = 8, SA_THREADS = 1 << SA_LOG, SA_WARPS = SA_THREADS / 32;
-constexpr int SA_BINS = 4 * SA_THREADS;      // steps of a histogram of counts
+constexpr int SA_BINS = 8 * SA_THREADS;      // steps of a histogram of counts
 constexpr int SA_FINE = 2 * SA_THREADS;      // steps among the elements set aside
-constexpr int SA_ASIDE = 1024;         // elements that a CTA can set aside
+constexpr int SA_ASIDE = 512;          // elements that a CTA can set aside
 constexpr int SA_LIST = SA_THREADS;    // elements of a list: one per thread
 constexpr int SA_CLUSTER = 8;          // CTAs of a row at most
 constexpr int SA_STEPS = 128;          // vectors of a lane at most
@@ -450,8 +450,9 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     return __float_as_int(y + 12582912.f) - 0x4b400000;      // 1.5 2^23
   };
   const uint32_t hist_s = smem_u32(s.hist);
-  const auto count_step = [&](float x, float scale) {
-    asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(hist_s + (uint32_t)step_of(x, scale) * 4) : "memory");
+  const auto count_step = [&](float x, float scale, float from) {      // of x >= from
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(hist_s + (uint32_t)step_of(x, scale) * 4), "f"(x),
+                 "f"(from) : "memory");
   };
   const auto scale_of = [&](float lo) {
     const float range = top - lo;
@@ -466,20 +467,23 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     if (part_max) atomicAdd(&s.hist[bin], 1);
     __syncthreads();
     u64 all;
-    uint32_t four = 0, v[4];
+    constexpr int OWN = SA_BINS / SA_THREADS;
+    uint32_t own = 0, v[OWN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = s.hist[tid * 4 + j], four += v[j];
-    const u64 upto = run(four, all);
+    for (int j = 0; j < OWN; ++j) v[j] = s.hist[tid * OWN + j], own += v[j];
+    const u64 upto = run(own, all);
     if (tid == 0) s.got[0] = SA_BINS;
     __syncthreads();
-    if (upto - four < (u64)k && (u64)k <= upto) {
-      u64 at = upto - four;
-      int j = 0;
-      while (at + v[j] < (u64)k) at += v[j++];
-      s.got[0] = tid * 4 + j;
+    if (upto - own < (u64)k && (u64)k <= upto) {
+      u64 at = upto - own;
+#pragma unroll
+      for (int j = 0; j < OWN; ++j) {
+        if (at < (u64)k && (u64)k <= at + v[j]) s.got[0] = tid * OWN + j;
+        at += v[j];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s.hist[tid * 4 + j] = 0;
+    for (int j = 0; j < OWN; ++j) s.hist[tid * OWN + j] = 0;
     __syncthreads();
     const int border = (int)s.got[0];
     const uint32_t low_max = __reduce_min_sync(0xffffffffu, part_max && bin <= border ? part_max : 0xffffffffu);
@@ -522,58 +526,79 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   float edge = -INFINITY;
   int last = V;
   const auto kept = [&](int i, float x) { return x > edge || (x == edge && i <= last); };
-  // Two steps of a histogram of the row at which the running sum of value(step) per element reaches aim(sum of all, of squares, ..), in fp32 (exact for
-  // counts) and a fixed order, all of it in each CTA.  got[]: the steps in the upper halves, the sums in front of them in the lower; ~0
-  // where it is not reached.  The histogram may be cleared behind the next barrier of the cluster.
+  const auto clear_hist = [&]() {
+    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
+    __syncthreads();
+  };
+  // Two steps of a histogram of the row at which the running sum of value(step) per element reaches aim(sum of all, of squares, ..), in
+  // fp32 (exact for counts) and a fixed order; each CTA adds up its part of the steps.  got[]: the steps in the upper halves, the sums in
+  // front of them in the lower; ~0 where it is not reached.  Clears the histogram.
   const auto find = [&](const auto& value, const auto& aim) {
+    constexpr int MOST = SA_BINS / SA_THREADS;
+    const int per = max(MOST >> lc, 1), b0 = (rank << SA_LOG) * per + tid * per;      // (eight CTAs have a step per thread)
+    static_assert(SA_BINS == SA_THREADS * SA_CLUSTER, "a step per thread at least");
     cluster_sync();
-    float v[4], four = 0.f, square = 0.f;      // square: of what one element of a step counts, over all
-    uint32_t n[4] = {0, 0, 0, 0};
+    float v[MOST], own = 0.f, square = 0.f;      // square: of what one element of a step counts, over all
 #pragma unroll
-    for (int c = 0; c < SA_CLUSTER; ++c) {
-      if (c < C) {
-        uint4 q;
-        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(there(&s.hist[tid * 4], c)) : "memory");
-        n[0] += q.x, n[1] += q.y, n[2] += q.z, n[3] += q.w;
+    for (int j = 0; j < MOST; ++j) {
+      v[j] = 0.f;
+      if (j < per) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int c = 0; c < SA_CLUSTER; ++c) n += c < C ? peek(&s.hist[b0 + j], c) : 0;
+        const float one = n ? value(b0 + j) : 0.f;
+        v[j] = (float)n * one, square += v[j] * one;
+        own += v[j];
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float one = n[j] ? value(tid * 4 + j) : 0.f;
-      v[j] = (float)n[j] * one, square += v[j] * one;
-      four += v[j];
-    }
-    const float up = warp_upto(four);
+    const float up = warp_upto(own);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
     float* part = reinterpret_cast<float*>(s.part);
     if (lane == 31) part[warp] = up, part[SA_WARPS + warp] = square;
-    if (tid < 2) s.got[tid] = ~0ull;
+    if (tid < 2) s.record[turn][tid] = ~0ull;
     __syncthreads();
-    float front = up - four, all = 0.f, squares = 0.f;
+    float front = up - own;
 #pragma unroll
-    for (int w = 0; w < SA_WARPS; ++w) {
-      const float q = part[w];
-      squares += part[SA_WARPS + w];
-      front += w < warp ? q : 0.f;
-      all += q;
+    for (int w = 0; w < SA_WARPS; ++w) front += w < warp ? part[w] : 0.f;
+    if (tid == 0) {
+      float all = 0.f, squares = 0.f;
+#pragma unroll
+      for (int w = 0; w < SA_WARPS; ++w) all += part[w], squares += part[SA_WARPS + w];
+      s.words[turn][0] = (u64)__float_as_uint(squares) << 32 | __float_as_uint(all);
     }
+    cluster_sync();
+    if (warp == 0) {
+      const u64 q = lane < C ? peek(&s.words[turn][0], lane) : 0;
+      const float upto = warp_upto(__uint_as_float((uint32_t)q)), squares = warp_upto(__uint_as_float((uint32_t)(q >> 32)));
+      if (lane == 31) s.got[0] = __float_as_uint(upto), s.got[1] = __float_as_uint(squares);
+      if (lane == rank) s.got[2] = __float_as_uint(upto - __uint_as_float((uint32_t)q));
+    }
+    clear_hist();
+    const float all = __uint_as_float((uint32_t)s.got[0]), squares = __uint_as_float((uint32_t)s.got[1]);
+    front += __uint_as_float((uint32_t)s.got[2]);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const float want = aim(all, squares, a);
       float at = front;
-      if (front < want && front + four >= want) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (v[j] > 0.f && at + v[j] >= want) {
-            atomicMin(&s.got[a], (u64)(tid * 4 + j) << 32 | __float_as_uint(at));
-            break;
-          }
-          at += v[j];
+      for (int j = 0; j < MOST; ++j) {
+        if (v[j] > 0.f && at + v[j] >= want) {
+          atomicMin(&s.record[turn][a], (u64)(b0 + j) << 32 | __float_as_uint(at));
+          break;
         }
+        at += v[j];
       }
     }
+    cluster_sync();
+    if (warp == 0) {
+      u64 q = lane < 2 * C ? peek(&s.record[turn][lane & 1], lane >> 1) : ~0ull;
+#pragma unroll
+      for (int o = 2; o < 2 * SA_CLUSTER; o <<= 1) q = min(q, __shfl_xor_sync(0xffffffffu, q, o));
+      if (lane < 2) s.got[lane] = q;
+    }
     __syncthreads();
+    turn ^= 1;
   };
   // The smallest logit (as `order`) of step `b` or one further up, found by all lanes of a warp
   const auto first_of = [&](int b, float scale) {
@@ -727,10 +752,6 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     }
     return true;
   };
-  const auto clear_hist = [&]() {
-    for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
-    __syncthreads();
-  };
   // The kept elements of logits lo .. hi are set aside; of 16-bit logits there are few values in between, of many elements each
   constexpr bool ASIDE = sizeof(T) == 4;
   const auto put_aside = [&](float lo_x, float hi_x) {
@@ -742,7 +763,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   if (k < V) {
     const float scale = scale_of(fmaxf(lowest, top - 48.f));
     each([&](int, float x) {
-      if (x > -INFINITY) count_step(x, scale);
+      count_step(x, scale, -3.402823466e38f);
     });
     find([](int) { return 1.f; }, [&](float, float, int) { return (float)k; });
     const u64 got = s.got[0];
@@ -754,13 +775,10 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
       if (ASIDE) put_aside(ordered(lo), ordered(hi));
       v[0] = tid == 0 ? s.n_aside : 0, v[1] = tid == 0 && s.n_aside > SA_ASIDE;
       all_of(v);
-      clear_hist();
+      __syncthreads();
       inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - (u64)__uint_as_float((uint32_t)got));
       if (tid == 0) s.n_aside = 0;
       __syncthreads();
-    } else {
-      cluster_sync();
-      clear_hist();
     }
   }
   // What counts of each element: from what on it weighs anything, and whether it is kept
@@ -774,9 +792,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   if (p < 1.f) {
     const float from = fmaxf(weigh.floor, edge), scale = scale_of(fmaxf(lowest, from));
     const bool ties = edge >= from;
-    each([&](int, float x) {
-      if (x >= from) count_step(x, scale);
-    });
+    each([&](int, float x) { count_step(x, scale, from); });
     // A step's elements by the weight of its middle: each is off by up to half a step's factor, 1/sqrt(12) of a step on average and either
     // way, so that the border is between the two steps where their sums pass p of it all less and more four times that in the square mean
     const float per_bin = scale > 0.f ? 1.f / (scale * t) : 0.f;
@@ -789,8 +805,19 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     between(b1, b2, scale);
     uint32_t lo = (uint32_t)s.got[0], hi = (uint32_t)s.got[1];
     const float lo_x = fmaxf(ordered(lo), from), hi_x = ordered(hi);
-    const uint32_t one = logit_below(hi);
-    const bool single = one >= lo && (one == 0 || logit_below(one - 1) < lo);      // one value: its elements need not be looked at
+    // up to four values between: their elements are only counted
+    float value[4];
+    int values = 0;
+    {
+      uint32_t o = logit_below(hi);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        value[j] = ordered(o);
+        if (o >= lo && value[j] >= from && values == j) ++values;
+        o = logit_below(o - 1);
+      }
+      if (o >= lo && ordered(o) >= from) values = 0;
+    }
     u64 all = 0, above = 0;
     each([&](int, float x) {
       const u64 w = weigh(x);
@@ -803,33 +830,59 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
       all -= out * weigh(edge);
     }
     u64 v[4] = {all, above, 0, 0};
-    if (ASIDE && !single) {
+    uint32_t many[4] = {0, 0, 0, 0};
+    if (values) {
+      each([&](int, float x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) many[j] += x == value[j];
+      });
+      if (ties) {
+        each([&](int i, float x) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) many[j] -= x == value[j] && x == edge && i > last;
+        });
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= values) many[j] = 0;
+        many[j] = __reduce_add_sync(0xffffffffu, many[j]);      // of the warp
+      }
+      v[2] = lane == 0 ? (u64)many[0] << 32 | many[1] : 0, v[3] = lane == 0 ? (u64)many[2] << 32 | many[3] : 0;
+    } else if (ASIDE) {
       put_aside(lo_x, hi_x);
       v[2] = tid == 0 ? s.n_aside : 0, v[3] = tid == 0 && s.n_aside > SA_ASIDE;
     }
     const int own = min((int)s.n_aside, SA_ASIDE);
-    const u64 warps_above = warp_sum(above);
+    u64 kept_sum = warp_sum(above);      // of this warp
     all_of(v);
-    clear_hist();
+    __syncthreads();
     const u64 limit = max(share_of<true>(v[0], p), 1ull);
     const bool over = !ASIDE || v[3];
-    lo = max(lo, order_of(from));
-    u64 stay = 0;
     bool guessed = v[1] < limit;
-    if (guessed) {
-      if (single) {
-        const float value = ordered(one);
-        const int until = value == edge ? last : V;
-        guessed = value >= from && among_equal(one, weigh(value), sum_of([&](int i, float x) -> uint32_t { return x == value && i <= until; }), limit - v[1], stay);
-      } else {
-        guessed = inside(lo, hi, over ? SA_LIST + 1 : v[2], over, true, limit - v[1]);
+    if (guessed && values) {
+      u64 need = limit - v[1];
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 n = j & 1 ? (uint32_t)v[2 + (j >> 1)] : v[2 + (j >> 1)] >> 32, one = j < values ? weigh(value[j]) : 0;
+        if (found || j >= values) continue;
+        if (n * one >= need) {
+          u64 stay;
+          found = among_equal(order_of(value[j]), one, many[j], need, stay);
+          kept_sum += stay * one;
+        } else {
+          need -= n * one, kept_sum += many[j] * one;
+        }
       }
+      guessed = found;
+    } else if (guessed) {
+      guessed = inside(max(lo, order_of(from)), hi, over ? SA_LIST + 1 : v[2], over, true, limit - v[1]);
     }
     if (!guessed) inside(order_of(from), order_of(top), V, true, true, limit);      // not between those two: among all
     if (low == 0 && guessed) {      // the warps' sums: what was above, and the kept ones between the two
-      if (lane == 0) s.sums[turn][warp] = warps_above + stay * (single ? weigh(ordered(one)) : 0);
+      if (lane == 0) s.sums[turn][warp] = kept_sum;
       __syncthreads();
-      if (single) {
+      if (values) {
       } else if (!over) {
         for (int j = tid; j < own; j += SA_THREADS) {
           const u64 e = s.aside[j];
