@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   };
   // Equal steps of the logits from the top down, to the nearest: no less for a smaller logit
   const auto step_of = [&](float x, float scale) {
-    const float y = fminf((top - x) * scale, (float)(SA_BINS - 1));
-    return __float_as_int(y + 12582912.f) - 0x4b400000;      // 1.5 2^23
+    const float y = fminf(fmaf(top - x, scale, 12582912.f), 12582912.f + (SA_BINS - 1));      // 1.5 2^23
+    return __float_as_int(y) - 0x4b400000;
   };
   const uint32_t hist_s = smem_u32(s.hist);
   const auto count_step = [&](float x, float scale, float from) {      // of x >= from
@@ -832,10 +832,14 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     u64 v[4] = {all, above, 0, 0};
     uint32_t many[4] = {0, 0, 0, 0};
     if (values) {
-      each([&](int, float x) {
+      if (values <= 2) {
+        each([&](int, float x) { many[0] += x == value[0], many[1] += x == value[1]; });
+      } else {
+        each([&](int, float x) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) many[j] += x == value[j];
-      });
+          for (int j = 0; j < 4; ++j) many[j] += x == value[j];
+        });
+      }
       if (ties) {
         each([&](int i, float x) {
 #pragma unroll
