@@ -15,6 +15,12 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
+// The same of values of up to 448 and NaN
+__device__ __forceinline__ uint32_t e4m3_finite(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+  return r;
+}
 // Two values of the low 16 bits as fp16, which holds every one of them
 __device__ __forceinline__ uint32_t e4m3_up(uint32_t pair) {
   uint32_t r;

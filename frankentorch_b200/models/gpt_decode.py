@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import functools
-from typing import Callable, List, Optional, Sequence, Tuple, Union
+from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -38,20 +38,38 @@ class CacheFull(RuntimeError):
 
 class PagedKVCache:
     """Pages of all layers, ``[layers, pages, heads, page, hd]`` for keys and for values, and the page table of ``batch``
-    sequences.  A page number means the same page in every layer."""
+    sequences.  A page number means the same page in every layer.
+
+    With ``dtype`` ``torch.float8_e4m3fn`` keys and values take 8 bits, under a scale for every ``block`` rows of a page and head
+    (a power of two up to 64; the page, or 64): ``k_scales`` and ``v_scales``, ``[layers, pages, heads, page / block]``."""
 
     def __init__(self, layers: int, heads: int, hd: int, *, pages: int, batch: int, max_tokens: int, page: int = 64,
-                 device="cuda", dtype: torch.dtype = torch.bfloat16):
+                 device="cuda", dtype: torch.dtype = torch.bfloat16, block: Optional[int] = None):
         if page < 1 or page & (page - 1):
             raise ValueError(f"a page holds a power of two of tokens, not {page}")
         if pages < 1 or batch < 1 or max_tokens < 1:
             raise ValueError("pages, batch and max_tokens are positive")
+        if dtype != torch.float8_e4m3fn and block is not None:
+            raise ValueError(f"a cache of {dtype} has no scales")
         self.page, self.max_tokens = page, max_tokens
-        self.k = torch.zeros((layers, pages, heads, page, hd), dtype=dtype, device=device)
-        self.v = torch.zeros_like(self.k)
+        shape = (layers, pages, heads, page, hd)
+        self.k_scales = self.v_scales = None
+        if dtype == torch.float8_e4m3fn:
+            block = min(page, 64) if block is None else block
+            if not 1 <= block <= min(page, 64) or block & (block - 1):
+                raise ValueError(f"a scale is for a power of two of rows, up to {min(page, 64)} here, not {block}")
+            self.k, self.v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
+            self.k_scales, self.v_scales = (torch.zeros((layers, pages, heads, page // block), device=device) for _ in range(2))
+        else:
+            self.k = torch.zeros(shape, dtype=dtype, device=device)
+            self.v = torch.zeros_like(self.k)
         self.table = torch.zeros((batch, -(-max_tokens // page)), dtype=torch.int32, device=device)
         self._free: List[int] = list(range(pages - 1, -1, -1))
         self._held: List[List[int]] = [[] for _ in range(batch)]
+
+    def scales(self, layer: int) -> Dict[str, torch.Tensor]:
+        """The scales of a layer as the operators take them (none for a cache in 16 bits)."""
+        return {} if self.k_scales is None else {"k_scales": self.k_scales[layer], "v_scales": self.v_scales[layer]}
 
     @property
     def free_pages(self) -> int:
@@ -78,10 +96,11 @@ class PagedKVCache:
 
 
 class GPTDecoder:
-    """Decoding state of ``batch`` sequences over ``model``; ``pages`` (default: enough for all) bounds the cache."""
+    """Decoding state of ``batch`` sequences over ``model``; ``pages`` (default: enough for all) bounds the cache, ``cache_dtype``
+    ``torch.float8_e4m3fn`` halves it, with a scale for every ``cache_block`` rows (see :class:`PagedKVCache`)."""
 
     def __init__(self, model: GPT, batch: int, max_tokens: int, *, page: int = 64, pages: Optional[int] = None,
-                 use_cuda_graph: bool = True):
+                 use_cuda_graph: bool = True, cache_dtype: torch.dtype = torch.bfloat16, cache_block: Optional[int] = None):
         cfg = model.cfg
         if cfg.pos == "learned" and max_tokens > cfg.max_seq:
             raise ValueError(f"{max_tokens} tokens, the model has {cfg.max_seq} learned positions")
@@ -90,10 +109,12 @@ class GPTDecoder:
         self.hd = cfg.d_model // cfg.n_head
         if self.hd not in D.HEAD_SIZES:
             raise ValueError(f"head size must be one of {D.HEAD_SIZES}, not {self.hd}")
+        if cache_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"the cache is held in bfloat16 or float8_e4m3fn, not {cache_dtype}")
         if pages is None:
             pages = batch * -(-max_tokens // page)
         self.cache = PagedKVCache(cfg.n_layer, cfg.n_head, self.hd, pages=pages, batch=batch, max_tokens=max_tokens,
-                                  page=page, device=self.device)
+                                  page=page, device=self.device, dtype=cache_dtype, block=cache_block)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)      # tokens in the cache
         self.ids = torch.zeros(batch, dtype=torch.int64, device=self.device)
         self._host_lengths = [0] * batch
@@ -151,7 +172,7 @@ class GPTDecoder:
                 q, k, v = qkv.view(B, S, 3, H, hd).unbind(2)
                 if self.model.inv_freq is not None:
                     q, k = D.rotary(q, k, self.model.inv_freq)
-                D.paged_append(cache.k[l], cache.v[l], cache.table, k, v, start, counts)
+                D.paged_append(cache.k[l], cache.v[l], cache.table, k, v, start, counts, **cache.scales(l))
                 return K.attention_fwd(q, k, v, causal=True)[0].view(B * S, d)
             x = self._layer(l, x, attend)
         last = torch.arange(0, B * S, S, device=self.device) + counts - 1
@@ -170,12 +191,13 @@ class GPTDecoder:
         for l in range(cfg.n_layer):
             def attend(qkv, l=l):
                 q, k, v = qkv.view(B, 1, 3, H, hd).unbind(2)
+                scales = cache.scales(l)
                 if self.model.inv_freq is None:
-                    D.paged_append(cache.k[l], cache.v[l], cache.table, k, v, self.lengths)
+                    D.paged_append(cache.k[l], cache.v[l], cache.table, k, v, self.lengths, **scales)
                 else:
                     q = D.paged_append(cache.k[l], cache.v[l], cache.table, k, v, self.lengths, q=q,
-                                       inv_freq=self.model.inv_freq)
-                return D.paged_attention(q[:, 0], cache.k[l], cache.v[l], cache.table, reach)[0].view(B, d)
+                                       inv_freq=self.model.inv_freq, **scales)
+                return D.paged_attention(q[:, 0], cache.k[l], cache.v[l], cache.table, reach, **scales)[0].view(B, d)
             x = self._layer(l, x, attend)
         out = self._head(x)
         self.lengths.copy_(reach)
@@ -222,16 +244,26 @@ class GPTDecoder:
                  eos: Optional[int] = None, repetition=None, frequency=None, presence=None,
                  bias: Optional[torch.Tensor] = None,
                  allowed: Union[torch.Tensor, Callable[[torch.Tensor, torch.Tensor], torch.Tensor], None] = None,
-                 choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 choose: Optional[Callable[[torch.Tensor], torch.Tensor]] = None, temperature=None, top_k=None, top_p=None,
+                 min_p=None, generator: Optional[torch.Generator] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Continue the prompts by up to ``max_new_tokens`` tokens; returns ``(tokens [batch, S + max_new_tokens], totals [batch])``.
 
         Row ``b`` holds its prompt and what was generated behind it, ``totals[b]`` tokens; the rest of the row is 0.  The penalties,
         ``bias`` and ``allowed`` are those of :func:`~frankentorch_b200.ops.decode.logits_process`; ``allowed`` may be a function of the
-        tokens and totals so far.  ``choose`` takes the processed logits ``[batch, vocabulary]`` to the next ids (default: the
-        highest).  A row ends behind ``eos``, and where mask and bias leave it no token; with a mask or a bias ``choose`` gets
-        zeros for the rows that have ended, and what it returns for them is not used."""
+        tokens and totals so far.
+
+        The next ids are the highest; or drawn, where ``temperature``, ``top_k``, ``top_p`` or ``min_p`` is given, as
+        :func:`~frankentorch_b200.ops.decode.sample` does, with random numbers of ``generator`` (the device's own); or what ``choose``
+        makes of the processed logits ``[batch, vocabulary]``.  A row ends behind ``eos``, and where mask and bias leave it no token;
+        with a mask or a bias ``choose`` gets zeros for the rows that have ended, and what it returns for them is not used."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens is positive")
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        drawn = any(v is not None for v in settings.values())
+        if choose is not None and (drawn or generator is not None):
+            raise ValueError("tokens are drawn or chosen by a function, not both")
+        if generator is not None and not drawn:
+            raise ValueError("a generator is for tokens that are drawn: temperature, top_k, top_p or min_p is missing")
         B, S = ids.shape
         logits = self.prefill(ids, lengths)
         for b, n in enumerate(self._host_lengths):
@@ -245,14 +277,20 @@ class GPTDecoder:
         penalised = not (repetition is None and frequency is None and presence is None)
         for i in range(max_new_tokens):
             words = allowed(tokens, totals) if callable(allowed) else allowed
-            x = D.logits_process(logits, vocab=self.cfg.vocab_size, tokens=tokens if penalised else None,
-                                 lengths=totals if penalised else None, prompt_lengths=prompt if penalised else None,
-                                 repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=words)
-            if words is not None or bias is not None:
+            plain = drawn and not penalised and words is None and bias is None      # the sampler reads the head's own rows
+            x = logits if plain else D.logits_process(
+                logits, vocab=self.cfg.vocab_size, tokens=tokens if penalised else None, lengths=totals if penalised else None,
+                prompt_lengths=prompt if penalised else None, repetition=repetition, frequency=frequency, presence=presence,
+                bias=bias, allowed=words)
+            if drawn:
+                u = torch.rand(B, generator=generator, device=self.device)
+                picked = D.sample(x, u, vocab=self.cfg.vocab_size, **settings)[0]
+                live &= picked >= 0             # -1: there is none
+            elif words is not None or bias is not None:
                 live &= x.amax(-1) != float("-inf")
                 if choose is not None:          # a sampler would make NaN of a row of -inf
                     x = torch.where(live[:, None], x, 0.0)
-            new = torch.where(live, x.argmax(-1) if choose is None else choose(x), 0)
+            new = torch.where(live, picked if drawn else x.argmax(-1) if choose is None else choose(x), 0)
             place = totals.to(torch.int64)[:, None]
             tokens.scatter_(1, place, torch.where(live[:, None], new[:, None], tokens.gather(1, place)))
             totals += live

@@ -81,6 +81,8 @@ def _fill(g, pages, scales, table, ends, powers=True):
     (1, 70, 4, 2, 256, 256, 64, 32, [3], [70]),
     (2, 5, 1, 1, 1024, 512, 16, 4, [14, 3], [5, 2]),
     (3, 33, 5, 5, 64, 32, 16, 2, [0, 1, 17], [33, 32, 31]),
+    (1, 64, 1, 1, 1024, 1024, 64, 64, [0], None),        # more angles than shared memory holds
+    (40, 3, 30, 10, 64, 64, 16, 16, [i * 7 for i in range(40)], [i % 4 for i in range(40)]),
 ])
 def test_append(cuda_device, B, S, H, Hk, hd, turn, page, block, start, counts, dtype, interleaved, layout):
     from frankentorch_b200.ops import decode as D
