@@ -31,6 +31,7 @@
 namespace ftk {
 
 typedef unsigned long long u64;
+#define SA_INLINE __attribute__((always_inline))      // left out of line, a lambda keeps what it captures in local memory
 constexpr int SA_LOG = 8, SA_THREADS = 1 << SA_LOG, SA_WARPS = SA_THREADS / 32;
 constexpr int SA_BINS = 8 * SA_THREADS;      // steps of a histogram of counts
 constexpr int SA_FINE = 2 * SA_THREADS;      // steps among the elements set aside
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     }
   };
   // Sums of up to four numbers over the row
-  const auto all_of = [&](u64 (&v)[4]) {
+  const auto all_of = [&](u64 (&v)[4]) SA_INLINE {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[j] = warp_sum(v[j]);
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     u64 front, target;                 // sum in front of that warp's run, and what was looked for
   };
   // `leaves`: the answer of the row, written by who finds it; the CTAs end with it
-  const auto locate_from = [&](u64 warps_sum, bool leaves, const auto& value, const auto& aim) -> Place {
+  const auto locate_from = [&](u64 warps_sum, bool leaves, const auto& value, const auto& aim) SA_INLINE -> Place {
     u64* w = s.sums[turn];
     if (lane == 0) w[warp] = warps_sum;
     cluster_sync();
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     turn ^= 1;
     return got;
   };
-  const auto sum_of = [&](const auto& value) {      // of this warp's elements
+  const auto sum_of = [&](const auto& value) SA_INLINE {      // of this warp's elements
     decltype(value(0, 0.f)) sum = 0;
     each([&](int i, float x) { sum += value(i, x); });
     return (u64)warp_sum(sum);
@@ -399,8 +400,8 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
 
   // ---- lists: `order` and inverted id of elements, the largest first: sorted[] of the CTAs that sort.  Returns how many there are.
   // Elements have been put into list[], n_list of them by this CTA (more than SA_LIST: not all).
-  const auto sort_list = [&](bool here) {
-    cluster_sync();
+  const auto sort_list = [&](bool here, bool seen) SA_INLINE {      // seen: the lists have been published
+    if (!seen) cluster_sync();
     if (warp == 0) {
       const uint32_t n = lane < C ? min(peek(&s.n_list, lane), 1u << 21) : 0, upto = warp_upto(n);
       if (lane < SA_CLUSTER) s.part[lane][0] = upto;      // (behind the last CTA: all)
@@ -425,12 +426,12 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     }
     return n;
   };
-  const auto to_list = [&](int i, float x) {
+  const auto to_list = [&](int i, float x) SA_INLINE {
     const uint32_t at = atomicAdd(&s.n_list, 1);
     if (at < SA_LIST) s.list[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
   };
   // Running sum of a number per thread, and the sum of all
-  const auto run = [&](u64 v, u64& all) {
+  const auto run = [&](u64 v, u64& all) SA_INLINE {
     const u64 up = warp_upto(v);
     if (lane == 31) s.part[warp][1] = up;
     __syncthreads();
@@ -443,6 +444,20 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     }
     __syncthreads();
     return front;
+  };
+  // The choice among the elements of a list, of which a thread has `key` with the weight `stays`
+  const auto from_list = [&](int n, u64 key, u64 stays) SA_INLINE {
+    u64 sum;
+    run(stays, sum);
+    const u64 target = at_random(sum);
+    s.value[tid] = stays;
+    __syncthreads();
+    if (stays) {      // the sum in front of it in the order of the ids, which are held inverted
+      u64 front = 0;
+      for (int j = 0; j < n; ++j)
+        if ((uint32_t)s.sorted[j] > (uint32_t)key) front += s.value[j];
+      if (front <= target && target < front + stays) leave((long long)(uint32_t)~(uint32_t)key, (float)log((double)stays / (double)sum));
+    }
   };
   // Equal steps of the logits from the top down, to the nearest: no less for a smaller logit
   const auto step_of = [&](float x, float scale) {
@@ -494,25 +509,15 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     each([&](int i, float x) {
       if (x >= reach) to_list(i, x);
     });
-    const int n = sort_list(rank == 0);
+    const int n = sort_list(rank == 0, false);
     if (n <= SA_LIST) {
       if (rank == 0) {
         const u64 key = tid < n ? s.sorted[tid] : 0;
         const float x = ordered((uint32_t)(key >> 32));
         const u64 w = tid < n && tid < k && x >= weigh.floor ? weigh(x) : 0;
-        u64 total, sum;
-        const u64 before = run(w, total) - w, limit = p < 1.f ? share_of<true>(total, p) : ~0ull;
-        const u64 stays = (tid == 0 || before < limit) && w >= low ? w : 0;
-        run(stays, sum);
-        const u64 target = at_random(sum);
-        s.value[tid] = stays;
-        __syncthreads();
-        if (stays) {      // the sum in front of it in the order of the ids, which are held inverted
-          u64 front = 0;
-          for (int j = 0; j < n; ++j)
-            if ((uint32_t)s.sorted[j] > (uint32_t)key) front += s.value[j];
-          if (front <= target && target < front + stays) leave((long long)(uint32_t)~(uint32_t)key, (float)log((double)stays / (double)sum));
-        }
+        u64 total;
+        const u64 before = run(w, total) - w;
+        from_list(n, key, (tid == 0 || before < (p < 1.f ? share_of<true>(total, p) : ~0ull)) && w >= low ? w : 0);
       }
       cluster_sync();
       return;
@@ -526,22 +531,23 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   float edge = -INFINITY;
   int last = V;
   const auto kept = [&](int i, float x) { return x > edge || (x == edge && i <= last); };
-  const auto clear_hist = [&]() {
+  const auto clear_hist = [&]() SA_INLINE {
     for (int i = tid; i < SA_BINS; i += SA_THREADS) s.hist[i] = 0;
     __syncthreads();
   };
   // Two steps of a histogram of the row at which the running sum of value(step) per element reaches aim(sum of all, of squares, ..), in
-  // fp32 (exact for counts) and a fixed order; each CTA adds up its part of the steps.  got[]: the steps in the upper halves, the sums in
-  // front of them in the lower; ~0 where it is not reached.  Clears the histogram.
-  const auto find = [&](const auto& value, const auto& aim) {
+  // fp32 (exact for counts) and a fixed order; each CTA adds up its part of the steps.  got[]: the steps in the upper halves, in the lower
+  // how many elements are in front of the first and up to the second; ~0 where it is not reached.  Clears the histogram.
+  const auto find = [&](const auto& value, const auto& aim) SA_INLINE {
     constexpr int MOST = SA_BINS / SA_THREADS;
     const int per = max(MOST >> lc, 1), b0 = (rank << SA_LOG) * per + tid * per;      // (eight CTAs have a step per thread)
     static_assert(SA_BINS == SA_THREADS * SA_CLUSTER, "a step per thread at least");
     cluster_sync();
     float v[MOST], own = 0.f, square = 0.f;      // square: of what one element of a step counts, over all
+    uint32_t m[MOST], own_m = 0;
 #pragma unroll
     for (int j = 0; j < MOST; ++j) {
-      v[j] = 0.f;
+      v[j] = 0.f, m[j] = 0;
       if (j < per) {
         uint32_t n = 0;
 #pragma unroll
@@ -549,45 +555,54 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
         const float one = n ? value(b0 + j) : 0.f;
         v[j] = (float)n * one, square += v[j] * one;
         own += v[j];
+        m[j] = n, own_m += n;
       }
     }
     const float up = warp_upto(own);
+    const uint32_t up_m = warp_upto(own_m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
     float* part = reinterpret_cast<float*>(s.part);
-    if (lane == 31) part[warp] = up, part[SA_WARPS + warp] = square;
+    uint32_t* part_m = reinterpret_cast<uint32_t*>(part) + 2 * SA_WARPS;
+    if (lane == 31) part[warp] = up, part[SA_WARPS + warp] = square, part_m[warp] = up_m;
     if (tid < 2) s.record[turn][tid] = ~0ull;
     __syncthreads();
     float front = up - own;
+    uint32_t front_m = up_m - own_m;
 #pragma unroll
-    for (int w = 0; w < SA_WARPS; ++w) front += w < warp ? part[w] : 0.f;
+    for (int w = 0; w < SA_WARPS; ++w) front += w < warp ? part[w] : 0.f, front_m += w < warp ? part_m[w] : 0;
     if (tid == 0) {
       float all = 0.f, squares = 0.f;
 #pragma unroll
       for (int w = 0; w < SA_WARPS; ++w) all += part[w], squares += part[SA_WARPS + w];
-      s.words[turn][0] = (u64)__float_as_uint(squares) << 32 | __float_as_uint(all);
+      uint32_t all_m = 0;
+#pragma unroll
+      for (int w = 0; w < SA_WARPS; ++w) all_m += part_m[w];
+      s.words[turn][0] = (u64)__float_as_uint(squares) << 32 | __float_as_uint(all), s.words[turn][1] = all_m;
     }
     cluster_sync();
     if (warp == 0) {
       const u64 q = lane < C ? peek(&s.words[turn][0], lane) : 0;
       const float upto = warp_upto(__uint_as_float((uint32_t)q)), squares = warp_upto(__uint_as_float((uint32_t)(q >> 32)));
       if (lane == 31) s.got[0] = __float_as_uint(upto), s.got[1] = __float_as_uint(squares);
-      if (lane == rank) s.got[2] = __float_as_uint(upto - __uint_as_float((uint32_t)q));
+      const uint32_t q_m = lane < C ? (uint32_t)peek(&s.words[turn][1], lane) : 0, upto_m = warp_upto(q_m);
+      if (lane == rank) s.got[2] = (u64)(upto_m - q_m) << 32 | __float_as_uint(upto - __uint_as_float((uint32_t)q));
     }
     clear_hist();
     const float all = __uint_as_float((uint32_t)s.got[0]), squares = __uint_as_float((uint32_t)s.got[1]);
-    front += __uint_as_float((uint32_t)s.got[2]);
+    front += __uint_as_float((uint32_t)s.got[2]), front_m += (uint32_t)(s.got[2] >> 32);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const float want = aim(all, squares, a);
       float at = front;
+      uint32_t at_m = front_m;
 #pragma unroll
       for (int j = 0; j < MOST; ++j) {
         if (v[j] > 0.f && at + v[j] >= want) {
-          atomicMin(&s.record[turn][a], (u64)(b0 + j) << 32 | __float_as_uint(at));
+          atomicMin(&s.record[turn][a], (u64)(b0 + j) << 32 | (at_m + (a ? m[j] : 0)));
           break;
         }
-        at += v[j];
+        at += v[j], at_m += m[j];
       }
     }
     cluster_sync();
@@ -601,7 +616,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     turn ^= 1;
   };
   // The smallest logit (as `order`) of step `b` or one further up, found by all lanes of a warp
-  const auto first_of = [&](int b, float scale) {
+  const auto first_of = [&](int b, float scale) SA_INLINE {
     uint32_t lo = 0x00800000u, hi = order_of(top);      // the lowest finite number; step_of(top) = 0
     {      // about there
       const uint32_t at = order_of(fmaxf(top - ((float)b + 0.5f) / scale, -3.4e38f)) - 16 + lane;
@@ -620,7 +635,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     return lo;
   };
   // The logits of steps b1 to b2: got[0] the smallest, got[1] the largest (as `order`)
-  const auto between = [&](int b1, int b2, float scale) {
+  const auto between = [&](int b1, int b2, float scale) SA_INLINE {
     if (warp < 2) {
       const int b = warp == 0 ? b2 : b1 - 1;
       const uint32_t o = b >= SA_BINS - 1 ? 0x00800000u : b < 0 ? order_of(top) + 1 : first_of(b, scale);
@@ -628,7 +643,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     }
     __syncthreads();
   };
-  const auto set_aside = [&](int i, float x) {
+  const auto set_aside = [&](int i, float x) SA_INLINE {
     const uint32_t at = atomicAdd(&s.n_aside, 1);
     if (at < SA_ASIDE) s.aside[at] = (u64)order_of(x) << 32 | (uint32_t)~i;
   };
@@ -639,7 +654,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   };
   // The border among the kept elements of one value, of which this warp has `many`: it has as many of them as are needed, by their ids.
   // Sets how many of the warp's own that are.  False where there are not so many.
-  const auto among_equal = [&](uint32_t o, u64 one, u64 many, u64 need, u64& stay) {
+  const auto among_equal = [&](uint32_t o, u64 one, u64 many, u64 need, u64& stay) SA_INLINE {
     const float value = ordered(o);
     const int until = value == edge ? last : V;
     const u64 take = (need + one - 1) / max(one, 1ull);
@@ -657,7 +672,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   };
   // The border among n kept elements of logits lo .. hi (as `order`) is where the running count or sum of weights reaches `need`.  They have
   // been set aside, or where there was no room all look at the whole row for them.  False where they do not reach it.
-  const auto inside = [&](uint32_t lo, uint32_t hi, u64 n, bool over, bool mass, u64 need) {
+  const auto inside = [&](uint32_t lo, uint32_t hi, u64 n, bool over, bool mass, u64 need) SA_INLINE {
     const float lo0 = ordered(lo), hi0 = ordered(hi);
     const int own = min((int)s.n_aside, SA_ASIDE);
     const auto members = [&](const auto& fn) {      // fn(order, inverted id)
@@ -731,7 +746,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     for (int i = tid; i < SA_FINE; i += SA_THREADS) s.hist[i] = 0;
     if (lo < hi) {
       members([&](uint32_t o, uint32_t inverted) { to_list((int)~inverted, ordered(o)); });
-      const int m = sort_list(true);
+      const int m = sort_list(true, false);
       const u64 key = tid < m ? s.sorted[tid] : 0, w = tid < m ? weight_of((uint32_t)(key >> 32)) : 0;
       u64 sum;
       const u64 upto = run(w, sum);
@@ -754,7 +769,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   };
   // The kept elements of logits lo .. hi are set aside; of 16-bit logits there are few values in between, of many elements each
   constexpr bool ASIDE = sizeof(T) == 4;
-  const auto put_aside = [&](float lo_x, float hi_x) {
+  const auto put_aside = [&](float lo_x, float hi_x) SA_INLINE {
     each([&](int i, float x) {
       if (lo_x <= x && x <= hi_x && kept(i, x)) set_aside(i, x);
     });
@@ -776,7 +791,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
       v[0] = tid == 0 ? s.n_aside : 0, v[1] = tid == 0 && s.n_aside > SA_ASIDE;
       all_of(v);
       __syncthreads();
-      inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - (u64)__uint_as_float((uint32_t)got));
+      inside(lo, hi, ASIDE ? v[0] : SA_LIST + 1, !ASIDE || v[1], false, (u64)k - (uint32_t)got);
       if (tid == 0) s.n_aside = 0;
       __syncthreads();
     }
@@ -800,6 +815,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
       const float off = 1.2f * fminf(per_bin, 1.f) * sqrtf(squares) + 1e-5f * all;
       return p * all + (a ? off : -off);
     });
+    const bool listed = s.got[1] != ~0ull && (uint32_t)s.got[1] <= SA_LIST;      // all down to the second step fit a list
     const int b1 = s.got[0] == ~0ull ? 0 : (int)(s.got[0] >> 32), b2 = s.got[1] == ~0ull ? SA_BINS - 1 : (int)(s.got[1] >> 32);
     __syncthreads();
     between(b1, b2, scale);
@@ -819,68 +835,98 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
       if (o >= lo && ordered(o) >= from) values = 0;
     }
     u64 all = 0, above = 0;
-    each([&](int, float x) {
-      const u64 w = weigh(x);
-      if (x >= from) all += w;
-      if (x > hi_x) above += w;
-    });
+    if (listed) {
+      each([&](int i, float x) {
+        const u64 w = weigh(x);
+        if (x >= from) all += w;
+        if (x >= lo_x && kept(i, x)) to_list(i, x);
+      });
+    } else {
+      each([&](int, float x) {
+        const u64 w = weigh(x);
+        if (x >= from) all += w;
+        if (x > hi_x) above += w;
+      });
+    }
     if (ties) {      // equal ones that top-k has not kept
       uint32_t out = 0;
       each([&](int i, float x) { out += x == edge && i > last; });
       all -= out * weigh(edge);
     }
-    u64 v[4] = {all, above, 0, 0};
-    uint32_t many[4] = {0, 0, 0, 0};
-    if (values) {
-      if (values <= 2) {
-        each([&](int, float x) { many[0] += x == value[0], many[1] += x == value[1]; });
-      } else {
-        each([&](int, float x) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) many[j] += x == value[j];
-        });
-      }
-      if (ties) {
-        each([&](int i, float x) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) many[j] -= x == value[j] && x == edge && i > last;
-        });
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= values) many[j] = 0;
-        many[j] = __reduce_add_sync(0xffffffffu, many[j]);      // of the warp
-      }
-      v[2] = lane == 0 ? (u64)many[0] << 32 | many[1] : 0, v[3] = lane == 0 ? (u64)many[2] << 32 | many[3] : 0;
-    } else if (ASIDE) {
-      put_aside(lo_x, hi_x);
-      v[2] = tid == 0 ? s.n_aside : 0, v[3] = tid == 0 && s.n_aside > SA_ASIDE;
-    }
-    const int own = min((int)s.n_aside, SA_ASIDE);
-    u64 kept_sum = warp_sum(above);      // of this warp
-    all_of(v);
-    __syncthreads();
-    const u64 limit = max(share_of<true>(v[0], p), 1ull);
-    const bool over = !ASIDE || v[3];
-    bool guessed = v[1] < limit;
-    if (guessed && values) {
-      u64 need = limit - v[1];
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 n = j & 1 ? (uint32_t)v[2 + (j >> 1)] : v[2 + (j >> 1)] >> 32, one = j < values ? weigh(value[j]) : 0;
-        if (found || j >= values) continue;
-        if (n * one >= need) {
-          u64 stay;
-          found = among_equal(order_of(value[j]), one, many[j], need, stay);
-          kept_sum += stay * one;
-        } else {
-          need -= n * one, kept_sum += many[j] * one;
+    u64 limit, kept_sum = 0;             // kept_sum: of this warp
+    bool guessed = false, over = false;
+    int own = 0;
+    if (listed) {
+      u64 v[4] = {all, 0, 0, 0}, sum;
+      all_of(v);
+      limit = max(share_of<true>(v[0], p), 1ull);
+      const int n = sort_list(true, true);
+      if (n <= SA_LIST) {
+        const u64 key = tid < n ? s.sorted[tid] : 0;
+        const u64 w = tid < n ? weigh(ordered((uint32_t)(key >> 32))) : 0, upto = run(w, sum);
+        if (sum >= limit) {
+          if (rank == 0) from_list(n, key, upto - w < limit && w >= low ? w : 0);
+          cluster_sync();      // nobody leaves while its words are read
+          return;
         }
       }
-      guessed = found;
-    } else if (guessed) {
-      guessed = inside(max(lo, order_of(from)), hi, over ? SA_LIST + 1 : v[2], over, true, limit - v[1]);
+      cluster_sync();      // the border is further down
+      if (tid == 0) s.n_list = 0;
+      __syncthreads();
+    } else {
+      u64 v[4] = {all, above, 0, 0};
+      uint32_t many[4] = {0, 0, 0, 0};
+      if (values) {
+        if (values <= 2) {
+          each([&](int, float x) { many[0] += x == value[0], many[1] += x == value[1]; });
+        } else {
+          each([&](int, float x) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) many[j] += x == value[j];
+          });
+        }
+        if (ties) {
+          each([&](int i, float x) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) many[j] -= x == value[j] && x == edge && i > last;
+          });
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= values) many[j] = 0;
+          many[j] = __reduce_add_sync(0xffffffffu, many[j]);      // of the warp
+        }
+        v[2] = lane == 0 ? (u64)many[0] << 32 | many[1] : 0, v[3] = lane == 0 ? (u64)many[2] << 32 | many[3] : 0;
+      } else if (ASIDE) {
+        put_aside(lo_x, hi_x);
+        v[2] = tid == 0 ? s.n_aside : 0, v[3] = tid == 0 && s.n_aside > SA_ASIDE;
+      }
+      own = min((int)s.n_aside, SA_ASIDE);
+      kept_sum = warp_sum(above);
+      all_of(v);
+      __syncthreads();
+      limit = max(share_of<true>(v[0], p), 1ull);
+      over = !ASIDE || v[3];
+      guessed = v[1] < limit;
+      if (guessed && values) {
+        u64 need = limit - v[1];
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u64 n = j & 1 ? (uint32_t)v[2 + (j >> 1)] : v[2 + (j >> 1)] >> 32, one = j < values ? weigh(value[j]) : 0;
+          if (found || j >= values) continue;
+          if (n * one >= need) {
+            u64 stay;
+            found = among_equal(order_of(value[j]), one, many[j], need, stay);
+            kept_sum += stay * one;
+          } else {
+            need -= n * one, kept_sum += many[j] * one;
+          }
+        }
+        guessed = found;
+      } else if (guessed) {
+        guessed = inside(max(lo, order_of(from)), hi, over ? SA_LIST + 1 : v[2], over, true, limit - v[1]);
+      }
     }
     if (!guessed) inside(order_of(from), order_of(top), V, true, true, limit);      // not between those two: among all
     if (low == 0 && guessed) {      // the warps' sums: what was above, and the kept ones between the two
