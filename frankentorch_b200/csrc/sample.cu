@@ -200,23 +200,40 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   };
   // ---- the row comes in: its largest element, and about its smallest finite one
   float most = -INFINITY, fewest = INFINITY;
-  const auto take = [&](const uint4& v, int it) {
-    if (RES) kept_row[(warp * its + it) * 32 + lane] = v;
+  const auto take = [&](const uint4& v) {
     float x[N];
     logits_of<T>(v, x);
 #pragma unroll
     for (int e = 0; e < N; ++e) most = max_or_nan(most, x[e]);
     fewest = x[0] > -INFINITY ? fminf(fewest, x[0]) : fewest;
   };
-  int it0 = 0;
-  for (; it0 + 4 <= mine; it0 += 4) {
-    uint4 v[4];
+  if (RES && VEC) {      // all of a thread's vectors are on their way at once
+    for (int it = 0; it < mine; ++it) {
+      uint4* to = kept_row + (warp * its + it) * 32 + lane;
+      const int from = begin + (it * 32 + lane) * N;
+      if (from + N <= V) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(row + from) : "memory");
+      else *to = fetch(from);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    for (int it = 0; it < mine; ++it) take(kept_row[(warp * its + it) * 32 + lane]);
+  } else {
+    int it0 = 0;
+    for (; it0 + 4 <= mine; it0 += 4) {
+      uint4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = fetch(begin + ((it0 + j) * 32 + lane) * N);
+      for (int j = 0; j < 4; ++j) v[j] = fetch(begin + ((it0 + j) * 32 + lane) * N);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) take(v[j], it0 + j);
+      for (int j = 0; j < 4; ++j) {
+        if (RES) kept_row[(warp * its + it0 + j) * 32 + lane] = v[j];
+        take(v[j]);
+      }
+    }
+    for (; it0 < mine; ++it0) {
+      const uint4 v = fetch(begin + (it0 * 32 + lane) * N);
+      if (RES) kept_row[(warp * its + it0) * 32 + lane] = v;
+      take(v);
+    }
   }
-  for (; it0 < mine; ++it0) take(fetch(begin + (it0 * 32 + lane) * N), it0);
   bool odd = most != most || !(t >= 0.f) || p != p || least != least || u != u;
 
   // ---- what all CTAs of the row agree on.  Published words take turns: between two uses of a set lies a barrier of the cluster.
@@ -294,7 +311,8 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
     for (int j = 0; j < 4; ++j) v[j] = s.got[j];
     turn ^= 1;
   };
-  // The first element by id whose running sum of value(id, logit) passes aim(sum of all).  `sum`: of this thread's elements
+  // The first element by id whose running sum of value(id, logit) passes aim(sum of all); what aim() leaves there is what the answer's weight is
+  // a share of
   struct Place {
     int id, owner;                     // id; warp of the row
     u64 front, target;                 // sum in front of that warp's run, and what was looked for
@@ -311,9 +329,10 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
         const int at = lane * 2 + j;
         v[j] = at < C * SA_WARPS ? peek(&w[at % SA_WARPS], at / SA_WARPS) : 0;
       }
-      const u64 upto = warp_upto(v[0] + v[1]), total = __shfl_sync(0xffffffffu, upto, 31), target = aim(total), front = upto - v[0] - v[1];
+      u64 total = __shfl_sync(0xffffffffu, warp_upto(v[0] + v[1]), 31);
+      const u64 upto = warp_upto(v[0] + v[1]), most = total, target = aim(total), front = upto - v[0] - v[1];
       const bool here = front <= target && target < upto, second = target >= front + v[0];
-      if (here || (lane == 0 && target >= total))
+      if (here || (lane == 0 && target >= most))
         s.got[2] = lane * 2 + second, s.got[3] = second ? front + v[0] : front, s.got[4] = target, s.got[5] = total;
     }
     if (leaves) leave_arrive();
@@ -386,15 +405,12 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   const long long k = t == 0.f ? 1 : (k0 <= 0 || k0 > V ? V : k0);
   const u64 low = least >= 1.f ? 1ull << 43 : (u64)ceil(fmax((double)least, 0.0) * 0x1p43);
   if (k == 1 || top == INFINITY) {      // of the largest the first, or the first few: they weigh the same
-    u64 kept_ones = 1;
     const auto largest = [&](int, float x) -> uint32_t { return x == top; };
-    const Place at = locate_from(sum_of(largest), false, largest, [&](u64 total) {
-      kept_ones = min(total, (u64)k);
-      if (p < 1.f) kept_ones = max((share_of<true>(kept_ones << 43, p) + (1ull << 43) - 1) >> 43, 1ull);
-      return at_random(kept_ones << 43) >> 43;
+    locate_from(sum_of(largest), true, largest, [&](u64& total) {
+      total = min(total, (u64)k);
+      if (p < 1.f) total = max((share_of<true>(total << 43, p) + (1ull << 43) - 1) >> 43, 1ull);
+      return at_random(total << 43) >> 43;
     });
-    if (rank == 0 && tid == 0) leave(at.id, kept_ones == 1 ? 0.f : (float)-log((double)kept_ones));
-    cluster_sync();
     return;
   }
 
@@ -985,10 +1001,10 @@ template <typename T> static int launch(FtkSampleDesc d, cudaStream_t s) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const auto its_of = [&](int c) { return (int)((d.V + (long long)STEP * c - 1) / ((long long)STEP * c)); };
-  // As many CTAs for a row as fill the SMs four times, with two steps each at least, and as many as it takes to keep 32 KB each: four
-  // CTAs share an SM then, and one works while others wait
+  // As many CTAs for a row as fill the SMs four times, with two steps each at least, and as many as it takes to keep 56 KB each: three
+  // share an SM then, and one works while others wait
   int c = 1;
-  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 4ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > 32 * 1024)) c *= 2;
+  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 4ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > 56 * 1024)) c *= 2;
   int lc = 0;
   while ((1 << lc) < c) ++lc;
   d.cluster = lc;
