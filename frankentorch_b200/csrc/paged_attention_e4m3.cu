@@ -547,7 +547,8 @@ static int launch(const FtkPagedAttnDesc& d, const Plan8& p, void* scratch, cuda
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(A8_WARPS * 32), bytes, s, a, by, status);
   if (rc || !p.split) return rc;
-  return launch_join<T, HD, ROWS, 0>(a, p.heads, p.ctas, p.headers, s);
+  // Few heads have up to a hundred parts each
+  return p.heads > 32 ? launch_join<T, HD, ROWS, 0>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, 1024>(a, p.heads, p.ctas, p.headers, s);
 }
 
 // Strides of 64 GB and more are refused: offsets are 32 bits times 16 bytes (4 of scales and of the table) of each kind, added up in 64

@@ -102,9 +102,9 @@ __device__ __forceinline__ Place first_place(const int B, const int heads, const
 // Joins the parts of a head that several CTAs had, if header blockIdx.x is of one: `together` rows from together * blockIdx.y on, and
 // where that leaves threads over, several of them share a row's parts.  Sums are in a fixed order.  And since sequences of no tokens are in
 // nobody's piece, the blocks write them, a sequence each.  Sums and accumulators are carried times 2^SHIFT.
-template <typename T, int HD, int ROWS, int SHIFT>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
-  constexpr int PART = PA_PART<ROWS, HD>, LANES = HD / 4, SLOTS = 256 / LANES;      // threads of a row, and how many times those
+template <typename T, int HD, int ROWS, int SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
+  constexpr int PART = PA_PART<ROWS, HD>, LANES = HD / 4, SLOTS = THREADS / LANES;      // threads of a row, and how many times those
   constexpr int FIRST = 4;               // parts whose accumulators a thread requests along with the statistics
   extern __shared__ float2 part_ml[];    // [parts][together]: maximum and sum, then (factor, -)
   __shared__ float sums[SLOTS], tops[SLOTS];
@@ -130,13 +130,13 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
 #pragma unroll
     for (int k = 0; k < FIRST; ++k)
       if (j < some && share + k * sharing < n) x[k] = acc_of(share + k * sharing);
-    for (int i = threadIdx.x; i < n * together; i += 256) {
+    for (int i = threadIdx.x; i < n * together; i += THREADS) {
       const int p = i / together, row = i % together;
       if (row < some) part_ml[i] = make_float2(part(p)[ROWS * HD + r0 + row], part(p)[ROWS * (HD + 1) + r0 + row]);
     }
     __syncthreads();
     // a warp per row: the largest maximum, every part's factor, the sum
-    for (int row = warp; row < some; row += 8) {
+    for (int row = warp; row < some; row += THREADS / 32) {
       float top = -INFINITY;
       for (int i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i * together + row].x);
 #pragma unroll
@@ -181,21 +181,21 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
   }
   for (int b = blockIdx.x; b < (int)d.B; b += gridDim.x) {
     if (d.lengths[b] > 0) continue;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq * LANES; i += gridDim.y * 256)
+    for (int i = blockIdx.y * THREADS + threadIdx.x; i < (int)d.Hq * LANES; i += gridDim.y * THREADS)
       *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + (i / LANES) * d.o_hs + (i % LANES) * 4) = make_uint2(0, 0);
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)d.Hq; i += gridDim.y * 256) d.lse[(long long)b * d.Hq + i] = -INFINITY;
+    for (int i = blockIdx.y * THREADS + threadIdx.x; i < (int)d.Hq; i += gridDim.y * THREADS) d.lse[(long long)b * d.Hq + i] = -INFINITY;
   }
 }
 
 // The launch of the join: few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a
 // head, as far as shared memory goes.
-template <typename T, int HD, int ROWS, int SHIFT>
+template <typename T, int HD, int ROWS, int SHIFT, int THREADS = 256>
 static int launch_join(const PagedAttn& a, long long heads, long long ctas, long long headers, cudaStream_t s) {
-  constexpr int slots = 256 / (HD / 4);
+  constexpr int slots = THREADS / (HD / 4);
   int together = 1;
   while (heads > 32 && together < a.sub_heads && together < slots && ctas * together * 2 * sizeof(float2) <= 40 * 1024)
     together *= 2;
-  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS, SHIFT>, dim3((unsigned)headers, (unsigned)((a.sub_heads + together - 1) / together)), dim3(256),
+  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS, SHIFT, THREADS>, dim3((unsigned)headers, (unsigned)((a.sub_heads + together - 1) / together)), dim3(THREADS),
                     (size_t)ctas * together * sizeof(float2), s, a, together);
 }
 
