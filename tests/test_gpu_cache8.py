@@ -82,6 +82,7 @@ def _fill(g, pages, scales, table, ends, powers=True):
     (2, 5, 1, 1, 1024, 512, 16, 4, [14, 3], [5, 2]),
     (3, 33, 5, 5, 64, 32, 16, 2, [0, 1, 17], [33, 32, 31]),
     (1, 64, 1, 1, 1024, 1024, 64, 64, [0], None),        # more angles than shared memory holds
+    (2, 1100, 16, 1, 128, 64, 64, 64, [5, 0], [1100, 900]),      # so many queries that they have a launch of their own
     (40, 3, 30, 10, 64, 64, 16, 16, [i * 7 for i in range(40)], [i % 4 for i in range(40)]),
 ])
 def test_append(cuda_device, B, S, H, Hk, hd, turn, page, block, start, counts, dtype, interleaved, layout):
@@ -425,4 +426,60 @@ def test_empty_calls(cuda_device):
     assert bool(k8.float().isnan().all()) and bool(ks.isnan().all())
     o, lse = D.paged_attention(_rnd(g, 0, 4, 64), k8, v8, table[:0], _i32([]), **kw)
     assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_behind_32_bits(cuda_device, hd):
+    """Pages whose first byte is more than 2^32 from the cache's: appended to and read where they are."""
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    g = _gen(31)
+    P, H, page = (1 << 32) // (2 * 64 * hd) + 40, 2, 64
+    k8, v8 = (torch.empty(P, H, page, hd, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    ks, vs = (torch.ones(P, H, 2, device="cuda") for _ in range(2))
+    assert (P - 30) * H * page * hd > 1 << 32
+    table = torch.tensor([[P - 1, 3, P - 20, P - 7], [P - 30, P - 2, 0, P - 9]], dtype=torch.int32, device="cuda")
+    small = [t[table.flatten().long()].clone() if t.dtype != E4M3 else t.view(torch.uint8)[table.flatten().long()].view(E4M3).clone()
+             for t in (k8, ks, v8, vs)]
+    near = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    x, y = _rnd(g, 2, 200, H, hd), _rnd(g, 2, 200, H, hd)
+    n = _i32([200, 150])
+    D.paged_append(k8, v8, table, x, y, _i32([0, 0]), n, k_scales=ks, v_scales=vs)
+    D.paged_append(small[0], small[2], near, x, y, _i32([0, 0]), n, k_scales=small[1], v_scales=small[3])
+    q = _rnd(g, 2, 4, hd)
+    far = D.paged_attention(q, k8, v8, table, n, k_scales=ks, v_scales=vs)
+    want = D.paged_attention(q, small[0], small[2], near, n, k_scales=small[1], v_scales=small[3])
+    assert torch.equal(far[0], want[0]) and torch.equal(far[1], want[1]) and bool(far[0].isfinite().all())
+    K.check_status()
+
+
+def test_calls_of_several_threads(cuda_device):
+    """Two threads with streams and caches of their own at once: what each has alone."""
+    import threading
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+
+    def work(seed, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g = _gen(seed)
+            lengths = [300 + seed, 50, 2000]
+            q, k8, v8, ks, vs, table = _attend(g, 3, 8, 2, 64, 16, 16, lengths, BF)
+            x = _rnd(g, 3, 1, 2, 64)
+            for _ in range(20):
+                D.paged_append(k8, v8, table, x, x, _i32([n - 1 for n in lengths]), k_scales=ks, v_scales=vs)
+                o = D.paged_attention(q, k8, v8, table, _i32(lengths), k_scales=ks, v_scales=vs)
+            torch.cuda.current_stream().synchronize()
+            out[seed] = (o[0].clone(), o[1].clone(), k8.view(torch.uint8).clone())
+    alone, both = {}, {}
+    for seed in (1, 2):
+        work(seed, alone)
+    threads = [threading.Thread(target=work, args=(seed, both)) for seed in (1, 2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for seed in (1, 2):
+        for a, b in zip(alone[seed], both[seed]):
+            assert torch.equal(a, b)
     K.check_status()

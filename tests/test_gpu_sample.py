@@ -206,3 +206,64 @@ def test_streams_and_graphs(cuda_device):
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
     none = D.sample(x[:0], u[:0])
     assert none[0].shape == none[1].shape == (0,)
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=127), dict(top_k=128), dict(top_k=129), dict(top_k=256), dict(top_k=257), dict(top_k=2000),
+                                dict(top_k=400, top_p=0.6), dict(top_k=700, top_p=0.9, min_p=0.01)], ids=str)
+@pytest.mark.parametrize("dtype", [FF, BF])
+@pytest.mark.parametrize("V", [300, 5000, 40000])
+def test_large_k(cuda_device, V, dtype, kw):
+    """Around the sizes of a list, where the border is found by counts."""
+    g = _gen(V)
+    x = (2.0 * torch.randn(3, V, generator=g, device="cuda")).to(dtype)
+    _check(x, torch.rand(3, generator=g, device="cuda"), **kw)
+
+
+def _rows(kind, V, g):
+    x = torch.randn(4, V, generator=g, device="cuda")
+    if kind == "outlier":            # all others are in one step of the range
+        x = 1e-3 * x
+        x[:, V // 3] = 50.0
+    elif kind == "cluster":          # a spread of a few units of fp32
+        x = 100.0 + 2e-5 * x
+    elif kind == "lowest":           # masked by the type's lowest value
+        x[torch.rand(4, V, generator=g, device="cuda") < 0.7] = torch.finfo(FF).min
+    elif kind == "scales":           # clusters within clusters
+        x = torch.sign(x) * torch.exp2(-40 * torch.rand(4, V, generator=g, device="cuda"))
+    elif kind == "two":              # two values, most of them the lower
+        x = torch.where(x > 2.0, 1.0, -1.0)
+    elif kind == "few":              # hardly any allowed
+        x[torch.rand(4, V, generator=g, device="cuda") < 0.999] = -math.inf
+        x[:, V - 1] = 0.0
+    elif kind == "huge":
+        x = 1e37 * x
+    return x
+
+
+@pytest.mark.parametrize("kw", [dict(temperature=20.0, top_p=0.9), dict(temperature=20.0, top_p=0.3, top_k=3000), dict(top_k=1500),
+                                dict(top_k=100, temperature=50.0, top_p=0.99), dict(top_p=0.999, min_p=0.5), dict(temperature=1e38, top_p=0.5),
+                                dict(temperature=30.0)], ids=str)
+@pytest.mark.parametrize("kind", ["outlier", "cluster", "lowest", "scales", "two", "few", "huge"])
+@pytest.mark.parametrize("dtype", [FF, HF, BF])
+def test_rows_of_odd_spread(cuda_device, kind, kw, dtype):
+    if dtype is HF and kind in ("huge", "lowest"):
+        pytest.skip("no such numbers in fp16")
+    g = _gen(17)
+    _check(_rows(kind, 9001, g).to(dtype), torch.tensor([0.0, 0.3, 0.9, 0.999999], device="cuda"), **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50, top_p=0.9), dict(top_k=5000), dict(top_p=0.8), dict(temperature=0.0)], ids=str)
+@pytest.mark.parametrize("dtype,V", [(FF, 400003), (BF, 800009)])
+def test_rows_that_shared_memory_does_not_hold(cuda_device, dtype, V, kw):
+    g = _gen(23)
+    x = (3.0 * torch.randn(1, V, generator=g, device="cuda")).to(dtype)
+    _check(x, torch.tensor([0.6], device="cuda"), **kw)
+    odd = torch.empty(V + 1, dtype=dtype, device="cuda")[1:].view(1, V)      # rows that start anywhere
+    odd.copy_(x)
+    _check(odd, torch.tensor([0.6], device="cuda"), **kw)
+
+
+def test_many_rows(cuda_device):
+    g = _gen(29)
+    x = torch.randn(3000, 40, generator=g, device="cuda")
+    _check(x, torch.rand(3000, generator=g, device="cuda"), temperature=1.3, top_k=11, top_p=0.9)
