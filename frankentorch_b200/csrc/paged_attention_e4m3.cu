@@ -23,7 +23,13 @@ namespace ftk {
 
 constexpr int A8_WARPS = 2, A8_TOKENS = 32;      // of a CTA that shares its SM; tokens that a warp takes at a time
 constexpr float A8_SHIFT = 16384.f;
-__host__ inline long long a8_whole(long long heads, long long sms) { return heads <= sms ? 9 + 28 * heads / sms : 20; }
+// Tiles of 64 tokens, by the width of the table, up to which a head is left whole: a second launch and the join cost 4 - 6 us.  Whole and cut
+// (us), all positions in use, 64 to a tile: 12 heads of 64, 16 tiles 7.2 and 9.5, 24 tiles 9.3 and 9.9, 32 tiles 11.2 and 9.9; 32 heads of
+// 128, 16 tiles 9.7 and 11.1, 32 tiles 15.9 and 12.9; 128 heads of 128, 16 tiles 10.6 and 16.2, 40 tiles 19.7 and 23.8.  With several heads
+// per SM, which fill the time among themselves: 256 of 128, 16 tiles 21.1 and 21.9, 32 tiles 37.8 and 31.9; 768 of 64, 16 tiles 29.4 and
+// 32.6, 32 tiles 53.2 and 48.8; 1024 of 128, 16 tiles 60.5 and 54.5, 24 tiles 87.3 and 72.5.  A straight line below these borders up to a
+// head per SM, and one border above.
+__host__ inline long long a8_whole(long long heads, long long sms) { return heads <= sms ? 18 + 32 * heads / sms : 16; }
 
 // ROWS query heads of a head of the cache: 1, up to 8 or up to 16
 template <int ROWS, int HD, int W> struct A8Smem {
