@@ -11,7 +11,13 @@
 // Work.  A CTA has the tokens of a call that fall into one block of rows of a sequence, and some of their heads: it forms the angles' sines
 // and cosines once per token and pair.  A unit is one head of those tokens, of the keys, the values or the queries; a group of as many
 // lanes as have one to four items of 16 elements each takes units in turn, holds a unit's elements in registers until their largest is
-// known (two exchanges in shared memory where a group is several warps), and writes them.
+// known (through shared memory where a group is several warps), and writes them.  Queries in a launch of their own took 75.5 us where
+// they take 71.0 with the rest (16 prompts of up to 2048, 16 + 4 heads of 128), and 81.4 against 79.6 (8 x 2048, 16 + 16 heads).
+// Measured: those prompts 71 us, 3470 GB/s of what the call needs and 4700 with the queries behind the counts, which leave as they came;
+// a token of 256 sequences, 16 heads of 128, 5.8 us; one token, 12 heads of 64, 2.9 us.  Instructions hold the long calls, about 500 of a
+// warp for 32 items: the rotation is done twice, before the largest is known and after, because the floats of four items are too many
+// registers (held as floats, 75.9, 90.7 and 34.7 us for the prompts and the two calls below with two items a lane: 2 % less and 3 % and
+// 8 % more than turning twice).
 #include "e4m3.cuh"
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
@@ -25,8 +31,10 @@ extern "C" int* ftk_status_word(void);
 namespace ftk {
 
 constexpr int A8_THREADS = 128;
-constexpr int A8_HELD = 2;             // items of a unit that a lane holds
-constexpr long long A8_APART = 4 << 20;      // elements of the queries from which on they have a launch of their own
+// Items of a unit that a lane holds: one where a warp has a lane for each, else four, so that a group of few warps holds a block and the
+// elements come once.  One, two and four (us): a token of 256 sequences 5.8, 6.3, 7.5; 8 x 2048 tokens of 16 heads of 128 -, 88.3, 81.5;
+// 16 x 2048 of 4 heads without queries -, 32.0, 28.4.
+constexpr int A8_ONE = 1, A8_MORE = 4;
 
 struct AppendShape {
   long long blocks;                    // blocks of rows that a sequence's tokens can touch
@@ -35,8 +43,8 @@ struct AppendShape {
   int hq;                              // heads of the queries that take part
 };
 
-// TABLE: sines and cosines in shared memory; else (more than 200 KB of them) where they are used
-template <typename T, bool INTER, bool TABLE>
+// HELD: items of a lane.  TABLE: sines and cosines in shared memory; else (more than 200 KB of them) where they are used
+template <typename T, bool INTER, bool TABLE, int HELD>
 __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ AppendShape w, int* status) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float largest[2][A8_THREADS / 32];
@@ -62,9 +70,9 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
   if (s0 >= s1) return;
   const int fresh = max(0, min(s1, count) - s0);      // tokens for the cache
   // this lane's items of a unit: 16 elements of a token, eight whole pairs
-  int tok[A8_HELD], chunk[A8_HELD];
+  int tok[HELD], chunk[HELD];
 #pragma unroll
-  for (int k = 0; k < A8_HELD; ++k) tok[k] = (l + k * L) / (unsigned)chunks, chunk[k] = (l + k * L) % (unsigned)chunks;
+  for (int k = 0; k < HELD; ++k) tok[k] = (l + k * L) / (unsigned)chunks, chunk[k] = (l + k * L) % (unsigned)chunks;
   const auto place = [&](int c, bool apart, int& o0, int& o1) { o0 = apart ? c * 8 : c * 16, o1 = apart ? half + c * 8 : c * 16 + 8; };
   const auto fetch = [&](int unit, int t, int c, uint4& u, uint4& v) {
     const int g = first + unit, kv = (int)d.Hkv;
@@ -76,11 +84,11 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
     place(c, !INTER && c * 16 < (int)d.turn && (key || query), o0, o1);
     u = *reinterpret_cast<const uint4*>(at + o0), v = *reinterpret_cast<const uint4*>(at + o1);
   };
-  uint4 u[A8_HELD], v[A8_HELD], u_next[A8_HELD], v_next[A8_HELD];
+  uint4 u[HELD], v[HELD], u_next[HELD], v_next[HELD];
   const auto fetch_all = [&](int unit) {
     const int n = unit < units ? (first + unit < 2 * (int)d.Hkv ? fresh : s1 - s0) : 0;
 #pragma unroll
-    for (int k = 0; k < A8_HELD; ++k)
+    for (int k = 0; k < HELD; ++k)
       if (tok[k] < n) fetch(unit, tok[k], chunk[k], u_next[k], v_next[k]);
   };
   fetch_all(group);
@@ -134,7 +142,7 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
     const int unit = base + group, g = first + unit;
     const bool key = g < (int)d.Hkv, cache = g < 2 * (int)d.Hkv;
 #pragma unroll
-    for (int k = 0; k < A8_HELD; ++k) u[k] = u_next[k], v[k] = v_next[k];
+    for (int k = 0; k < HELD; ++k) u[k] = u_next[k], v[k] = v_next[k];
     fetch_all(unit + groups);            // the next unit, on its way while this one is worked on
     if (unit < units && !cache) {      // queries: turned, and as they are behind the sequence's tokens
       T* const to = (T*)d.q_out + b * d.qo_bs + (g - 2 * d.Hkv) * d.qo_hs;
@@ -151,9 +159,9 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
         *reinterpret_cast<uint4*>(at + o0) = y0, *reinterpret_cast<uint4*>(at + o1) = y1;
       };
 #pragma unroll
-      for (int k = 0; k < A8_HELD; ++k)
+      for (int k = 0; k < HELD; ++k)
         if (tok[k] < s1 - s0) put(tok[k], chunk[k], u[k], v[k]);
-      for (int i = l + A8_HELD * L; i < (s1 - s0) * chunks; i += L) {
+      for (int i = l + HELD * L; i < (s1 - s0) * chunks; i += L) {
         uint4 a, e;
         fetch(unit, i / chunks, i % chunks, a, e);
         put(i / chunks, i % chunks, a, e);
@@ -165,14 +173,14 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
     const auto largest_of = [&](auto finite) {
       float top = 0.f, x[16];
 #pragma unroll
-      for (int k = 0; k < A8_HELD; ++k) {
+      for (int k = 0; k < HELD; ++k) {
         if (tok[k] < fresh) {
           turned(u[k], v[k], tok[k], chunk[k], key, x);
 #pragma unroll
           for (int e = 0; e < 16; ++e) top = fmaxf(top, finite() ? finite_size(x[e]) : fabsf(x[e]));
         }
       }
-      for (int i = l + A8_HELD * L; i < fresh * chunks; i += L) {
+      for (int i = l + HELD * L; i < fresh * chunks; i += L) {
         uint4 a, e;
         fetch(unit, i / chunks, i % chunks, a, e);
         turned(a, e, i / chunks, i % chunks, key, x);
@@ -253,9 +261,9 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
     };
     const auto put_all = [&](auto finite) {
 #pragma unroll
-      for (int k = 0; k < A8_HELD; ++k)
+      for (int k = 0; k < HELD; ++k)
         if (tok[k] < fresh) put(tok[k], chunk[k], u[k], v[k], finite);
-      for (int i = l + A8_HELD * L; i < fresh * chunks; i += L) {
+      for (int i = l + HELD * L; i < fresh * chunks; i += L) {
         uint4 a, e;
         fetch(unit, i / chunks, i % chunks, a, e);
         put(i / chunks, i % chunks, a, e, finite);
@@ -266,15 +274,15 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
   }
 }
 
-template <typename T>
+template <typename T, int HELD>
 static int launch(const FtkRotaryDesc& d, AppendShape w, cudaStream_t s) {
   const long long ctas = d.B * w.blocks * w.parts, tokens = d.S < (1ll << d.block_shift) ? d.S : 1ll << d.block_shift;
   if (ctas > 0x7fffffff) return -2;
   size_t bytes = (size_t)tokens * (d.turn >> 1) * sizeof(float2);
   const bool table = bytes <= 200 * 1024;
   if (!table) bytes = 0;
-  const auto kernel = d.interleaved ? (table ? append_e4m3_kernel<T, true, true> : append_e4m3_kernel<T, true, false>)
-                                    : (table ? append_e4m3_kernel<T, false, true> : append_e4m3_kernel<T, false, false>);
+  const auto kernel = d.interleaved ? (table ? append_e4m3_kernel<T, true, true, HELD> : append_e4m3_kernel<T, true, false, HELD>)
+                                    : (table ? append_e4m3_kernel<T, false, true, HELD> : append_e4m3_kernel<T, false, false, HELD>);
   if (bytes > 40 * 1024) {
     const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (rc) return rc;
@@ -292,19 +300,11 @@ extern "C" int ftk_append_e4m3(const FtkRotaryDesc* d, void* stream) {
   if (d->page_shift < 0 || d->page_shift > 30 || d->block_shift < 0 || d->block_shift > 6 || d->block_shift > d->page_shift) return -2;
   if (d->S > 0x3fffffff || d->B > (1 << 30) || d->Hkv > (1 << 20) || (d->q && (d->Hq < 0 || d->Hq > (1 << 20)))) return -2;
   AppendShape w = {};
-  // Queries take no part in a block's scale: many are turned by the kernel that does nothing else
-  const bool apart = d->q && d->B * d->S * d->Hq * d->hd > A8_APART;
-  if (apart) {
-    FtkRotaryDesc q = *d;
-    q.k = q.v = nullptr, q.k_pages = q.v_pages = nullptr;
-    const int rc = ftk_rotary(&q, stream);
-    if (rc) return rc;
-  }
-  w.hq = d->q && !apart ? (int)d->Hq : 0;
+  w.hq = d->q ? (int)d->Hq : 0;
   const long long block = 1ll << d->block_shift, tokens = d->S < block ? d->S : block, items = tokens * (d->hd >> 4), all = 2 * d->Hkv + w.hq;
   w.blocks = (d->S + block - 2) / block + 1;
   // A lane per item up to a warp's, then up to four items a lane
-  for (w.lanes = 4; w.lanes < A8_THREADS && (items > 32 ? w.lanes < 32 || items > (long long)A8_HELD * w.lanes : items > w.lanes);) w.lanes *= 2;
+  for (w.lanes = 4; w.lanes < A8_THREADS && (items > 32 ? w.lanes < 32 || items > (long long)A8_MORE * w.lanes : items > w.lanes);) w.lanes *= 2;
   // Heads are shared out among CTAs where there are too few for the SMs
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -313,5 +313,7 @@ extern "C" int ftk_append_e4m3(const FtkRotaryDesc* d, void* stream) {
   const long long parts = want < most ? want : most;
   w.units = (int)((all + parts - 1) / parts);
   w.parts = (int)((all + w.units - 1) / w.units);
-  return d->type == FTK_T_BF16 ? launch<__nv_bfloat16>(*d, w, (cudaStream_t)stream) : launch<__half>(*d, w, (cudaStream_t)stream);
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (items <= w.lanes) return d->type == FTK_T_BF16 ? launch<__nv_bfloat16, A8_ONE>(*d, w, s) : launch<__half, A8_ONE>(*d, w, s);
+  return d->type == FTK_T_BF16 ? launch<__nv_bfloat16, A8_MORE>(*d, w, s) : launch<__half, A8_MORE>(*d, w, s);
 }
