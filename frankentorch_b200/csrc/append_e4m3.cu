@@ -14,10 +14,10 @@
 // known (through shared memory where a group is several warps), and writes them.  Queries in a launch of their own took 75.5 us where
 // they take 71.0 with the rest (16 prompts of up to 2048, 16 + 4 heads of 128), and 81.4 against 79.6 (8 x 2048, 16 + 16 heads).
 // Measured: those prompts 71 us, 3470 GB/s of what the call needs and 4700 with the queries behind the counts, which leave as they came;
-// a token of 256 sequences, 16 heads of 128, 5.8 us; one token, 12 heads of 64, 2.9 us.  Instructions hold the long calls, about 500 of a
-// warp for 32 items: the rotation is done twice, before the largest is known and after, because the floats of four items are too many
-// registers (held as floats, 75.9, 90.7 and 34.7 us for the prompts and the two calls below with two items a lane: 2 % less and 3 % and
-// 8 % more than turning twice).
+// a token of 256 sequences, 16 heads of 128, 5.8 us; one token, 12 heads of 64, 2.9 us.  What holds the
+// long calls are chains of instructions of few warps (three CTAs of 152 registers to an SM, issuing in 49 % of the cycles).  The rotation
+// is done twice, before the largest is known and after: turned elements held as floats are too many registers (with two items a lane
+// 75.9, 90.7 and 34.7 us for the prompts and the two calls below, where turning twice took 77.4, 88.6 and 32.0).
 #include "e4m3.cuh"
 #include "ft_sm100.cuh"
 #include "half_types.cuh"

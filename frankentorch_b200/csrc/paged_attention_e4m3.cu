@@ -7,13 +7,24 @@
 // the pieces, the rings and the join are the same.
 //
 // What bounds it: every key and value is read once, in 8 bits; the copy bandwidth, with twice the arithmetic per byte of a 16-bit cache.
+// 128 sequences of 700 to 4096, 16 heads of 128: 204 - 218 us on three boxes, 6.0 - 6.4 TB/s (16-bit cache 388 - 410); 32 of up to 2048 31.6 (51);
+// two of up to 65537, 32 heads over 4, 36.2 (51); one of 301 tokens, 12 heads of 64, 5.1.  A warp's 32 tokens of 128 bytes are 640
+// instructions, of which 64 convert; the SMs issue in 47 % of the cycles, so few heads are bound by the first tiles' way and by the join.
 //
 // A warp takes 32 tokens of a tile at a time.  fp16 holds every e4m3 value, so keys and values go into the matrix instructions as they
 // are, converted in registers, and the scales are applied to scores and probabilities, which are few.  The queries are in fp16 too, a
-// row at a time times the power of two that brings its largest element to 2^14 .. 2^15: what that loses is below 2^-39 of it.  The
-// elements of a product's inner dimension may come in any order that both operands share: a thread's four neighbouring bytes of a key
-// row are two operand registers as they are, and of a value column one byte permutation brings the bytes of two tokens together, with
-// even columns in one product and odd ones in another.  Probabilities times scales are split into two halves of fp16, carried times 2^14.
+// row at a time times the power of two that brings its largest element to 2^14 .. 2^15: what that loses is below 2^-39 of it.
+// Matrix products of the 8-bit values as they are, with queries and probabilities in several parts, took 284 us where these took 276.
+//
+// Scores are formed with the tokens as rows and the heads as columns: of 16 x 8 results none is wasted for up to eight heads, where heads as
+// rows would fill half.  The elements of a product's inner dimension may come in any order that both operands share, so a thread's four
+// neighbouring bytes of a key are two operand registers as they are.  For the output the heads are rows; a register's transposition in the warp
+// turns the probabilities, and of a value column one byte permutation brings the bytes of two tokens together, even columns in one
+// product and odd ones in another.  Probabilities times scales are split into two halves of fp16, carried times 2^14: 22 bits of them count.
+// With one head to a head of the cache three of four lanes would hold nothing, so its scores go through shared memory to a token per
+// lane, and the two halves of its probabilities are two rows of one product: 118 us and 123, 128 sequences of 16 heads of 64.
+//
+// Two warps and six CTAs to an SM, two tiles in flight: 218 us; four warps and three CTAs 231 (heads of 128, the largest batch above).
 #include "e4m3.cuh"
 #include "paged_attn.cuh"
 
@@ -62,7 +73,7 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there)
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 
-// What the loads of a tile take, in 32 bits: with 64 bits of everything and a division for the head they were 100 of 770 instructions
+// What the loads of a tile take, in 32 bits: with 64 bits of everything and a division for the head they were 100 instructions more
 struct Strides8 {
   unsigned k_page, k_head, k_row, v_page, v_head, v_row;      // of pages, in 16 bytes
   unsigned ks_page, ks_head, vs_page, vs_head;                // of scales
@@ -553,7 +564,8 @@ static int launch(const FtkPagedAttnDesc& d, const Plan8& p, void* scratch, cuda
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(A8_WARPS * 32), bytes, s, a, by, status);
   if (rc || !p.split) return rc;
-  // Few heads have up to a hundred parts each
+  // Few heads have up to a hundred parts each: 1024 threads 36.2 us for two sequences of 65537 (8 heads), 256 threads 38.9; for 464 heads
+  // with a part or two 39.1 and 31.6, for 32 heads of 16 queries each 96.7 and 82.4
   return p.heads > 32 ? launch_join<T, HD, ROWS, 0>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, 1024>(a, p.heads, p.ctas, p.headers, s);
 }
 
