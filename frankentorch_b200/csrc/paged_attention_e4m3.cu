@@ -7,7 +7,7 @@
 // the pieces, the rings and the join are the same.
 //
 // What bounds it: every key and value is read once, in 8 bits; the copy bandwidth, with twice the arithmetic per byte of a 16-bit cache.
-// 128 sequences of 700 to 4096, 16 heads of 128: 204 - 218 us on three boxes, 6.0 - 6.4 TB/s (16-bit cache 388 - 410); 32 of up to 2048 31.6 (51);
+// 128 sequences of 700 to 4096, 16 heads of 128: 204 us in a burst of calls, 6.4 TB/s, 230 under sustained load (16-bit cache 388 - 410); 32 of up to 2048 31.6 (51);
 // two of up to 65537, 32 heads over 4, 36.2 (51); one of 301 tokens, 12 heads of 64, 5.1.  A warp's 32 tokens of 128 bytes are 640
 // instructions, of which 64 convert; the SMs issue in 47 % of the cycles, so few heads are bound by the first tiles' way and by the join.
 //
