@@ -483,3 +483,56 @@ def test_calls_of_several_threads(cuda_device):
         for a, b in zip(alone[seed], both[seed]):
             assert torch.equal(a, b)
     K.check_status()
+
+
+@pytest.mark.parametrize("group", [1, 3, 9])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tiles", [16, 17, 60])
+def test_more_heads_than_ctas_under_any_width_of_table(cuda_device, tiles, hd, group):
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    g = _gen(tiles + hd + group)
+    lengths = [(i * 53) % 131 for i in range(96)]
+    lengths[5], lengths[94] = 64 * 16, 64 * 15 + 1
+    q, k8, v8, ks, vs, table = _attend(g, 96, 16 * group, 16, hd, 16, 8, lengths, BF)
+    wide = torch.full((96, 4 * tiles), -7, dtype=torch.int32, device="cuda")
+    wide[:, : min(4 * tiles, table.shape[1])] = table[:, : 4 * tiles]
+    o, lse = D.paged_attention(q, k8, v8, wide, _i32(lengths), k_scales=ks, v_scales=vs)
+    wo, wl, to, tl = _want(q, k8, v8, ks, vs, table, lengths)
+    close(o, wo, to, "o")
+    close(lse, wl, tl, "lse")
+    again = D.paged_attention(q, k8, v8, wide, _i32(lengths), k_scales=ks, v_scales=vs)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+    K.check_status()
+
+
+def test_many_queries_turned_where_they_are(cuda_device):
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    g = _gen(77)
+    B, S, H, Hk, hd, page, block = 5, 700, 16, 3, 128, 64, 32
+    start, counts = [0, 31, 5, 64, 1], [700, 699, 0, 1, 350]
+    x = _rnd(g, B, S, H + 2 * Hk, hd)
+    before = x.clone()
+    q, k, v = x.split([H, Hk, Hk], 2)
+    w = 10000.0 ** (-torch.arange(hd // 2, dtype=torch.float64, device="cuda") / (hd // 2))
+    k8, v8, ks, vs, table = _cache(g, Hk, page, block, hd, [s + c for s, c in zip(start, counts)])
+    other = tuple(t.clone() for t in (k8.view(torch.uint8), v8.view(torch.uint8), ks, vs))
+    apart = D.paged_append(other[0].view(E4M3), other[1].view(E4M3), table, k, v, _i32(start), _i32(counts), q=q, inv_freq=w,
+                           q_out=torch.empty(B, S, H, hd, dtype=BF, device="cuda"), k_scales=other[2], v_scales=other[3])
+    D.paged_append(k8, v8, table, k, v, _i32(start), _i32(counts), q=q, inv_freq=w, q_out=q, k_scales=ks, v_scales=vs)
+    assert torch.equal(q, apart) and torch.equal(x[:, :, H:], before[:, :, H:])
+    for b, n in enumerate(counts):
+        assert torch.equal(q[b, n:], before[b, n:, :H])
+        if n:
+            at = start[b] + torch.arange(n, device="cuda")
+            angle = at.double()[:, None] * w
+            c, s = angle.cos()[:, None], angle.sin()[:, None]
+            lo, hi = before[b, :n, :H].double().split(hd // 2, -1)
+            want = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+            size = torch.cat([(lo * c).abs() + (hi * s).abs(), (hi * c).abs() + (lo * s).abs()], -1)
+            assert bool(((q[b, :n].double() - want).abs() <= want.abs() * 2.0 ** -8 + size * 2.0 ** -20).all())
+    for mine, theirs in ((k8.view(torch.uint8), other[0]), (v8.view(torch.uint8), other[1]), (ks.view(torch.int32), other[2].view(torch.int32)),
+                         (vs.view(torch.int32), other[3].view(torch.int32))):
+        assert torch.equal(mine, theirs)
+    K.check_status()
