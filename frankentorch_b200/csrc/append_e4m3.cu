@@ -11,11 +11,11 @@
 // Work.  A CTA has the tokens of a call that fall into one block of rows of a sequence, and some of their heads: it forms the angles' sines
 // and cosines once per token and pair.  A unit is one head of those tokens, of the keys, the values or the queries; a group of as many
 // lanes as have one to four items of 16 elements each takes units in turn, holds a unit's elements in registers until their largest is
-// known (through shared memory where a group is several warps), and writes them.  Queries in a launch of their own took 75.5 us where
-// they take 71.0 with the rest (16 prompts of up to 2048, 16 + 4 heads of 128), and 81.4 against 79.6 (8 x 2048, 16 + 16 heads).
-// Measured: those prompts 71 us, 3470 GB/s of what the call needs and 4700 with the queries behind the counts, which leave as they came;
-// a token of 256 sequences, 16 heads of 128, 5.8 us; one token, 12 heads of 64, 2.9 us.  What holds the
-// long calls are chains of instructions of few warps (three CTAs of 152 registers to an SM, issuing in 49 % of the cycles).  The rotation
+// known (through shared memory where a group is several warps), and writes them.  Queries in a launch of their own took 75.5 us
+// where they took 71.0 with the rest (16 prompts of up to 2048, 16 + 4 heads of 128), and 81.4 against 79.6 (8 x 2048, 16 + 16 heads).
+// Measured: those prompts 68.3 us, 3600 GB/s of what the call needs and 4900 with the queries behind the counts, which leave as they came;
+// a token of 256 sequences, 16 heads of 128, 4.6 us; one token, 12 heads of 64, 2.8 us.  What holds the
+// long calls are chains of instructions of few warps (three or four CTAs to an SM, issuing in half of the cycles).  The rotation
 // is done twice, before the largest is known and after: turned elements held as floats are too many registers (with two items a lane
 // 75.9, 90.7 and 34.7 us for the prompts and the two calls below, where turning twice took 77.4, 88.6 and 32.0).
 #include "e4m3.cuh"
@@ -32,9 +32,14 @@ namespace ftk {
 
 constexpr int A8_THREADS = 128;
 // Items of a unit that a lane holds: one where a warp has a lane for each, else four, so that a group of few warps holds a block and the
-// elements come once.  One, two and four (us): a token of 256 sequences 5.8, 6.3, 7.5; 8 x 2048 tokens of 16 heads of 128 -, 88.3, 81.5;
+// elements come once.  One, two and four (us): a token of 256 sequences 5.8, 6.3, 7.5 (without the bound below); 8 x 2048 tokens of 16 heads of 128 -, 88.3, 81.5;
 // 16 x 2048 of 4 heads without queries -, 32.0, 28.4.
 constexpr int A8_ONE = 1, A8_MORE = 4;
+// CTAs of an SM that the registers are bounded for.  With one item a lane six, where five fit without a bound: 4.6 us for the 256 sequences
+// and 5.8 (seven 5.1).  With four items a lane four or three (152 registers): in groups of up to 64 lanes, 25.3 and 28.2 us for the call without
+// queries, 68.3 and 71.1 for 16 ragged prompts, 11.9 and 13.7 for 8 x 1024 tokens of 12 heads of 64; a group of 128 lanes, where all warps
+// wait for one another, 83.0 and 79.7 for the 16 heads of 128, 8.9 and 8.3 for 16 x 40 tokens of 16 + 4 heads.
+constexpr int A8_CTAS_ONE = 6, A8_CTAS = 4, A8_CTAS_WIDE = 3;
 
 struct AppendShape {
   long long blocks;                    // blocks of rows that a sequence's tokens can touch
@@ -43,9 +48,9 @@ struct AppendShape {
   int hq;                              // heads of the queries that take part
 };
 
-// HELD: items of a lane.  TABLE: sines and cosines in shared memory; else (more than 200 KB of them) where they are used
-template <typename T, bool INTER, bool TABLE, int HELD>
-__global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ AppendShape w, int* status) {
+// HELD: items of a lane, CTAS: of an SM.  TABLE: sines and cosines in shared memory; else (more than 200 KB of them) where they are used
+template <typename T, bool INTER, bool TABLE, int HELD, int CTAS>
+__global__ void __launch_bounds__(A8_THREADS, CTAS) append_e4m3_kernel(const __grid_constant__ FtkRotaryDesc d, const __grid_constant__ AppendShape w, int* status) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float largest[2][A8_THREADS / 32];
   // Cosines and sines of two pairs, (c, c', s, s'), as [token][two pairs of an item][items]: the items' lanes read 16 bytes side by side
@@ -274,15 +279,15 @@ __global__ void __launch_bounds__(A8_THREADS) append_e4m3_kernel(const __grid_co
   }
 }
 
-template <typename T, int HELD>
+template <typename T, int HELD, int CTAS>
 static int launch(const FtkRotaryDesc& d, AppendShape w, cudaStream_t s) {
   const long long ctas = d.B * w.blocks * w.parts, tokens = d.S < (1ll << d.block_shift) ? d.S : 1ll << d.block_shift;
   if (ctas > 0x7fffffff) return -2;
   size_t bytes = (size_t)tokens * (d.turn >> 1) * sizeof(float2);
   const bool table = bytes <= 200 * 1024;
   if (!table) bytes = 0;
-  const auto kernel = d.interleaved ? (table ? append_e4m3_kernel<T, true, true, HELD> : append_e4m3_kernel<T, true, false, HELD>)
-                                    : (table ? append_e4m3_kernel<T, false, true, HELD> : append_e4m3_kernel<T, false, false, HELD>);
+  const auto kernel = d.interleaved ? (table ? append_e4m3_kernel<T, true, true, HELD, CTAS> : append_e4m3_kernel<T, true, false, HELD, CTAS>)
+                                    : (table ? append_e4m3_kernel<T, false, true, HELD, CTAS> : append_e4m3_kernel<T, false, false, HELD, CTAS>);
   if (bytes > 40 * 1024) {
     const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (rc) return rc;
@@ -314,6 +319,8 @@ extern "C" int ftk_append_e4m3(const FtkRotaryDesc* d, void* stream) {
   w.units = (int)((all + parts - 1) / parts);
   w.parts = (int)((all + w.units - 1) / w.units);
   const cudaStream_t s = (cudaStream_t)stream;
-  if (items <= w.lanes) return d->type == FTK_T_BF16 ? launch<__nv_bfloat16, A8_ONE>(*d, w, s) : launch<__half, A8_ONE>(*d, w, s);
-  return d->type == FTK_T_BF16 ? launch<__nv_bfloat16, A8_MORE>(*d, w, s) : launch<__half, A8_MORE>(*d, w, s);
+  const bool bf = d->type == FTK_T_BF16;
+  if (items <= w.lanes) return bf ? launch<__nv_bfloat16, A8_ONE, A8_CTAS_ONE>(*d, w, s) : launch<__half, A8_ONE, A8_CTAS_ONE>(*d, w, s);
+  if (w.lanes < A8_THREADS) return bf ? launch<__nv_bfloat16, A8_MORE, A8_CTAS>(*d, w, s) : launch<__half, A8_MORE, A8_CTAS>(*d, w, s);
+  return bf ? launch<__nv_bfloat16, A8_MORE, A8_CTAS_WIDE>(*d, w, s) : launch<__half, A8_MORE, A8_CTAS_WIDE>(*d, w, s);
 }
