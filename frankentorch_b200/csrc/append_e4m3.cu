@@ -14,10 +14,10 @@
 // known (through shared memory where a group is several warps), and writes them.  Queries in a launch of their own took 75.5 us
 // where they took 71.0 with the rest (16 prompts of up to 2048, 16 + 4 heads of 128), and 81.4 against 79.6 (8 x 2048, 16 + 16 heads).
 // Measured: those prompts 68.3 us, 3600 GB/s of what the call needs and 4900 with the queries behind the counts, which leave as they came;
-// a token of 256 sequences, 16 heads of 128, 4.6 us; one token, 12 heads of 64, 2.8 us.  What holds the
-// long calls are chains of instructions of few warps (three or four CTAs to an SM, issuing in half of the cycles).  The rotation
-// is done twice, before the largest is known and after: turned elements held as floats are too many registers (with two items a lane
-// 75.9, 90.7 and 34.7 us for the prompts and the two calls below, where turning twice took 77.4, 88.6 and 32.0).
+// a token of 256 sequences, 16 heads of 128, 4.6 us; one token, 12 heads of 64, 2.8 us.  What holds the long calls are chains of instructions
+// of few warps (three or four CTAs to an SM, issuing in 59 % of the cycles).  The rotation is done twice, before the largest is known and
+// after: turned elements held as floats are too many registers (with two items a lane 75.9, 90.7 and 34.7 us for the prompts and the two
+// calls below, where turning twice took 77.4, 88.6 and 32.0).
 #include "e4m3.cuh"
 #include "ft_sm100.cuh"
 #include "half_types.cuh"
@@ -32,8 +32,8 @@ namespace ftk {
 
 constexpr int A8_THREADS = 128;
 // Items of a unit that a lane holds: one where a warp has a lane for each, else four, so that a group of few warps holds a block and the
-// elements come once.  One, two and four (us): a token of 256 sequences 5.8, 6.3, 7.5 (without the bound below); 8 x 2048 tokens of 16 heads of 128 -, 88.3, 81.5;
-// 16 x 2048 of 4 heads without queries -, 32.0, 28.4.
+// elements come once.  One, two and four, before the bounds below (us): a token of 256 sequences 5.8, 6.3, 7.5; 8 x 2048 tokens of 16 heads
+// of 128 -, 88.3, 81.5; 16 x 2048 of 4 heads without queries -, 32.0, 28.4.
 constexpr int A8_ONE = 1, A8_MORE = 4;
 // CTAs of an SM that the registers are bounded for.  With one item a lane six, where five fit without a bound: 4.6 us for the 256 sequences
 // and 5.8 (seven 5.1).  With four items a lane four or three (152 registers): in groups of up to 64 lanes, 25.3 and 28.2 us for the call without
