@@ -1,10 +1,17 @@
 // Attention of one new token per sequence over a paged key-value cache held in 8 bits (e4m3) with a scale per block of rows and head.
 //
 // Mathematics.  With ks and vs the scales of token t's key and value, x_t = scale ks_t (q . k_t), o = sum_t softmax_t(x) vs_t v_t and
-// lse = log sum_t exp(x_t).  What is added up for the output are terms of size exp(x_t) vs_t, so the running maximum m is that of
-// y_t = x_t + log2 vs_t (base 2; of vs_t its power of two): the accumulator is sum_t 2^(x_t - m) vs_t v_t, the sum l = sum_t 2^(x_t - m),
-// which no scale from 2^-100 to 2^100 takes out of fp32.  Parts join as in paged_attention.cu, which this follows: the list of tiles,
-// the pieces, the rings and the join are the same.
+// lse = log sum_t exp(x_t).  Terms of the output have size 2^(x_t) vs_t, terms of the sum 2^(x_t), so each has a reference of its own, a whole
+// number of base 2: the accumulators are sum_t 2^(y_t - m) (vs_t / 2^e_t) v_t with e_t the power of two in vs_t, y_t = x_t + e_t and m the largest
+// y_t, rounded up; l = sum_t 2^(x_t - n) with n the largest x_t.  One reference for both takes tokens out of the sum that weigh as much as
+// others, where scales are 2^126 apart.  Whole numbers leave x_t - (m - e_t) as exact as x_t.  As long as a head's scales are within 2^40 of
+// its first ones, n = m - e of those serves, and a weight is its term of l times a power of two and the scale; from the first tile on
+// where they are not, n is each lane's own and weights have an exponential of their own (32 heads over 8 of 128, 16 x 2048 tokens: 20.0 us that
+// way throughout, 18.9 now); with one head to a head of the cache, a token per lane, that costs nothing and is always so.  Parts are given on as m and l 2^(n - m), which |n - m| <= 129 keeps in fp32; where parts
+// meet, sums are compared by their own powers of two.  The list of tiles, the pieces, the rings and the join are paged_attention.cu's.
+//
+// What is lost: weights are held in two halves of fp16, the largest as 2^13 or more, each to 2^-25: what adds less than 2^-38 of the largest weight
+// (value scale and all) times 448 to an element of the output does not count.
 //
 // What bounds it: every key and value is read once, in 8 bits; the copy bandwidth, with twice the arithmetic per byte of a 16-bit cache.
 // 128 sequences of 700 to 4096, 16 heads of 128: 204 us in a burst of calls, 6.4 TB/s, 230 under sustained load (16-bit cache 388 - 410); 32 of up to 2048 31.6 (51);
@@ -33,7 +40,9 @@ extern "C" int* ftk_status_word(void);
 namespace ftk {
 
 constexpr int A8_WARPS = 2, A8_TOKENS = 32;      // of a CTA that shares its SM; tokens that a warp takes at a time
-constexpr float A8_SHIFT = 16384.f;
+constexpr float A8_NONE = -3.402823466e38f;      // the reference where there is no token yet
+// Scales within 2^40 of one another: x - (m - unit) is 40 at most, and what it loses to fp32 below 2^-126 is below 2^-46 of l and of the accumulator
+constexpr float A8_NEAR = 40.f;
 // Tiles of 64 tokens, by the width of the table, up to which a head is left whole: a second launch and the join cost 4 - 6 us.  Whole and cut
 // (us), all positions in use, 64 to a tile: 12 heads of 64, 16 tiles 7.2 and 9.5, 24 tiles 9.3 and 9.9, 32 tiles 11.2 and 9.9; 32 heads of
 // 128, 16 tiles 9.7 and 11.1, 32 tiles 15.9 and 12.9; 128 heads of 128, 16 tiles 10.6 and 16.2, 40 tiles 19.7 and 23.8.  With several heads
@@ -52,7 +61,7 @@ template <int ROWS, int HD, int W> struct A8Smem {
   static constexpr int RING = STAGES * STAGE;
   static constexpr int COLS = ONE ? HD : (HD == 128 ? 32 : 64);      // columns of the accumulators of all warps that are joined at a time
   static constexpr int MERGE = W * ROWS * COLS * 4;
-  static constexpr int BYTES = W * (RING + TURN) + (OWN ? MERGE : 0) + 2 * W * ROWS * 4 + W * STAGES * 4;
+  static constexpr int BYTES = W * (RING + TURN) + (OWN ? MERGE : 0) + (3 * W + 1) * ROWS * 4 + W * STAGES * 4;
   static_assert(OWN || MERGE <= W * RING, "the accumulators fit the rings");
   static_assert(STAGE % 128 == 0, "chunks of a row are exchanged by address bits");
   static_assert(CTAS * (BYTES + 1024) <= 228 * 1024 && BYTES <= 227 * 1024, "the CTAs of an SM share its memory");
@@ -64,6 +73,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t pair) {      // of 8 x 8
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(pair));
   return r;
 }
+constexpr int A8_SHIFT = 14;      // weights are carried times 2^14
+// v / 2^e, times 2^14
+__device__ __forceinline__ float unscaled(float v, float e) { return v * __uint_as_float((uint32_t)(127 + A8_SHIFT - (int)e) << 23); }
 __device__ __forceinline__ float max_of(float x) {      // over the warp; NaN is not counted
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -95,8 +107,9 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
   unsigned char* ring = smem + warp * SM::RING;
   unsigned char* turn = smem + W * SM::RING + warp * SM::TURN;      // ONE: scores, then 16 rows of weights; else the scales of each token
   float* merge = reinterpret_cast<float*>(smem + (SM::OWN ? W * (SM::RING + SM::TURN) : 0));
-  float* stat = reinterpret_cast<float*>(smem + W * (SM::RING + SM::TURN) + (SM::OWN ? SM::MERGE : 0));      // [2][warps][ROWS]
-  unsigned* there = reinterpret_cast<unsigned*>(stat + 2 * W * ROWS) + warp * STAGES;
+  // [3][warps][ROWS]: m, then the sum as own_power has it; [ROWS]: what the output is multiplied by
+  float* stat = reinterpret_cast<float*>(smem + W * (SM::RING + SM::TURN) + (SM::OWN ? SM::MERGE : 0));
+  unsigned* there = reinterpret_cast<unsigned*>(stat + (3 * W + 1) * ROWS) + warp * STAGES;
   const PagedTable table = {d.table, d.table_stride, d.table_cols, d.n_pages, (int)d.page_shift};
   const auto length = [&](int b) {
     bool bad;
@@ -245,7 +258,10 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
 
   // ---- tiles
   uint32_t q[CH][2 * RR];               // of chunk c: elements 2 c0 .. + 3 of head r0, then of head r0 + 8
-  float acc[NT][4], m[2 * RR], l[2 * RR], sc[2 * RR];      // of heads c0, c0 + 1, c0 + 8, c0 + 9; ONE: [0], of all lanes
+  // of heads c0, c0 + 1, c0 + 8, c0 + 9; ONE: [0].  m of the accumulators, of all lanes; n and l of this lane's tokens
+  float acc[NT][4], m[2 * RR], n[2 * RR], l[2 * RR], sc[2 * RR];
+  float unit;                           // power of two of the first tokens' value scales
+  bool near;                            // all so far are within A8_NEAR powers of it: then n = m - unit, and a weight is taken from its term of l
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
   const auto begin = [&]() {            // queries of the head at `p`; rows beyond the group are zero
     const int first = row0(p.h), rows = rows_of(p.h);
@@ -279,7 +295,8 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2 * RR; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < 2 * RR; ++r) m[r] = n[r] = A8_NONE, l[r] = 0.f;
+    unit = A8_NONE, near = true;
   };
   bool begun = p.t == 0;                // the piece has the beginning of the head at `p`
   int parts = 0;
@@ -301,7 +318,6 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       load(stage == 0 ? STAGES - 1 : stage - 1);      // the stage that the tile before left: its reads are behind the warp's barrier
       const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);      // keys', values', the values' exponents
       const float k_scale = scales[lane], v_scale = scales[N + lane], v_exp = (float)max((int)(__float_as_uint(v_scale) >> 23 & 255) - 127, -100);
-      if (!ONE) reinterpret_cast<float4*>(turn)[lane] = make_float4(k_scale, v_exp, v_scale * A8_SHIFT, 0.f);
       // Scores with the tokens as rows: s[2 r + t] of tokens 16 t and on, the r-th eight heads
       float s[2 * RR][4] = {};
 #pragma unroll
@@ -328,15 +344,16 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
         }
         __syncwarp();
         const float x = ok >> lane & 1u ? score[lane] * (k_scale * sc[0]) : -INFINITY;
-        const float top = fmaxf(m[0], max_of(x + v_exp)), base = top == -INFINITY ? 0.f : top, e = exp2_of(x - base), w = e * (v_scale * A8_SHIFT);
+        const float top = fmaxf(m[0], ceilf(max_of(x + v_exp))), own = fmaxf(n[0], ceilf(x));
+        const float w = exp2_of(x - (top - v_exp)) * unscaled(v_scale, v_exp);
         if (top != m[0]) {
-          const float grow = exp2_of(m[0] - base);
-          l[0] *= grow;
+          const float grow = exp2_of(m[0] - top);
 #pragma unroll
           for (int i = 0; i < NT; ++i) acc[i][0] *= grow, acc[i][1] *= grow, acc[i][2] *= grow, acc[i][3] *= grow;
           m[0] = top;
         }
-        l[0] += e;
+        l[0] = fmaf(l[0], exp2_of(n[0] - own), exp2_of(x - own));
+        n[0] = own;
         const __half h = __float2half_rn(w);
         weight[lane] = __half_as_ushort(h);
         weight[8 * (SM::WEIGHT_ROW / 2) + lane] = __half_as_ushort(__float2half_rn(w - __half2float(h)));
@@ -344,17 +361,23 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
         ldm4(weights_at, hi[0]);
         ldm4(weights_at + 32, hi[1]);
       } else {
-        // masked scores of heads c0, c0 + 1 at tokens r0, r0 + 8 .., and the larger maximum of the head's tokens and what was there
+        // masked scores of heads c0, c0 + 1 at tokens r0, r0 + 8 .., and the larger references of the head's tokens and what was there
+        {
+        const bool there = ok >> lane & 1u;
+        if (unit == A8_NONE) unit = max_of(there ? v_exp : A8_NONE);
+        near = near && !__any_sync(0xffffffffu, there && fabsf(v_exp - unit) > A8_NEAR);
+        reinterpret_cast<float4*>(turn)[lane] = make_float4(k_scale, v_exp, there ? unscaled(v_scale, near ? unit : v_exp) : 0.f, 0.f);
+      }
         __syncwarp();
-        float grow[2 * RR], v14[4];
+        float grow[2 * RR], v14[4], v_of[4];
         bool moved = false;
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
           float x[4][2], top[2] = {m[2 * r], m[2 * r + 1]};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {        // token 8 i + r0: key's scale, exponent of the value's, that times 2^14
+          for (int i = 0; i < 4; ++i) {        // token 8 i + r0: key's scale, exponent of the value's, the rest of that
             const float4 f = reinterpret_cast<const float4*>(turn)[8 * i + r0];
-            v14[i] = f.z;
+            v_of[i] = f.y, v14[i] = f.z;
             const bool there = ok >> (8 * i + r0) & 1u;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -366,15 +389,34 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-            const float base = top[e] == -INFINITY ? 0.f : top[e];
+            top[e] = ceilf(top[e]);
             moved |= top[e] != m[2 * r + e];
-            grow[2 * r + e] = exp2_of(m[2 * r + e] - base);
+            grow[2 * r + e] = exp2_of(m[2 * r + e] - top[e]);
             m[2 * r + e] = top[e];
-            l[2 * r + e] *= grow[2 * r + e];
+          }
+          if (near) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[i][e] = exp2_of(x[i][e] - base);
-              l[2 * r + e] += x[i][e];
+            for (int e = 0; e < 2; ++e) {
+              const float own = top[e] - unit;
+              l[2 * r + e] *= grow[2 * r + e];
+              n[2 * r + e] = own;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                x[i][e] = exp2_of(x[i][e] - own);
+                l[2 * r + e] += x[i][e];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float own = fmaxf(n[2 * r + e], ceilf(fmaxf(fmaxf(x[0][e], x[1][e]), fmaxf(x[2][e], x[3][e]))));
+              l[2 * r + e] *= exp2_of(n[2 * r + e] - own);
+              n[2 * r + e] = own;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                l[2 * r + e] += exp2_of(x[i][e] - own);
+                x[i][e] = exp2_of(x[i][e] - (top[e] - v_of[i]));
+              }
             }
           }
 #pragma unroll
@@ -428,12 +470,21 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
     // ---- the end of a head, or of the piece: the warps' parts become one
 #pragma unroll
     for (int r = 0; r < (ONE ? 1 : 2 * RR); ++r) {
+      float most = n[r];
+      if (ONE) most = max_of(most);
+      if (!ONE && !near) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if (ONE || !near) l[r] *= exp2_of(n[r] - most);
 #pragma unroll
       for (int o = ONE ? 1 : 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
       if (r0 == 0 && (!ONE || c0 == 0)) {
         const int head = ONE ? 0 : (r >> 1) * 8 + c0 + (r & 1);
         stat[warp * ROWS + head] = m[r];
-        stat[(W + warp) * ROWS + head] = l[r];
+        const float2 x = own_power(most, l[r]);
+        stat[(W + warp) * ROWS + head] = x.x;
+        stat[(2 * W + warp) * ROWS + head] = x.y;
       }
     }
     const bool whole = begun && p.t == p.tiles;
@@ -448,7 +499,20 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       float top = own;
 #pragma unroll
       for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w * ROWS + head]);
-      scale[r] = exp2f(own - (top == -INFINITY ? 0.f : top)) * (1.f / A8_SHIFT);
+      scale[r] = exp2_of(own - top) * (1.f / (1 << A8_SHIFT));
+      if (warp == 0 && c0 == 0 && head < rows && (!ONE || r0 == 0)) {      // the sum of all warps, and where it belongs
+        float most = A8_NONE, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) most = fmaxf(most, stat[(W + w) * ROWS + head]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += exp2_of(stat[(W + w) * ROWS + head] - most) * stat[(2 * W + w) * ROWS + head];
+        if (!SPLIT || whole) {
+          stat[3 * W * ROWS + head] = sum == 0.f ? 0.f : exp2f(top - most) / sum;
+          d.lse[(long long)p.b * d.Hq + first + head] = sum == 0.f ? -INFINITY : (most + log2f(sum)) * LN2;
+        } else {
+          part[ROWS * HD + head] = top, part[ROWS * (HD + 1) + head] = sum * exp2f(most - top);
+        }
+      }
     }
     // all columns of a few rows at once, else some of all rows
     const int cols = rows * HD <= ROWS * SM::COLS ? HD : SM::COLS;
@@ -470,24 +534,17 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       for (int i = threadIdx.x; i < rows * cols / 2; i += W * 32) {
         const int row = i / (cols / 2), in = (i % (cols / 2)) * 2, col = from + in;
         float2 v = make_float2(0.f, 0.f);
-        float top = stat[row], sum = 0.f;
-#pragma unroll
-        for (int w = 1; w < W; ++w) top = fmaxf(top, stat[w * ROWS + row]);
-        const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const float2 x = *reinterpret_cast<const float2*>(merge + (w * rows + row) * cols + in);
           v.x += x.x, v.y += x.y;
-          sum += exp2f(stat[w * ROWS + row] - base) * stat[(W + w) * ROWS + row];
         }
         if (!SPLIT || whole) {
-          const float by = sum == 0.f ? 0.f : 1.f / sum;
+          const float by = stat[3 * W * ROWS + row];
           T* o = (T*)d.o + p.b * d.o_bs + (first + row) * d.o_hs + col;
-          *reinterpret_cast<uint32_t*>(o) = Half16<T>::down(sum == 0.f ? 0.f : v.x * by, sum == 0.f ? 0.f : v.y * by);
-          if (col == 0) d.lse[(long long)p.b * d.Hq + first + row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+          *reinterpret_cast<uint32_t*>(o) = Half16<T>::down(by == 0.f ? 0.f : v.x * by, by == 0.f ? 0.f : v.y * by);
         } else {
           *reinterpret_cast<float2*>(part + row * HD + col) = v;
-          if (col == 0) part[ROWS * HD + row] = top, part[ROWS * (HD + 1) + row] = sum;
         }
       }
       __syncthreads();
@@ -566,7 +623,7 @@ static int launch(const FtkPagedAttnDesc& d, const Plan8& p, void* scratch, cuda
   if (rc || !p.split) return rc;
   // Few heads have up to a hundred parts each: 1024 threads 36.2 us for two sequences of 65537 (8 heads), 256 threads 38.9; for 464 heads
   // with a part or two 39.1 and 31.6, for 32 heads of 16 queries each 96.7 and 82.4
-  return p.heads > 32 ? launch_join<T, HD, ROWS, 0>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, 1024>(a, p.heads, p.ctas, p.headers, s);
+  return p.heads > 32 ? launch_join<T, HD, ROWS, 0, true>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, true, 1024>(a, p.heads, p.ctas, p.headers, s);
 }
 
 // Strides of 64 GB and more are refused: offsets are 32 bits times 16 bytes (4 of scales and of the table) of each kind, added up in 64

@@ -99,15 +99,22 @@ __device__ __forceinline__ Place first_place(const int B, const int heads, const
   return p;
 }
 
+// A part's sum l, relative to its accumulators' reference m: the reference by the sum's own power of two, and what is left of it
+__device__ __forceinline__ float2 own_power(float m, float l) {
+  if (l == 0.f) return make_float2(-3.402823466e38f, 0.f);      // of no tokens
+  const int e = min((int)(__float_as_uint(l) >> 23 & 255) - 127, 126);
+  return make_float2(m + (float)e, l * __uint_as_float((uint32_t)(127 - e) << 23));
+}
 // Joins the parts of a head that several CTAs had, if header blockIdx.x is of one: `together` rows from together * blockIdx.y on, and
 // where that leaves threads over, several of them share a row's parts.  Sums are in a fixed order.  And since sequences of no tokens are in
-// nobody's piece, the blocks write them, a sequence each.  Sums and accumulators are carried times 2^SHIFT.
-template <typename T, int HD, int ROWS, int SHIFT, int THREADS>
+// nobody's piece, the blocks write them, a sequence each.  Sums and accumulators are carried times 2^SHIFT.  FAR: a part's sum may be
+// any power of two away from its accumulators, so the sums are added up by their own largest.
+template <typename T, int HD, int ROWS, int SHIFT, bool FAR, int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttn a, const int together) {
   constexpr int PART = PA_PART<ROWS, HD>, LANES = HD / 4, SLOTS = THREADS / LANES;      // threads of a row, and how many times those
   constexpr int FIRST = 4;               // parts whose accumulators a thread requests along with the statistics
   extern __shared__ float2 part_ml[];    // [parts][together]: maximum and sum, then (factor, -)
-  __shared__ float sums[SLOTS], tops[SLOTS];
+  __shared__ float sums[SLOTS], tops[SLOTS], backs[SLOTS];
   __shared__ float4 shares[SLOTS][LANES];
   const FtkPagedAttnDesc& d = a.d;
   pdl_wait();
@@ -137,20 +144,30 @@ __global__ void __launch_bounds__(THREADS) paged_attn_join_kernel(const __grid_c
     __syncthreads();
     // a warp per row: the largest maximum, every part's factor, the sum
     for (int row = warp; row < some; row += THREADS / 32) {
-      float top = -INFINITY;
-      for (int i = lane; i < n; i += 32) top = fmaxf(top, part_ml[i * together + row].x);
+      float top = -INFINITY, most = -INFINITY;
+      for (int i = lane; i < n; i += 32) {
+        top = fmaxf(top, part_ml[i * together + row].x);
+        if (FAR) most = fmaxf(most, own_power(part_ml[i * together + row].x, part_ml[i * together + row].y).x);
+      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 16; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (FAR) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
       for (int i = lane; i < n; i += 32) {
         float2& ml = part_ml[i * together + row];
+        if (FAR) {
+          const float2 x = own_power(ml.x, ml.y);
+          sum += exp2_of(x.x - most) * x.y;
+        }
         ml.x = exp2f(ml.x - base);
-        sum += ml.x * ml.y;
+        if (!FAR) sum += ml.x * ml.y;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) sums[row] = sum, tops[row] = top;
+      if (lane == 0) sums[row] = sum, tops[row] = FAR ? most : top, backs[row] = FAR ? exp2f(top - most) / sum : 1.f;
     }
     __syncthreads();
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -172,10 +189,11 @@ __global__ void __launch_bounds__(THREADS) paged_attn_join_kernel(const __grid_c
         const float4 y = shares[k * together + j][quad];
         v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
       }
-      const float sum = sums[j], by = sum == 0.f ? 0.f : 1.f / sum;
+      const float sum = sums[j], by = sum == 0.f ? 0.f : FAR ? backs[j] : 1.f / sum;
       const int q = (head / a.subs) * a.group + (head % a.subs) * a.sub_heads + r0 + j;
       if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x * by, v.y * by), Half16<T>::down(v.z * by, v.w * by));
+      v.x *= by, v.y *= by, v.z *= by, v.w *= by;
+      *reinterpret_cast<uint2*>((T*)d.o + b * d.o_bs + q * d.o_hs + quad * 4) = make_uint2(Half16<T>::down(v.x, v.y), Half16<T>::down(v.z, v.w));
       if (quad == 0) d.lse[(long long)b * d.Hq + q] = sum == 0.f ? -INFINITY : (tops[j] + log2f(sum) - (float)SHIFT) * LN2;
     }
   }
@@ -189,13 +207,13 @@ __global__ void __launch_bounds__(THREADS) paged_attn_join_kernel(const __grid_c
 
 // The launch of the join: few heads have many parts each: a row per block, its parts shared by the block's threads.  Else the rows of a
 // head, as far as shared memory goes.
-template <typename T, int HD, int ROWS, int SHIFT, int THREADS = 256>
+template <typename T, int HD, int ROWS, int SHIFT, bool FAR = false, int THREADS = 256>
 static int launch_join(const PagedAttn& a, long long heads, long long ctas, long long headers, cudaStream_t s) {
   constexpr int slots = THREADS / (HD / 4);
   int together = 1;
   while (heads > 32 && together < a.sub_heads && together < slots && ctas * together * 2 * sizeof(float2) <= 40 * 1024)
     together *= 2;
-  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS, SHIFT, THREADS>, dim3((unsigned)headers, (unsigned)((a.sub_heads + together - 1) / together)), dim3(THREADS),
+  return launch_pdl(paged_attn_join_kernel<T, HD, ROWS, SHIFT, FAR, THREADS>, dim3((unsigned)headers, (unsigned)((a.sub_heads + together - 1) / together)), dim3(THREADS),
                     (size_t)ctas * together * sizeof(float2), s, a, together);
 }
 

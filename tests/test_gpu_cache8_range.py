@@ -1,0 +1,136 @@
+"""The 8-bit cache's attention over values and keys whose scales are as far apart as the append makes them, against 64-bit arithmetic."""
+import math
+
+import pytest
+import torch
+
+from _decode_oracle import attention as attention64
+from _decode_oracle import close
+from _served_oracle import E4M3, whole
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _weights_apart(q, k, v, ks, vs, table, lengths, scale=None):
+    """What weights held in two halves of fp16 add to the bound: the largest weight of a head, value scale and all, is carried as 2^13 at
+    least, and every weight is off by half of 2^-24 at most, so by 2^-38 of the largest; a value is 448 of its scale's unit at most."""
+    n = vs.shape[2]
+    q, table = q.double().cpu(), table.cpu()
+    keys, scales = whole(k, ks), vs.cpu().double().repeat_interleave(k.shape[2] // n, 2)
+    H, Hk = q.shape[1], k.shape[1]
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    extra = torch.zeros(q.shape, dtype=torch.float64)
+    for b, m in enumerate(lengths):
+        if m == 0:
+            continue
+        p = torch.arange(m)
+        at = table[b].long()[p // k.shape[2]], slice(None), p % k.shape[2]
+        for h in range(H):
+            g = h // (H // Hk)
+            w = torch.softmax(scale * (keys[at][:, g] @ q[b, h]), 0) * scales[at][:, g]
+            extra[b, h] = m * 448 * 2.0 ** -38 * float(w.max())
+    return extra
+
+
+def _check(q, k, v, table, lengths, ks, vs, scale=None):
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    wo, wl, to, tl = attention64(q, whole(k, ks), whole(v, vs), table, lengths, scale)
+    to = to + _weights_apart(q, k, v, ks, vs, table, lengths, scale)
+    page = k.shape[2]
+    for cols in (table.shape[1], 60 * 64 // page + 1):          # left whole, and cut into pieces
+        t = torch.full((table.shape[0], max(cols, table.shape[1])), -7, dtype=torch.int32, device="cuda")
+        t[:, : table.shape[1]] = table
+        o, lse = D.paged_attention(q, k, v, t, _i32(lengths), scale=scale, k_scales=ks, v_scales=vs)
+        close(o, wo, to, ("o", cols))
+        close(lse, wl, tl, ("lse", cols))
+    K.check_status()
+
+
+# powers of two of the blocks' value scales, over and over: in the same 32 tokens, by 32 tokens (a warp's), by 64 and more (other tiles), and
+# from one end to the other; None: a scale of 0
+PATTERNS = {
+    "low then high": lambda i, n: -100 if i < n // 2 else 40,
+    "high then low": lambda i, n: 40 if i < n // 2 else -100,
+    "ends, up": lambda i, n: -100 if i < n // 2 else 100,
+    "ends, down": lambda i, n: 100 if i < n // 2 else -100,
+    "within a warp's tokens": lambda i, n: (-100, 40, 100, None)[i % 4],
+    "by warp": lambda i, n: (-100, 60)[i // 4 % 2],
+    "by tile": lambda i, n: (60, None, -100)[i // 8 % 3],
+    "slowly up": lambda i, n: -100 + 200 * i // max(n - 1, 1),
+    "slowly down": lambda i, n: 100 - 200 * i // max(n - 1, 1),
+    "one high": lambda i, n: 100 if i == n // 3 else -90,
+}
+
+
+@pytest.mark.parametrize("pattern", PATTERNS, ids=lambda p: p.replace(" ", "_"))
+@pytest.mark.parametrize("H,Hk,hd", [(1, 1, 64), (3, 3, 128), (8, 2, 64), (6, 1, 128), (12, 1, 64), (32, 2, 128)])
+def test_value_scales_far_apart(cuda_device, H, Hk, hd, pattern):
+    """No token is left out of the sum, wherever the scales change."""
+    g = _gen(H + hd)
+    page, block, lengths = 16, 8, [1900, 61, 200, 9]
+    cols = -(-max(lengths) // page)
+    need = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(need), generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(lengths), cols), -7, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(sum(need), Hk, page, hd, generator=g, device="cuda").mul(100).clamp(-448, 448).to(E4M3) for _ in range(2))
+    ks = torch.full((sum(need), Hk, page // block), 2.0 ** -7, device="cuda")
+    vs = torch.ones(sum(need), Hk, page // block, device="cuda")
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at: at + n]
+        at += n
+        blocks = -(-lengths[b] // block)
+        for i in range(blocks):
+            e = PATTERNS[pattern](i, blocks)
+            vs[int(table[b, i // 2]), :, i % 2] = 0.0 if e is None else 2.0 ** e
+    # 1.3 of a score on average: tokens of all blocks weigh about the same
+    q = torch.randn(len(lengths), H, hd, generator=g, device="cuda").to(BF)
+    _check(q, k, v, table, lengths, ks, vs)
+
+
+def test_equal_scores_under_scales_far_apart(cuda_device):
+    """Two tiles of equal scores: each has half of the weight."""
+    from frankentorch_b200.ops import decode as D
+    for low, high in ((-100, 40), (-100, 100), (None, 30)):
+        for first in (0, 1):
+            k = torch.zeros(2, 1, 64, 64, dtype=torch.uint8, device="cuda").view(E4M3)
+            v = torch.ones(2, 1, 64, 64, device="cuda").to(E4M3)
+            ks = torch.ones(2, 1, 1, device="cuda")
+            vs = torch.full((2, 1, 1), 2.0 ** high, device="cuda")
+            vs[first] = 0.0 if low is None else 2.0 ** low
+            for H in (1, 4, 16):
+                for cols in (2, 60):
+                    table = torch.tensor([[0, 1] + [-1] * (cols - 2)], dtype=torch.int32, device="cuda")
+                    o, lse = D.paged_attention(torch.ones(1, H, 64, dtype=BF, device="cuda"), k, v, table, _i32([128]), k_scales=ks, v_scales=vs)
+                    assert bool((o.float() == 2.0 ** (high - 1)).all()), (low, high, first, H, cols)
+                    assert float((lse - math.log(128)).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("H,Hk", [(2, 2), (8, 2)])
+@pytest.mark.parametrize("zero_first", [True, False])
+def test_a_zero_block_beside_large_values(cuda_device, H, Hk, zero_first):
+    """A block of zeros, which the append gives its smallest scale, beside one of values of 2^90."""
+    from frankentorch_b200.ops import decode as D
+    g = _gen(3)
+    n, page, hd = 256, 64, 64
+    x = torch.randn(1, n, Hk, hd, generator=g, device="cuda").to(BF)
+    y = (torch.randn(1, n, Hk, hd, generator=g, device="cuda") * 2.0 ** 90).to(BF)
+    y[:, : n // 2] = 0
+    if not zero_first:
+        y = y.flip(1)
+    k, v = (torch.zeros(n // page, Hk, page, hd, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    ks, vs = (torch.zeros(n // page, Hk, 2, device="cuda") for _ in range(2))
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None]
+    D.paged_append(k, v, table, x, y, _i32([0]), k_scales=ks, v_scales=vs)
+    assert float(vs.min()) == 2.0 ** -100 and float(vs.max()) > 2.0 ** 80
+    _check(torch.randn(1, H, hd, generator=g, device="cuda").to(BF), k, v, table, [n], ks, vs)
