@@ -20,7 +20,7 @@
 //
 // A warp takes 32 tokens of a tile at a time.  fp16 holds every e4m3 value, so keys and values go into the matrix instructions as they
 // are, converted in registers, and the scales are applied to scores and probabilities, which are few.  The queries are in fp16 too, a
-// row at a time times the power of two that brings its largest element to 2^14 .. 2^15: what that loses is below 2^-39 of it.
+// row at a time times the power of two, up to 2^127, that brings its largest element to 2^14 .. 2^15: what that loses is below 2^-39 of it.
 // Matrix products of the 8-bit values as they are, with queries and probabilities in several parts, took 284 us where these took 276.
 //
 // Scores are formed with the tokens as rows and the heads as columns: of 16 x 8 results none is wasted for up to eight heads, where heads as
@@ -74,8 +74,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t pair) {      // of 8 x 8
   return r;
 }
 constexpr int A8_SHIFT = 14;      // weights are carried times 2^14
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // 2^e of -126 to 127
 // v / 2^e, times 2^14
-__device__ __forceinline__ float unscaled(float v, float e) { return v * __uint_as_float((uint32_t)(127 + A8_SHIFT - (int)e) << 23); }
+__device__ __forceinline__ float unscaled(float v, float e) { return v * power(A8_SHIFT - (int)e); }
 __device__ __forceinline__ float max_of(float x) {      // over the warp; NaN is not counted
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -260,11 +261,13 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
   uint32_t q[CH][2 * RR];               // of chunk c: elements 2 c0 .. + 3 of head r0, then of head r0 + 8
   // of heads c0, c0 + 1, c0 + 8, c0 + 9; ONE: [0].  m of the accumulators, of all lanes; n and l of this lane's tokens
   float acc[NT][4], m[2 * RR], n[2 * RR], l[2 * RR], sc[2 * RR];
+  float k_by;                           // what keys' scales are multiplied by
   float unit;                           // power of two of the first tokens' value scales
   bool near;                            // all so far are within A8_NEAR powers of it: then n = m - unit, and a weight is taken from its term of l
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
   const auto begin = [&]() {            // queries of the head at `p`; rows beyond the group are zero
     const int first = row0(p.h), rows = rows_of(p.h);
+    int e[RR];
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
       const int row = r * 8 + r0;
@@ -279,16 +282,27 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
-      const float by = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-      const float own = (float)d.scale * LOG2E * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-      sc[2 * r] = __shfl_sync(0xffffffffu, own, ONE ? 0 : c0 * 4);
-      sc[2 * r + 1] = __shfl_sync(0xffffffffu, own, c0 * 4 + 4);
+      e[r] = min(max((int)(__float_as_uint(most) >> 23) - 127, -113), 127);
+      const float by = power(14 - e[r]);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const float2 x = Half16<T>::up(u[c].x), y = Half16<T>::up(u[c].y);
         q[c][2 * r] = Half16<__half>::down(x.x * by, x.y * by), q[c][2 * r + 1] = Half16<__half>::down(y.x * by, y.y * by);
       }
+    }
+    // What a score is multiplied by beside its key's scale, scale log2(e) 2^(e - 14): the power of two of the row that has the largest goes
+    // to the keys' scales, so that neither of the two is beyond fp32 where their product is not
+    const float factor = (float)d.scale * LOG2E;
+    const int of_factor = min(max((int)(__float_as_uint(factor) >> 23 & 255) - 127, -126), 126);
+    if (ONE) e[0] = __shfl_sync(0xffffffffu, e[0], 0);
+    const int largest = ONE ? e[0] : __reduce_max_sync(0xffffffffu, max(e[0], e[RR - 1]));
+    const int with_key = min(max(largest - 14 + of_factor, -126), 127);
+    k_by = power(with_key);
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      const float own = factor * power(-of_factor) * power(max(e[r] - 14 + of_factor - with_key, -126));
+      sc[2 * r] = ONE ? own : __shfl_sync(0xffffffffu, own, c0 * 4);
+      if (!ONE) sc[2 * r + 1] = __shfl_sync(0xffffffffu, own, c0 * 4 + 4);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -317,7 +331,7 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       const unsigned ok = there[stage];
       load(stage == 0 ? STAGES - 1 : stage - 1);      // the stage that the tile before left: its reads are behind the warp's barrier
       const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);      // keys', values', the values' exponents
-      const float k_scale = scales[lane], v_scale = scales[N + lane], v_exp = (float)max((int)(__float_as_uint(v_scale) >> 23 & 255) - 127, -100);
+      const float k_scale = scales[lane] * k_by, v_scale = scales[N + lane], v_exp = (float)max((int)(__float_as_uint(v_scale) >> 23 & 255) - 127, -100);
       // Scores with the tokens as rows: s[2 r + t] of tokens 16 t and on, the r-th eight heads
       float s[2 * RR][4] = {};
 #pragma unroll

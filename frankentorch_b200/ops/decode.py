@@ -17,7 +17,8 @@ may be strided.  Lengths, positions and counts are int32 on the device, so a cap
 The cache may be held in 8 bits: pages of ``torch.float8_e4m3fn`` with fp32 scales, ``[pages, heads, blocks]`` with unit inner stride,
 for keys (``k_scales``) and for values (``v_scales``).  A block is ``page / blocks`` neighbouring rows of a page and head (a power of two,
 64 at most), and an element stands for its 8 bits times its block's scale.  :func:`paged_append` makes the scales, powers of two;
-:func:`paged_attention` takes any from 2^-100 to 2^100, or 0.
+:func:`paged_attention` takes those and any other from 2^-100 to 2^120, or 0, in any mixture.  What adds less than 2^-38 of the largest
+product of a probability and a value's scale, times 448, to an element of the output does not count.
 
 A call enqueues on the current stream of its tensors' device, also where another device is the current one, and returns.
 Arguments that the host can check are refused with :class:`~.kernels.KernelError`; a page, token or length out of range on the
@@ -70,7 +71,7 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     returned turned; queries behind ``counts[b]`` are copied as they are.  ``q_out`` may be ``q`` itself.
 
     Into a cache in 8 bits a block's new elements (keys in fp32 behind their rotation) get the smallest power of two, 2^-100 at least, of
-    which 448 times reaches the largest finite one, and each is rounded once to a multiple of it; infinities and NaN are held as NaN.
+    which 448 times reaches the largest finite one, and each is rounded once to a multiple of it; infinities and NaN are held as NaN.  (From 1.9375 2^127 on the nearest multiple is 2^128, which neither fp32 nor bf16 holds.)
     A block that has rows in front of ``start[b]`` keeps at least its own scale; where it grows, those rows are rounded anew (exact but
     for the smallest ones).  What stands in a block behind the last new token has no meaning any more."""
     return _lib.bind().paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out, k_scales, v_scales)

@@ -51,7 +51,11 @@ def _check(q, k, v, table, lengths, ks, vs, scale=None):
         t = torch.full((table.shape[0], max(cols, table.shape[1])), -7, dtype=torch.int32, device="cuda")
         t[:, : table.shape[1]] = table
         o, lse = D.paged_attention(q, k, v, t, _i32(lengths), scale=scale, k_scales=ks, v_scales=vs)
-        close(o, wo, to, ("o", cols))
+        # The nearest multiple of 2^120 of 1.99 2^127 is 256, and 2^128 is beyond bf16: what passes the type's largest number by the bound,
+        # or does not by less, may be infinite
+        got = o.cpu().double()
+        over = got.isinf() & (got.sign() == wo.sign()) & (wo.abs() + to > torch.finfo(o.dtype).max)
+        close(torch.where(over, 0.0, got), torch.where(over, 0.0, wo), to, ("o", cols))
         close(lse, wl, tl, ("lse", cols))
     K.check_status()
 
@@ -134,3 +138,29 @@ def test_a_zero_block_beside_large_values(cuda_device, H, Hk, zero_first):
     D.paged_append(k, v, table, x, y, _i32([0]), k_scales=ks, v_scales=vs)
     assert float(vs.min()) == 2.0 ** -100 and float(vs.max()) > 2.0 ** 80
     _check(torch.randn(1, H, hd, generator=g, device="cuda").to(BF), k, v, table, [n], ks, vs)
+
+
+@pytest.mark.parametrize("H,Hk", [(2, 2), (8, 2), (12, 1)])
+@pytest.mark.parametrize("q_size,k_size,v_size,scale", [
+    (0, 0, 127, None), (-124, 127, 0, None), (-124, 127, 127, None), (0, 127, 0, 2.0 ** -126), (-20, 127, -99, 2.0 ** -106),
+    (98, -95, 0, None), (127, -95, 127, 2.0 ** -31), (-60, 60, -95, None)])
+def test_every_scale_that_the_append_makes(cuda_device, H, Hk, q_size, k_size, v_size, scale):
+    """Keys and values up to the largest numbers of bf16, whose scales are 2^120, and as small ones; queries of a size that leaves scores of
+    about 8."""
+    from frankentorch_b200.ops import decode as D
+    g = _gen(H + q_size + 200)
+    n, page, hd = 300, 64, 64
+    # 1 to 1.99, of either sign, times 2^k_size
+    x, y = ((torch.rand(1, n, Hk, hd, generator=g, device="cuda").double() * 0.99 + 1) * torch.where(
+        torch.rand(1, n, Hk, hd, generator=g, device="cuda") < 0.5, -1, 1) * 2.0 ** e for e in (k_size, v_size))
+    x, y = x.to(BF), y.to(BF)
+    assert bool(x.isfinite().all()) and bool(y.isfinite().all())
+    q = (torch.randn(1, H, hd, generator=g, device="cuda").clamp(-1.9, 1.9).double() * 2.0 ** q_size).to(BF)
+    P = -(-n // page)
+    k, v = (torch.zeros(P, Hk, page, hd, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    ks, vs = (torch.zeros(P, Hk, 1, device="cuda") for _ in range(2))
+    table = torch.arange(P, dtype=torch.int32, device="cuda")[None]
+    D.paged_append(k, v, table, x, y, _i32([0]), k_scales=ks, v_scales=vs)
+    for size, s in ((k_size, ks), (v_size, vs)):
+        assert float(s.max()) == float(s.min()) == 2.0 ** max(size - 7, -100)
+    _check(q, k, v, table, [n], ks, vs, scale)
