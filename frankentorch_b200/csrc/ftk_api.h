@@ -441,7 +441,7 @@ typedef struct FtkLogitsDesc {
 } FtkLogitsDesc;
 int ftk_logits(const FtkLogitsDesc* d, void* stream);
 
-// Row r: token i < V weighs w_i = round(2^43 exp((x_i - max x) / T)), nothing where x_i is -inf.  In the order of x, equal ones by
+// Row r: token i < V weighs w_i = round(2^43 exp((x_i - max x) / T)) (within 2^-8 of a half, either neighbour), nothing where x_i is -inf.  In the order of x, equal ones by
 // their ids, are kept the first k (k <= 0: all), of those the ones before which less than p of their sum lies (p >= 1: all; the first
 // always), of those the ones of at least min_p of the largest; T = 0 keeps the first.  token[r] is the first kept one by id with
 // sum_{j <= i} w_j > floor(u sum_j w_j), logprob[r] = log(w_i / sum_j w_j).  A row of nothing but -inf: -1, -inf; with a NaN among its

@@ -1,11 +1,11 @@
 // The choice of a token from the logits of a step: temperature, top-k, top-p, min-p, and a given random number.
 //
-// Mathematics.  Weights are whole numbers, w_i = 2^43 exp((x_i - max x) / T) to a unit, so their sums (63 bits for up to 2^20 tokens) are
+// Mathematics.  Weights are whole numbers, w_i = 2^43 exp((x_i - max x) / T) rounded, so their sums (63 bits for up to 2^20 tokens) are
 // exact whatever their order, and a row's choice is a function of its logits, settings and random number alone.  With tokens in the
 // order of their logits (equal ones by their ids): the first k; of those the ones before which less than p of the sum lies; of those the
 // ones of at least min_p of the largest; then the first by id whose running sum passes u times the sum.
 //
-// What bounds it: each logit is read once.  A weight takes 9 operations in 64 bits, at half the rate of fp32, so where all are needed they are
+// What bounds it: each logit is read once.  A weight takes 10 operations in 64 bits, at half the rate of fp32, so where all are needed they are
 // next: with what is around them 6 to 7 cycles of an SM for 32.
 //
 // Work.  A cluster of CTAs has a row, each an equal run of its columns, which it keeps in shared memory (rows of more than that are read
@@ -154,8 +154,10 @@ struct SampleShared {
   uint32_t n_list, n_aside;
 };
 
-// A row's settings.  2^43 exp((x - top) / T): 2^(k / 256) out of the table, the rest by three terms of the exponential series (relative
-// error 2^-46), and by adding 2^9 a number of up to 1 is rounded to units of 2^-43.
+// A row's settings.  2^43 exp((x - top) / T): 2^(k / 256) out of the table, the rest by four terms of the exponential series, up to
+// (ln(2) / 512)^4 / 24 (the next one is 2^-54), and by adding 2^9 a number of up to 1 is rounded to units of 2^-43.  What is rounded is within
+// 2^-8 of the exact number of units: z exp(-z) 2^43, 0.37 2^43 at most, times the 2^-52 by which z = (top - x) / T is off, and some
+// roundings of the result.
 struct Weigh {
   const double* table;
   double top, by;                      // 256 log2(e) / T
@@ -165,7 +167,7 @@ struct Weigh {
     const double d = (double)x - top, kd = fma(d, by, MAGIC), r = fma(d, by, MAGIC - kd);
     const int k = __double2loint(kd);
     constexpr double C = 0.0027076061740622863;       // ln(2) / 256
-    const double p = r * fma(r, fma(r, C * C * C / 6, C * C / 2), C), t = table[k & 255];
+    const double p = r * fma(r, fma(r, fma(r, C * C * C * C / 24, C * C * C / 6), C * C / 2), C), t = table[k & 255];
     double v = fma(t, p, t);
     v = __hiloint2double(__double2hiint(v) + (int)((uint32_t)(k & ~255) << 12), __double2loint(v)) + 512.0;
     return (u64)(uint32_t)(__double2hiint(v) - 0x40800000) << 32 | (uint32_t)__double2loint(v);

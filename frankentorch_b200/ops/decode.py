@@ -119,7 +119,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, vocab: Optional[int] 
     """A token for each row of ``logits`` (the first ``vocab`` columns, 2^20 at most, of ``[R, columns]``; bf16, fp16 or fp32) from
     ``uniform`` (fp32 ``[R]``, in [0, 1)); returns ``(token int64 [R], logprob fp32 [R])``.
 
-    Token ``i`` weighs ``w_i = round(2^43 exp((x_i - max x) / temperature))``.  In the order of the logits, equal ones by their ids, are kept
+    Token ``i`` weighs ``w_i = round(2^43 exp((x_i - max x) / temperature))`` (formed in 64 bits: within 2^-8 of a half, either neighbour).  In the order of the logits, equal ones by their ids, are kept
 
     * ``top_k``: the first ``top_k`` (0: all);
     * ``top_p``: of those the ones before which less than ``top_p`` of their sum lies (1: all; the first always);
