@@ -255,7 +255,9 @@ class GPTDecoder:
         The next ids are the highest; or drawn, where ``temperature``, ``top_k``, ``top_p`` or ``min_p`` is given, as
         :func:`~frankentorch_b200.ops.decode.sample` does, with random numbers of ``generator`` (the device's own); or what ``choose``
         makes of the processed logits ``[batch, vocabulary]``.  A row ends behind ``eos``, and where mask and bias leave it no token;
-        with a mask or a bias ``choose`` gets zeros for the rows that have ended, and what it returns for them is not used."""
+        with a mask or a bias ``choose`` gets zeros for the rows that have ended, and what it returns for them is not used.  Where a token
+        is to be drawn from NaN, under a setting that is NaN or a negative temperature, a KernelError names the rows when the others are
+        through."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens is positive")
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
@@ -274,6 +276,7 @@ class GPTDecoder:
         tokens = torch.zeros((B, S + max_new_tokens), dtype=torch.int64, device=self.device)
         tokens[:, :S] = torch.where(at[None, :] < prompt[:, None], ids.to(self.device), 0)
         live = torch.ones(B, dtype=torch.bool, device=self.device)
+        undefined = torch.zeros_like(live)      # rows that ended for logits or settings that are no numbers
         penalised = not (repetition is None and frequency is None and presence is None)
         for i in range(max_new_tokens):
             words = allowed(tokens, totals) if callable(allowed) else allowed
@@ -284,7 +287,8 @@ class GPTDecoder:
                 bias=bias, allowed=words)
             if drawn:
                 u = torch.rand(B, generator=generator, device=self.device)
-                picked = D.sample(x, u, vocab=self.cfg.vocab_size, **settings)[0]
+                picked, logprob = D.sample(x, u, vocab=self.cfg.vocab_size, **settings)
+                undefined |= live & logprob.isnan()
                 live &= picked >= 0             # -1: there is none
             elif words is not None or bias is not None:
                 live &= x.amax(-1) != float("-inf")
@@ -301,4 +305,7 @@ class GPTDecoder:
             if i + 1 < max_new_tokens:
                 logits = self.step(new)
         K.check_status()
+        if drawn and bool(undefined.any()):
+            raise K.KernelError(f"nothing could be drawn for rows {undefined.nonzero().flatten().tolist()}: NaN among their logits or "
+                                "settings, or a negative temperature")
         return tokens, totals
