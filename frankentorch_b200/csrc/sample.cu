@@ -153,6 +153,8 @@ struct SampleShared {
   uint32_t maxima[SA_THREADS];         // published: of parts of the row
   uint32_t n_list, n_aside;
 };
+constexpr int SA_OWN = (sizeof(SampleShared) + 15) / 16 * 16;      // bytes of a CTA beside its part of the row
+static_assert(SA_OWN <= 48 * 1024 && SA_OWN + SA_SHARE <= 227 * 1024, "a CTA's shared memory, where it keeps none of the row and where it keeps the most");
 
 // A row's settings.  2^43 exp((x - top) / T): 2^(k / 256) out of the table, the rest by four terms of the exponential series, up to
 // (ln(2) / 512)^4 / 24 (the next one is 2^-54), and by adding 2^9 a number of up to 1 is rounded to units of 2^-43.  What is rounded is within
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
   constexpr int N = 16 / (int)sizeof(T), STEP = 32 * N;      // elements of a vector, of a warp's step
   extern __shared__ __align__(16) unsigned char smem[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
-  uint4* kept_row = reinterpret_cast<uint4*>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
+  uint4* kept_row = reinterpret_cast<uint4*>(smem + SA_OWN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = (int)d.V;
   const int rank = (int)cluster_rank(), lc = (int)d.cluster, C = 1 << lc;
   const long long r = blockIdx.x >> lc;
@@ -985,9 +987,11 @@ __global__ void __launch_bounds__(SA_THREADS, 4) sample_kernel(const __grid_cons
 template <typename T, bool RES, bool VEC>
 static int launch(const FtkSampleDesc& d, int its, cudaStream_t s) {
   const auto kernel = sample_kernel<T, RES, VEC>;
-  const size_t bytes = (sizeof(SampleShared) + 15) / 16 * 16 + (RES ? (size_t)its * SA_THREADS * 16 : 0);
-  int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (rc) return rc;
+  const size_t bytes = SA_OWN + (RES ? (size_t)its * SA_THREADS * 16 : 0);
+  if (RES) {      // the most for any row: the limit is the function's, and calls of other sizes may be on their way to their launch
+    const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_OWN + SA_SHARE);
+    if (rc) return rc;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(d.R << d.cluster));
   cfg.blockDim = dim3(SA_THREADS);
