@@ -154,6 +154,8 @@ struct SampleShared {
   uint32_t n_list, n_aside;
 };
 constexpr int SA_OWN = (sizeof(SampleShared) + 15) / 16 * 16;      // bytes of a CTA beside its part of the row
+constexpr int SA_THREE = (228 * 1024 / 3 - 1024 - SA_OWN) / (SA_THREADS * 16);      // steps up to which three CTAs share an SM's memory
+static_assert(SA_THREE == 13, "the sizes measured at the launcher are on either side of it");
 static_assert(SA_OWN <= 48 * 1024 && SA_OWN + SA_SHARE <= 227 * 1024, "a CTA's shared memory, where it keeps none of the row and where it keeps the most");
 
 // A row's settings.  2^43 exp((x - top) / T): 2^(k / 256) out of the table, the rest by four terms of the exponential series, up to
@@ -1013,11 +1015,12 @@ template <typename T> static int launch(FtkSampleDesc d, cudaStream_t s) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const auto its_of = [&](int c) { return (int)((d.V + (long long)STEP * c - 1) / ((long long)STEP * c)); };
-  // As many CTAs for a row as fill the SMs four times, with two steps each at least, and as many as it takes to keep 56 KB each: three
-  // share an SM then, and one works while others wait.  256 rows of 50257 fp32: 65.5 us with 56 KB, 74.7 with 32 KB (clusters twice as large);
-  // 512 rows of 128003 bf16 the same with both
+  // As many CTAs for a row as fill the SMs four times, with two steps each at least, and as many as it takes for three to share an SM, so
+  // that one works while others wait.  With 13 steps, the most for that: 256 rows of 50257 fp32, settings by row, 65.8 us, and 74.7 in clusters twice
+  // as large.  With 14, in clusters twice as large as against two CTAs to an SM: 256 rows of 55000 with settings by row 77.7 and 81.3, k = 50
+  // 43.5 and 46.6, the whole distribution 51.9 and 54.3, p = 0.9 116.1 and 110.9; 640 of 14000, p = 0.9, 68.2 and 74.8; 512 of 110000 in bf16 the same
   int c = 1;
-  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 4ll * sms && its_of(c) > 2) || its_of(c) * SA_THREADS * 16 > 56 * 1024)) c *= 2;
+  while (c < SA_CLUSTER && its_of(c) > 1 && ((d.R * c < 4ll * sms && its_of(c) > 2) || its_of(c) > SA_THREE)) c *= 2;
   int lc = 0;
   while ((1 << lc) < c) ++lc;
   d.cluster = lc;
