@@ -376,12 +376,10 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
         ldm4(weights_at + 32, hi[1]);
       } else {
         // masked scores of heads c0, c0 + 1 at tokens r0, r0 + 8 .., and the larger references of the head's tokens and what was there
-        {
-        const bool there = ok >> lane & 1u;
-        if (unit == A8_NONE) unit = max_of(there ? v_exp : A8_NONE);
-        near = near && !__any_sync(0xffffffffu, there && fabsf(v_exp - unit) > A8_NEAR);
-        reinterpret_cast<float4*>(turn)[lane] = make_float4(k_scale, v_exp, there ? unscaled(v_scale, near ? unit : v_exp) : 0.f, 0.f);
-      }
+        const bool own_there = ok >> lane & 1u;
+        if (unit == A8_NONE) unit = max_of(own_there ? v_exp : A8_NONE);
+        near = near && !__any_sync(0xffffffffu, own_there && fabsf(v_exp - unit) > A8_NEAR);
+        reinterpret_cast<float4*>(turn)[lane] = make_float4(k_scale, v_exp, own_there ? unscaled(v_scale, near ? unit : v_exp) : 0.f, 0.f);
         __syncwarp();
         float grow[2 * RR], v14[4], v_of[4];
         bool moved = false;
@@ -411,7 +409,7 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
           if (near) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float own = top[e] - unit;
+              const float own = top[e] == A8_NONE ? A8_NONE : top[e] - unit;      // (a tile may have no token: pages that are none)
               l[2 * r + e] *= grow[2 * r + e];
               n[2 * r + e] = own;
 #pragma unroll

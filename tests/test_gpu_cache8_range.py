@@ -164,3 +164,27 @@ def test_every_scale_that_the_append_makes(cuda_device, H, Hk, q_size, k_size, v
     for size, s in ((k_size, ks), (v_size, vs)):
         assert float(s.max()) == float(s.min()) == 2.0 ** max(size - 7, -100)
     _check(q, k, v, table, [n], ks, vs, scale)
+
+
+@pytest.mark.parametrize("H", [1, 4, 12])
+def test_a_page_that_is_none_before_scales_far_apart(cuda_device, H):
+    """What is left of the sequence counts in full, however low its scores are."""
+    from frankentorch_b200.ops import decode as D
+    from frankentorch_b200.ops import kernels as K
+    page, n, hd = 32, 600, 64
+    P = -(-n // page)
+    k = torch.ones(P, 1, page, hd, device="cuda").to(E4M3)
+    v = torch.ones(P, 1, page, hd, device="cuda").to(E4M3)
+    ks = torch.full((P, 1, 4), 64.0, device="cuda")
+    vs = torch.tensor([2.0 ** 40, 2.0 ** -100] * 2, device="cuda").expand(P, 1, 4).contiguous()
+    q = torch.full((1, H, hd), -0.5, dtype=BF, device="cuda")            # scores of -256
+    for cols in (P, 60):
+        table = torch.full((1, cols), -7, dtype=torch.int32, device="cuda")
+        table[0, :P] = torch.arange(P, dtype=torch.int32, device="cuda")
+        table[0, 0] = -3
+        o, lse = D.paged_attention(q, k, v, table, _i32([n]), k_scales=ks, v_scales=vs)
+        with pytest.raises(K.KernelError, match="BAD_INDEX"):
+            K.check_status()
+        assert float((lse.double() - (math.log(n - page) - 256)).abs().max()) < 256 * 68 * 2.0 ** -24
+        high = sum(1 for t in range(page, n) if t // 8 % 2 == 0)
+        assert float((o.double() / 2.0 ** 40 - high / (n - page)).abs().max()) <= 2.0 ** -8
