@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
 
 struct Plan8 {
   int subs, sub_heads, rows;
-  bool split, alone;               // heads cut into pieces; a CTA per SM, for few heads
+  bool split, alone, wide_join;    // heads cut into pieces; a CTA per SM, for few heads; 1024 threads for a row of the join
   long long ctas, heads, headers, bytes;      // heads: of all sequences, a part of a group counting as one
 };
 template <int ROWS, int HD> constexpr int A8_CTAS = A8Smem<ROWS, HD, A8_WARPS>::CTAS;
@@ -603,6 +603,10 @@ static Plan8 plan_of(const FtkPagedAttnDesc& d) {
   const long long tiles = ((d.table_cols << d.page_shift) + 63) / 64;
   p.alone = p.heads <= sms;
   p.split = tiles > a8_whole(p.heads, sms);
+  // Few heads have up to a hundred parts each, which 1024 threads join faster than 256, as long as the rows, a block each, have an SM each (us):
+  // 8 heads of 8 queries, 2 x 65537, 36.1 and 38.7; 16 of 8 31.3 and 32.2; 32 of 1 22.3 and 22.1; 32 of 8 50.1 and 46.7; 32 of 16 72.0 and 62.7.
+  // Many heads have a part or two: 464 heads 50.8 and 40.6, 48 42.6 and 42.2
+  p.wide_join = p.heads <= 32 && p.heads * p.sub_heads <= sms;
   if (p.split) {
     p.ctas = (d.hd == 64 ? (p.rows == 1 ? A8_CTAS<1, 64> : p.rows == 8 ? A8_CTAS<8, 64> : A8_CTAS<16, 64>)
                          : (p.rows == 1 ? A8_CTAS<1, 128> : p.rows == 8 ? A8_CTAS<8, 128> : A8_CTAS<16, 128>)) * (long long)sms;
@@ -633,9 +637,7 @@ static int launch(const FtkPagedAttnDesc& d, const Plan8& p, void* scratch, cuda
   if (rc) return rc;
   rc = launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(A8_WARPS * 32), bytes, s, a, by, status);
   if (rc || !p.split) return rc;
-  // Few heads have up to a hundred parts each: 1024 threads 36.2 us for two sequences of 65537 (8 heads), 256 threads 38.9; for 464 heads
-  // with a part or two 39.1 and 31.6, for 32 heads of 16 queries each 96.7 and 82.4
-  return p.heads > 32 ? launch_join<T, HD, ROWS, 0, true>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, true, 1024>(a, p.heads, p.ctas, p.headers, s);
+  return p.wide_join ? launch_join<T, HD, ROWS, 0, true, 1024>(a, p.heads, p.ctas, p.headers, s) : launch_join<T, HD, ROWS, 0, true>(a, p.heads, p.ctas, p.headers, s);
 }
 
 // Strides of 64 GB and more are refused: offsets are 32 bits times 16 bytes (4 of scales and of the table) of each kind, added up in 64

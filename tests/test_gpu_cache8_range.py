@@ -188,3 +188,15 @@ def test_a_page_that_is_none_before_scales_far_apart(cuda_device, H):
         assert float((lse.double() - (math.log(n - page) - 256)).abs().max()) < 256 * 68 * 2.0 ** -24
         high = sum(1 for t in range(page, n) if t // 8 % 2 == 0)
         assert float((o.double() / 2.0 ** 40 - high / (n - page)).abs().max()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("B,H,Hk,hd,n", [(2, 16, 1, 64, 2600), (4, 64, 4, 128, 2500), (8, 16, 4, 64, 2400), (8, 32, 4, 128, 1900), (3, 33, 11, 128, 2000)])
+def test_few_heads_of_many_queries_in_pieces(cuda_device, B, H, Hk, hd, n):
+    """Rows of the join that have an SM each, and more of them than SMs."""
+    g = _gen(B * H)
+    page, lengths = 64, [n - 37 * b for b in range(B)]
+    P = -(-n // page)
+    k, v = (torch.randn(B * P, Hk, page, hd, generator=g, device="cuda").mul(100).clamp(-448, 448).to(E4M3) for _ in range(2))
+    ks, vs = (torch.exp2(torch.randint(-9, -5, (B * P, Hk, 2), generator=g, device="cuda").float()) for _ in range(2))
+    table = torch.randperm(B * P, generator=g, device="cuda").to(torch.int32).view(B, P)
+    _check(torch.randn(B, H, hd, generator=g, device="cuda").to(BF), k, v, table, lengths, ks, vs)
