@@ -7,16 +7,18 @@
 // others, where scales are 2^126 apart.  Whole numbers leave x_t - (m - e_t) as exact as x_t.  As long as a head's scales are within 2^40 of
 // its first ones, n = m - e of those serves, and a weight is its term of l times a power of two and the scale; from the first tile on
 // where they are not, n is each lane's own and weights have an exponential of their own (32 heads over 8 of 128, 16 x 2048 tokens: 20.0 us that
-// way throughout, 18.9 now); with one head to a head of the cache, a token per lane, that costs nothing and is always so.  Parts are given on as m and l 2^(n - m), which |n - m| <= 129 keeps in fp32; where parts
-// meet, sums are compared by their own powers of two.  The list of tiles, the pieces, the rings and the join are paged_attention.cu's.
+// way throughout, 18.9 this way); with one head to a head of the cache, a token per lane, that costs nothing and is always so.  Parts are
+// given on as m and l 2^(n - m), which |n - m| <= 129 keeps in fp32; where parts meet, sums are compared by their own powers of two.  The
+// list of tiles, the pieces, the rings and the join are paged_attention.cu's.
 //
 // What is lost: weights are held in two halves of fp16, the largest as 2^13 or more, each to 2^-25: what adds less than 2^-38 of the largest weight
 // (value scale and all) times 448 to an element of the output does not count.
 //
 // What bounds it: every key and value is read once, in 8 bits; the copy bandwidth, with twice the arithmetic per byte of a 16-bit cache.
-// 128 sequences of 700 to 4096, 16 heads of 128: 204 us in a burst of calls, 6.4 TB/s, 230 under sustained load (16-bit cache 388 - 410); 32 of up to 2048 31.6 (51);
-// two of up to 65537, 32 heads over 4, 36.2 (51); one of 301 tokens, 12 heads of 64, 5.1.  A warp's 32 tokens of 128 bytes are 640
-// instructions, of which 64 convert; the SMs issue in 47 % of the cycles, so few heads are bound by the first tiles' way and by the join.
+// 128 sequences of 700 to 4096, 16 heads of 128: 211 - 230 us in calls one after another, by the power that is left, 5.7 - 6.2 TB/s, and 203 - 205
+// in a captured burst of them (16-bit cache 388 - 410); 32 of up to 2048 31.8 (51); two of up to 65537, 32 heads over 4, 36.2 (51); one of 301
+// tokens, 12 heads of 64, 5.4.  A warp's 32 tokens of 128 bytes are 620 instructions, of which 64 convert; the SMs issue in 45 - 47 % of the
+// cycles, so few heads are bound by the first tiles' way and by the join.
 //
 // A warp takes 32 tokens of a tile at a time.  fp16 holds every e4m3 value, so keys and values go into the matrix instructions as they
 // are, converted in registers, and the scales are applied to scores and probabilities, which are few.  The queries are in fp16 too, a
@@ -44,10 +46,10 @@ constexpr float A8_NONE = -3.402823466e38f;      // the reference where there is
 // Scales within 2^40 of one another: x - (m - unit) is 40 at most, and what it loses to fp32 below 2^-126 is below 2^-46 of l and of the accumulator
 constexpr float A8_NEAR = 40.f;
 // Tiles of 64 tokens, by the width of the table, up to which a head is left whole: a second launch and the join cost 4 - 6 us.  Whole and cut
-// (us), all positions in use, 64 to a tile: 12 heads of 64, 16 tiles 7.2 and 9.5, 24 tiles 9.3 and 9.9, 32 tiles 11.2 and 9.9; 32 heads of
-// 128, 16 tiles 9.7 and 11.1, 32 tiles 15.9 and 12.9; 128 heads of 128, 16 tiles 10.6 and 16.2, 40 tiles 19.7 and 23.8.  With several heads
-// per SM, which fill the time among themselves: 256 of 128, 16 tiles 21.1 and 21.9, 32 tiles 37.8 and 31.9; 768 of 64, 16 tiles 29.4 and
-// 32.6, 32 tiles 53.2 and 48.8; 1024 of 128, 16 tiles 60.5 and 54.5, 24 tiles 87.3 and 72.5.  A straight line below these borders up to a
+// (us), all positions in use, 64 to a tile: 12 heads of 64, 16 tiles 7.5 and 10.1, 24 tiles 9.5 and 10.3, 32 tiles 11.4 and 10.2; 32 heads of
+// 128, 16 tiles 9.9 and 11.4, 32 tiles 15.9 and 13.1; 128 heads of 128, 16 tiles 10.7 and 16.3, 40 tiles 19.7 and 24.2.  With several heads
+// per SM, which fill the time among themselves: 256 of 128, 16 tiles 22.0 and 21.8, 32 tiles 39.4 and 32.0; 768 of 64, 16 tiles 30.5 and
+// 33.1, 32 tiles 55.4 and 49.4; 1024 of 128, 16 tiles 61.6 and 54.4, 24 tiles 87.6 and 72.1.  A straight line below these borders up to a
 // head per SM, and one border above.
 __host__ inline long long a8_whole(long long heads, long long sms) { return heads <= sms ? 18 + 32 * heads / sms : 16; }
 

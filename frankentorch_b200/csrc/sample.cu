@@ -20,11 +20,14 @@
 //   * The choice: sums per warp in the order of the ids, the warp with the target, the 32 vectors, the lane.
 // The random sums of shared memory's counters take 10 cycles of an SM for 32 elements; collectives of a cluster 1500 cycles each.
 //
-// Measured: 256 rows of 50257 fp32, 51 MB in 22 us with the largest alone, 36 with k = 50 and p, 82 with k = 200, 73 - 92 with p = 0.9, 45
-// with the whole distribution, 65 with settings that change from row to row; 512 rows of 128003 bf16 with p = 0.9 262; one
-// row of 50257 with k = 50 and p 8, 64 with the whole distribution 15 a call.  Reading is a small part of it.  Of the 65 us the SMs issue in 42 % of
-// the cycles, of the 262 in 54 %, with 64-bit arithmetic in 8 and 13 %: barriers, the CTA's own and the cluster's, are the largest stall
+// Measured: 256 rows of 50257 fp32, 51 MB in 22 us with the largest alone, 36 with k = 50 and p, 84 with k = 200, 74 - 93 with p = 0.9, 46
+// with the whole distribution, 66 with settings that change from row to row; 512 rows of 128003 bf16 with p = 0.9 268; one
+// row of 50257 with k = 50 and p 8, 64 with the whole distribution 15 a call.  Reading is a small part of it.  Of the 66 us the SMs issue in 43 % of
+// the cycles, of the 268 in 53 %, with 64-bit arithmetic in 9 and 13 %: barriers, the CTA's own and the cluster's, are the largest stall
 // (3.6 and 4.1 of 8 and 11 cycles of a warp per instruction).
+//
+// Registers are bounded for four CTAs to an SM, 64 each, which leaves 8 to 204 bytes of spills.  Bounded for three, where nothing spills, and five:
+// the 66 us become 65.4 and 69.7, the 268 302 and 279, the 15.3 of 64 whole distributions 19.1 and 15.6, the 84 of k = 200 82.8 and 84.9.
 #include <math.h>
 
 #include <type_traits>

@@ -25,8 +25,8 @@ Arguments that the host can check are refused with :class:`~.kernels.KernelError
 device is reported by that device's :func:`~.kernels.check_status`, and what it leads to is not read and not written.  A call keeps
 nothing: its scratch is its own, so calls of several streams, threads and captured graphs do not meet, and the same call gives
 the same bits.  (The attention cuts a sequence's heads by the work of the whole call: beside other sequences its last bits may
-be others.)  Two tokens of one append must not have the same place (over 8 bits: two sequences no common block), and an output must not overlap an input other than where
-the function says so; one whose own rows overlap is refused.
+be others.)  Two tokens of one append must not have the same place (over 8 bits: two sequences no common block), and an output must not
+overlap an input other than where the function says so; one whose own rows overlap is refused.
 """
 from __future__ import annotations
 
@@ -71,7 +71,8 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     returned turned; queries behind ``counts[b]`` are copied as they are.  ``q_out`` may be ``q`` itself.
 
     Into a cache in 8 bits a block's new elements (keys in fp32 behind their rotation) get the smallest power of two, 2^-100 at least, of
-    which 448 times reaches the largest finite one, and each is rounded once to a multiple of it; infinities and NaN are held as NaN.  (From 1.9375 2^127 on the nearest multiple is 2^128, which neither fp32 nor bf16 holds.)
+    which 448 times reaches the largest finite one, and each is rounded once to a multiple of it; infinities and NaN are held as NaN.
+    (From 1.9375 2^127 on the nearest multiple is 2^128, which neither fp32 nor bf16 holds.)
     A block that has rows in front of ``start[b]`` keeps at least its own scale; where it grows, those rows are rounded anew (exact but
     for the smallest ones).  What stands in a block behind the last new token has no meaning any more."""
     return _lib.bind().paged_append(k_pages, v_pages, table, k, v, start, counts, q, inv_freq, interleaved, q_out, k_scales, v_scales)
@@ -119,7 +120,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, vocab: Optional[int] 
     """A token for each row of ``logits`` (the first ``vocab`` columns, 2^20 at most, of ``[R, columns]``; bf16, fp16 or fp32) from
     ``uniform`` (fp32 ``[R]``, in [0, 1)); returns ``(token int64 [R], logprob fp32 [R])``.
 
-    Token ``i`` weighs ``w_i = round(2^43 exp((x_i - max x) / temperature))`` (formed in 64 bits: within 2^-8 of a half, either neighbour).  In the order of the logits, equal ones by their ids, are kept
+    Token ``i`` weighs ``w_i = round(2^43 exp((x_i - max x) / temperature))`` (formed in 64 bits: within 2^-8 of a half, either neighbour).
+    In the order of the logits, equal ones by their ids, are kept
 
     * ``top_k``: the first ``top_k`` (0: all);
     * ``top_p``: of those the ones before which less than ``top_p`` of their sum lies (1: all; the first always);
