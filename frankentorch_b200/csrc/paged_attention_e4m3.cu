@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
     k_by = power(with_key);
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      const float own = factor * power(-of_factor) * power(max(e[r] - 14 + of_factor - with_key, -126));
+      const int rest = e[r] - 14 + of_factor - with_key;      // -240 to 112: rows may be that far apart
+      const float own = factor * power(-of_factor) * power(rest >> 1) * power(rest - (rest >> 1));
       sc[2 * r] = ONE ? own : __shfl_sync(0xffffffffu, own, c0 * 4);
       if (!ONE) sc[2 * r + 1] = __shfl_sync(0xffffffffu, own, c0 * 4 + 4);
     }
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(W * 32, A8Smem<ROWS, HD, W>::CTAS) paged_attn_
       const uint32_t ks = ring_s + stage * STAGE + l_at, vs = ks + N * HD;
       const unsigned ok = there[stage];
       load(stage == 0 ? STAGES - 1 : stage - 1);      // the stage that the tile before left: its reads are behind the warp's barrier
-      const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);      // keys', values', the values' exponents
+      const float* scales = reinterpret_cast<const float*>(ring + stage * STAGE + SM::DATA);      // keys', values'
       const float k_scale = scales[lane] * k_by, v_scale = scales[N + lane], v_exp = (float)max((int)(__float_as_uint(v_scale) >> 23 & 255) - 127, -100);
       // Scores with the tokens as rows: s[2 r + t] of tokens 16 t and on, the r-th eight heads
       float s[2 * RR][4] = {};

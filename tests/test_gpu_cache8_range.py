@@ -200,3 +200,19 @@ def test_few_heads_of_many_queries_in_pieces(cuda_device, B, H, Hk, hd, n):
     ks, vs = (torch.exp2(torch.randint(-9, -5, (B * P, Hk, 2), generator=g, device="cuda").float()) for _ in range(2))
     table = torch.randperm(B * P, generator=g, device="cuda").to(torch.int32).view(B, P)
     _check(torch.randn(B, H, hd, generator=g, device="cuda").to(BF), k, v, table, lengths, ks, vs)
+
+
+@pytest.mark.parametrize("H", [2, 7, 12, 16])
+def test_queries_of_a_group_far_apart(cuda_device, H):
+    """One head's queries are 2^140 times those of the others, whose scores are next to 0."""
+    g = _gen(H)
+    n, page, hd = 500, 64, 64
+    P = -(-n // page)
+    k, v = (torch.randn(P, 1, page, hd, generator=g, device="cuda").mul(100).clamp(-448, 448).to(E4M3) for _ in range(2))
+    ks = torch.full((P, 1, 1), 2.0 ** -10, device="cuda")
+    vs = torch.full((P, 1, 1), 2.0 ** -7, device="cuda")
+    q = torch.randn(1, H, hd, generator=g, device="cuda").clamp(-1.9, 1.9) * 2.0 ** -13
+    q[:, H // 2] *= 2.0 ** 70      # (2^140 is no number of fp32)
+    q[:, H // 2] *= 2.0 ** 70
+    assert bool(q.isfinite().all())
+    _check(q.to(BF), k, v, torch.arange(P, dtype=torch.int32, device="cuda")[None], [n], ks, vs)
